@@ -29,8 +29,9 @@ EXPORTS = (
     "dlt_timing_enable", "dlt_timing_collect", "dlt_debug_copy",
     "dlt_swa_fwd_image", "dlt_swa_bwd_image", "dlt_swa_image_offsets", "dlt_swa_fwd_rot", "dlt_swa_bwd_rot",
     "dlt_swa_bwd_noalloc", "dlt_dry_run", "dlt_last_kernel_family",
+    "dlt_rope_axes", "dlt_window_workspace", "dlt_window_fwd", "dlt_window_bwd", "dlt_paged_append", "dlt_paged_workspace", "dlt_paged_attn",
 )
-KERNEL_FAMILIES = ("none", "marching", "streaming", "tile", "flash", "generic")   # DLT_FAMILY_* of include/dlt.h
+KERNEL_FAMILIES = ("none", "marching", "streaming", "tile", "flash", "generic", "band")   # DLT_FAMILY_* of include/dlt.h
 NOALLOC_MAX_DELTA = 1 << 20  # DLT_NOALLOC_MAX_DELTA of include/dlt.h
 KERNEL_NAMES = ("rope2d", "attn_fwd", "attn_delta", "attn_bwd_kv", "attn_bwd_q")
 
@@ -71,6 +72,27 @@ class FlashShape(Structure):
     _fields_ = [
         ("B", c_int32), ("H", c_int32), ("Lq", c_int32), ("Lk", c_int32), ("dk", c_int32), ("dv", c_int32),
         ("sm_scale", c_float), ("causal", c_int32), ("dtype", c_int32),
+    ]
+
+
+class WindowShape(Structure):
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("Hkv", c_int32), ("Lq", c_int32), ("Lk", c_int32), ("dk", c_int32), ("dv", c_int32),
+        ("window", c_int32), ("n_sink", c_int32), ("sm_scale", c_float), ("dtype", c_int32),
+    ]
+
+
+class PagedShape(Structure):
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("Hkv", c_int32), ("T", c_int32), ("dk", c_int32), ("dv", c_int32),
+        ("page", c_int32), ("n_pages", c_int32), ("cols", c_int32), ("window", c_int32), ("n_sink", c_int32), ("sm_scale", c_float), ("dtype", c_int32),
+    ]
+
+
+class RopeAxesDesc(Structure):
+    _fields_ = [
+        ("n_axes", c_int32), ("layout", c_int32), ("pos", c_void_p), ("pos_strides", c_int64 * 3), ("table", c_void_p * 4),
+        ("table_stride0", c_int64 * 4), ("n_rdim", c_int32 * 4), ("len", c_int32 * 4),
     ]
 
 
@@ -139,6 +161,21 @@ def _declare(lib) -> None:
     lib.dlt_flash_fwd_ws.argtypes = fwd + [POINTER(FlashShape), c_void_p, c_int64, c_void_p]
     lib.dlt_flash_bwd_ws.restype = c_int
     lib.dlt_flash_bwd_ws.argtypes = bwd + [POINTER(FlashShape), c_void_p, c_int64, c_void_p]
+    tensor = [c_void_p, P64]
+    lib.dlt_rope_axes.restype = c_int
+    lib.dlt_rope_axes.argtypes = (tensor * 2 + [c_int32]) * 2 + [c_int32, c_int64, c_int64, POINTER(RopeAxesDesc), c_int, c_int, c_void_p]
+    lib.dlt_window_workspace.restype = c_int
+    lib.dlt_window_workspace.argtypes = [POINTER(WindowShape), c_int, P64]
+    lib.dlt_window_fwd.restype = c_int
+    lib.dlt_window_fwd.argtypes = tensor * 4 + [c_void_p, POINTER(WindowShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_window_bwd.restype = c_int
+    lib.dlt_window_bwd.argtypes = tensor * 5 + [c_void_p, c_void_p] + tensor * 3 + [POINTER(WindowShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_paged_append.restype = c_int
+    lib.dlt_paged_append.argtypes = tensor * 6 + [c_void_p, c_int64, c_void_p, c_void_p, POINTER(RopeAxesDesc), POINTER(PagedShape), c_void_p]
+    lib.dlt_paged_workspace.restype = c_int
+    lib.dlt_paged_workspace.argtypes = [POINTER(PagedShape), P64]
+    lib.dlt_paged_attn.restype = c_int
+    lib.dlt_paged_attn.argtypes = tensor * 4 + [c_void_p, c_int64, c_void_p, c_void_p, POINTER(PagedShape), c_void_p, c_int64, c_void_p]
     lib.dlt_debug_copy.restype = c_int
     lib.dlt_debug_copy.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
     lib.dlt_timing_enable.restype = c_int

@@ -1,0 +1,353 @@
+// Entry points of the 1D window attention, the paged cache's attention and append: argument checks, how a call is cut into workgroups, and
+// the launches that sum partial results.
+#include <cmath>
+#include "band_common.h"
+#include "band_shapes.h"
+#include "rope_axes.h"
+
+namespace {
+
+// ---- sums of shares -------------------------------------------------------------------------------------------------------------
+// Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row.  A thread takes 4 dims of a row and the shares
+// in their order.
+template <typename TIO>
+__global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
+  const int per = a.dv_ / 4;
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = gid / per;
+  const int d = 4 * (int)(gid - at * per);
+  if (at >= (int64_t)a.B * a.Hkv * a.rows) return;
+  const int bh = (int)(at / a.rows), r = (int)(at - (int64_t)bh * a.rows), b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int n_q = a.pg.n_new != nullptr ? dlt_imax(0, dlt_imin(a.pg.n_new[b], a.Lq)) : a.Lq;
+  const float* ml = a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (r < n_q * a.G)
+    for (int s = 0; s < a.shares; s++) {
+      const int64_t row = ((int64_t)bh * a.shares + s) * a.rows + r;
+      const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
+      if (x.x == -INFINITY && x.y == 0.f) continue;   // the share held no key of the row
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + row * a.dv_ + d);
+      float f1, f2;
+      flash_merge(m, x.x, 1.f, f1, f2);
+      l = flash_add(l, f1, x.y, f2);
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[i] = flash_add(o[i], f1, v[i], f2);
+    }
+  const float f = l == 0.f ? 0.f : 1.f / l;
+  TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r) + d;
+  u32x2 w;
+  w.x = pack2<TIO>(o[0] * f, o[1] * f);
+  w.y = pack2<TIO>(o[2] * f, o[3] * f);
+  store_stream8(p, w);
+  if (d == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
+}
+
+// dK (times sm_scale) or dV: partial sums [bh][share][key][dims], added in the order of the shares
+template <typename TIO>
+__global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
+  const bool keys = blockIdx.y == 0;
+  const int dims = keys ? a.dk_ : a.dv_, per = dims / 4;
+  const float* part = a.part + (keys ? 0 : (int64_t)a.B * a.Hkv * a.shares * a.Lk * a.dk_);
+  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t at = gid / per;
+  const int d = 4 * (int)(gid - at * per);
+  if (at >= (int64_t)a.B * a.Hkv * a.Lk) return;
+  const int bh = (int)(at / a.Lk), j = (int)(at - (int64_t)bh * a.Lk), b = bh / a.Hkv, h = bh - b * a.Hkv;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < a.shares; i++) s += *reinterpret_cast<const f32x4*>(part + (((int64_t)bh * a.shares + i) * a.Lk + j) * dims + d);
+  if (keys) s *= a.sm_scale;
+  TIO* p = keys ? reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1] + j * a.dks[2] : reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1] + j * a.dvs[2];
+  u32x2 w;
+  w.x = pack2<TIO>(s[0], s[1]);
+  w.y = pack2<TIO>(s[2], s[3]);
+  store_stream8(p + d, w);
+}
+
+int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
+  if (a.shares <= 1) return DLT_OK;
+  const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.Lk : a.rows);
+  const int per = (backward ? dlt_imax(a.dk_, a.dv_) : a.dv_) / 4;
+  const dim3 grid((unsigned)((rows * per + 255) / 256), backward ? 2 : 1);
+  dlt_timing_before(backward ? DLT_K_BWD_KV : DLT_K_FWD, stream);
+  if (backward) {
+    if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kv_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(band_join_kv_kernel<f16_t>, grid, dim3(256), 0, stream, a);
+  } else {
+    if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(band_join_kernel<f16_t>, grid, dim3(256), 0, stream, a);
+  }
+  dlt_timing_after(stream);
+  DLT_CHECK_LAUNCH("window sum launch");
+  return DLT_OK;
+}
+
+// ---- checks ------------------------------------------------------------------------------------------------------------------------
+int check_rows(const char* who, const char* name, const void* p, const int64_t* st, bool empty, int64_t span /* largest offset inside a slab that must fit 32 bits, elements */) {
+  DLT_REQUIRE(st != nullptr && (p != nullptr || empty), "%s: %s is NULL", who, name);
+  if (empty) return DLT_OK;
+  DLT_REQUIRE(st[3] == 1 && (uintptr_t)p % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0,
+              "%s: rows of %s must be contiguous and start at multiples of 16 bytes", who, name);
+  DLT_REQUIRE(st[0] >= 0 && st[1] >= 0 && st[2] >= 0, "%s: negative stride of %s", who, name);
+  if (span >= (int64_t)1 << 30) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: strides of %s are too large", who, name);
+  return DLT_OK;
+}
+
+int check_common(const char* who, int B, int H, int Hkv, int dk, int dv, int window, int n_sink, float sm_scale, int dtype) {
+  DLT_REQUIRE(B > 0 && H > 0 && Hkv > 0, "%s: B=%d H=%d Hkv=%d must be positive", who, B, H, Hkv);
+  DLT_REQUIRE(H % Hkv == 0, "%s: %d query heads do not share %d key heads evenly", who, H, Hkv);
+  DLT_REQUIRE(dk > 0 && dv > 0, "%s: dk=%d dv=%d must be positive", who, dk, dv);
+  DLT_REQUIRE(window >= 1 && n_sink >= 0, "%s: window %d must be at least 1, n_sink %d at least 0", who, window, n_sink);
+  DLT_REQUIRE(std::isfinite(sm_scale) && sm_scale > 0.f, "%s: sm_scale must be positive and finite", who);
+  DLT_REQUIRE(dtype == DLT_BF16 || dtype == DLT_FP16 || dtype == DLT_FP32, "%s: bad dtype %d", who, dtype);
+  if (dtype == DLT_FP32) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: fp32 tensors are not covered, expected bfloat16 or float16", who);
+  if (dk > 128 || dv > 128 || dk % 8 != 0 || dv % 8 != 0)
+    return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: head dims dk=%d dv=%d must be multiples of 8 up to 128", who, dk, dv);
+  return DLT_OK;
+}
+
+void set_scalars(BandArgs& a, float sm_scale, int Hkv, int G) {
+  a.sm_scale = sm_scale;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.Hkv = Hkv;
+  a.G = G;
+  dlt_fastdiv_make((uint32_t)G, a.mG, a.sG);
+  a.q16 = 16 % G == 0;
+}
+
+int window_problem(const char* who, const dlt_window_shape_t* s, BandArgs& a) {
+  DLT_REQUIRE(s != nullptr, "%s: shape is NULL", who);
+  const int rc = check_common(who, s->B, s->H, s->Hkv, s->dk, s->dv, s->window, s->n_sink, s->sm_scale, s->dtype);
+  if (rc != DLT_OK) return rc;
+  DLT_REQUIRE(s->Lq >= 0 && s->Lk >= 0, "%s: negative length", who);
+  const int G = s->H / s->Hkv;
+  if ((int64_t)s->Lq * G >= 1 << 30 || s->Lk >= 1 << 30) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  a = BandArgs{};
+  a.B = s->B; a.Lq = s->Lq; a.Lk = s->Lk; a.dk_ = s->dk; a.dv_ = s->dv;
+  a.W = dlt_imin(s->window, dlt_imax(s->Lk, 1));
+  a.S = dlt_imin(s->n_sink, s->Lk);
+  a.off = s->Lk - s->Lq;
+  a.rows = s->Lq * G;
+  a.shares = 1;
+  set_scalars(a, s->sm_scale, s->Hkv, G);
+  a.group = flash_causal_group(dlt_imax(s->Lk, 1), s->dk, s->dv);
+  return DLT_OK;
+}
+
+int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
+  DLT_REQUIRE(s != nullptr, "%s: shape is NULL", who);
+  const int rc = check_common(who, s->B, s->H, s->Hkv, s->dk, s->dv, s->window, s->n_sink, s->sm_scale, s->dtype);
+  if (rc != DLT_OK) return rc;
+  DLT_REQUIRE(s->T >= 0 && s->cols > 0 && s->n_pages > 0 && s->page > 0, "%s: T=%d cols=%d n_pages=%d page=%d", who, s->T, s->cols, s->n_pages, s->page);
+  if (s->page % 16 != 0) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: pages of %d tokens, expected a multiple of 16", who, s->page);
+  const int G = s->H / s->Hkv;
+  if ((int64_t)s->T * G >= 1 << 30 || (int64_t)s->cols * s->page >= 1 << 30) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many tokens", who);
+  a = BandArgs{};
+  a.B = s->B; a.Lq = s->T; a.Lk = s->cols * s->page; a.dk_ = s->dk; a.dv_ = s->dv;
+  a.W = dlt_imin(s->window, a.Lk);
+  a.S = dlt_imin(s->n_sink, a.Lk);
+  a.rows = s->T * G;
+  a.shares = 1;
+  set_scalars(a, s->sm_scale, s->Hkv, G);
+  a.group = 1;
+  a.pg.cols = s->cols;
+  a.pg.n_pages = s->n_pages;
+  a.pg.p16 = s->page / 16;
+  dlt_fastdiv_make((uint32_t)a.pg.p16, a.pg.m16, a.pg.s16);
+  return DLT_OK;
+}
+
+// ---- cutting a call into workgroups ---------------------------------------------------------------------------------------------------
+// Rows: 128 a workgroup, 64 where that leaves CUs idle.  Where even those are few, the keys of a block are taken by several workgroups (shares).
+int plan_rows(BandArgs& a, bool shares) {
+  const int cus = dlt_device_cus();
+  const int64_t bh = (int64_t)a.B * a.Hkv;
+  int np = bh * ((a.rows + 127) / 128) < 2 * cus ? 1 : 2;
+  a.nblk = (a.rows + 64 * np - 1) / (64 * np);
+  a.shares = 1;
+  if (shares) {
+    const int64_t wgs = bh * a.nblk;
+    const int most = (int)dlt_imin64((int64_t)a.W + a.S + 64 * np / a.G + 1, a.Lk) / 64 + 1;   // chunks of a block
+    int64_t n = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
+    n = dlt_imin64(n, most / 4);
+    const int64_t row_bytes = bh * a.rows * (a.dv_ + 2) * 4;
+    n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(row_bytes > 0 ? row_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
+    a.shares = n < 1 ? 1 : (int)n;
+  }
+  return np;
+}
+int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
+// Keys: the rows that see a block of keys taken by several workgroups where blocks are few
+void plan_keys(BandArgs& a) {
+  const int cus = dlt_device_cus();
+  const int own = band_kv_own(band_class(a.dk_, a.dv_));
+  a.nblk = (a.Lk + own - 1) / own;
+  const int64_t bh = (int64_t)a.B * a.Hkv, wgs = bh * a.nblk;
+  const int64_t most = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;
+  int64_t n = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
+  n = dlt_imin64(n, most / 4);
+  const int64_t key_bytes = bh * a.Lk * (a.dk_ + a.dv_) * 4;
+  n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(key_bytes > 0 ? key_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
+  a.shares = n < 1 ? 1 : (int)n;
+}
+int64_t keys_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.Lk * (a.dk_ + a.dv_) * 4 : 0; }
+
+int check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
+  DLT_REQUIRE(need == 0 || (ws != nullptr && have >= need && (uintptr_t)ws % 16 == 0), "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", who,
+              (long long)need, (long long)(ws != nullptr ? have : 0));
+  return DLT_OK;
+}
+int check_grid(const char* who, const BandArgs& a) {
+  if ((int64_t)a.B * a.Hkv * a.nblk * a.shares > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  return DLT_OK;
+}
+void strides3(int64_t (&to)[3], const int64_t* st) {
+  for (int i = 0; i < 3; i++) to[i] = st[i];
+}
+// queries of a (batch, kv head) are addressed with 32-bit offsets over 16 tokens and the heads of the group; keys over 16 tokens
+int64_t row_span(const int64_t* st, int G) { return st == nullptr ? 0 : 17 * st[2] + (int64_t)G * st[1]; }
+int64_t key_span(const int64_t* st) { return st == nullptr ? 0 : 17 * st[2]; }
+
+}  // namespace
+
+extern "C" int dlt_window_workspace(const dlt_window_shape_t* shape, int backward, int64_t* bytes) {
+  DLT_REQUIRE(bytes != nullptr, "window_workspace: bytes is NULL");
+  BandArgs a;
+  const int rc = window_problem("window_workspace", shape, a);
+  if (rc != DLT_OK) return rc;
+  if (backward) plan_keys(a);
+  else plan_rows(a, true);
+  *bytes = backward ? keys_bytes(a) : rows_bytes(a);
+  return DLT_OK;
+}
+
+extern "C" int dlt_window_fwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                              void* o, const int64_t o_strides[4], float* lse2, const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
+  const char* who = "window_fwd";
+  hipStream_t stream = (hipStream_t)stream_;
+  BandArgs a;
+  int rc = window_problem(who, shape, a);
+  if (rc != DLT_OK) return rc;
+  if ((rc = check_rows(who, "q", q, q_strides, a.Lq == 0, row_span(q_strides, a.G))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "k", k, k_strides, a.Lk == 0, key_span(k_strides))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "v", v, v_strides, a.Lk == 0, key_span(v_strides))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
+  DLT_REQUIRE(lse2 != nullptr || a.Lq == 0, "%s: lse2 is NULL", who);
+  const int np = plan_rows(a, true);
+  if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
+  if ((rc = check_grid(who, a)) != DLT_OK) return rc;
+  if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
+  a.q = q; a.k = k; a.v = v; a.out = o; a.lse = lse2; a.part = (float*)ws;
+  strides3(a.qs, q_strides); strides3(a.ks, k_strides); strides3(a.vs, v_strides); strides3(a.os, o_strides);
+  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_fwd_64(a, shape->dtype, np, stream) : dlt_band_fwd_128(a, shape->dtype, np, stream);
+  return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
+}
+
+extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                              const void* o, const int64_t o_strides[4], const void* d_o, const int64_t do_strides[4], const float* lse2, float* delta,
+                              void* dq, const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4], void* dv, const int64_t dv_strides[4],
+                              const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
+  const char* who = "window_bwd";
+  hipStream_t stream = (hipStream_t)stream_;
+  BandArgs a;
+  int rc = window_problem(who, shape, a);
+  if (rc != DLT_OK) return rc;
+  const bool nq = a.Lq == 0, nk = a.Lk == 0;
+  struct { const char* name; const void* p; const int64_t* st; bool none; int64_t span; } ts[] = {
+      {"q", q, q_strides, nq, row_span(q_strides, a.G)}, {"k", k, k_strides, nk, key_span(k_strides)}, {"v", v, v_strides, nk, key_span(v_strides)},
+      {"o", o, o_strides, nq, 0}, {"d_o", d_o, do_strides, nq, row_span(do_strides, a.G)}, {"dq", dq, dq_strides, nq, 0}, {"dk", dk, dk_strides, nk, 0},
+      {"dv", dv, dv_strides, nk, 0}};
+  for (const auto& t : ts)
+    if ((rc = check_rows(who, t.name, t.p, t.st, t.none, t.span)) != DLT_OK) return rc;
+  DLT_REQUIRE((lse2 != nullptr && delta != nullptr) || nq, "%s: lse2 or delta is NULL", who);
+  BandArgs kv = a;
+  plan_keys(kv);
+  const int np = plan_rows(a, false);
+  if ((rc = check_ws(who, ws, ws_bytes, keys_bytes(kv))) != DLT_OK) return rc;
+  if ((rc = check_grid(who, a)) != DLT_OK || (rc = check_grid(who, kv)) != DLT_OK) return rc;
+  if (dlt_route_note(DLT_FAMILY_BAND)) return DLT_OK;
+  for (BandArgs* x : {&a, &kv}) {
+    x->q = q; x->k = k; x->v = v; x->o = o; x->d_o = d_o; x->dq = dq; x->dk = dk; x->dv = dv;
+    x->lse = const_cast<float*>(lse2); x->delta = delta; x->part = (float*)ws;
+    strides3(x->qs, q_strides); strides3(x->ks, k_strides); strides3(x->vs, v_strides); strides3(x->os, o_strides); strides3(x->dos, do_strides);
+    strides3(x->dqs, dq_strides); strides3(x->dks, dk_strides); strides3(x->dvs, dv_strides);
+  }
+  const bool small = band_class(a.dk_, a.dv_) == 64;
+  if (!nq && (rc = small ? dlt_band_bwd_q_64(a, shape->dtype, np, stream) : dlt_band_bwd_q_128(a, shape->dtype, np, stream)) != DLT_OK) return rc;
+  if (nk) return DLT_OK;
+  if ((rc = small ? dlt_band_bwd_kv_64(kv, shape->dtype, stream) : dlt_band_bwd_kv_128(kv, shape->dtype, stream)) != DLT_OK) return rc;
+  return join(kv, true, shape->dtype, stream);
+}
+
+extern "C" int dlt_paged_workspace(const dlt_paged_shape_t* shape, int64_t* bytes) {
+  DLT_REQUIRE(bytes != nullptr, "paged_workspace: bytes is NULL");
+  BandArgs a;
+  const int rc = paged_problem("paged_workspace", shape, a);
+  if (rc != DLT_OK) return rc;
+  plan_rows(a, true);
+  *bytes = rows_bytes(a);
+  return DLT_OK;
+}
+
+extern "C" int dlt_paged_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4], const void* v_cache,
+                              const int64_t v_cache_strides[4], void* o, const int64_t o_strides[4], const int32_t* table, int64_t table_stride, const int32_t* seq_len,
+                              const int32_t* n_new, const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
+  const char* who = "paged_attn";
+  hipStream_t stream = (hipStream_t)stream_;
+  BandArgs a;
+  int rc = paged_problem(who, shape, a);
+  if (rc != DLT_OK) return rc;
+  if ((rc = check_rows(who, "q", q, q_strides, a.Lq == 0, row_span(q_strides, a.G))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "k_cache", k_cache, k_cache_strides, false, key_span(k_cache_strides))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "v_cache", v_cache, v_cache_strides, false, key_span(v_cache_strides))) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
+  DLT_REQUIRE(table != nullptr && seq_len != nullptr, "%s: table or seq_len is NULL", who);
+  DLT_REQUIRE(table_stride >= 0, "%s: negative table stride", who);
+  const int np = plan_rows(a, true);
+  if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
+  if ((rc = check_grid(who, a)) != DLT_OK) return rc;
+  if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
+  a.q = q; a.k = k_cache; a.v = v_cache; a.out = o; a.part = (float*)ws;
+  strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);
+  a.pg.table = table; a.pg.seq = seq_len; a.pg.n_new = n_new; a.pg.ts = table_stride;
+  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged_64(a, shape->dtype, np, stream) : dlt_band_paged_128(a, shape->dtype, np, stream);
+  return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
+}
+
+extern "C" int dlt_paged_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4], const void* q, const int64_t q_strides[4],
+                                void* q_out, const int64_t q_out_strides[4], void* k_cache, const int64_t k_cache_strides[4], void* v_cache,
+                                const int64_t v_cache_strides[4], const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
+                                const dlt_rope_axes_t* rope, const dlt_paged_shape_t* s, void* stream) {
+  const char* who = "paged_append";
+  DLT_REQUIRE(s != nullptr, "%s: shape is NULL", who);
+  DLT_REQUIRE(s->dtype == DLT_BF16 || s->dtype == DLT_FP16 || s->dtype == DLT_FP32, "%s: bad dtype %d", who, s->dtype);
+  DLT_REQUIRE(s->B > 0 && s->H >= 0 && s->Hkv > 0 && s->T >= 0 && s->dk > 0 && s->dv > 0, "%s: B=%d H=%d Hkv=%d T=%d dk=%d dv=%d", who, s->B, s->H, s->Hkv, s->T, s->dk,
+              s->dv);
+  DLT_REQUIRE(s->cols > 0 && s->n_pages > 0 && s->page > 0 && (int64_t)s->cols * s->page < 1 << 30, "%s: cols=%d n_pages=%d page=%d", who, s->cols, s->n_pages, s->page);
+  DLT_REQUIRE((int64_t)s->H + 2 * (int64_t)s->Hkv <= 0x7fffffff, "%s: too many heads", who);
+  DLT_REQUIRE(table != nullptr && seq_len != nullptr && table_stride >= 0, "%s: table or seq_len is NULL, or the table's stride negative", who);
+  RotArgs a{};
+  const int rc = dlt_rope_axes_make(rope, s->dk, false, 0, who, a.r);
+  if (rc != DLT_OK) return rc;
+  auto stream_of = [&](const void* src, const int64_t* ss, const void* dst, const int64_t* ds, int H, int C, int rot, int paged) {
+    RotStream& x = a.s[a.n++];
+    x.src = src; x.dst = const_cast<void*>(dst);
+    for (int i = 0; i < 4; i++) { x.ss[i] = ss[i]; x.ds[i] = ds[i]; }
+    x.H = H; x.C = C; x.rot = rot; x.paged = paged;
+  };
+  const bool none = s->T == 0;
+  DLT_REQUIRE(k_strides != nullptr && v_strides != nullptr && k_cache_strides != nullptr && v_cache_strides != nullptr && k_cache != nullptr && v_cache != nullptr &&
+                  (none || (k != nullptr && v != nullptr)), "%s: a tensor of keys or values is NULL", who);
+  if (s->H > 0) {
+    DLT_REQUIRE(q_strides != nullptr && q_out_strides != nullptr && (none || (q != nullptr && q_out != nullptr)), "%s: q or q_out is NULL", who);
+    DLT_REQUIRE(none || q != q_out, "%s: q and q_out must be two buffers", who);
+    stream_of(q, q_strides, q_out, q_out_strides, s->H, s->dk, 1, 0);
+  }
+  stream_of(k, k_strides, k_cache, k_cache_strides, s->Hkv, s->dk, 1, 1);
+  stream_of(v, v_strides, v_cache, v_cache_strides, s->Hkv, s->dv, 0, 1);
+  if (none) return DLT_OK;
+  a.B = s->B; a.T = s->T;
+  a.table = table; a.seq = seq_len; a.n_new = n_new; a.tbs = table_stride;
+  a.cols = s->cols; a.n_pages = s->n_pages; a.page = s->page;
+  return dlt_rotate_rows(a, s->dtype, "paged_append launch", (hipStream_t)stream);
+}

@@ -1,0 +1,524 @@
+// Backward pass of attention over a 1D window with sinks and grouped heads (band_common.h).
+//
+//   P = exp2(scale q.k - lse2), dP = dO.v, dS = P (dP - delta), delta = rowsum(dO o)
+//   dQ = sm_scale dS K  (rows own, K and V stream; this kernel runs first and stores delta)
+//   dK = sm_scale dS^T Q, dV = P^T dO  (keys own; the rows of all heads of the group stream, so the sum over the heads that share a
+//   key is part of the product: no atomics, one order of summation)
+// P and dS are rounded to 16 bits for the second products, as their operands have to be; sums stay in 32 bits to the end.
+#pragma once
+#include "band_common.h"
+
+// ---- dQ ---------------------------------------------------------------------------------------------------------------------------
+template <typename TIO, int D, int NP, int CK, int NW, int PAD>
+__global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_q_kernel(const BandArgs a) {
+  typedef BandBuf<D, CK> B;
+  extern __shared__ __align__(16) char smem[];
+  constexpr int KC = D / 32, KB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NG = CK / NW / 16;
+  static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
+  constexpr int PER_CHUNK = 2 * NG * BandStage<D>::NI;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const int lin = xcd_remap(blockIdx.x, gridDim.x);
+  int bh, r_, blk;
+  flash_block_causal(lin, a.nblk, a.B * a.Hkv, a.group, 1, true, bh, r_, blk);
+  const int x0 = blk * OWN;
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];
+  const TIO* dob = reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1];
+  const TIO* ob = reinterpret_cast<const TIO*>(a.o) + b * a.os[0] + (int64_t)h * a.G * a.os[1];
+  const TIO* kh = reinterpret_cast<const TIO*>(a.k) + b * a.ks[0] + h * a.ks[1];
+  const TIO* vh = reinterpret_cast<const TIO*>(a.v) + b * a.vs[0] + h * a.vs[1];
+
+  BandWalk<CK> W;
+  const int xl = dlt_imin(x0 + OWN, a.rows) - 1;
+  W.init(a.off + band_row(a, x0).tok, a.off + band_row(a, xl).tok, a.W, a.S);
+
+  BandStage<D> stk, stv;
+  stk.init(lane, a.dk_, a.ks[2]);
+  stv.init(lane, a.dv_, a.vs[2]);
+  if constexpr (PAD) {
+#pragma unroll
+    for (int i = 0; i < NBUF; i++) {
+      flashd_zero_pads<D>(smem + i * B::BUF, CK, a.dk_ >> 3, tid, 64 * NW);
+      flashd_zero_pads<D>(smem + i * B::BUF + B::REG, CK, a.dv_ >> 3, tid, 64 * NW);
+    }
+  }
+  auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NG; u++) {
+      const int t0 = W.x(i) + wave * 16 * NG + 16 * u;
+      char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
+      if (t0 + 16 <= a.Lk) {
+        stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (int64_t)t0 * a.ks[2]), dst);
+        stv.template issue<PAD>(reinterpret_cast<const char*>(vh + (int64_t)t0 * a.vs[2]), dst + B::REG);
+      } else {
+        keep_branch();
+        const int tc = dlt_imin(t0, a.Lk - 1);
+        stk.template issue_clamped<PAD>(reinterpret_cast<const char*>(kh + (int64_t)tc * a.ks[2]), a.Lk - 1 - tc, dst);
+        stv.template issue_clamped<PAD>(reinterpret_cast<const char*>(vh + (int64_t)tc * a.vs[2]), a.Lk - 1 - tc, dst + B::REG);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < AHEAD; i++)
+    if (i < W.n) issue(i, smem + i * B::BUF);
+
+  const int wq0 = x0 + wave * 16 * NP;
+  u32x4 qf[NP][KC], dof[NP][KC];
+  float nlse[NP], del[NP];
+  int hi[NP], lo[NP];
+  const int64_t row0 = (int64_t)bh * a.rows;
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    const int r = wq0 + 16 * p + n;
+    const bool on = r < a.rows;
+    const int rc = on ? r : 0, pos = a.off + band_row(a, rc).tok;
+    hi[p] = on ? pos : -1;
+    lo[p] = pos - a.W;
+    band_load_own<KC>(qf[p], band_row_ptr(qb, a.qs, a, rc), on, a.dk_, g);
+    band_load_own<KC>(dof[p], band_row_ptr(dob, a.dos, a, rc), on, a.dv_, g);
+    nlse[p] = on ? -a.lse[row0 + r] : 0.f;
+    u32x4 of[KC];
+    band_load_own<KC>(of, band_row_ptr(ob, a.os, a, rc), on, a.dv_, g);
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+      float fo[8], fd[8];
+      unpack8<TIO>(of[c], fo);
+      unpack8<TIO>(dof[p][c], fd);
+#pragma unroll
+      for (int j = 0; j < 8; j++) sum += fo[j] * fd[j];
+    }
+    del[p] = wave_sum4(sum);
+    if (g == 0 && on) store_stream4(a.delta + row0 + r, del[p]);
+  }
+  const int wl = dlt_imin(wq0 + 16 * NP, a.rows) - 1;
+  const int pa = wl >= wq0 ? a.off + band_row(a, wq0).tok : 0, pb = wl >= wq0 ? a.off + band_row(a, wl).tok : -1;
+
+  f32x4 acc[NP][KB];
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int d = 0; d < KB; d++) acc[p][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float scale = a.scale_log2;
+  FlashDLane<D> L;
+  flashd_lane_init(L, n, g);
+
+  swa2_wait_copies();
+  pin_loaded(qf);
+  pin_loaded(dof);
+#pragma unroll
+  for (int p = 0; p < NP; p++) { pin_loaded(nlse[p]); pin_loaded(del[p]); }
+  // the dP products start from -delta: the matrix pipe delivers dP - delta
+  f32x4 dinit[NP];
+#pragma unroll
+  for (int p = 0; p < NP; p++) dinit[p] = f32x4{-del[p], -del[p], -del[p], -del[p]};
+  __syncthreads();
+
+  auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    Swa2Lds sK = cur, sV = cur + B::REG;
+    constexpr int N1H = 2 * KC, N1 = 2 * N1H, NB = N1 + KB, NT = NKB * NB;
+    u32x4 ring[2];
+    auto rd = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
+      constexpr int kb = k / NB, j = k % NB;
+      if constexpr (j < N1) {
+        constexpr int mb = j / N1H, r = j % N1H, T0 = 32 * kb + 16 * mb;
+        if constexpr (r < KC) ring[k % 2] = swa2_lds16(sK + T0 * FlashDRow<D>::ROW + L.a[r]);
+        else ring[k % 2] = swa2_lds16(sV + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
+      } else {
+        ring[k % 2] = flashd_read_tr<D, 32 * kb>(sK, L, j - N1);
+      }
+    };
+    rd(std::integral_constant<int, 0>{});
+    swa2_for<0, NKB>([&](auto kbc) __attribute__((always_inline)) {
+      constexpr int kb = decltype(kbc)::value;
+      float ds[NP][8];
+      f32x4 sv[NP], dp[NP];
+      u32x4 dsb[NP];
+      swa2_for<0, NB>([&](auto jc) __attribute__((always_inline)) {
+        constexpr int j = decltype(jc)::value, k = kb * NB + j;
+        if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+        __builtin_amdgcn_sched_barrier(0);
+        const u32x4 op = ring[k % 2];
+        if constexpr (j < N1) {
+          constexpr int mb = j / N1H, r = j % N1H;
+#pragma unroll
+          for (int p = 0; p < NP; p++) {
+            if constexpr (r < KC) sv[p] = Mma<TIO>::mfma(op, qf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[p]);
+            else dp[p] = Mma<TIO>::mfma(op, dof[p][r - KC], r == KC ? dinit[p] : dp[p]);
+          }
+          if constexpr (r == N1H - 1) {
+#pragma unroll
+            for (int p = 0; p < NP; p++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                float v = fast_exp2(fmaf(sv[p][i], scale, nlse[p])) * dp[p][i];
+                if constexpr (MASK) {
+                  const int j_ = x + 32 * kb + 16 * mb + 4 * g + i;
+                  v = j_ <= hi[p] && (j_ > lo[p] || j_ < a.S) ? v : 0.f;
+                }
+                ds[p][4 * mb + i] = v;
+              }
+            if constexpr (mb == 1) {
+#pragma unroll
+              for (int p = 0; p < NP; p++) dsb[p] = pack8<TIO>(ds[p]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < NP; p++) acc[p][j - N1] = Mma<TIO>::mfma(op, dsb[p], acc[p][j - N1]);
+        }
+      });
+    });
+  };
+  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int x = W.x(i), xe = x + CK - 1;
+    if (x > pb || (xe <= pa - a.W && x >= a.S)) return;
+    if (xe <= pa && (x > pb - a.W || xe < a.S)) consume(x, (Swa2Lds)buf, std::false_type{});
+    else consume(x, (Swa2Lds)buf, std::true_type{});
+  };
+  int bi = 0, i = 0;
+  auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
+#pragma unroll 1
+  for (; i + AHEAD < W.n; i++) {
+    issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi));
+    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    __syncthreads();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  }
+#pragma unroll 1
+  for (; i < W.n; i++) {
+    chunk(i, buf_of(bi));
+    swa2_wait_copies();
+    __syncthreads();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  }
+  __syncthreads();
+  float mul[NP];
+  unsigned odd[NP];
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    mul[p] = a.sm_scale;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < a.rows && band_odd_row(acc, p));
+    odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
+  }
+  TIO* dqb = reinterpret_cast<TIO*>(a.dq) + b * a.dqs[0] + (int64_t)h * a.G * a.dqs[1];
+  constexpr int PT = D * 2 + 16;
+  band_store_rows<D, NP, TIO>(smem, acc, mul, NW, a.dk_, wave, n, g, tid,
+                              [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(dqb, a.dqs, a, x0 + row) : nullptr; },
+                              [&]() {
+                                // rows with an infinite or NaN sum once more, over the keys that they see alone (band_common.h)
+#pragma unroll 1
+                                for (int p = 0; p < NP; p++)
+                                  for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+                                    const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w, pos = a.off + band_row(a, r).tok;
+                                    const TIO *q = band_row_ptr(qb, a.qs, a, r), *d_o = band_row_ptr(dob, a.dos, a, r);
+                                    const float lse = a.lse[row0 + r], delta = band_dot(band_row_ptr(ob, a.os, a, r), d_o, a.dv_);
+                                    float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+                                    for (int c = 0; c < W.n; c++)
+#pragma unroll 1
+                                      for (int x = W.x(c); x < W.x(c) + CK; x += 64) {
+                                        const int j = x + lane;
+                                        const bool sees = j < a.Lk && band_sees(pos, j, a.W, a.S);
+                                        uint64_t left = __builtin_amdgcn_ballot_w64(sees);
+                                        float ds = 0.f;
+                                        if (sees)
+                                          ds = fast_exp2(band_dot(q, kh + j * a.ks[2], a.dk_) * scale - lse) * (band_dot(d_o, vh + j * a.vs[2], a.dv_) - delta);
+                                        for (; left != 0; left &= left - 1) {
+                                          const int u = __builtin_ctzll(left);
+                                          band_axpy(sum, band_lane(ds, u), kh + (x + u) * a.ks[2], a.dk_, lane);
+                                        }
+                                      }
+                                    if (2 * lane < D)
+                                      *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * a.sm_scale, sum[1] * a.sm_scale);
+                                  }
+                              });
+}
+
+// ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
+template <typename TIO, int D, int NP, int CK, int NW, int PAD>
+__global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs a) {
+  typedef BandBuf<D, CK> B;
+  extern __shared__ __align__(16) char smem[];
+  constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NG = CK / NW / 16;
+  static_assert(NG >= 1 && NG * NW * 16 == CK && CK == 64, "whole groups of 16 rows per wave; one copy of scalars a chunk");
+  constexpr int PER_CHUNK = 2 * NG * BandStageRows<D>::NI;   // waves 0 and 1: one more
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const int lin = xcd_remap(blockIdx.x, gridDim.x);
+  int bh, r_, unit;
+  flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, false, bh, r_, unit);
+  const int blk = unit / a.shares, share = unit - blk * a.shares;
+  const int x0 = blk * OWN, xe = dlt_imin(x0 + OWN, a.Lk);
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const char* qb = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1]);
+  const char* dob = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1]);
+  const TIO* kh = reinterpret_cast<const TIO*>(a.k) + b * a.ks[0] + h * a.ks[1];
+  const TIO* vh = reinterpret_cast<const TIO*>(a.v) + b * a.vs[0] + h * a.vs[1];
+  const int64_t row0 = (int64_t)bh * a.rows;
+
+  // rows [r_beg, r_end) see some own key; key j is seen by rows [rlo(j), rhi(j))
+  auto rlo_of = [&](int j) { return (int)dlt_imin64((int64_t)dlt_imax(j - a.off, 0) * a.G, a.rows); };
+  auto rhi_of = [&](int j) { return j < a.S ? a.rows : (int)dlt_imin64((int64_t)dlt_imax(j - a.off + a.W, 0) * a.G, a.rows); };
+  const int r_beg = rlo_of(x0), r_end = x0 < a.S ? a.rows : rhi_of(xe - 1);
+  int nch = r_end > r_beg ? (r_end - r_beg + CK - 1) / CK : 0;
+  const int per = (nch + a.shares - 1) / a.shares;
+  const int i_beg = dlt_imin(share * per, nch), i_end = dlt_imin(i_beg + per, nch);
+
+  BandStageRows<D> stq, std_;
+  stq.init(a, lane, a.dk_, a.qs);
+  std_.init(a, lane, a.dv_, a.dos);
+  if constexpr (PAD) {
+#pragma unroll
+    for (int i = 0; i < NBUF; i++) {
+      flashd_zero_pads<D>(smem + i * B::BUF_KV, CK, a.dk_ >> 3, tid, 64 * NW);
+      flashd_zero_pads<D>(smem + i * B::BUF_KV + B::REG, CK, a.dv_ >> 3, tid, 64 * NW);
+    }
+  }
+  const float* scal = (wave == 0 ? a.lse : a.delta) + row0;
+  auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int r0 = r_beg + i * CK;
+#pragma unroll
+    for (int u = 0; u < NG; u++) {
+      const int at = wave * 16 * NG + 16 * u;
+      stq.template issue<PAD>(a, qb, a.qs, r0 + at, a.rows - 1, buf + at * 2 * D);
+      std_.template issue<PAD>(a, dob, a.dos, r0 + at, a.rows - 1, buf + B::REG + at * 2 * D);
+    }
+    if (wave < 2) dlt_copy4_to_lds(reinterpret_cast<const char*>(scal + r0), (uint32_t)dlt_imin(lane, a.rows - 1 - r0) * 4u, buf + 2 * B::REG + wave * (CK * 4));
+  };
+#pragma unroll 1
+  for (int i = 0; i < AHEAD; i++)
+    if (i_beg + i < i_end) issue(i_beg + i, smem + i * B::BUF_KV);
+
+  const int wk0 = x0 + wave * 16 * NP;
+  u32x4 kf[NP][KC], vf[NP][KC];
+  int rlo[NP], rhi[NP];
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    const int xk = wk0 + 16 * p + n;
+    const bool on = xk < a.Lk;
+    rlo[p] = on ? rlo_of(xk) : a.rows;
+    rhi[p] = on ? rhi_of(xk) : 0;
+    band_load_own<KC>(kf[p], kh + (on ? xk : 0) * a.ks[2], on, a.dk_, g);
+    band_load_own<KC>(vf[p], vh + (on ? xk : 0) * a.vs[2], on, a.dv_, g);
+  }
+  // rows that see some key of the wave: [wlo, whi); rows that see all of them: [flo, fhi)
+  const int wk1 = dlt_imin(wk0 + 16 * NP, xe) - 1;
+  const bool wave_on = wk1 >= wk0;
+  const int wlo = wave_on ? rlo_of(wk0) : 0, whi = !wave_on ? 0 : wk0 < a.S ? a.rows : rhi_of(wk1);
+  const int flo = wave_on ? rlo_of(wk1) : 0, fhi = !wave_on ? 0 : wk0 >= a.S ? rhi_of(wk0) : wk1 < a.S ? a.rows : rhi_of(a.S);
+
+  f32x4 dk_acc[NP][KB], dv_acc[NP][KB];
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int d = 0; d < KB; d++) dk_acc[p][d] = dv_acc[p][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const float scale = a.scale_log2;
+  FlashDLane<D> L;
+  flashd_lane_init(L, n, g);
+
+  swa2_wait_copies();
+  pin_loaded(kf);
+  pin_loaded(vf);
+  // the own values are negated and the dP products start from the rows' delta: the matrix pipe delivers -(dP - delta)
+#pragma unroll
+  for (int p = 0; p < NP; p++)
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+      vf[p][c].x ^= 0x80008000u; vf[p][c].y ^= 0x80008000u; vf[p][c].z ^= 0x80008000u; vf[p][c].w ^= 0x80008000u;
+    }
+  __syncthreads();
+
+  auto consume = [&](const int q0, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    Swa2Lds sQ = cur, sDO = cur + B::REG;
+    Swa2Lds sLse = cur + 2 * B::REG + 16 * g, sDel = sLse + CK * 4;
+    // the first products (S, dP) of every 16-row half, then the second ones (dV, dK) block by block; the element-wise work of a half is
+    // issued in pieces behind the matrix instructions of the following segment
+    constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NP2 = 2 * KB, NT = N1 + NQB * NP2;
+    constexpr int NU = 2 * NP;
+    static_assert(NP2 >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
+    u32x4 ring[2];
+    auto rd = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
+      if constexpr (k < N1) {
+        constexpr int hh = k / N1H, r = k % N1H, T0 = 16 * hh;
+        if constexpr (r < KC) ring[k % 2] = swa2_lds16(sQ + T0 * FlashDRow<D>::ROW + L.a[r]);
+        else ring[k % 2] = swa2_lds16(sDO + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
+      } else {
+        constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
+        if constexpr (d < KB) ring[k % 2] = flashd_read_tr<D, 32 * qb_>(sDO, L, d);
+        else ring[k % 2] = flashd_read_tr<D, 32 * qb_>(sQ, L, d - KB);
+      }
+    };
+    rd(std::integral_constant<int, 0>{});
+    f32x4 sv[2][NP], dp[2][NP], lq[2], dl[2];   // by the parity of the half
+    dl[0] = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
+    u32x4 pb[NQB][NP], dsb[NQB][NP];
+    auto ew = [&](auto hhc, auto uc) __attribute__((always_inline)) {
+      constexpr int hh = decltype(hhc)::value, u = decltype(uc)::value;
+      constexpr int qb_ = hh / 2, mb = hh % 2, p = u / 2, i0_ = 2 * (u % 2);
+      float pr[2], ds[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const int i = i0_ + t;
+        float pv = fast_exp2(fmaf(sv[hh & 1][p][i], scale, -lq[hh & 1][i]));
+        float dv = -pv * dp[hh & 1][p][i];
+        if constexpr (MASK) {
+          const int r = q0 + 16 * hh + 4 * g + i;
+          const bool sees = r >= rlo[p] && r < rhi[p];
+          pv = sees ? pv : 0.f;
+          dv = sees ? dv : 0.f;
+        }
+        pr[t] = pv;
+        ds[t] = dv;
+      }
+      const unsigned pw = pack2<TIO>(pr[0], pr[1]), dw = pack2<TIO>(ds[0], ds[1]);
+      if constexpr (mb == 0 && i0_ == 0) { pb[qb_][p].x = pw; dsb[qb_][p].x = dw; }
+      if constexpr (mb == 0 && i0_ == 2) { pb[qb_][p].y = pw; dsb[qb_][p].y = dw; }
+      if constexpr (mb == 1 && i0_ == 0) { pb[qb_][p].z = pw; dsb[qb_][p].z = dw; }
+      if constexpr (mb == 1 && i0_ == 2) { pb[qb_][p].w = pw; dsb[qb_][p].w = dw; }
+    };
+    swa2_for<0, NT>([&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
+      if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+      if constexpr (k < N1 && k % N1H == 0) {
+        constexpr int hh = k / N1H;
+        lq[hh & 1] = __builtin_bit_cast(f32x4, swa2_lds16(sLse + 16 * hh * 4));
+      }
+      if constexpr (k < N1 && k % N1H == KC && k / N1H + 1 < NH) {
+        constexpr int hn = k / N1H + 1;
+        dl[hn & 1] = __builtin_bit_cast(f32x4, swa2_lds16(sDel + 16 * hn * 4));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x4 op = ring[k % 2];
+      if constexpr (k < N1) {
+        constexpr int hh = k / N1H, r = k % N1H;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          if constexpr (r < KC) sv[hh & 1][p] = Mma<TIO>::mfma(op, kf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[hh & 1][p]);
+          else dp[hh & 1][p] = Mma<TIO>::mfma(op, vf[p][r - KC], r == KC ? dl[hh & 1] : dp[hh & 1][p]);
+        }
+        if constexpr (hh >= 1 && r < NU) {
+          ew(std::integral_constant<int, hh - 1>{}, std::integral_constant<int, r>{});
+          SWA2_MIX(NP, 12 / NP)
+        }
+      } else {
+        constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          if constexpr (d < KB) dv_acc[p][d] = Mma<TIO>::mfma(op, pb[qb_][p], dv_acc[p][d]);
+          else dk_acc[p][d - KB] = Mma<TIO>::mfma(op, dsb[qb_][p], dk_acc[p][d - KB]);
+        }
+        if constexpr (qb_ == 0 && d < NU) {
+          ew(std::integral_constant<int, NH - 1>{}, std::integral_constant<int, d>{});
+          SWA2_MIX(NP, 12 / NP)
+        }
+      }
+    });
+  };
+  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int q0 = r_beg + i * CK;
+    if (q0 >= whi || q0 + CK <= wlo) return;
+    if (q0 >= flo && q0 + CK <= fhi) consume(q0, (Swa2Lds)buf, std::false_type{});
+    else consume(q0, (Swa2Lds)buf, std::true_type{});
+  };
+  int bi = 0, i = i_beg;
+  auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF_KV; };
+#pragma unroll 1
+  for (; i + AHEAD < i_end; i++) {
+    issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi));
+    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    __syncthreads();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  }
+#pragma unroll 1
+  for (; i < i_end; i++) {
+    chunk(i, buf_of(bi));
+    swa2_wait_copies();
+    __syncthreads();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  }
+  __syncthreads();
+
+  // ---- epilogue
+  unsigned odd[NP];
+  float mulk[NP], mulv[NP];
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    mulk[p] = a.sm_scale;
+    mulv[p] = 1.f;
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(wk0 + 16 * p + n < a.Lk && (band_odd_row(dk_acc, p) || band_odd_row(dv_acc, p)));
+    odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
+  }
+  // one own key once more over the rows of chunks [i_beg, i_end) that see it: two dims of dK (without sm_scale) and dV
+  auto exact = [&](int xk, float (&sk)[2], float (&sv)[2]) __attribute__((always_inline)) {
+    const TIO *k = kh + xk * a.ks[2], *v = vh + xk * a.vs[2];
+    const int lo = dlt_imax(rlo_of(xk), r_beg + i_beg * CK), hi = dlt_imin(rhi_of(xk), r_beg + i_end * CK);
+    sk[0] = sk[1] = sv[0] = sv[1] = 0.f;
+#pragma unroll 1
+    for (int r0 = lo; r0 < hi; r0 += 64) {
+      const int r = r0 + lane;
+      float p = 0.f, ds = 0.f;
+      if (r < hi) {
+        const TIO *q = band_row_ptr(reinterpret_cast<const TIO*>(qb), a.qs, a, r), *d_o = band_row_ptr(reinterpret_cast<const TIO*>(dob), a.dos, a, r);
+        p = fast_exp2(band_dot(q, k, a.dk_) * scale - a.lse[row0 + r]);
+        ds = p * (band_dot(d_o, v, a.dv_) - a.delta[row0 + r]);
+      }
+      for (int u = 0; u < 64 && r0 + u < hi; u++) {
+        band_axpy(sv, band_lane(p, u), band_row_ptr(reinterpret_cast<const TIO*>(dob), a.dos, a, r0 + u), a.dv_, lane);
+        band_axpy(sk, band_lane(ds, u), band_row_ptr(reinterpret_cast<const TIO*>(qb), a.qs, a, r0 + u), a.dk_, lane);
+      }
+    }
+  };
+  if (a.shares > 1) {
+    float* pk = a.part + ((int64_t)bh * a.shares + share) * a.Lk * a.dk_;
+    float* pv = a.part + (int64_t)a.B * a.Hkv * a.shares * a.Lk * a.dk_ + ((int64_t)bh * a.shares + share) * a.Lk * a.dv_;
+    flash_share_put<NP>(pk, dk_acc, a.dk_, wk0 + n, a.Lk, g);
+    flash_share_put<NP>(pv, dv_acc, a.dv_, wk0 + n, a.Lk, g);
+#pragma unroll 1
+    for (int p = 0; p < NP; p++)
+      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+        const int xk = wk0 + 16 * p + __builtin_ctz(todo);
+        float sk[2], sv[2];
+        exact(xk, sk, sv);
+        __threadfence();   // behind the wave's own stores of the row
+        if (2 * lane < a.dk_) *reinterpret_cast<float2*>(pk + (int64_t)xk * a.dk_ + 2 * lane) = float2{sk[0], sk[1]};
+        if (2 * lane < a.dv_) *reinterpret_cast<float2*>(pv + (int64_t)xk * a.dv_ + 2 * lane) = float2{sv[0], sv[1]};
+      }
+    return;
+  }
+  constexpr int PT = D * 2 + 16;
+  auto again = [&](bool keys) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int p = 0; p < NP; p++)
+      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+        const int w = 16 * p + __builtin_ctz(todo);
+        float sk[2], sv[2];
+        exact(wk0 + w, sk, sv);
+        const float f = keys ? a.sm_scale : 1.f;
+        if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>((keys ? sk[0] : sv[0]) * f, (keys ? sk[1] : sv[1]) * f);
+      }
+  };
+  TIO* dkb = reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1];
+  TIO* dvb = reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1];
+  band_store_rows<D, NP, TIO>(smem, dk_acc, mulk, NW, a.dk_, wave, n, g, tid,
+                              [&](int row) -> TIO* { return x0 + row < a.Lk ? dkb + (x0 + row) * a.dks[2] : nullptr; }, [&]() { again(true); });
+  band_store_rows<D, NP, TIO>(smem, dv_acc, mulv, NW, a.dv_, wave, n, g, tid,
+                              [&](int row) -> TIO* { return x0 + row < a.Lk ? dvb + (x0 + row) * a.dvs[2] : nullptr; }, [&]() { again(false); });
+}

@@ -1,0 +1,233 @@
+// Attention over a 1D window with first tokens that stay visible (sinks), heads of q in groups that share one head of k and v:
+// what the forward, backward and paged kernels share.
+//
+// Query token i of a sequence stands at position p = off + i (off = Lk - Lq, paged: length - new tokens) and sees key j iff
+//   j <= p  and  (p - j < W  or  j < S).
+// The G query heads of a group read the same keys, so they are rows of one tile: row r = i G + (head in the group).  A tile of 128 rows
+// then spans 128 / G tokens: the keys that only some of its rows see shrink with G, and a key is fetched once for the whole group.
+// lse2 and delta are contiguous [B, Hkv, Lq G] in that row order.
+#pragma once
+#include "flash_dma_kernel.hpp"
+
+struct BandPages {          // keys and values in pages (paged calls); strides in elements
+  const int32_t* table;     // [B, cols] page numbers
+  const int32_t* seq;       // [B] tokens of a sequence, the new ones included
+  const int32_t* n_new;     // [B] new tokens, or NULL: T of every sequence
+  int64_t ts;               // row stride of the table
+  int32_t cols, n_pages;
+  int32_t p16;              // 16-token groups of a page
+  uint32_t m16, s16;        // division by p16
+};
+
+struct BandArgs {
+  const void *q, *k, *v, *o, *d_o;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta, *part;
+  int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // batch (pages: page), head, token; head dims are contiguous
+  int32_t B, Hkv, G, Lq, Lk, dk_, dv_;
+  uint32_t mG, sG;          // division by G
+  int32_t W, S, off, rows;  // W <= Lk; rows = Lq G
+  int32_t nblk, group;      // own blocks of a (batch, kv head); heads interleaved at launch (flash_block_causal)
+  int32_t shares;           // workgroups that share the keys of an own block (forward)
+  int32_t q16;              // 16 is a multiple of G: 16 rows are whole tokens
+  float scale_log2, sm_scale;
+  BandPages pg;
+};
+
+DLT_HD int64_t dlt_imin64(int64_t a, int64_t b) { return a < b ? a : b; }
+
+// Of the rows of a tile: token and head in the group
+struct BandRow { int tok, head; };
+DLT_DEV BandRow band_row(const BandArgs& a, int r) {
+  const int t = (int)dlt_fastdiv((uint32_t)r, a.mG, a.sG);
+  return BandRow{t, r - t * a.G};
+}
+template <typename T>
+DLT_DEV T* band_row_ptr(T* base, const int64_t (&st)[3], const BandArgs& a, int r) {
+  const BandRow w = band_row(a, r);
+  return base + (w.tok * st[2] + w.head * st[1]);
+}
+
+// Chunks of CK keys that the rows of a block at positions [first, last] see: those with sinks, then those of the window.
+template <int CK>
+struct BandWalk {
+  int ns, c0, n;
+  DLT_DEV void init(int first, int last, int W, int S) {
+    ns = c0 = n = 0;
+    if (last < 0) return;
+    first = dlt_imax(first, 0);
+    c0 = first >= W ? (first - W + 1) / CK : 0;
+    ns = dlt_imin((dlt_imin(S, last + 1) + CK - 1) / CK, c0);
+    n = ns + last / CK + 1 - c0;
+  }
+  DLT_DEV int x(int i) const { return CK * (i < ns ? i : c0 + i - ns); }
+};
+
+// Own rows as B operands: lane (n, g) holds head dims 32 c + 8 g .. + 7 of row n; r < 0: no row
+template <int KC, typename TIO>
+DLT_DEV void band_load_own(u32x4 (&f)[KC], const TIO* row, bool on, int dims, int g) {
+#pragma unroll
+  for (int c = 0; c < KC; c++) {
+    f[c] = u32x4{0u, 0u, 0u, 0u};
+    if (on && 8 * (4 * c + g) < dims) f[c] = *reinterpret_cast<const u32x4*>(row + 8 * (4 * c + g));
+  }
+}
+
+// Copies of keys or values HBM -> LDS, 16 tokens at a time (one wave): token t of the group, piece c of its row lies at piece
+// c ^ swz(t) (FlashDRow).  The place of the group is wave-uniform, a lane's offset inside it is kept in registers.
+template <int D>
+struct BandStage {
+  typedef FlashDRow<D> R;
+  static constexpr int NI = 16 / R::TPI;                    // copy instructions per 16 tokens
+  static constexpr int NOFF = R::TPI >= 8 ? 1 : 8 / R::TPI; // instructions NOFF apart: 8 tokens apart, same swizzle
+  uint32_t off[NOFF];
+  int t0, lp, npieces;
+  uint32_t sn2;
+  DLT_DEV uint32_t piece(int i) const { return (uint32_t)(lp ^ R::swz(t0 + R::TPI * i)); }
+  DLT_DEV void init(int lane, int dims, int64_t sn) {
+    t0 = lane / R::PIECES;
+    lp = lane % R::PIECES;
+    npieces = dims >> 3;
+    sn2 = (uint32_t)sn * 2u;
+#pragma unroll
+    for (int i = 0; i < NOFF; i++) off[i] = (uint32_t)(t0 + R::TPI * i) * sn2 + 16u * piece(i);
+  }
+  template <int PAD>
+  DLT_DEV void issue(const char* base, char* dst) const {   // all 16 tokens are there
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+      if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(base + (uint32_t)(i / NOFF * NOFF * R::TPI) * sn2, off[i % NOFF], dst + R::TPI * i * R::ROW);
+  }
+  template <int PAD>
+  DLT_DEV void issue_clamped(const char* base, int last, char* dst) const {   // tokens behind `last` repeat it
+#pragma unroll 1
+    for (int i = 0; i < NI; i++)
+      if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(base, (uint32_t)dlt_imin(t0 + R::TPI * i, last) * sn2 + 16u * piece(i), dst + R::TPI * i * R::ROW);
+  }
+};
+
+// Rows r0 .. r0 + 15 of a query-side tensor -> LDS (dK / dV kernel).  `base`: of the (batch, kv head).
+template <int D>
+struct BandStageRows {
+  typedef FlashDRow<D> R;
+  static constexpr int NI = 16 / R::TPI;
+  uint32_t off[NI];   // q16: of the lane's row inside a group of 16 that starts with a token
+  int t0, lp, npieces;
+  DLT_DEV uint32_t piece(int i) const { return (uint32_t)(lp ^ R::swz(t0 + R::TPI * i)); }
+  DLT_DEV void init(const BandArgs& a, int lane, int dims, const int64_t (&st)[3]) {
+    t0 = lane / R::PIECES;
+    lp = lane % R::PIECES;
+    npieces = dims >> 3;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const BandRow w = band_row(a, t0 + R::TPI * i);
+      off[i] = (uint32_t)(w.tok * (int)st[2] + w.head * (int)st[1]) * 2u + 16u * piece(i);
+    }
+  }
+  // rows behind `last` repeat it
+  template <int PAD>
+  DLT_DEV void issue(const BandArgs& a, const char* base, const int64_t (&st)[3], int r0, int last, char* dst) const {
+    const int f0 = dlt_imin(r0, last);
+    const int tk = (int)dlt_fastdiv((uint32_t)f0, a.mG, a.sG);
+    const char* b = base + (int64_t)tk * st[2] * 2;   // wave-uniform
+    if (a.q16 != 0 && r0 + 15 <= last) {
+#pragma unroll
+      for (int i = 0; i < NI; i++)
+        if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(b, off[i], dst + R::TPI * i * R::ROW);
+    } else {
+      keep_branch();
+#pragma unroll 1
+      for (int i = 0; i < NI; i++) {
+        const BandRow w = band_row(a, dlt_imin(r0 + t0 + R::TPI * i, last));
+        const uint32_t o = (uint32_t)((w.tok - tk) * (int)st[2] + w.head * (int)st[1]) * 2u + 16u * piece(i);
+        if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(b, o, dst + R::TPI * i * R::ROW);
+      }
+    }
+  }
+};
+
+// bytes of a chunk of CK tokens of both streamed tensors, and of the scalars of CK rows (dK / dV kernel)
+template <int D, int CK>
+struct BandBuf {
+  static constexpr int REG = CK * 2 * D;
+  static constexpr int BUF = 2 * REG;
+  static constexpr int BUF_KV = 2 * REG + 2 * CK * 4;
+};
+
+// Accumulators in C layout (lane (n, g): dims 16 d + 4 g .. + 3 of own row n, times mul[p]) -> LDS tile of 16-bit values -> rows.
+// `ptr(row)`: the row's place or NULL.  The tile takes the chunk buffers' LDS.
+// `again()`: the wave writes rows of its own part of the tile once more (see below).
+template <int D, int NP, typename TIO, int NA, typename PtrFn, typename AgainFn>
+DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int dims, int wave, int n, int g, int tid, PtrFn ptr,
+                             AgainFn again) {
+  constexpr int PT = D * 2 + 16;
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    char* row = sT + (wave * 16 * NP + 16 * p + n) * PT + 8 * g;
+#pragma unroll
+    for (int d = 0; d < NA; d++) {
+      u32x2 w;
+      w.x = pack2<TIO>(acc[p][d][0] * mul[p], acc[p][d][1] * mul[p]);
+      w.y = pack2<TIO>(acc[p][d][2] * mul[p], acc[p][d][3] * mul[p]);
+      *reinterpret_cast<u32x2*>(row + 32 * d) = w;
+    }
+  }
+  again();
+  __syncthreads();
+  int tw = tid;   // opaque copy: keeps the addresses out of the registers that live across the chunk loop
+  asm volatile("" : "+v"(tw));
+  constexpr int CH = D / 8;
+  const int c = tw % CH;
+  if (8 * c < dims)
+    for (int row = tw / CH; row < 16 * NP * nw; row += 64 * nw / CH) {
+      TIO* p = ptr(row);
+      if (p == nullptr) continue;
+      const u32x4 v = lds_read16(sT + row * PT + 16 * c);
+      store_stream16(p + 8 * c, v);
+    }
+  __syncthreads();
+}
+
+DLT_DEV bool band_odd(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }   // infinite or NaN
+template <int NP, int NA>
+DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {
+  bool odd = false;
+#pragma unroll
+  for (int d = 0; d < NA; d++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) odd = odd || band_odd(acc[p][d][i]);
+  return odd;
+}
+
+// ---- rows whose sums came out infinite or NaN ------------------------------------------------------------------------------------
+// The matrix products of a chunk at the edge of a window multiply hidden pairs by 0, and 0 times an infinity or a NaN is NaN: a hidden key
+// (in the backward pass a hidden query) with such values would reach rows that do not see it.  Every kernel therefore looks at its sums once,
+// at the end, and takes rows with such a value again, one wave a row, over the pairs that see each other alone.  Ordinary data never
+// comes here.
+template <typename TIO>
+DLT_DEV float band_dot(const TIO* x, const TIO* y, int dims) {
+  float s = 0.f;
+  for (int d = 0; d < dims; d += 8) {
+    float fx[8], fy[8];
+    unpack8<TIO>(*reinterpret_cast<const u32x4*>(x + d), fx);
+    unpack8<TIO>(*reinterpret_cast<const u32x4*>(y + d), fy);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s = fmaf(fx[j], fy[j], s);
+  }
+  return s;
+}
+DLT_DEV float band_lane(float v, int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); }
+DLT_DEV float band_wave_max(float v) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+// acc[2] += w * (dims 2 lane, 2 lane + 1 of x)
+template <typename TIO>
+DLT_DEV void band_axpy(float (&acc)[2], float w, const TIO* x, int dims, int lane) {
+  if (2 * lane < dims) {
+    acc[0] = fmaf(w, (float)x[2 * lane], acc[0]);
+    acc[1] = fmaf(w, (float)x[2 * lane + 1], acc[1]);
+  }
+}
+DLT_DEV bool band_sees(int p, int j, int W, int S) { return j <= p && (p - j < W || j < S); }

@@ -1,0 +1,3 @@
+#define DLT_BAND_D 128
+#define DLT_BAND_PART 0
+#include "band_inst.h"

@@ -1,0 +1,358 @@
+// Forward pass of attention over a 1D window with sinks and grouped heads (band_common.h), keys and values dense or in pages.
+//
+// A workgroup of NW waves owns 16 NP NW rows (query token, head) of one group; K and V stream through LDS in chunks of CK keys, copied
+// asynchronously, 16 tokens a wave (in pages: one page lookup).  Per chunk: S^T = K Q^T, one update of the running maximum and sum, O^T +=
+// V^T P^T.  Chunks that every row of a wave sees whole run without a mask, chunks that no row sees are left out.
+// P is rounded to 16 bits for the second product, as its operand has to be; sums, maxima and outputs stay in 32 bits to the end.
+#pragma once
+#include "band_common.h"
+
+// What one sequence of a call holds
+struct BandSeq {
+  int off, n_q, n_k;   // position of query token 0, query tokens, keys
+};
+template <bool PAGED>
+DLT_DEV BandSeq band_seq(const BandArgs& a, int b) {
+  BandSeq s{a.off, a.Lq, a.Lk};
+  if constexpr (PAGED) {
+    s.n_q = a.pg.n_new != nullptr ? dlt_imax(0, dlt_imin(a.pg.n_new[b], a.Lq)) : a.Lq;
+    s.n_k = dlt_imax(0, dlt_imin(a.pg.seq[b], a.Lk));   // Lk: what the table's row can hold
+    s.off = s.n_k - s.n_q;
+  }
+  return s;
+}
+// Page of the 16 tokens that hold position 16 t16.  A number outside the pool is the caller's mistake: the nearest page is read.
+DLT_DEV int band_page(const BandPages& pg, const int32_t* row, int t16, int& in16) {
+  const int pi = (int)dlt_fastdiv((uint32_t)t16, pg.m16, pg.s16);
+  in16 = t16 - pi * pg.p16;
+  return dlt_imax(0, dlt_imin(row[pi], pg.n_pages - 1));
+}
+// Element offset of key j inside the tensor at the head's base
+template <bool PAGED>
+DLT_DEV int64_t band_key_off(const BandArgs& a, const int32_t* row, const int64_t (&st)[3], int j) {
+  if constexpr (!PAGED) return j * st[2];
+  int in16;
+  const int page = band_page(a.pg, row, j >> 4, in16);
+  return page * st[0] + (in16 * 16 + (j & 15)) * st[2];
+}
+
+// One row again over the keys of chunks [i0, i1) that it sees: maximum (log2 units), sum, two dims of the unnormalised output
+template <typename TIO, bool PAGED, int CK>
+DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, const TIO* vb, const int32_t* pages, const BandWalk<CK>& W, int i0, int i1, int pos,
+                            int n_k, int lane, float& m, float& l, float (&acc)[2]) {
+  m = -INFINITY;
+  l = acc[0] = acc[1] = 0.f;
+#pragma unroll 1
+  for (int i = i0; i < i1; i++)
+#pragma unroll 1
+    for (int x = W.x(i); x < W.x(i) + CK; x += 64) {
+      const int j = x + lane;
+      const bool sees = j < n_k && band_sees(pos, j, a.W, a.S);
+      uint64_t todo = __builtin_amdgcn_ballot_w64(sees);
+      if (todo == 0) continue;
+      const float s = sees ? band_dot(q, kb + band_key_off<PAGED>(a, pages, a.ks, j), a.dk_) * a.scale_log2 : -INFINITY;
+      const float m_new = fmaxf(m, band_wave_max(s));
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - ref);
+      const float p = sees ? fast_exp2(s - ref) : 0.f;
+      m = m_new;
+      l *= alpha; acc[0] *= alpha; acc[1] *= alpha;
+      while (todo != 0) {
+        const int u = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const float w = band_lane(p, u);
+        l += w;
+        band_axpy(acc, w, vb + band_key_off<PAGED>(a, pages, a.vs, x + u), a.dv_, lane);
+      }
+    }
+}
+
+template <typename TIO, int D, int NP, int CK, int NW, bool PAGED, int PAD>
+__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
+  typedef BandBuf<D, CK> B;
+  extern __shared__ __align__(16) char smem[];
+  constexpr int KC = D / 32, VB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NG = CK / NW / 16;                              // groups of 16 tokens that a wave copies
+  static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
+  constexpr int PER_CHUNK = 2 * NG * BandStage<D>::NI;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  const int lin = xcd_remap(blockIdx.x, gridDim.x);
+  int bh, r_, unit;
+  flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, true, bh, r_, unit);
+  const int blk = unit / a.shares, share = unit - blk * a.shares;
+  const int x0 = blk * OWN;
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const BandSeq sq = band_seq<PAGED>(a, b);
+  const int n_rows = sq.n_q * a.G;                              // rows with a query; those behind get zeros
+  const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];
+  const TIO* kh = reinterpret_cast<const TIO*>(a.k) + (PAGED ? 0 : b * a.ks[0]) + h * a.ks[1];
+  const TIO* vh = reinterpret_cast<const TIO*>(a.v) + (PAGED ? 0 : b * a.vs[0]) + h * a.vs[1];
+  const int32_t* pages = PAGED ? a.pg.table + b * a.pg.ts : nullptr;
+
+  // chunks of the block and of this share of it
+  BandWalk<CK> W;
+  const int xl = dlt_imin(x0 + OWN, n_rows) - 1;
+  W.init(sq.off + band_row(a, x0).tok, xl >= x0 ? dlt_imin(sq.off + band_row(a, dlt_imax(xl, 0)).tok, sq.n_k - 1) : -1, a.W, a.S);
+  const int per = (W.n + a.shares - 1) / a.shares;
+  const int i_beg = dlt_imin(share * per, W.n), i_end = dlt_imin(i_beg + per, W.n);
+
+  BandStage<D> stk, stv;
+  stk.init(lane, a.dk_, a.ks[2]);
+  stv.init(lane, a.dv_, a.vs[2]);
+  if constexpr (PAD) {
+#pragma unroll
+    for (int i = 0; i < NBUF; i++) {
+      flashd_zero_pads<D>(smem + i * B::BUF, CK, a.dk_ >> 3, tid, 64 * NW);
+      flashd_zero_pads<D>(smem + i * B::BUF + B::REG, CK, a.dv_ >> 3, tid, 64 * NW);
+    }
+  }
+  auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int x = W.x(i) + wave * 16 * NG;
+#pragma unroll
+    for (int u = 0; u < NG; u++) {
+      char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
+      if constexpr (PAGED) {
+        int in16;
+        const int page = band_page(a.pg, pages, dlt_imin(x / 16 + u, (sq.n_k - 1) >> 4), in16);
+        const int64_t row = 16 * in16;
+        stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (page * a.ks[0] + row * a.ks[2])), dst);
+        stv.template issue<PAD>(reinterpret_cast<const char*>(vh + (page * a.vs[0] + row * a.vs[2])), dst + B::REG);
+      } else {
+        const int t0 = x + 16 * u;
+        if (t0 + 16 <= a.Lk) {
+          stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (int64_t)t0 * a.ks[2]), dst);
+          stv.template issue<PAD>(reinterpret_cast<const char*>(vh + (int64_t)t0 * a.vs[2]), dst + B::REG);
+        } else {
+          keep_branch();
+          const int tc = dlt_imin(t0, a.Lk - 1);
+          stk.template issue_clamped<PAD>(reinterpret_cast<const char*>(kh + (int64_t)tc * a.ks[2]), a.Lk - 1 - tc, dst);
+          stv.template issue_clamped<PAD>(reinterpret_cast<const char*>(vh + (int64_t)tc * a.vs[2]), a.Lk - 1 - tc, dst + B::REG);
+        }
+      }
+    }
+  };
+  // Pages hold anything behind the last key: those value rows, which no row sees, are cleared by the wave that copied them
+  auto settle = [&](int i, char* buf) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+      const int x = W.x(i) + wave * 16 * NG;
+      if (x + 16 * NG > sq.n_k) {
+        keep_branch();
+        char* v = buf + B::REG + wave * 16 * NG * 2 * D;
+        for (int s = lane; s < 16 * NG * D / 8; s += 64)
+          if (x + s / (D / 8) >= sq.n_k) lds_write16(v + 16 * s, u32x4{0u, 0u, 0u, 0u});
+      }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < AHEAD; i++)
+    if (i_beg + i < i_end) issue(i_beg + i, smem + i * B::BUF);
+
+  const int wq0 = x0 + wave * 16 * NP;
+  u32x4 qf[NP][KC];
+  int hi[NP], lo[NP];   // the row sees keys lo < j <= hi, and the sinks
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    const int r = wq0 + 16 * p + n;
+    const bool on = r < n_rows;
+    const int pos = sq.off + band_row(a, on ? r : 0).tok;
+    hi[p] = on ? dlt_imin(pos, sq.n_k - 1) : -1;
+    lo[p] = pos - a.W;
+    band_load_own<KC>(qf[p], band_row_ptr(qb, a.qs, a, on ? r : 0), on, a.dk_, g);
+  }
+  // positions of the wave's first and last row
+  const int wl = dlt_imin(wq0 + 16 * NP, n_rows) - 1;
+  const int pa = wl >= wq0 ? sq.off + band_row(a, wq0).tok : 0, pb = wl >= wq0 ? sq.off + band_row(a, wl).tok : -1;
+
+  float m_run[NP];
+  f32x4 acc[NP][VB], acc_l[NP];
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    m_run[p] = -INFINITY;
+    acc_l[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < VB; d++) acc[p][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float scale = a.scale_log2;
+  const unsigned one2 = pack2<TIO>(1.f, 1.f);
+  const u32x4 ones = n == 0 ? u32x4{one2, one2, one2, one2} : u32x4{0u, 0u, 0u, 0u};
+  FlashDLane<D> L;
+  flashd_lane_init(L, n, g);
+
+  swa2_wait_copies();
+  pin_loaded(qf);
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++)
+    if (i_beg + i < i_end) settle(i_beg + i, smem + i * B::BUF);
+  __syncthreads();
+
+  auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
+    constexpr bool MASK = decltype(mask_tag)::value;
+    Swa2Lds sK = cur, sV = cur + B::REG;
+    constexpr int N1 = NKB * 2 * KC, NT = N1 + NKB * VB;
+    u32x4 ring[2];
+    auto rd = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
+      if constexpr (k < N1) {
+        constexpr int kb = k / (2 * KC), mb = (k / KC) % 2, r = k % KC;
+        ring[k % 2] = swa2_lds16(sK + (32 * kb + 16 * mb) * FlashDRow<D>::ROW + L.a[r]);
+      } else {
+        constexpr int kb = (k - N1) / VB, d = (k - N1) % VB;
+        ring[k % 2] = flashd_read_tr<D, 32 * kb>(sV, L, d);
+      }
+    };
+    rd(std::integral_constant<int, 0>{});
+    float t[NP][NKB][8];
+    u32x4 pb_[NP][NKB];
+    f32x4 s[NP];
+    swa2_for<0, NT>([&](auto kc) __attribute__((always_inline)) {
+      constexpr int k = decltype(kc)::value;
+      if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x4 op = ring[k % 2];
+      if constexpr (k < N1) {
+        constexpr int kb = k / (2 * KC), mb = (k / KC) % 2, r = k % KC;
+#pragma unroll
+        for (int p = 0; p < NP; p++) s[p] = Mma<TIO>::mfma(op, qf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[p]);
+        if constexpr (r == KC - 1) {
+#pragma unroll
+          for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              float v = s[p][i];
+              if constexpr (MASK) {
+                const int j = x + 32 * kb + 16 * mb + 4 * g + i;
+                v = j <= hi[p] && (j > lo[p] || j < a.S) ? v : -INFINITY;
+              }
+              t[p][kb][4 * mb + i] = v;
+            }
+        }
+        if constexpr (k == N1 - 1) {
+#pragma unroll
+          for (int p = 0; p < NP; p++) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int kb2 = 0; kb2 < NKB; kb2++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) mx[i] = fmaxf(fmaxf(mx[i], t[p][kb2][2 * i]), t[p][kb2][2 * i + 1]);
+            const float mloc = wave_max4(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            // the reference maximum moves only when a score exceeds it by more than 2^8 after scaling: P stays below 2^8, its sum in
+            // 32 bits below 2^8 times the keys
+            if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > 8.f)) {
+              keep_branch();
+              const float m_new = fmaxf(m_run[p], mloc);
+              const float alpha = fast_exp2((m_run[p] - m_new) * scale);
+              m_run[p] = m_new;
+              const float al = m_new == -INFINITY ? 1.f : alpha;
+#pragma unroll
+              for (int d = 0; d < VB; d++) acc[p][d] *= al;
+              acc_l[p] *= al;
+            }
+            const float neg_m2 = m_run[p] == -INFINITY ? 0.f : -m_run[p] * scale;
+#pragma unroll
+            for (int kb2 = 0; kb2 < NKB; kb2++) {
+#pragma unroll
+              for (int i = 0; i < 8; i++) t[p][kb2][i] = fast_exp2(fmaf(t[p][kb2][i], scale, neg_m2));
+              pb_[p][kb2] = pack8<TIO>(t[p][kb2]);
+            }
+          }
+        }
+      } else {
+        constexpr int kb = (k - N1) / VB, d = (k - N1) % VB;
+#pragma unroll
+        for (int p = 0; p < NP; p++) acc[p][d] = Mma<TIO>::mfma(op, pb_[p][kb], acc[p][d]);
+        if constexpr (d == VB - 1) {
+#pragma unroll
+          for (int p = 0; p < NP; p++) acc_l[p] = Mma<TIO>::mfma(ones, pb_[p][kb], acc_l[p]);
+        }
+      }
+    });
+  };
+  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
+    const int x = W.x(i), xe = x + CK - 1;
+    if (x > pb || (xe <= pa - a.W && x >= a.S)) return;                       // no row of the wave sees any of it
+    if (xe <= pa && (x > pb - a.W || xe < a.S)) consume(x, (Swa2Lds)buf, std::false_type{});
+    else consume(x, (Swa2Lds)buf, std::true_type{});
+  };
+  int bi = 0;
+  auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
+  int i = i_beg;
+#pragma unroll 1
+  for (; i + AHEAD < i_end; i++) {
+    issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi));
+    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+    settle(i + 1, buf_of(bi));
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (; i < i_end; i++) {
+    chunk(i, buf_of(bi));
+    swa2_wait_copies();
+    bi = bi + 1 == NBUF ? 0 : bi + 1;
+    if (i + 1 < i_end) settle(i + 1, buf_of(bi));
+    __syncthreads();
+  }
+
+  // ---- epilogue
+  float lt[NP], inv[NP];
+  unsigned odd[NP];   // rows of the wave to be taken again
+#pragma unroll
+  for (int p = 0; p < NP; p++) {
+    lt[p] = wave_sum4(acc_l[p][0]);
+    inv[p] = lt[p] > 0.f && wq0 + 16 * p + n < n_rows ? fast_rcp(lt[p]) : 0.f;   // rows that see nothing, and rows behind the last query: zeros
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < n_rows && (band_odd_row(acc, p) || band_odd(lt[p])));
+    odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
+  }
+  const int64_t row0 = (int64_t)bh * a.rows;
+  if (a.shares > 1) {
+    const int64_t at = ((int64_t)bh * a.shares + share) * a.rows;
+    float* part = a.part + at * a.dv_;
+    float* ml = a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_ + 2 * at;
+    flash_share_put<NP>(part, acc, a.dv_, wq0 + n, n_rows, g);
+#pragma unroll
+    for (int p = 0; p < NP; p++)
+      if (g == 0 && wq0 + 16 * p + n < n_rows) *reinterpret_cast<float2*>(ml + 2 * (wq0 + 16 * p + n)) = float2{m_run[p] * scale, lt[p]};
+#pragma unroll 1
+    for (int p = 0; p < NP; p++)
+      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+        const int r = wq0 + 16 * p + __builtin_ctz(todo);
+        float m, l, o2[2];
+        band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
+        __threadfence();   // behind the wave's own stores of the row
+        if (2 * lane < a.dv_) *reinterpret_cast<float2*>(part + (int64_t)r * a.dv_ + 2 * lane) = float2{o2[0], o2[1]};
+        if (lane == 0) *reinterpret_cast<float2*>(ml + 2 * r) = float2{m, l};
+      }
+    return;
+  }
+  if (a.lse != nullptr) {
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      const int r = wq0 + 16 * p + n;
+      if (g == 0 && r < n_rows && (odd[p] >> n & 1) == 0) store_stream4(a.lse + row0 + r, m_run[p] * scale + fast_log2(lt[p]));
+    }
+  }
+  __syncthreads();
+  TIO* ob = reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1];
+  constexpr int PT = D * 2 + 16;
+  band_store_rows<D, NP, TIO>(smem, acc, inv, NW, a.dv_, wave, n, g, tid,
+                              [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(ob, a.os, a, x0 + row) : nullptr; },
+                              [&]() {
+#pragma unroll 1
+                                for (int p = 0; p < NP; p++)
+                                  for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+                                    const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w;
+                                    float m, l, o2[2];
+                                    band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok,
+                                                                   sq.n_k, lane, m, l, o2);
+                                    const float f = l == 0.f ? 0.f : 1.f / l;
+                                    if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(o2[0] * f, o2[1] * f);
+                                    if (lane == 0 && a.lse != nullptr) a.lse[row0 + r] = m + fast_log2(l);
+                                  }
+                              });
+}

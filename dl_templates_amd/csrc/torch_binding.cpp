@@ -28,6 +28,7 @@
 #include <array>
 #include <mutex>
 #include <string>
+#include <vector>
 
 #include "../../include/dlt.h"
 
@@ -157,13 +158,14 @@ Rope make_rope_for(const Tensor& idx, const Tensor& row, const Tensor& col, cons
 }
 
 // ---- the attention operators --------------------------------------------------------------------
-enum class Op { Swa, Image, Flash };
+enum class Op { Swa, Image, Flash, Window };
 
 struct Spec {
   Op op = Op::Swa;
   dlt_swa_shape_t swa{};
   dlt_swa_tile_t tile{};
   dlt_flash_shape_t flash{};
+  dlt_window_shape_t window{};
   bool narrow = false;   // Swa: see small_tiles
 };
 
@@ -208,6 +210,32 @@ Spec flash_spec(const Tensor& q, const Tensor& k, const Tensor& v, bool causal, 
   return s;
 }
 
+Spec window_spec(const Tensor& q, const Tensor& k, const Tensor& v, const int64_t* dims /* window, n_sink */, double scale) {
+  check_assert(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
+  check_assert(q.size(3) == k.size(3), "q and k must have one head dim");
+  check_assert(q.size(0) == k.size(0) && k.sizes().slice(0, 3) == v.sizes().slice(0, 3), "k and v must match q");
+  check_assert(q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type(), "q, k and v must have one dtype");
+  Spec s;
+  s.op = Op::Window;
+  s.window = {(int32_t)q.size(0), (int32_t)q.size(1), (int32_t)k.size(1), (int32_t)q.size(2), (int32_t)k.size(2), (int32_t)q.size(3), (int32_t)v.size(3),
+              (int32_t)dims[0], (int32_t)dims[1], (float)scale, dtype_code(q)};
+  return s;
+}
+// The window and paged kernels read rows in 16-byte pieces; anything else is copied first.
+bool rows16(const Tensor& x) {
+  if (x.dim() != 4 || x.numel() == 0) return true;
+  bool ok = (x.stride(3) == 1 || x.size(3) == 1) && (uintptr_t)x.const_data_ptr() % 16 == 0;
+  for (int i = 0; i < 3; i++) ok = ok && (x.size(i) == 1 || (x.stride(i) % 8 == 0 && x.stride(i) >= 0));
+  return ok;
+}
+Tensor as_rows16(const Tensor& x) { return rows16(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
+// strides of a [.., .., .., D] tensor as the C ABI takes them: those of dims of one element do not matter
+std::array<int64_t, 4> st16(const Tensor& x) {
+  std::array<int64_t, 4> s;
+  for (int i = 0; i < 4; i++) s[i] = i == 3 ? 1 : x.size(i) == 1 || x.numel() == 0 ? 0 : x.stride(i);
+  return s;
+}
+
 // Partial results of a flash pass that splits its other side: from the caching allocator, on the call's stream, for the call alone.
 struct Workspace {
   Tensor t;
@@ -217,6 +245,16 @@ struct Workspace {
 Workspace flash_workspace(const dlt_flash_shape_t& shape, int backward, const Tensor& like) {
   Workspace w;
   check_rc(dlt_flash_workspace(&shape, backward, &w.bytes));
+  if (w.bytes > 0) {
+    w.t = empty({w.bytes / 4}, at::kFloat, like);
+    w.ptr = w.t.mutable_data_ptr();
+  }
+  return w;
+}
+
+Workspace window_workspace(const dlt_window_shape_t& shape, int backward, const Tensor& like) {
+  Workspace w;
+  check_rc(dlt_window_workspace(&shape, backward, &w.bytes));
   if (w.bytes > 0) {
     w.t = empty({w.bytes / 4}, at::kFloat, like);
     w.ptr = w.t.mutable_data_ptr();
@@ -239,6 +277,14 @@ Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tenso
     const Workspace ws = flash_workspace(s.flash, 0, q);
     check_rc(dlt_flash_fwd_ws(q.const_data_ptr(), st(q), k.const_data_ptr(), st(k), v.const_data_ptr(), st(v), f.o.mutable_data_ptr(), st(f.o),
                               (float*)f.lse.mutable_data_ptr(), st(f.lse), &s.flash, ws.ptr, ws.bytes, stream));
+    return f;
+  }
+  if (s.op == Op::Window) {
+    const Workspace ws = window_workspace(s.window, 0, q);
+    f.o = empty({q.size(0), q.size(1), q.size(2), v.size(3)}, dt, q);
+    f.lse = empty({q.size(0), k.size(1), q.size(2), q.size(1) / k.size(1)}, at::kFloat, q);
+    check_rc(dlt_window_fwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), f.o.mutable_data_ptr(),
+                            st16(f.o).data(), (float*)f.lse.mutable_data_ptr(), &s.window, ws.ptr, ws.bytes, stream));
     return f;
   }
   if (s.op == Op::Image) {
@@ -272,8 +318,19 @@ std::array<Tensor, 3> run_backward(const Spec& s, const Tensor& q, const Tensor&
                                    const Tensor& d_o, const Rope* rope, bool rotated) {
   require_gpu(q, k, v, o, lse, d_o);
   c10::DeviceGuard guard(q.device());
-  Tensor dq = grad_like(q), dk = grad_like(k), dv = grad_like(v), delta = grad_like(lse);
   void* stream = stream_of(q);
+  if (s.op == Op::Window) {
+    const Workspace ws = window_workspace(s.window, 1, q);
+    Tensor dq = empty(q.sizes(), q.scalar_type(), q), dk = empty(k.sizes(), k.scalar_type(), k), dv = empty(v.sizes(), v.scalar_type(), v);
+    Tensor delta = empty(lse.sizes(), at::kFloat, lse);
+    const Tensor g = as_rows16(d_o);
+    check_rc(dlt_window_bwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), o.const_data_ptr(),
+                            st16(o).data(), g.const_data_ptr(), st16(g).data(), (const float*)lse.const_data_ptr(), (float*)delta.mutable_data_ptr(),
+                            dq.mutable_data_ptr(), st16(dq).data(), dk.mutable_data_ptr(), st16(dk).data(), dv.mutable_data_ptr(), st16(dv).data(), &s.window,
+                            ws.ptr, ws.bytes, stream));
+    return {dq, dk, dv};
+  }
+  Tensor dq = grad_like(q), dk = grad_like(k), dv = grad_like(v), delta = grad_like(lse);
   auto call = [&](auto fn, auto... shape) {
     check_rc(fn(q.const_data_ptr(), st(q), k.const_data_ptr(), st(k), v.const_data_ptr(), st(v), o.const_data_ptr(), st(o), d_o.const_data_ptr(),
                 st(d_o), (const float*)lse.const_data_ptr(), (float*)delta.mutable_data_ptr(), st(lse), dq.mutable_data_ptr(), st(dq),
@@ -396,13 +453,20 @@ Tensor attention(Op op, const Tensor& q, const Tensor& k, const Tensor& v, const
   {
     at::AutoDispatchBelowADInplaceOrView below;
     const bool narrow = op == Op::Swa && rope_t == nullptr && small_tiles(q, k, v, dims[0], scale);
-    const Pad pad = narrow ? Pad{dk, dv} : op == Op::Flash ? flash_pad(dk, dv, q.scalar_type()) : op == Op::Swa ? swa_pad(dk, dv, q.scalar_type(), dims[0]) : Pad{dk, dv};
+    const Pad pad = narrow ? Pad{dk, dv} : op == Op::Flash || op == Op::Window ? flash_pad(dk, dv, q.scalar_type()) : op == Op::Swa ? swa_pad(dk, dv, q.scalar_type(), dims[0]) : Pad{dk, dv};
     if (C10_UNLIKELY(pad.dk != dk || pad.dv != dv)) {
       pq = pad_last(q, pad.dk);
       pk = pad_last(k, pad.dk);
       pv = pad_last(v, pad.dv);
     }
-    spec = op == Op::Flash ? flash_spec(pq, pk, pv, causal, scale) : op == Op::Image ? image_spec(pq, pk, pv, dims, scale) : swa_spec(pq, pk, pv, dims, scale);
+    if (op == Op::Window) {
+      check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
+      require_gpu(q, k, v);
+      pq = as_rows16(pq);
+      pk = as_rows16(pk);
+      pv = as_rows16(pv);
+    }
+    spec = op == Op::Window ? window_spec(pq, pk, pv, dims, scale) : op == Op::Flash ? flash_spec(pq, pk, pv, causal, scale) : op == Op::Image ? image_spec(pq, pk, pv, dims, scale) : swa_spec(pq, pk, pv, dims, scale);
     spec.narrow = narrow;
     Rope rope;
     if (rope_t != nullptr) {
@@ -511,6 +575,158 @@ void rope_apply(const Tensor& x, const Rows& r, const Tensor& idx, const Tensor&
   }
   torch::autograd::increment_version(x);
   if (grad) torch::autograd::rebase_history(x, node);
+}
+
+// ---- rotation with several axes -------------------------------------------------------------------------
+struct Axes {
+  Tensor pos;                   // int32 [axes, N] or [axes, B, N]
+  std::vector<Tensor> tables;   // fp32 [len, R, 2]
+  int layout = DLT_ROPE_BLOCKS;
+};
+
+// n_tokens, batch: those of the tensors; `d` holds pointers into `t`, whose tables it may replace by dense fp32 copies
+void make_axes(Axes& t, int64_t batch, int64_t n_tokens, const Tensor& like, dlt_rope_axes_t& d) {
+  d = {};
+  require(!t.tables.empty() && t.tables.size() <= DLT_ROPE_AXES_MAX, PyExc_ValueError, "one to four axes are supported");
+  d.n_axes = (int32_t)t.tables.size();
+  d.layout = t.layout;
+  if (t.pos.defined()) {
+    require(t.pos.scalar_type() == at::kInt && (t.pos.dim() == 2 || t.pos.dim() == 3), PyExc_TypeError, "pos must be an int32 tensor [axes, N] or [axes, B, N]");
+    require(t.pos.size(0) == d.n_axes && t.pos.size(-1) == n_tokens && (t.pos.dim() == 2 || t.pos.size(1) == batch), PyExc_ValueError,
+            "pos must have an entry for every axis and token");
+    require_gpu(like, t.pos);
+    d.pos = t.pos.const_data_ptr<int32_t>();
+    d.pos_strides[0] = t.pos.stride(0);
+    d.pos_strides[1] = t.pos.dim() == 3 ? t.pos.stride(1) : 0;
+    d.pos_strides[2] = t.pos.stride(-1);
+  }
+  for (int i = 0; i < d.n_axes; i++) {
+    Tensor& x = t.tables[i];
+    require(x.dim() == 3 && x.size(2) == 2, PyExc_ValueError, "cos/sin table must have shape [len, R, 2]");
+    require_gpu(like, x);
+    const bool dense = x.scalar_type() == at::kFloat && (x.numel() == 0 || (x.stride(2) == 1 && (x.size(1) == 1 || x.stride(1) == 2) && x.stride(0) % 2 == 0 &&
+                                                         x.stride(0) >= 2 * x.size(1) && (uintptr_t)x.const_data_ptr() % 8 == 0));
+    if (!dense) x = x.to(at::kFloat).clone(at::MemoryFormat::Contiguous);
+    d.table[i] = (const float*)x.const_data_ptr();
+    d.table_stride0[i] = std::max<int64_t>(x.size(0) == 1 ? 2 * x.size(1) : x.stride(0), 2 * x.size(1));
+    d.n_rdim[i] = (int32_t)x.size(1);
+    d.len[i] = (int32_t)x.size(0);
+  }
+}
+
+// q and k (k undefined: q alone) into q_out and k_out, which may be q and k themselves
+void run_axes(const Tensor& q, const Tensor& k, const Tensor& q_out, const Tensor& k_out, Axes t, bool inverse) {
+  check_assert(q.dim() == 4 && (!k.defined() || k.dim() == 4), "q and k must have shape [B, heads, N, C]");
+  check_assert(!k.defined() || (k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3) && k.scalar_type() == q.scalar_type()),
+               "q and k must have one batch, token count, head dim and dtype");
+  check_assert(t.pos.defined(), "pos is needed");
+  if (k.defined()) require_gpu(q, k);
+  else require_gpu(q);
+  dlt_rope_axes_t d;
+  make_axes(t, q.size(0), q.size(2), q, d);
+  c10::DeviceGuard guard(q.device());
+  check_rc(dlt_rope_axes(q.const_data_ptr(), st(q), q_out.mutable_data_ptr(), st(q_out), (int32_t)q.size(1), k.defined() ? k.const_data_ptr() : nullptr,
+                         k.defined() ? st(k) : nullptr, k.defined() ? k_out.mutable_data_ptr() : nullptr, k.defined() ? st(k_out) : nullptr,
+                         k.defined() ? (int32_t)k.size(1) : 0, (int32_t)q.size(0), q.size(2), q.size(3), &d, inverse, dtype_code(q), stream_of(q)));
+}
+std::array<Tensor, 2> run_axes_new(const Tensor& q, const Tensor& k, const Axes& t, bool inverse) {
+  if (k.defined()) require_gpu(q, k);
+  else require_gpu(q);
+  c10::DeviceGuard guard(q.device());
+  std::array<Tensor, 2> out{empty(q.sizes(), q.scalar_type(), q), k.defined() ? empty(k.sizes(), k.scalar_type(), k) : Tensor()};
+  run_axes(q, k, out[0], out[1], t, inverse);
+  return out;
+}
+
+std::array<Tensor, 2> rope_axes(const Tensor& q, const Tensor& k, const Axes& t, bool inverse);
+
+struct RopeAxesBackward : public Node {
+  SavedVariable pos;
+  std::vector<SavedVariable> tables;
+  int layout = 0;
+  bool inverse = false, pair = false;
+  std::string name() const override { return "DltRopeAxesBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    pos.reset_data();
+    for (SavedVariable& s : tables) s.reset_data();
+  }
+  // The backward pass of a rotation is the inverse one: the same operator, which records its own graph where one is wanted.
+  variable_list apply(variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    Axes t;
+    t.pos = pos.unpack();
+    for (SavedVariable& s : tables) t.tables.push_back(s.unpack());
+    t.layout = layout;
+    const bool a = grads[0].defined(), b = pair && grads[1].defined();
+    variable_list out(pair ? 2 : 1);
+    if (a && b) {
+      auto g = rope_axes(grads[0], grads[1], t, !inverse);
+      out[0] = g[0];
+      out[1] = g[1];
+    } else if (a || b) {
+      out[a ? 0 : 1] = rope_axes(grads[a ? 0 : 1], Tensor(), t, !inverse)[0];
+    }
+    return out;
+  }
+};
+
+// rotated copies, with the graph recorded when q or k asks for it
+std::array<Tensor, 2> rope_axes(const Tensor& q, const Tensor& k, const Axes& t, bool inverse) {
+  const bool pair = k.defined();
+  std::shared_ptr<RopeAxesBackward> node;
+  if (pair ? torch::autograd::compute_requires_grad(q, k) : torch::autograd::compute_requires_grad(q)) {
+    node = make_node<RopeAxesBackward>();
+    node->set_next_edges(pair ? torch::autograd::collect_next_edges(q, k) : torch::autograd::collect_next_edges(q));
+    node->inverse = inverse;
+    node->pair = pair;
+    node->layout = t.layout;
+  }
+  std::array<Tensor, 2> out;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    out = run_axes_new(q, k, t, inverse);
+  }
+  if (node) {
+    node->pos = SavedVariable(t.pos, false);
+    for (const Tensor& x : t.tables) node->tables.emplace_back(x, false);
+    torch::autograd::set_history(out[0], node);
+    if (pair) torch::autograd::set_history(out[1], node);
+  }
+  return out;
+}
+
+// ---- the paged cache ---------------------------------------------------------------------------------------
+struct Paged {
+  dlt_paged_shape_t s{};
+  const int32_t *table = nullptr, *seq = nullptr, *n_new = nullptr;
+  int64_t ts = 0;
+};
+Paged paged_args(const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor* n_new, int64_t B, int64_t T, int64_t H) {
+  check_assert(kc.dim() == 4 && vc.dim() == 4 && kc.sizes().slice(0, 3) == vc.sizes().slice(0, 3), "caches must have shape [pages, heads, page, D], all but D alike");
+  check_assert(kc.scalar_type() == vc.scalar_type(), "caches must have one dtype");
+  require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), PyExc_TypeError,
+          "page_table must be an int32 tensor [B, pages of a sequence] with contiguous rows");
+  require(seq.scalar_type() == at::kInt && seq.dim() == 1 && (seq.size(0) <= 1 || seq.stride(0) == 1), PyExc_TypeError, "seq_len must be a contiguous 1-D int32 tensor");
+  check_assert(table.size(0) == B && seq.size(0) == B, "page_table and seq_len must have a row for every sequence");
+  require_gpu(kc, vc, table, seq);
+  Paged p;
+  if (n_new != nullptr) {
+    require(n_new->scalar_type() == at::kInt && n_new->dim() == 1 && (n_new->size(0) <= 1 || n_new->stride(0) == 1), PyExc_TypeError,
+            "n_new must be a contiguous 1-D int32 tensor");
+    check_assert(n_new->size(0) == B, "n_new must have an entry for every sequence");
+    require_gpu(kc, *n_new);
+    p.n_new = n_new->const_data_ptr<int32_t>();
+  }
+  check_assert(kc.size(0) <= INT32_MAX && kc.size(2) <= INT32_MAX && table.size(1) <= INT32_MAX && T <= INT32_MAX, "too many pages or tokens");
+  p.table = table.const_data_ptr<int32_t>();
+  p.seq = seq.const_data_ptr<int32_t>();
+  p.ts = table.stride(0);
+  p.s.B = (int32_t)B; p.s.H = (int32_t)H; p.s.Hkv = (int32_t)kc.size(1); p.s.T = (int32_t)T;
+  p.s.dk = (int32_t)kc.size(3); p.s.dv = (int32_t)vc.size(3);
+  p.s.page = (int32_t)kc.size(2); p.s.n_pages = (int32_t)kc.size(0); p.s.cols = (int32_t)table.size(1);
+  p.s.dtype = dtype_code(kc);
+  return p;
 }
 
 // ---- arguments --------------------------------------------------------------------------------------------
@@ -687,6 +903,169 @@ PyObject* py_flash_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+int32_t window_arg(PyObject* o) { return o == Py_None ? INT32_MAX : (int32_t)int_arg(o); }
+
+// (q, k, v, window or None, n_sink, scale)
+PyObject* py_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6, 6);
+  const int64_t dims[2] = {window_arg(a[3]), int_arg(a[4])};
+  if (!plain(tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]))) Py_RETURN_NOTIMPLEMENTED;
+  return THPVariable_Wrap(attention(Op::Window, tensor_arg(a[0]), tensor_arg(a[1]), tensor_arg(a[2]), nullptr, dims, false, float_arg(a[5]), false, true));
+  END_HANDLE_TH_ERRORS
+}
+
+// the same -> (o, lse2) and (q, k, v, o, lse2, do, the same 3 numbers) -> (dq, dk, dv): no graph, no padding
+PyObject* py_window_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6, 6);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]);
+  const int64_t dims[2] = {window_arg(a[3]), int_arg(a[4])};
+  require_gpu(q, k, v);
+  const Tensor q_ = as_rows16(q), k_ = as_rows16(k), v_ = as_rows16(v);
+  const Forward f = run_forward(window_spec(q_, k_, v_, dims, float_arg(a[5])), q_, k_, v_, nullptr, false);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(f.o), THPVariable_Wrap(f.lse));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_window_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9, 9);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &o = tensor_arg(a[3]), &lse = tensor_arg(a[4]), &d_o = tensor_arg(a[5]);
+  const int64_t dims[2] = {window_arg(a[6]), int_arg(a[7])};
+  require_gpu(q, k, v, o, lse, d_o);
+  const Tensor q_ = as_rows16(q), k_ = as_rows16(k), v_ = as_rows16(v), o_ = as_rows16(o);
+  auto g = run_backward(window_spec(q_, k_, v_, dims, float_arg(a[8])), q_, k_, v_, o_, lse.contiguous(), d_o, nullptr, false);
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(g[0]), THPVariable_Wrap(g[1]), THPVariable_Wrap(g[2]));
+  END_HANDLE_TH_ERRORS
+}
+
+Axes axes_arg(PyObject* pos, PyObject* tables, PyObject* layout) {
+  Axes t;
+  if (pos != Py_None) t.pos = tensor_arg(pos);
+  PyObject* seq = PySequence_Fast(tables, "tables must be a sequence of cos/sin tables");
+  if (seq == nullptr) throw python_error();
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(seq);
+  for (Py_ssize_t i = 0; i < n; i++) {
+    PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+    if (!THPVariable_Check(o)) {
+      Py_DECREF(seq);
+      raise_py(PyExc_TypeError, "tables must hold tensors");
+    }
+    t.tables.push_back(THPVariable_Unpack(o));
+  }
+  Py_DECREF(seq);
+  t.layout = (int)int_arg(layout);
+  return t;
+}
+PyObject* wrap_pair(const Tensor& q, const Tensor& k) {
+  if (!k.defined()) return Py_BuildValue("(NO)", THPVariable_Wrap(q), Py_None);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(k));
+}
+
+// (q, k or None, pos, tables, layout number, inverse, mode): mode 0: new tensors, with a graph; 1: new tensors, no graph; 2: in place, no graph
+PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 7, 7);
+  const Tensor& q = tensor_arg(a[0]);
+  const Tensor k = a[1] == Py_None ? Tensor() : tensor_arg(a[1]);
+  const Axes t = axes_arg(a[2], a[3], a[4]);
+  const bool inverse = bool_arg(a[5]);
+  const int64_t mode = int_arg(a[6]);
+  if (mode == 0) {
+    bool ordinary = plain(q) && (!k.defined() || plain(k)) && (!t.pos.defined() || plain(t.pos));
+    for (const Tensor& x : t.tables) ordinary = ordinary && plain(x);
+    if (!ordinary) Py_RETURN_NOTIMPLEMENTED;
+    const auto out = rope_axes(q, k, t, inverse);
+    return wrap_pair(out[0], out[1]);
+  }
+  if (mode == 2) {
+    torch::autograd::check_inplace(q, torch::autograd::compute_requires_grad(q));
+    if (k.defined()) torch::autograd::check_inplace(k, torch::autograd::compute_requires_grad(k));
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      run_axes(q, k, q, k, t, inverse);
+    }
+    torch::autograd::increment_version(q);
+    if (k.defined()) torch::autograd::increment_version(k);
+    return PyTuple_Pack(2, a[0], a[1]);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  const auto out = run_axes_new(q, k, t, inverse);
+  return wrap_pair(out[0], out[1]);
+  END_HANDLE_TH_ERRORS
+}
+
+// (k_cache, v_cache, k, v, page_table, seq_len, n_new or None, pos or None, tables or None, layout number, q or None) -> rotated q or None
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 11, 11);
+  const Tensor &kc = tensor_arg(a[0]), &vc = tensor_arg(a[1]), &k = tensor_arg(a[2]), &v = tensor_arg(a[3]), &table = tensor_arg(a[4]), &seq = tensor_arg(a[5]);
+  const Tensor n_new = a[6] == Py_None ? Tensor() : tensor_arg(a[6]), q = a[10] == Py_None ? Tensor() : tensor_arg(a[10]);
+  const bool rope = a[8] != Py_None;
+  Axes t;
+  if (rope) t = axes_arg(a[7], a[8], a[9]);
+  check_assert(k.dim() == 4 && v.dim() == 4 && k.sizes().slice(0, 3) == v.sizes().slice(0, 3), "k and v must have shape [B, heads, T, D], all but D alike");
+  check_assert(k.size(1) == kc.size(1) && k.size(3) == kc.size(3) && v.size(3) == vc.size(3), "k and v must match their caches");
+  check_assert(k.scalar_type() == kc.scalar_type() && v.scalar_type() == kc.scalar_type(), "k, v and the caches must have one dtype");
+  check_assert(!q.defined() || (q.dim() == 4 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.size(3) == k.size(3) && q.scalar_type() == k.scalar_type()),
+               "q must match k");
+  Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, k.size(0), k.size(2), q.defined() ? q.size(1) : 0);
+  require_gpu(kc, k, v);
+  if (q.defined()) require_gpu(kc, q);
+  for (const Tensor* c : {&kc, &vc}) torch::autograd::check_inplace(*c, torch::autograd::compute_requires_grad(*c));
+  Tensor q_out;
+  if (p.s.B > 0) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::DeviceGuard guard(kc.device());
+    if (q.defined()) q_out = empty(q.sizes(), q.scalar_type(), q);
+    dlt_rope_axes_t d;
+    if (rope) make_axes(t, k.size(0), k.size(2), kc, d);
+    check_rc(dlt_paged_append(k.const_data_ptr(), st(k), v.const_data_ptr(), st(v), q.defined() ? q.const_data_ptr() : nullptr, q.defined() ? st(q) : nullptr,
+                              q.defined() ? q_out.mutable_data_ptr() : nullptr, q.defined() ? st(q_out) : nullptr, kc.mutable_data_ptr(), st(kc),
+                              vc.mutable_data_ptr(), st(vc), p.table, p.ts, p.seq, p.n_new, rope ? &d : nullptr, &p.s, stream_of(kc)));
+  } else if (q.defined()) {
+    q_out = empty(q.sizes(), q.scalar_type(), q);
+  }
+  torch::autograd::increment_version(kc);
+  torch::autograd::increment_version(vc);
+  if (!q_out.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(q_out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, v_cache, page_table, seq_len, window or None, n_sink, scale, n_new or None) -> o, no graph
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9, 9);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const Tensor &q0 = tensor_arg(a[0]), &kc = tensor_arg(a[1]), &vc = tensor_arg(a[2]), &table = tensor_arg(a[3]), &seq = tensor_arg(a[4]);
+  const Tensor n_new = a[8] == Py_None ? Tensor() : tensor_arg(a[8]);
+  check_assert(q0.dim() == 4 && q0.size(3) == kc.size(-1) && q0.scalar_type() == kc.scalar_type(), "q must have shape [B, heads, T, D] and match the cache");
+  Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, q0.size(0), q0.size(2), q0.size(1));
+  p.s.window = window_arg(a[5]);
+  p.s.n_sink = (int32_t)int_arg(a[6]);
+  p.s.sm_scale = (float)float_arg(a[7]);
+  require_gpu(kc, q0);
+  require(rows16(kc) && rows16(vc), PyExc_ValueError, "rows of the caches must be contiguous and start at multiples of 16 bytes");
+  c10::DeviceGuard guard(kc.device());
+  Tensor o = empty({q0.size(0), q0.size(1), q0.size(2), vc.size(3)}, q0.scalar_type(), q0);
+  if (o.numel() == 0) return THPVariable_Wrap(o);
+  const Tensor q = as_rows16(q0);
+  Workspace ws;
+  check_rc(dlt_paged_workspace(&p.s, &ws.bytes));
+  if (ws.bytes > 0) {
+    ws.t = empty({ws.bytes / 4}, at::kFloat, q);
+    ws.ptr = ws.t.mutable_data_ptr();
+  }
+  check_rc(dlt_paged_attn(q.const_data_ptr(), st16(q).data(), kc.const_data_ptr(), st16(kc).data(), vc.const_data_ptr(), st16(vc).data(), o.mutable_data_ptr(),
+                          st16(o).data(), p.table, p.ts, p.seq, p.n_new, &p.s, ws.ptr, ws.bytes, stream_of(q)));
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
 // (x[B', N, C], idx, row, col): rotated in place, returned
 PyObject* py_rope_apply(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -772,7 +1151,8 @@ PyObject* py_pad_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define DLT_FN(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef METHODS[] = {DLT_FN(tiled_swa), DLT_FN(tiled_swa_fwd), DLT_FN(tiled_swa_rope), DLT_FN(tiled_swa_image), DLT_FN(flash), DLT_FN(swa_forward),
                          DLT_FN(swa_backward), DLT_FN(image_forward), DLT_FN(image_backward), DLT_FN(flash_forward), DLT_FN(flash_backward), DLT_FN(rope_apply), DLT_FN(rope_heads), DLT_FN(rope_inplace), DLT_FN(rope_pair),
-                         DLT_FN(pad_plan), {nullptr, nullptr, 0, nullptr}};
+                         DLT_FN(pad_plan), DLT_FN(window), DLT_FN(window_forward), DLT_FN(window_backward), DLT_FN(rope_axes), DLT_FN(paged_append), DLT_FN(paged_attention),
+                         {nullptr, nullptr, 0, nullptr}};
 #undef DLT_FN
 
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_dlt_torch", "torch binding of libdlt_hip.so", -1, METHODS, nullptr, nullptr, nullptr, nullptr};

@@ -277,6 +277,90 @@ int dlt_flash_bwd_ws(const void* q, const int64_t q_strides[4], const void* k, c
                      void* dv, const int64_t dv_strides[4],
                      const dlt_flash_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
 
+/* ---- rotation by positions with several axes -----------------------------------------------
+ * The rotation above for any number of axes (time, height and width of a video, say), tables and clamping as there.  Axis a
+ * turns n_rdim[a] pairs of dims by the row of table[a] that pos gives for it; a negative position leaves its dims as they are.  With
+ * off_a = n_rdim[0] + .. + n_rdim[a - 1] and P = sum n_rdim, pair i of axis a is
+ *   DLT_ROPE_BLOCKS  dims 2 off_a + i and 2 off_a + n_rdim[a] + i   (the layout of dlt_rope2d)
+ *   DLT_ROPE_HALVES  dims off_a + i and P + off_a + i
+ * Dims from 2 P on pass through. */
+#define DLT_ROPE_AXES_MAX 4
+enum { DLT_ROPE_BLOCKS = 0, DLT_ROPE_HALVES = 1 };
+typedef struct {
+  int32_t n_axes, layout;
+  const int32_t* pos;       /* pos[axis, batch, token] by element strides; batch stride 0: one set for all.  dlt_paged_append: NULL
+                               takes a token's place in its sequence on every axis */
+  int64_t pos_strides[3];
+  const float* table[DLT_ROPE_AXES_MAX];        /* fp32 [len, n_rdim, 2], (cos, sin) innermost */
+  int64_t table_stride0[DLT_ROPE_AXES_MAX];     /* elements between rows */
+  int32_t n_rdim[DLT_ROPE_AXES_MAX], len[DLT_ROPE_AXES_MAX];
+} dlt_rope_axes_t;
+
+/* q [B, Hq, N, C] and k [B, Hk, N, C] (Hk == 0: q alone) rotated into q_out and k_out in one launch, the inverse rotation (its transpose:
+ * what a gradient takes) when inverse != 0.  q_out == q with the same strides rotates in place; otherwise outputs must not overlap inputs. */
+int dlt_rope_axes(const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4], int32_t Hq,
+                  const void* k, const int64_t k_strides[4], void* k_out, const int64_t k_out_strides[4], int32_t Hk,
+                  int32_t B, int64_t n_tokens, int64_t n_dim, const dlt_rope_axes_t* rope, int inverse, int dtype, void* stream);
+
+/* ---- attention over a 1D window with sinks ---------------------------------------------------
+ * q [B, H, Lq, dk], k [B, Hkv, Lk, dk], v [B, Hkv, Lk, dv], o [B, H, Lq, dv]; head h of q reads head h / (H / Hkv) of k and v.  Query i
+ * stands at position p = Lk - Lq + i and sees key j iff j <= p and (p - j < window or j < n_sink): the last `window` keys up to its own
+ * and the first n_sink ones.  A query that sees nothing (p < 0) gives zeros and lse2 = -inf.  lse2 and delta are fp32, contiguous
+ * [B, Hkv, Lq, H / Hkv].  DLT_BF16 and DLT_FP16; dk and dv multiples of 8 up to 128, rows of unit last stride in multiples of 16
+ * bytes; sm_scale > 0. */
+typedef struct {
+  int32_t B, H, Hkv, Lq, Lk, dk, dv;
+  int32_t window, n_sink;   /* window >= 1 (INT32_MAX: no limit), n_sink >= 0 */
+  float sm_scale;
+  int32_t dtype;
+} dlt_window_shape_t;
+
+/* Bytes of workspace that a pass needs (0: none): partial results where few rows or keys are split over workgroups, at most
+ * DLT_WINDOW_WORKSPACE_MAX.  The workspace is 16-byte aligned device memory that belongs to the call until its kernels have run. */
+#define DLT_WINDOW_WORKSPACE_MAX (256 << 20)
+int dlt_window_workspace(const dlt_window_shape_t* shape, int backward, int64_t* bytes);
+int dlt_window_fwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
+                   const void* v, const int64_t v_strides[4], void* o, const int64_t o_strides[4], float* lse2,
+                   const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
+/* delta: scratch of the size of lse2.  dk and dv are summed over the heads that share a key in a fixed order. */
+int dlt_window_bwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
+                   const void* v, const int64_t v_strides[4], const void* o, const int64_t o_strides[4],
+                   const void* d_o, const int64_t do_strides[4], const float* lse2, float* delta,
+                   void* dq, const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4],
+                   void* dv, const int64_t dv_strides[4],
+                   const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- keys and values in pages -----------------------------------------------------------------
+ * A cache is [n_pages, Hkv, page, d] by element strides (page, head, row, dim).  Row b of `table` (int32, `cols` pages, element stride
+ * table_stride) names the pages of sequence b in order: position p lies in row p % page of page table[b][p / page].  seq_len[b] counts the
+ * tokens of sequence b with its n_new[b] newest ones (n_new NULL: T of every sequence; n_new[b] is taken within 0 .. T, seq_len[b] within
+ * 0 .. cols * page); new token t < n_new[b] stands at position seq_len[b] - n_new[b] + t, tokens t >= n_new[b] are padding. */
+typedef struct {
+  int32_t B, H, Hkv, T, dk, dv;
+  int32_t page, n_pages, cols;
+  int32_t window, n_sink;   /* attention: as in dlt_window_shape_t */
+  float sm_scale;
+  int32_t dtype;
+} dlt_paged_shape_t;
+
+/* New keys k [B, Hkv, T, dk] and values v [B, Hkv, T, dv] into the cache; with `rope` keys are rotated on the way, and with q [B, H, T, dk]
+ * (H == 0: none) queries are rotated into q_out.  Padding, positions outside the table's row and page numbers outside the pool write nothing
+ * into the cache; padded rows of q are copied as they are.  No two tokens may name the same place.  All three dtypes, any strides. */
+int dlt_paged_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                     const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4],
+                     void* k_cache, const int64_t k_cache_strides[4], void* v_cache, const int64_t v_cache_strides[4],
+                     const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
+                     const dlt_rope_axes_t* rope, const dlt_paged_shape_t* shape, void* stream);
+
+/* The window attention above for the T newest tokens of every sequence, keys and values in pages (page a multiple of 16).  Padded rows and rows
+ * that see nothing give zeros.  What pages hold behind a sequence's last token does not matter.  A page number outside the pool reads
+ * another page of it. */
+int dlt_paged_workspace(const dlt_paged_shape_t* shape, int64_t* bytes);
+int dlt_paged_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4],
+                   const void* v_cache, const int64_t v_cache_strides[4], void* o, const int64_t o_strides[4],
+                   const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
+                   const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
+
 /* ---- per-kernel timing (measurement aid) ---------------------------------------------------
  * Counterpart of the reference's triton.testing.do_bench calls (src/tiled_swa.py:765-774,
  * src/flash_attn.py:592,606), at kernel granularity.  While enabled for the calling thread,
@@ -311,9 +395,10 @@ int dlt_debug_copy(void* dst, const void* src, int64_t bytes, void* stream);
  *             dlt_swa_*_narrow also at multiples of 8 below 64
  *   TILE      token grids, head dims in multiples of 32 up to 128, windows up to 21 columns (rotation in the tile loads)
  *   FLASH     dense / causal / tiles of 16 k tokens, 2-byte element types, head dims up to 128 (multiples of 8)
- *   GENERIC   everything else */
+ *   GENERIC   everything else
+ *   BAND      dlt_window_*, dlt_paged_attn */
 enum { DLT_FAMILY_NONE = 0, DLT_FAMILY_MARCHING = 1, DLT_FAMILY_STREAMING = 2, DLT_FAMILY_TILE = 3, DLT_FAMILY_FLASH = 4,
-       DLT_FAMILY_GENERIC = 5 };
+       DLT_FAMILY_GENERIC = 5, DLT_FAMILY_BAND = 6 };
 int dlt_dry_run(int on);
 int dlt_last_kernel_family(void);
 

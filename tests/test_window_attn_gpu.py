@@ -1,0 +1,55 @@
+"""Window attention with sinks against its 64-bit form (GPU)."""
+import math
+
+import pytest
+import torch
+
+from dl_templates_amd.window_attn import window_attention
+from tests import long_oracle as orc
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def make(seed, B, Hq, Hkv, Lq, Lk, dk, dv, dtype):
+    gen = torch.Generator().manual_seed(seed)
+    mk = lambda *s: torch.randn(s, generator=gen).to(dtype).cuda()  # noqa: E731
+    return mk(B, Hq, Lq, dk), mk(B, Hkv, Lk, dk), mk(B, Hkv, Lk, dv), mk(B, Hq, Lq, dv)
+
+
+def run(q, k, v, do, window, n_sink, scale):
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    o = window_attention(q, k, v, window, n_sink, scale)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, (q, k, v), do)))
+
+
+CASES = [
+    # B, Hq, Hkv, Lq, Lk, dk, dv, window, sinks, dtype
+    (1, 1, 1, 1, 1, 64, 64, 1, 0, BF),
+    (1, 2, 2, 64, 64, 64, 64, None, 0, BF),
+    (2, 4, 2, 200, 200, 64, 64, 64, 4, HF),
+    (1, 8, 1, 130, 130, 128, 128, 17, 1, BF),
+    (1, 6, 2, 257, 301, 80, 80, 100, 5, HF),
+    (1, 3, 1, 77, 500, 128, 128, 60, 33, BF),
+    (2, 5, 5, 65, 65, 32, 64, 1, 0, BF),
+    (1, 4, 4, 90, 40, 64, 64, 16, 2, HF),          # more queries than keys: the first ones see nothing
+    (1, 2, 1, 1, 700, 128, 128, None, 0, BF),
+    (1, 2, 1, 5, 700, 64, 64, 300, 70, HF),
+    (1, 7, 1, 333, 333, 96, 40, 1000, 3, BF),
+    (1, 1, 1, 513, 513, 128, 128, 128, 64, HF),
+    (1, 1, 1, 513, 513, 128, 128, 129, 65, BF),
+    (1, 32, 1, 40, 90, 64, 128, 31, 7, BF),
+    (3, 2, 2, 127, 129, 8, 16, 2, 1, BF),
+    (1, 2, 2, 700, 700, 64, 64, 64, 600, BF),      # sinks beyond the window's own reach
+    (1, 1, 1, 2000, 2000, 64, 64, 500, 4, HF),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_against_64_bits(case):
+    B, Hq, Hkv, Lq, Lk, dk, dv, window, n_sink, dtype = case
+    q, k, v, do = make(1, B, Hq, Hkv, Lq, Lk, dk, dv, dtype)
+    scale = 1.0 / math.sqrt(dk)
+    got = run(q, k, v, do, window, n_sink, scale)
+    for name, want in orc.window(q, k, v, window, n_sink, scale, do).items():
+        orc.check(got[name], want, name)
