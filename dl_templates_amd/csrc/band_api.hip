@@ -43,19 +43,25 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
   if (d == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
-// dK (times sm_scale) or dV: partial sums [bh][share][key][dims], added in the order of the shares
+// dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares
 template <typename TIO>
 __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
   const bool keys = blockIdx.y == 0;
   const int dims = keys ? a.dk_ : a.dv_, per = dims / 4;
-  const float* part = a.part + (keys ? 0 : (int64_t)a.B * a.Hkv * a.shares * a.Lk * a.dk_);
+  const BandParts P(a, band_kv_group(band_class(a.dk_, a.dv_)));
+  const float *part = a.part + (keys ? 0 : P.v_at), *fpart = a.part + (keys ? P.far_at : P.v_at + P.v_far_at);
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t at = gid / per;
   const int d = 4 * (int)(gid - at * per);
-  if (at >= (int64_t)a.B * a.Hkv * a.Lk) return;
-  const int bh = (int)(at / a.Lk), j = (int)(at - (int64_t)bh * a.Lk), b = bh / a.Hkv, h = bh - b * a.Hkv;
+  if (at >= (int64_t)a.B * a.Hkv * P.keys) return;
+  const int bh = (int)(at / P.keys), j = (int)(at - (int64_t)bh * P.keys), b = bh / a.Hkv, h = bh - b * a.Hkv;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < a.shares; i++) s += *reinterpret_cast<const f32x4*>(part + (((int64_t)bh * a.shares + i) * a.Lk + j) * dims + d);
+#pragma unroll 4
+  for (int i = 0; i < a.shares; i++) s += *reinterpret_cast<const f32x4*>(part + (((int64_t)bh * a.shares + i) * P.keys + j) * dims + d);
+  if (j < P.far_keys) {
+#pragma unroll 8
+    for (int i = 0; i < 4 * a.far; i++) s += *reinterpret_cast<const f32x4*>(fpart + (((int64_t)bh * a.far * 4 + i) * P.far_keys + j) * dims + d);
+  }
   if (keys) s *= a.sm_scale;
   TIO* p = keys ? reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1] + j * a.dks[2] : reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1] + j * a.dvs[2];
   u32x2 w;
@@ -65,8 +71,8 @@ __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
 }
 
 int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
-  if (a.shares <= 1) return DLT_OK;
-  const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.Lk : a.rows);
+  if (backward ? a.part_keys == 0 : a.shares <= 1) return DLT_OK;
+  const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.part_keys : a.rows);
   const int per = (backward ? dlt_imax(a.dk_, a.dv_) : a.dv_) / 4;
   const dim3 grid((unsigned)((rows * per + 255) / 256), backward ? 2 : 1);
   dlt_timing_before(backward ? DLT_K_BWD_KV : DLT_K_FWD, stream);
@@ -177,20 +183,36 @@ int plan_rows(BandArgs& a, bool shares) {
   return np;
 }
 int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
-// Keys: the rows that see a block of keys taken by several workgroups where blocks are few
+int64_t keys_bytes(const BandArgs& a) { return a.part_keys > 0 ? BandParts(a, band_kv_group(band_class(a.dk_, a.dv_))).floats * 4 : 0; }
+// Keys: the rows that see a block of keys taken by several workgroups where blocks are few, the far rows of sinks always
 void plan_keys(BandArgs& a) {
   const int cus = dlt_device_cus();
-  const int own = band_kv_own(band_class(a.dk_, a.dv_));
+  const int cls = band_class(a.dk_, a.dv_), own = band_kv_own(cls), group = band_kv_group(cls);
   a.nblk = (a.Lk + own - 1) / own;
+  a.shares = 1;
+  a.far = a.far_groups = a.part_keys = 0;
   const int64_t bh = (int64_t)a.B * a.Hkv, wgs = bh * a.nblk;
-  const int64_t most = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;
-  int64_t n = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
-  n = dlt_imin64(n, most / 4);
-  const int64_t key_bytes = bh * a.Lk * (a.dk_ + a.dv_) * 4;
-  n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(key_bytes > 0 ? key_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
-  a.shares = n < 1 ? 1 : (int)n;
+  const int64_t near_chunks = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;   // of a block without sinks
+  const int64_t want = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
+  const int64_t key_bytes = dlt_imax64(bh * a.Lk * (a.dk_ + a.dv_) * 4, 1);
+  a.shares = (int)dlt_imax64(1, dlt_imin64(dlt_imin64(want, near_chunks / 4), DLT_WINDOW_WORKSPACE_MAX / 2 / key_bytes));
+  const int64_t near_end = dlt_imin64((int64_t)dlt_imax(dlt_imin(own, a.Lk) - 1 - a.off + a.W, 0) * a.G, a.rows);
+  const int64_t far_chunks = (a.rows - near_end + 63) / 64;
+  if (a.S > 0 && far_chunks > 4) {
+    // about as many chunks as a near workgroup has (a far one takes a third of the time for one), fewer where that leaves CUs idle
+    a.far_groups = (a.S + group - 1) / group;
+    int64_t most = dlt_imax64(16, 2 * near_chunks / a.shares);
+    while (most > 8 && wgs * a.shares + bh * a.far_groups * (far_chunks / most) < 2 * cus) most /= 2;
+    const int64_t far_bytes = bh * 4 * a.far_groups * group * (a.dk_ + a.dv_) * 4;
+    a.far = (int)dlt_imax64(1, dlt_imin64((far_chunks + most - 1) / most, DLT_WINDOW_WORKSPACE_MAX / 4 / far_bytes));
+    a.part_keys = dlt_imin((a.S + own - 1) / own * own, a.Lk);
+  }
+  if (a.shares > 1) a.part_keys = a.Lk;
+  if (keys_bytes(a) > DLT_WINDOW_WORKSPACE_MAX) {   // sinks of very many heads
+    a.far = a.far_groups = 0;
+    a.part_keys = a.shares > 1 ? a.Lk : 0;
+  }
 }
-int64_t keys_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.Lk * (a.dk_ + a.dv_) * 4 : 0; }
 
 int check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
   DLT_REQUIRE(need == 0 || (ws != nullptr && have >= need && (uintptr_t)ws % 16 == 0), "%s: needs %lld bytes of 16-byte aligned workspace, got %lld", who,
@@ -198,7 +220,7 @@ int check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
   return DLT_OK;
 }
 int check_grid(const char* who, const BandArgs& a) {
-  if ((int64_t)a.B * a.Hkv * a.nblk * a.shares > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  if ((int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + (int64_t)a.far * a.far_groups) > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
   return DLT_OK;
 }
 void strides3(int64_t (&to)[3], const int64_t* st) {

@@ -244,6 +244,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
                               });
 }
 
+// Sinks are seen by every later row, so a block of keys with sinks would have the rows of the whole sequence where others have those of a
+// window.  The rows behind the block's window ("far" rows) are therefore taken by workgroups of their own, a share of the rows each: the 16 NP keys
+// of a far workgroup belong to all its waves, which take 16 of a chunk's 64 rows each, with half-filled second products.  Far workgroups
+// and the blocks with sinks leave partial sums, which a second launch adds in a fixed order.  16 heads on 4, 8192 tokens, window 1024, 4 sinks,
+// d = 128: 876 us with the far rows in the block, FARTIME with 22 shares of them beside it.
 // ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
 template <typename TIO, int D, int NP, int CK, int NW, int PAD>
 __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs a) {
@@ -260,10 +265,22 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  int bh, r_, unit;
-  flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, false, bh, r_, unit);
-  const int blk = unit / a.shares, share = unit - blk * a.shares;
-  const int x0 = blk * OWN, xe = dlt_imin(x0 + OWN, a.Lk);
+  const int n_far = a.far * a.far_groups, far_lin = lin - ((int)gridDim.x - a.B * a.Hkv * n_far);
+  const bool far = far_lin >= 0;
+  int bh, share, x0;
+  if (far) {
+    bh = far_lin / n_far;
+    const int rest = far_lin - bh * n_far, grp = rest / a.far;
+    share = rest - grp * a.far;
+    x0 = grp * 16 * NP;
+  } else {
+    int r_, unit;
+    flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, false, bh, r_, unit);
+    const int blk = unit / a.shares;
+    share = unit - blk * a.shares;
+    x0 = blk * OWN;
+  }
+  const int xe = dlt_imin(x0 + (far ? 16 * NP : OWN), a.Lk);
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   const char* qb = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1]);
   const char* dob = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1]);
@@ -273,10 +290,14 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
 
   // rows [r_beg, r_end) see some own key; key j is seen by rows [rlo(j), rhi(j))
   auto rlo_of = [&](int j) { return (int)dlt_imin64((int64_t)dlt_imax(j - a.off, 0) * a.G, a.rows); };
-  auto rhi_of = [&](int j) { return j < a.S ? a.rows : (int)dlt_imin64((int64_t)dlt_imax(j - a.off + a.W, 0) * a.G, a.rows); };
-  const int r_beg = rlo_of(x0), r_end = x0 < a.S ? a.rows : rhi_of(xe - 1);
-  int nch = r_end > r_beg ? (r_end - r_beg + CK - 1) / CK : 0;
-  const int per = (nch + a.shares - 1) / a.shares;
+  // far rows start behind the last row whose window holds a key of the block (far workgroups: of the block that their keys lie in)
+  auto near_end = [&](int last) { return (int)dlt_imin64((int64_t)dlt_imax(last - a.off + a.W, 0) * a.G, a.rows); };
+  const int r_beg = far ? near_end(dlt_imin(x0 / OWN * OWN + OWN, a.Lk) - 1) : rlo_of(x0);
+  const int r_end = far ? a.rows : x0 < a.S && a.far == 0 ? a.rows : near_end(xe - 1);
+  auto rhi_of = [&](int j) { return j < a.S ? r_end : near_end(j); };
+  const int nch = r_end > r_beg ? (r_end - r_beg + CK - 1) / CK : 0;
+  const int n_shares = far ? a.far : a.shares;
+  const int per = (nch + n_shares - 1) / n_shares;
   const int i_beg = dlt_imin(share * per, nch), i_end = dlt_imin(i_beg + per, nch);
 
   BandStageRows<D> stq, std_;
@@ -304,7 +325,7 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
   for (int i = 0; i < AHEAD; i++)
     if (i_beg + i < i_end) issue(i_beg + i, smem + i * B::BUF_KV);
 
-  const int wk0 = x0 + wave * 16 * NP;
+  const int wk0 = far ? x0 : x0 + wave * 16 * NP;
   u32x4 kf[NP][KC], vf[NP][KC];
   int rlo[NP], rhi[NP];
 #pragma unroll
@@ -319,8 +340,8 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
   // rows that see some key of the wave: [wlo, whi); rows that see all of them: [flo, fhi)
   const int wk1 = dlt_imin(wk0 + 16 * NP, xe) - 1;
   const bool wave_on = wk1 >= wk0;
-  const int wlo = wave_on ? rlo_of(wk0) : 0, whi = !wave_on ? 0 : wk0 < a.S ? a.rows : rhi_of(wk1);
-  const int flo = wave_on ? rlo_of(wk1) : 0, fhi = !wave_on ? 0 : wk0 >= a.S ? rhi_of(wk0) : wk1 < a.S ? a.rows : rhi_of(a.S);
+  const int wlo = wave_on ? rlo_of(wk0) : 0, whi = !wave_on ? 0 : wk0 < a.S ? r_end : rhi_of(wk1);
+  const int flo = wave_on ? rlo_of(wk1) : 0, fhi = !wave_on ? 0 : wk0 >= a.S ? rhi_of(wk0) : wk1 < a.S ? r_end : rhi_of(a.S);
 
   f32x4 dk_acc[NP][KB], dv_acc[NP][KB];
 #pragma unroll
@@ -431,8 +452,52 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
       }
     });
   };
+  // far: rows 16 wave .. + 15 of the chunk
+  auto consume_far = [&](const int q0, Swa2Lds __restrict__ cur) __attribute__((always_inline)) {
+    Swa2Lds sQ = cur + 16 * wave * FlashDRow<D>::ROW, sDO = sQ + B::REG;
+    Swa2Lds sLse = cur + 2 * B::REG + 16 * g + 64 * wave, sDel = sLse + CK * 4;
+    const f32x4 lq = __builtin_bit_cast(f32x4, swa2_lds16(sLse)), dl = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
+    f32x4 sv[NP], dp[NP];
+#pragma unroll
+    for (int r = 0; r < KC; r++) {
+      const u32x4 x = swa2_lds16(sQ + L.a[r]), y = swa2_lds16(sDO + L.a[r]);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        sv[p] = Mma<TIO>::mfma(x, kf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[p]);
+        dp[p] = Mma<TIO>::mfma(y, vf[p][r], r == 0 ? dl : dp[p]);
+      }
+    }
+    u32x4 pb[NP], dsb[NP];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      float pr[4], ds[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int r = q0 + 16 * wave + 4 * g + i;
+        const bool sees = r >= rlo[p] && r < rhi[p];
+        const float pv = fast_exp2(fmaf(sv[p][i], scale, -lq[i]));
+        pr[i] = sees ? pv : 0.f;
+        ds[i] = sees ? -pv * dp[p][i] : 0.f;
+      }
+      pb[p] = u32x4{pack2<TIO>(pr[0], pr[1]), pack2<TIO>(pr[2], pr[3]), 0u, 0u};
+      dsb[p] = u32x4{pack2<TIO>(ds[0], ds[1]), pack2<TIO>(ds[2], ds[3]), 0u, 0u};
+    }
+#pragma unroll
+    for (int d = 0; d < KB; d++) {
+      const u32x2 x = swa2_lds_tr(sDO + L.tr[d]), y = swa2_lds_tr(sQ + L.tr[d]);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        dv_acc[p][d] = Mma<TIO>::mfma(u32x4{x.x, x.y, 0u, 0u}, pb[p], dv_acc[p][d]);
+        dk_acc[p][d] = Mma<TIO>::mfma(u32x4{y.x, y.y, 0u, 0u}, dsb[p], dk_acc[p][d]);
+      }
+    }
+  };
   auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
     const int q0 = r_beg + i * CK;
+    if (far) {
+      consume_far(q0, (Swa2Lds)buf);
+      return;
+    }
     if (q0 >= whi || q0 + CK <= wlo) return;
     if (q0 >= flo && q0 + CK <= fhi) consume(q0, (Swa2Lds)buf, std::false_type{});
     else consume(q0, (Swa2Lds)buf, std::true_type{});
@@ -475,22 +540,27 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
     for (int r0 = lo; r0 < hi; r0 += 64) {
       const int r = r0 + lane;
       float p = 0.f, ds = 0.f;
-      if (r < hi) {
+      const bool mine = r < hi && (!far || ((r - r_beg) >> 4 & 3) == wave);
+      const uint64_t todo = __builtin_amdgcn_ballot_w64(mine);
+      if (mine) {
         const TIO *q = band_row_ptr(reinterpret_cast<const TIO*>(qb), a.qs, a, r), *d_o = band_row_ptr(reinterpret_cast<const TIO*>(dob), a.dos, a, r);
         p = fast_exp2(band_dot(q, k, a.dk_) * scale - a.lse[row0 + r]);
         ds = p * (band_dot(d_o, v, a.dv_) - a.delta[row0 + r]);
       }
-      for (int u = 0; u < 64 && r0 + u < hi; u++) {
+      for (uint64_t left = todo; left != 0; left &= left - 1) {
+        const int u = __builtin_ctzll(left);
         band_axpy(sv, band_lane(p, u), band_row_ptr(reinterpret_cast<const TIO*>(dob), a.dos, a, r0 + u), a.dv_, lane);
         band_axpy(sk, band_lane(ds, u), band_row_ptr(reinterpret_cast<const TIO*>(qb), a.qs, a, r0 + u), a.dk_, lane);
       }
     }
   };
-  if (a.shares > 1) {
-    float* pk = a.part + ((int64_t)bh * a.shares + share) * a.Lk * a.dk_;
-    float* pv = a.part + (int64_t)a.B * a.Hkv * a.shares * a.Lk * a.dk_ + ((int64_t)bh * a.shares + share) * a.Lk * a.dv_;
-    flash_share_put<NP>(pk, dk_acc, a.dk_, wk0 + n, a.Lk, g);
-    flash_share_put<NP>(pv, dv_acc, a.dv_, wk0 + n, a.Lk, g);
+  if (far || a.shares > 1 || (a.far != 0 && x0 < a.S)) {
+    const BandParts P(a, 16 * NP);
+    float* pk = a.part + (far ? P.far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dk_ : ((int64_t)bh * a.shares + share) * P.keys * a.dk_);
+    float* pv = a.part + P.v_at + (far ? P.v_far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dv_ : ((int64_t)bh * a.shares + share) * P.keys * a.dv_);
+    const int len = far ? (int)P.far_keys : a.Lk;
+    flash_share_put<NP>(pk, dk_acc, a.dk_, wk0 + n, len, g);
+    flash_share_put<NP>(pv, dv_acc, a.dv_, wk0 + n, len, g);
 #pragma unroll 1
     for (int p = 0; p < NP; p++)
       for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {

@@ -28,13 +28,30 @@ struct BandArgs {
   uint32_t mG, sG;          // division by G
   int32_t W, S, off, rows;  // W <= Lk; rows = Lq G
   int32_t nblk, group;      // own blocks of a (batch, kv head); heads interleaved at launch (flash_block_causal)
-  int32_t shares;           // workgroups that share the keys of an own block (forward)
+  int32_t shares;           // workgroups that share the keys (forward) or rows (dK / dV) of an own block
+  int32_t far, far_groups;  // dK / dV: workgroups that share the far rows of a group of sinks, such groups (band_bwd_kernel.h); 0: none
+  int32_t part_keys;        // keys of a (batch, kv head) with partial sums
   int32_t q16;              // 16 is a multiple of G: 16 rows are whole tokens
   float scale_log2, sm_scale;
   BandPages pg;
 };
 
 DLT_HD int64_t dlt_imin64(int64_t a, int64_t b) { return a < b ? a : b; }
+DLT_HD int64_t dlt_imax64(int64_t a, int64_t b) { return a > b ? a : b; }
+
+// Partial sums of the dK / dV kernel in `part`: dK rows [bh][share][keys], far dK rows [bh][far share, wave][far_keys], then the same of dV
+struct BandParts {
+  int64_t keys, far_keys, far_at, v_at, v_far_at, floats;   // far_at from the start, v_far_at from v_at on
+  DLT_HD BandParts(const BandArgs& a, int group) {
+    const int64_t bh = (int64_t)a.B * a.Hkv;
+    keys = a.part_keys;
+    far_keys = (int64_t)a.far_groups * group;
+    far_at = bh * a.shares * keys * a.dk_;
+    v_at = far_at + bh * a.far * 4 * far_keys * a.dk_;
+    v_far_at = bh * a.shares * keys * a.dv_;
+    floats = v_at + v_far_at + bh * a.far * 4 * far_keys * a.dv_;
+  }
+};
 
 // Of the rows of a tile: token and head in the group
 struct BandRow { int tok, head; };

@@ -15,3 +15,5 @@ int dlt_band_bwd_kv_64(const BandArgs& a, int dtype, hipStream_t stream);
 int dlt_band_bwd_kv_128(const BandArgs& a, int dtype, hipStream_t stream);
 // keys of a workgroup of the dK / dV kernel
 constexpr int band_kv_own(int d) { return d <= 64 ? 128 : 64; }
+// ... and of one of its workgroups for far rows
+constexpr int band_kv_group(int d) { return band_kv_own(d) / 4; }

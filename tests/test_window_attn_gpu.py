@@ -53,3 +53,18 @@ def test_against_64_bits(case):
     got = run(q, k, v, do, window, n_sink, scale)
     for name, want in orc.window(q, k, v, window, n_sink, scale, do).items():
         orc.check(got[name], want, name)
+
+
+FAR = [
+    (1, 4, 1, 3000, 3000, 64, 64, 33, 4, BF),
+    (1, 2, 2, 2500, 2600, 128, 128, 64, 17, HF),      # two groups of sinks, the second one partly filled
+    (2, 3, 1, 1500, 1500, 80, 72, 100, 70, BF),       # sinks over two blocks of keys
+    (1, 8, 8, 1111, 1111, 128, 128, 1, 1, BF),
+    (1, 1, 1, 4000, 4000, 64, 64, 17, 128, HF),
+]
+
+
+@pytest.mark.parametrize("case", FAR, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_rows_far_behind_the_sinks(case):
+    """Gradients of first keys that the rows of the whole sequence see."""
+    test_against_64_bits(case)
