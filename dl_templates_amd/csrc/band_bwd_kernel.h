@@ -36,7 +36,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 
   BandWalk<CK> W;
   const int xl = dlt_imin(x0 + OWN, a.rows) - 1;
-  W.init(a.off + band_row(a, x0).tok, a.off + band_row(a, xl).tok, a.W, a.S);
+  const int first = a.off + band_row(a, x0).tok, last = a.off + band_row(a, xl).tok;
+  W.init(first, last, a.W, a.S);
 
   BandStage<D> stk, stv;
   stk.init(lane, a.dk_, a.ks[2]);
@@ -136,6 +137,11 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
         ring[k % 2] = flashd_read_tr<D, 32 * kb>(sK, L, j - N1);
       }
     };
+    BandEdge edge[NP];
+    if constexpr (MASK) {
+#pragma unroll
+      for (int p = 0; p < NP; p++) edge[p] = band_edge(hi[p], lo[p], a.S, x, g);
+    }
     rd(std::integral_constant<int, 0>{});
     swa2_for<0, NKB>([&](auto kbc) __attribute__((always_inline)) {
       constexpr int kb = decltype(kbc)::value;
@@ -161,8 +167,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
               for (int i = 0; i < 4; i++) {
                 float v = fast_exp2(fmaf(sv[p][i], scale, nlse[p])) * dp[p][i];
                 if constexpr (MASK) {
-                  const int j_ = x + 32 * kb + 16 * mb + 4 * g + i;
-                  v = j_ <= hi[p] && (j_ > lo[p] || j_ < a.S) ? v : 0.f;
+                  v = band_formed(v);
+                  v = band_edge_sees(edge[p], 32 * kb + 16 * mb + i) ? v : 0.f;
                 }
                 ds[p][4 * mb + i] = v;
               }
@@ -178,28 +184,35 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
       });
     });
   };
-  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
-    const int x = W.x(i), xe = x + CK - 1;
-    if (x > pb || (xe <= pa - a.W && x >= a.S)) return;
-    if (xe <= pa && (x > pb - a.W || xe < a.S)) consume(x, (Swa2Lds)buf, std::false_type{});
-    else consume(x, (Swa2Lds)buf, std::true_type{});
+  auto chunk = [&](int i, char* buf, auto mask_tag) __attribute__((always_inline)) {
+    const int x = W.x(i);
+    if (decltype(mask_tag)::value && (x > pb || (x + CK - 1 <= pa - a.W && x >= a.S))) return;
+    consume(x, (Swa2Lds)buf, mask_tag);
   };
-  int bi = 0, i = 0;
+  int f0, f1;
+  W.whole(first, last, a.W, 0, W.n, f0, f1);
+  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
+  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
+  int bi = 0, i = 0, stop = f0;
   auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
-#pragma unroll 1
-  for (; i + AHEAD < W.n; i++) {
-    issue(i + AHEAD, buf_of(bi + AHEAD));
-    chunk(i, buf_of(bi));
-    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
-    __syncthreads();
+  auto step = [&](auto mask_tag) __attribute__((always_inline)) {
+    const bool more = i + AHEAD < W.n;
+    if (more) issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi), mask_tag);
+    if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    else swa2_wait_copies();
     bi = bi + 1 == NBUF ? 0 : bi + 1;
-  }
-#pragma unroll 1
-  for (; i < W.n; i++) {
-    chunk(i, buf_of(bi));
-    swa2_wait_copies();
+    i++;
     __syncthreads();
-    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  };
+#pragma unroll 1
+  for (;;) {
+#pragma unroll 1
+    while (i < stop) step(std::true_type{});
+    if (i >= W.n) break;
+#pragma unroll 1
+    while (i < f1) step(std::false_type{});
+    stop = W.n;
   }
   __syncthreads();
   float mul[NP];
@@ -337,11 +350,10 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
     band_load_own<KC>(kf[p], kh + (on ? xk : 0) * a.ks[2], on, a.dk_, g);
     band_load_own<KC>(vf[p], vh + (on ? xk : 0) * a.vs[2], on, a.dv_, g);
   }
-  // rows that see some key of the wave: [wlo, whi); rows that see all of them: [flo, fhi)
+  // rows that see some key of the wave: [wlo, whi)
   const int wk1 = dlt_imin(wk0 + 16 * NP, xe) - 1;
   const bool wave_on = wk1 >= wk0;
   const int wlo = wave_on ? rlo_of(wk0) : 0, whi = !wave_on ? 0 : wk0 < a.S ? r_end : rhi_of(wk1);
-  const int flo = wave_on ? rlo_of(wk1) : 0, fhi = !wave_on ? 0 : wk0 >= a.S ? rhi_of(wk0) : wk1 < a.S ? r_end : rhi_of(a.S);
 
   f32x4 dk_acc[NP][KB], dv_acc[NP][KB];
 #pragma unroll
@@ -386,6 +398,13 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
         else ring[k % 2] = flashd_read_tr<D, 32 * qb_>(sQ, L, d - KB);
       }
     };
+    int elo[NP], ehi[NP];   // row 16 hh + 4 g + i of the chunk is seen iff elo <= 16 hh + i < ehi (see band_edge)
+    if constexpr (MASK) {
+      int at = q0 + 4 * g;
+      asm volatile("" : "+v"(at));
+#pragma unroll
+      for (int p = 0; p < NP; p++) { elo[p] = rlo[p] - at; ehi[p] = rhi[p] - at; }
+    }
     rd(std::integral_constant<int, 0>{});
     f32x4 sv[2][NP], dp[2][NP], lq[2], dl[2];   // by the parity of the half
     dl[0] = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
@@ -400,8 +419,9 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
         float pv = fast_exp2(fmaf(sv[hh & 1][p][i], scale, -lq[hh & 1][i]));
         float dv = -pv * dp[hh & 1][p][i];
         if constexpr (MASK) {
-          const int r = q0 + 16 * hh + 4 * g + i;
-          const bool sees = r >= rlo[p] && r < rhi[p];
+          const bool sees = 16 * hh + i >= elo[p] && 16 * hh + i < ehi[p];
+          pv = band_formed(pv);
+          dv = band_formed(dv);
           pv = sees ? pv : 0.f;
           dv = sees ? dv : 0.f;
         }
@@ -492,32 +512,44 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
       }
     }
   };
-  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
+  struct Far {};
+  auto chunk = [&](int i, char* buf, auto tag) __attribute__((always_inline)) {
     const int q0 = r_beg + i * CK;
-    if (far) {
-      consume_far(q0, (Swa2Lds)buf);
-      return;
+    if constexpr (std::is_same<decltype(tag), Far>::value) consume_far(q0, (Swa2Lds)buf);
+    else {
+      if (decltype(tag)::value && (q0 >= whi || q0 + CK <= wlo)) return;
+      consume(q0, (Swa2Lds)buf, tag);
     }
-    if (q0 >= whi || q0 + CK <= wlo) return;
-    if (q0 >= flo && q0 + CK <= fhi) consume(q0, (Swa2Lds)buf, std::false_type{});
-    else consume(q0, (Swa2Lds)buf, std::true_type{});
   };
-  int bi = 0, i = i_beg;
+  // chunks whose rows see all keys of the workgroup: rows [rlo of the last key, rhi of the first one without sinks)
+  const int all_lo = rlo_of(xe - 1), all_hi = x0 >= a.S ? rhi_of(x0) : xe <= a.S ? r_end : rhi_of(a.S);
+  const int f0 = dlt_imin(dlt_imax(i_beg, (all_lo - r_beg + CK - 1) / CK), i_end), f1 = dlt_imax(f0, dlt_imin(i_end, all_hi > r_beg ? (all_hi - r_beg) / CK : 0));
+  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
+  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
+  int bi = 0, i = i_beg, stop = f0;
   auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF_KV; };
-#pragma unroll 1
-  for (; i + AHEAD < i_end; i++) {
-    issue(i + AHEAD, buf_of(bi + AHEAD));
-    chunk(i, buf_of(bi));
-    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
-    __syncthreads();
+  auto step = [&](auto mask_tag) __attribute__((always_inline)) {
+    const bool more = i + AHEAD < i_end;
+    if (more) issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi), mask_tag);
+    if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    else swa2_wait_copies();
     bi = bi + 1 == NBUF ? 0 : bi + 1;
+    i++;
+    __syncthreads();
+  };
+  if (far) {
+#pragma unroll 1
+    while (i < i_end) step(Far{});
   }
 #pragma unroll 1
-  for (; i < i_end; i++) {
-    chunk(i, buf_of(bi));
-    swa2_wait_copies();
-    __syncthreads();
-    bi = bi + 1 == NBUF ? 0 : bi + 1;
+  for (;;) {
+#pragma unroll 1
+    while (i < stop) step(std::true_type{});
+    if (i >= i_end) break;
+#pragma unroll 1
+    while (i < f1) step(std::false_type{});
+    stop = i_end;
   }
   __syncthreads();
 

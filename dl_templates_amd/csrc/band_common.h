@@ -78,6 +78,13 @@ struct BandWalk {
     n = ns + last / CK + 1 - c0;
   }
   DLT_DEV int x(int i) const { return CK * (i < ns ? i : c0 + i - ns); }
+  // of chunks [beg, end) those that every one of the rows sees whole (chunks of sinks not counted): [f0, f1)
+  DLT_DEV void whole(int first, int last, int W, int beg, int end, int& f0, int& f1) const {
+    const int lo = last >= W ? (last - W) / CK + 1 : 0;       // first chunk behind the last row's window start
+    const int hi = first >= 0 ? (first + 1) / CK : 0;         // first chunk that ends behind the first row
+    f0 = dlt_imin(dlt_imax(beg, ns + dlt_imax(lo - c0, 0)), end);
+    f1 = dlt_imax(f0, dlt_imin(end, ns + hi - c0));
+  }
 };
 
 // Own rows as B operands: lane (n, g) holds head dims 32 c + 8 g .. + 7 of row n; r < 0: no row
@@ -215,6 +222,31 @@ DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {
     for (int i = 0; i < 4; i++) odd = odd || band_odd(acc[p][d][i]);
   return odd;
 }
+
+// maximum of three scores.  fmaxf would first multiply every operand by 1 (to quiet signalling NaNs), one vector instruction in eight of the forward loop
+DLT_DEV float band_max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+// Hidden pairs of a chunk at the edge.  Key x + 4 g + c of own row p (c a constant of the unrolled code) is seen iff c <= h && (c > l || c < s).  The
+// bounds are formed here, per chunk, from a value the compiler cannot look through: left to itself it keeps one register for each c, in kernels that have none left.
+struct BandEdge { int h, l, s; };
+DLT_DEV BandEdge band_edge(int hi, int lo, int S, int x, int g) {
+  int at = x + 4 * g;
+  asm volatile("" : "+v"(at));
+  return BandEdge{hi - at, lo - at, S - at};
+}
+DLT_DEV bool band_edge_sees(const BandEdge& e, int c) { return c <= e.h && (c > e.l || c < e.s); }
+// a value formed for every lane, hidden pairs too (where it is an exponential the compiler would otherwise branch around it)
+DLT_DEV float band_formed(float v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+#ifndef BAND_RD
+#define BAND_RD 1
+#endif
 
 // ---- rows whose sums came out infinite or NaN ------------------------------------------------------------------------------------
 // The matrix products of a chunk at the edge of a window multiply hidden pairs by 0, and 0 times an infinity or a NaN is NaN: a hidden key

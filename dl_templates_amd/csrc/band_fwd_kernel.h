@@ -97,7 +97,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   // chunks of the block and of this share of it
   BandWalk<CK> W;
   const int xl = dlt_imin(x0 + OWN, n_rows) - 1;
-  W.init(sq.off + band_row(a, x0).tok, xl >= x0 ? dlt_imin(sq.off + band_row(a, dlt_imax(xl, 0)).tok, sq.n_k - 1) : -1, a.W, a.S);
+  const int first = sq.off + band_row(a, x0).tok, last = xl >= x0 ? dlt_imin(sq.off + band_row(a, dlt_imax(xl, 0)).tok, sq.n_k - 1) : -1;
+  W.init(first, last, a.W, a.S);
   const int per = (W.n + a.shares - 1) / a.shares;
   const int i_beg = dlt_imin(share * per, W.n), i_end = dlt_imin(i_beg + per, W.n);
 
@@ -194,26 +195,32 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1 = NKB * 2 * KC, NT = N1 + NKB * VB;
-    u32x4 ring[2];
+    constexpr int RD = BAND_RD;
+    u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
       if constexpr (k < N1) {
         constexpr int kb = k / (2 * KC), mb = (k / KC) % 2, r = k % KC;
-        ring[k % 2] = swa2_lds16(sK + (32 * kb + 16 * mb) * FlashDRow<D>::ROW + L.a[r]);
+        ring[k % (RD + 1)] = swa2_lds16(sK + (32 * kb + 16 * mb) * FlashDRow<D>::ROW + L.a[r]);
       } else {
         constexpr int kb = (k - N1) / VB, d = (k - N1) % VB;
-        ring[k % 2] = flashd_read_tr<D, 32 * kb>(sV, L, d);
+        ring[k % (RD + 1)] = flashd_read_tr<D, 32 * kb>(sV, L, d);
       }
     };
-    rd(std::integral_constant<int, 0>{});
+    swa2_for<0, RD>([&](auto kc) __attribute__((always_inline)) { rd(kc); });
+    BandEdge edge[NP];
+    if constexpr (MASK) {
+#pragma unroll
+      for (int p = 0; p < NP; p++) edge[p] = band_edge(hi[p], lo[p], a.S, x, g);
+    }
     float t[NP][NKB][8];
     u32x4 pb_[NP][NKB];
     f32x4 s[NP];
     swa2_for<0, NT>([&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
-      if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+      if constexpr (k + RD < NT) rd(std::integral_constant<int, k + RD>{});
       __builtin_amdgcn_sched_barrier(0);
-      const u32x4 op = ring[k % 2];
+      const u32x4 op = ring[k % (RD + 1)];
       if constexpr (k < N1) {
         constexpr int kb = k / (2 * KC), mb = (k / KC) % 2, r = k % KC;
 #pragma unroll
@@ -224,22 +231,21 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
 #pragma unroll
             for (int i = 0; i < 4; i++) {
               float v = s[p][i];
-              if constexpr (MASK) {
-                const int j = x + 32 * kb + 16 * mb + 4 * g + i;
-                v = j <= hi[p] && (j > lo[p] || j < a.S) ? v : -INFINITY;
-              }
+              if constexpr (MASK) v = band_edge_sees(edge[p], 32 * kb + 16 * mb + i) ? v : -INFINITY;
               t[p][kb][4 * mb + i] = v;
             }
         }
         if constexpr (k == N1 - 1) {
 #pragma unroll
           for (int p = 0; p < NP; p++) {
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx[4];
 #pragma unroll
-            for (int kb2 = 0; kb2 < NKB; kb2++)
+            for (int i = 0; i < 4; i++) mx[i] = band_max3(t[p][0][2 * i], t[p][0][2 * i + 1], t[p][0][2 * i]);
 #pragma unroll
-              for (int i = 0; i < 4; i++) mx[i] = fmaxf(fmaxf(mx[i], t[p][kb2][2 * i]), t[p][kb2][2 * i + 1]);
-            const float mloc = wave_max4(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            for (int kb2 = 1; kb2 < NKB; kb2++)
+#pragma unroll
+              for (int i = 0; i < 4; i++) mx[i] = band_max3(mx[i], t[p][kb2][2 * i], t[p][kb2][2 * i + 1]);
+            const float mloc = wave_max4(band_max3(band_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
             // the reference maximum moves only when a score exceeds it by more than 2^8 after scaling: P stays below 2^8, its sum in
             // 32 bits below 2^8 times the keys
             if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > 8.f)) {
@@ -272,31 +278,36 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
       }
     });
   };
-  auto chunk = [&](int i, char* buf) __attribute__((always_inline)) {
-    const int x = W.x(i), xe = x + CK - 1;
-    if (x > pb || (xe <= pa - a.W && x >= a.S)) return;                       // no row of the wave sees any of it
-    if (xe <= pa && (x > pb - a.W || xe < a.S)) consume(x, (Swa2Lds)buf, std::false_type{});
-    else consume(x, (Swa2Lds)buf, std::true_type{});
+  auto chunk = [&](int i, char* buf, auto mask_tag) __attribute__((always_inline)) {
+    const int x = W.x(i);
+    if (decltype(mask_tag)::value && (x > pb || (x + CK - 1 <= pa - a.W && x >= a.S))) return;   // no row of the wave sees any of it
+    consume(x, (Swa2Lds)buf, mask_tag);
   };
-  int bi = 0;
+  int f0, f1;
+  W.whole(first, last, a.W, i_beg, i_end, f0, f1);
+  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
+  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
+  int bi = 0, i = i_beg, stop = f0;
   auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
-  int i = i_beg;
-#pragma unroll 1
-  for (; i + AHEAD < i_end; i++) {
-    issue(i + AHEAD, buf_of(bi + AHEAD));
-    chunk(i, buf_of(bi));
-    flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+  auto step = [&](auto mask_tag) __attribute__((always_inline)) {
+    const bool more = i + AHEAD < i_end;
+    if (more) issue(i + AHEAD, buf_of(bi + AHEAD));
+    chunk(i, buf_of(bi), mask_tag);
+    if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
+    else swa2_wait_copies();
     bi = bi + 1 == NBUF ? 0 : bi + 1;
-    settle(i + 1, buf_of(bi));
+    i++;
+    if (i < i_end) settle(i, buf_of(bi));
     __syncthreads();
-  }
+  };
 #pragma unroll 1
-  for (; i < i_end; i++) {
-    chunk(i, buf_of(bi));
-    swa2_wait_copies();
-    bi = bi + 1 == NBUF ? 0 : bi + 1;
-    if (i + 1 < i_end) settle(i + 1, buf_of(bi));
-    __syncthreads();
+  for (;;) {
+#pragma unroll 1
+    while (i < stop) step(std::true_type{});
+    if (i >= i_end) break;
+#pragma unroll 1
+    while (i < f1) step(std::false_type{});
+    stop = i_end;
   }
 
   // ---- epilogue
