@@ -8,39 +8,67 @@
 namespace {
 
 // ---- sums of shares -------------------------------------------------------------------------------------------------------------
-// Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row.  A thread takes 4 dims of a row and the shares
-// in their order.
+// Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row.  A workgroup joins one row: every wave forms the
+// weights of all shares (a lane each), then adds up every fourth share, and the four sums are added in their order.  (One thread per 4 dims walking all shares:
+// 36 us for 96 rows of 64 shares; this way JOINTIME.)
 template <typename TIO>
 __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
-  const int per = a.dv_ / 4;
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t at = gid / per;
-  const int d = 4 * (int)(gid - at * per);
-  if (at >= (int64_t)a.B * a.Hkv * a.rows) return;
+  __shared__ float sum[4][128];
+  const int64_t at = blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int bh = (int)(at / a.rows), r = (int)(at - (int64_t)bh * a.rows), b = bh / a.Hkv, h = bh - b * a.Hkv;
   const int n_q = a.pg.n_new != nullptr ? dlt_imax(0, dlt_imin(a.pg.n_new[b], a.Lq)) : a.Lq;
-  const float* ml = a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_;
+  const bool on = r < n_q * a.G;   // the others have no partial results
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_) + (int64_t)bh * a.shares * a.rows + r;
+  float2 x[BAND_SHARES_MAX / 64];
   float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  if (r < n_q * a.G)
-    for (int s = 0; s < a.shares; s++) {
-      const int64_t row = ((int64_t)bh * a.shares + s) * a.rows + r;
-      const float2 x = *reinterpret_cast<const float2*>(ml + 2 * row);
-      if (x.x == -INFINITY && x.y == 0.f) continue;   // the share held no key of the row
-      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + row * a.dv_ + d);
-      float f1, f2;
-      flash_merge(m, x.x, 1.f, f1, f2);
-      l = flash_add(l, f1, x.y, f2);
 #pragma unroll
-      for (int i = 0; i < 4; i++) o[i] = flash_add(o[i], f1, v[i], f2);
+  for (int i = 0; i < BAND_SHARES_MAX / 64; i++) {
+    const int s = 64 * i + lane;
+    x[i] = on && s < a.shares ? ml[(int64_t)s * a.rows] : float2{-INFINITY, 0.f};
+    m = fmaxf(m, x[i].x);
+  }
+  m = band_wave_max(m);
+  float wgt[BAND_SHARES_MAX / 64];
+#pragma unroll
+  for (int i = 0; i < BAND_SHARES_MAX / 64; i++) {
+    // a share that held no key of the row has (-inf, 0); a sum that is infinite or NaN goes through
+    wgt[i] = x[i].x == -INFINITY ? (x[i].y == 0.f ? 0.f : 1.f) : fast_exp2(x[i].x - m);
+    l = fmaf(x[i].y, wgt[i], l);
+  }
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k);
+  float o[2] = {0.f, 0.f};
+  if (on && 2 * lane < a.dv_) {
+    const float* part = a.part + ((int64_t)bh * a.shares * a.rows + r) * a.dv_ + 2 * lane;
+    static_assert(BAND_SHARES_MAX == 128, "two weights a lane");
+    for (int s0 = wave; s0 < a.shares; s0 += 32) {
+      float2 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = *reinterpret_cast<const float2*>(part + (int64_t)dlt_imin(s0 + 4 * u, a.shares - 1) * a.rows * a.dv_);
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const int s = s0 + 4 * u;
+        const float f = s < 64 ? band_lane(wgt[0], s) : band_lane(wgt[1], s - 64);
+        if (s < a.shares && f != 0.f) {
+          o[0] = fmaf(v[u].x, f, o[0]);
+          o[1] = fmaf(v[u].y, f, o[1]);
+        }
+      }
     }
+  }
+  if (2 * lane < 128) { sum[wave][2 * lane] = o[0]; sum[wave][2 * lane + 1] = o[1]; }
+  __syncthreads();
+  if (wave != 0) return;
   const float f = l == 0.f ? 0.f : 1.f / l;
-  TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r) + d;
-  u32x2 w;
-  w.x = pack2<TIO>(o[0] * f, o[1] * f);
-  w.y = pack2<TIO>(o[2] * f, o[3] * f);
-  store_stream8(p, w);
-  if (d == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
+  TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r);
+  if (2 * lane < a.dv_) {
+    float y[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) y[j] = ((sum[0][2 * lane + j] + sum[1][2 * lane + j]) + sum[2][2 * lane + j]) + sum[3][2 * lane + j];
+    *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(y[0] * f, y[1] * f);
+  }
+  if (lane == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
 // dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares
@@ -73,8 +101,8 @@ __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
 int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
   if (backward ? a.part_keys == 0 : a.shares <= 1) return DLT_OK;
   const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.part_keys : a.rows);
-  const int per = (backward ? dlt_imax(a.dk_, a.dv_) : a.dv_) / 4;
-  const dim3 grid((unsigned)((rows * per + 255) / 256), backward ? 2 : 1);
+  const int per = dlt_imax(a.dk_, a.dv_) / 4;
+  const dim3 grid((unsigned)(backward ? (rows * per + 255) / 256 : rows), backward ? 2 : 1);
   dlt_timing_before(backward ? DLT_K_BWD_KV : DLT_K_FWD, stream);
   if (backward) {
     if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kv_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
@@ -168,14 +196,14 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
 int plan_rows(BandArgs& a, bool shares) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv;
-  int np = bh * ((a.rows + 127) / 128) < 2 * cus ? 1 : 2;
+  const int np = a.rows <= 64 || bh * ((a.rows + 127) / 128) < 2 * cus ? 1 : 2;
   a.nblk = (a.rows + 64 * np - 1) / (64 * np);
   a.shares = 1;
   if (shares) {
     const int64_t wgs = bh * a.nblk;
     const int most = (int)dlt_imin64((int64_t)a.W + a.S + 64 * np / a.G + 1, a.Lk) / 64 + 1;   // chunks of a block
     int64_t n = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
-    n = dlt_imin64(n, most / 4);
+    n = dlt_imin64(dlt_imin64(n, most / 4), BAND_SHARES_MAX);
     const int64_t row_bytes = bh * a.rows * (a.dv_ + 2) * 4;
     n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(row_bytes > 0 ? row_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
     a.shares = n < 1 ? 1 : (int)n;

@@ -13,6 +13,7 @@ int dlt_band_bwd_q_64(const BandArgs& a, int dtype, int np, hipStream_t stream);
 int dlt_band_bwd_q_128(const BandArgs& a, int dtype, int np, hipStream_t stream);
 int dlt_band_bwd_kv_64(const BandArgs& a, int dtype, hipStream_t stream);
 int dlt_band_bwd_kv_128(const BandArgs& a, int dtype, hipStream_t stream);
+constexpr int BAND_SHARES_MAX = 128;   // workgroups that share the keys of a block of rows (forward)
 // keys of a workgroup of the dK / dV kernel
 constexpr int band_kv_own(int d) { return d <= 64 ? 128 : 64; }
 // ... and of one of its workgroups for far rows

@@ -16,32 +16,15 @@ struct RopeAxes {
   int32_t n, pairs, halves, inverse;
 };
 
-// axis of pair i, and the first pair of that axis
-DLT_HD int rope_axes_axis(const RopeAxes& r, int i, int& off) {
+// axis of pair i, the first pair of that axis, and how many it has
+DLT_HD int rope_axes_axis(const RopeAxes& r, int i, int& off, int& R) {
   int a = 0;
   off = 0;
+  R = r.end[0];
 #pragma unroll
   for (int k = 0; k + 1 < DLT_ROPE_AXES_MAX; k++)
-    if (k + 1 < r.n && i >= r.end[k]) { a = k + 1; off = r.end[k]; }
+    if (k + 1 < r.n && i >= r.end[k]) { a = k + 1; off = r.end[k]; R = r.end[k + 1] - off; }
   return a;
-}
-// dim d < 2 P -> its pair, whether it is the pair's first dim, and the other dim
-DLT_HD int rope_axes_pair(const RopeAxes& r, int d, bool& first, int& other) {
-  if (r.halves) {
-    first = d < r.pairs;
-    other = first ? d + r.pairs : d - r.pairs;
-    return first ? d : d - r.pairs;
-  }
-  int off;
-  const int a = rope_axes_axis(r, d >> 1, off);   // 2 off_a <= d < 2 end_a
-  int R = 0;
-#pragma unroll
-  for (int k = 0; k < DLT_ROPE_AXES_MAX; k++)
-    if (k == a) R = r.end[k] - off;
-  const int i = d - 2 * off;
-  first = i < R;
-  other = first ? d + R : d - R;
-  return off + (first ? i : i - R);
 }
 
 // One call of the kernels in rope_axes.hip: rows of up to three tensors, token by token
