@@ -125,16 +125,17 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1H = 2 * KC, N1 = 2 * N1H, NB = N1 + KB, NT = NKB * NB;
-    u32x4 ring[2];
+    constexpr int RD = BAND_RD_Q;
+    u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
       constexpr int kb = k / NB, j = k % NB;
       if constexpr (j < N1) {
         constexpr int mb = j / N1H, r = j % N1H, T0 = 32 * kb + 16 * mb;
-        if constexpr (r < KC) ring[k % 2] = swa2_lds16(sK + T0 * FlashDRow<D>::ROW + L.a[r]);
-        else ring[k % 2] = swa2_lds16(sV + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
+        if constexpr (r < KC) ring[k % (RD + 1)] = swa2_lds16(sK + T0 * FlashDRow<D>::ROW + L.a[r]);
+        else ring[k % (RD + 1)] = swa2_lds16(sV + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
       } else {
-        ring[k % 2] = flashd_read_tr<D, 32 * kb>(sK, L, j - N1);
+        ring[k % (RD + 1)] = flashd_read_tr<D, 32 * kb>(sK, L, j - N1);
       }
     };
     BandEdge edge[NP];
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 #pragma unroll
       for (int p = 0; p < NP; p++) edge[p] = band_edge(hi[p], lo[p], a.S, x, g);
     }
-    rd(std::integral_constant<int, 0>{});
+    swa2_for<0, RD>([&](auto kc) __attribute__((always_inline)) { rd(kc); });
     swa2_for<0, NKB>([&](auto kbc) __attribute__((always_inline)) {
       constexpr int kb = decltype(kbc)::value;
       float ds[NP][8];
@@ -150,9 +151,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
       u32x4 dsb[NP];
       swa2_for<0, NB>([&](auto jc) __attribute__((always_inline)) {
         constexpr int j = decltype(jc)::value, k = kb * NB + j;
-        if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+        if constexpr (k + RD < NT) rd(std::integral_constant<int, k + RD>{});
         __builtin_amdgcn_sched_barrier(0);
-        const u32x4 op = ring[k % 2];
+        const u32x4 op = ring[k % (RD + 1)];
         if constexpr (j < N1) {
           constexpr int mb = j / N1H, r = j % N1H;
 #pragma unroll
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 // d = 128: 876 us with the far rows in the block, FARTIME with 22 shares of them beside it.
 // ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
 template <typename TIO, int D, int NP, int CK, int NW, int PAD>
-__global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs a) {
+__global__ __launch_bounds__(64 * NW, NP * D > 128 ? 1 : 2) void band_bwd_kv_kernel(const BandArgs a) {
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
@@ -277,13 +278,14 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
   const int lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
-  const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  const int n_far = a.far * a.far_groups, far_lin = lin - ((int)gridDim.x - a.B * a.Hkv * n_far);
-  const bool far = far_lin >= 0;
+  // far workgroups are launched first: behind the others, which fill the chip in whole rounds, they would be a tail of their own
+  const int n_far = a.far * a.far_groups, all_far = a.B * a.Hkv * n_far;
+  const bool far = (int)blockIdx.x < all_far;
+  const int lin = far ? xcd_remap(blockIdx.x, all_far) : xcd_remap((int)blockIdx.x - all_far, (int)gridDim.x - all_far);
   int bh, share, x0;
   if (far) {
-    bh = far_lin / n_far;
-    const int rest = far_lin - bh * n_far, grp = rest / a.far;
+    bh = lin / n_far;
+    const int rest = lin - bh * n_far, grp = rest / a.far;
     share = rest - grp * a.far;
     x0 = grp * 16 * NP;
   } else {
@@ -385,17 +387,18 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
     constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NP2 = 2 * KB, NT = N1 + NQB * NP2;
     constexpr int NU = 2 * NP;
     static_assert(NP2 >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
-    u32x4 ring[2];
+    constexpr int RD = BAND_RD_KV;
+    u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
       if constexpr (k < N1) {
         constexpr int hh = k / N1H, r = k % N1H, T0 = 16 * hh;
-        if constexpr (r < KC) ring[k % 2] = swa2_lds16(sQ + T0 * FlashDRow<D>::ROW + L.a[r]);
-        else ring[k % 2] = swa2_lds16(sDO + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
+        if constexpr (r < KC) ring[k % (RD + 1)] = swa2_lds16(sQ + T0 * FlashDRow<D>::ROW + L.a[r]);
+        else ring[k % (RD + 1)] = swa2_lds16(sDO + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
       } else {
         constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
-        if constexpr (d < KB) ring[k % 2] = flashd_read_tr<D, 32 * qb_>(sDO, L, d);
-        else ring[k % 2] = flashd_read_tr<D, 32 * qb_>(sQ, L, d - KB);
+        if constexpr (d < KB) ring[k % (RD + 1)] = flashd_read_tr<D, 32 * qb_>(sDO, L, d);
+        else ring[k % (RD + 1)] = flashd_read_tr<D, 32 * qb_>(sQ, L, d - KB);
       }
     };
     int elo[NP], ehi[NP];   // row 16 hh + 4 g + i of the chunk is seen iff elo <= 16 hh + i < ehi (see band_edge)
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
 #pragma unroll
       for (int p = 0; p < NP; p++) { elo[p] = rlo[p] - at; ehi[p] = rhi[p] - at; }
     }
-    rd(std::integral_constant<int, 0>{});
+    swa2_for<0, RD>([&](auto kc) __attribute__((always_inline)) { rd(kc); });
     f32x4 sv[2][NP], dp[2][NP], lq[2], dl[2];   // by the parity of the half
     dl[0] = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
     u32x4 pb[NQB][NP], dsb[NQB][NP];
@@ -436,7 +439,7 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
     };
     swa2_for<0, NT>([&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
-      if constexpr (k + 1 < NT) rd(std::integral_constant<int, k + 1>{});
+      if constexpr (k + RD < NT) rd(std::integral_constant<int, k + RD>{});
       if constexpr (k < N1 && k % N1H == 0) {
         constexpr int hh = k / N1H;
         lq[hh & 1] = __builtin_bit_cast(f32x4, swa2_lds16(sLse + 16 * hh * 4));
@@ -446,7 +449,7 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
         dl[hn & 1] = __builtin_bit_cast(f32x4, swa2_lds16(sDel + 16 * hn * 4));
       }
       __builtin_amdgcn_sched_barrier(0);
-      const u32x4 op = ring[k % 2];
+      const u32x4 op = ring[k % (RD + 1)];
       if constexpr (k < N1) {
         constexpr int hh = k / N1H, r = k % N1H;
 #pragma unroll

@@ -247,6 +247,12 @@ DLT_DEV float band_formed(float v) {
 #ifndef BAND_RD
 #define BAND_RD 1
 #endif
+#ifndef BAND_RD_Q
+#define BAND_RD_Q 1
+#endif
+#ifndef BAND_RD_KV
+#define BAND_RD_KV 3
+#endif
 
 // ---- rows whose sums came out infinite or NaN ------------------------------------------------------------------------------------
 // The matrix products of a chunk at the edge of a window multiply hidden pairs by 0, and 0 times an infinity or a NaN is NaN: a hidden key

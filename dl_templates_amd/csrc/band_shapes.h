@@ -15,6 +15,9 @@ int dlt_band_bwd_kv_64(const BandArgs& a, int dtype, hipStream_t stream);
 int dlt_band_bwd_kv_128(const BandArgs& a, int dtype, hipStream_t stream);
 constexpr int BAND_SHARES_MAX = 128;   // workgroups that share the keys of a block of rows (forward)
 // keys of a workgroup of the dK / dV kernel
-constexpr int band_kv_own(int d) { return d <= 64 ? 128 : 64; }
+#ifndef BAND_KV128
+#define BAND_KV128 64
+#endif
+constexpr int band_kv_own(int d) { return d <= 64 ? 128 : BAND_KV128; }
 // ... and of one of its workgroups for far rows
 constexpr int band_kv_group(int d) { return band_kv_own(d) / 4; }
