@@ -14,7 +14,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, KB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
-  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;
   static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
   constexpr int PER_CHUNK = 2 * NG * BandStage<D>::NI;
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1H = 2 * KC, N1 = 2 * N1H, NB = N1 + KB, NT = NKB * NB;
-    constexpr int RD = BAND_RD_Q;
+    constexpr int RD = NP == 1 ? BAND_RD1 : 1;
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(64 * NW, NP * D > 128 ? 1 : 2) void band_bwd_kv_ker
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
-  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;
   static_assert(NG >= 1 && NG * NW * 16 == CK && CK == 64, "whole groups of 16 rows per wave; one copy of scalars a chunk");
   constexpr int PER_CHUNK = 2 * NG * BandStageRows<D>::NI;   // waves 0 and 1: one more

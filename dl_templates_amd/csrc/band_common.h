@@ -97,14 +97,47 @@ DLT_DEV void band_load_own(u32x4 (&f)[KC], const TIO* row, bool on, int dims, in
   }
 }
 
+// Copies of 16 bytes a lane to `lds` + OA, + OB (and + OC, + OD) + 16 lane, as dlt_copy16_to_lds (swa2_common.hpp) with one set-up of M0 for all: the offset field of
+// the instruction counts for the memory address too, so `voff` of a copy is its lane's offset less that.  (A set-up for each copy was a sixth of a
+// chunk's instructions.)
+template <int OA, int OB>
+DLT_DEV void band_copy2(const char* base, uint32_t va, uint32_t vb, char* lds) {
+  const uint32_t m = (uint32_t)(uintptr_t)(DLT_LDS char*)lds;
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1 offset:%5\n\tglobal_load_lds_dwordx4 %3, %1 offset:%6\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved) : "s"(base), "v"(va), "v"(vb), "s"(m), "n"(OA), "n"(OB) : "memory");
+}
+DLT_DEV void band_copy4(const char* base, const uint32_t (&v)[4], char* lds) {
+  const uint32_t m = (uint32_t)(uintptr_t)(DLT_LDS char*)lds;
+  uint32_t saved;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024\n\t"
+               "global_load_lds_dwordx4 %4, %1 offset:2048\n\tglobal_load_lds_dwordx4 %5, %1 offset:3072\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved) : "s"(base), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(m) : "memory");
+}
+// All copies of a group of 16 tokens: copy i goes to `lds` + 1024 i; v[i] = the lane's offset + band_bias - 1024 i, taken from base - band_bias.  Under PAD lanes of pieces that
+// do not exist copy nothing; copies two apart move the same piece (8 tokens apart).
+template <int NI> constexpr int band_bias = 1024 * (NI - 1);
+template <int NI, int PAD>
+DLT_DEV void band_copy_group(const char* base, const uint32_t (&v)[NI], bool on0, bool on1, char* lds) {
+  static_assert(NI == 2 || NI == 4, "head dim 64 or 128");
+  const char* b = base - band_bias<NI>;
+  if constexpr (NI == 2) {
+    if (!PAD || on0) band_copy2<0, 1024>(b, v[0], v[1], lds);
+  } else if constexpr (!PAD) {
+    band_copy4(b, v, lds);
+  } else {
+    if (on0) band_copy2<0, 2048>(b, v[0], v[2], lds);
+    if (on1) band_copy2<1024, 3072>(b, v[1], v[3], lds);
+  }
+}
+
 // Copies of keys or values HBM -> LDS, 16 tokens at a time (one wave): token t of the group, piece c of its row lies at piece
 // c ^ swz(t) (FlashDRow).  The place of the group is wave-uniform, a lane's offset inside it is kept in registers.
 template <int D>
 struct BandStage {
   typedef FlashDRow<D> R;
   static constexpr int NI = 16 / R::TPI;                    // copy instructions per 16 tokens
-  static constexpr int NOFF = R::TPI >= 8 ? 1 : 8 / R::TPI; // instructions NOFF apart: 8 tokens apart, same swizzle
-  uint32_t off[NOFF];
+  uint32_t off[NI];
   int t0, lp, npieces;
   uint32_t sn2;
   DLT_DEV uint32_t piece(int i) const { return (uint32_t)(lp ^ R::swz(t0 + R::TPI * i)); }
@@ -114,13 +147,11 @@ struct BandStage {
     npieces = dims >> 3;
     sn2 = (uint32_t)sn * 2u;
 #pragma unroll
-    for (int i = 0; i < NOFF; i++) off[i] = (uint32_t)(t0 + R::TPI * i) * sn2 + 16u * piece(i);
+    for (int i = 0; i < NI; i++) off[i] = (uint32_t)(t0 + R::TPI * i) * sn2 + 16u * piece(i) + (uint32_t)(band_bias<NI> - 1024 * i);
   }
   template <int PAD>
   DLT_DEV void issue(const char* base, char* dst) const {   // all 16 tokens are there
-#pragma unroll
-    for (int i = 0; i < NI; i++)
-      if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(base + (uint32_t)(i / NOFF * NOFF * R::TPI) * sn2, off[i % NOFF], dst + R::TPI * i * R::ROW);
+    band_copy_group<NI, PAD>(base, off, (int)piece(0) < npieces, (int)piece(1) < npieces, dst);
   }
   template <int PAD>
   DLT_DEV void issue_clamped(const char* base, int last, char* dst) const {   // tokens behind `last` repeat it
@@ -145,7 +176,7 @@ struct BandStageRows {
 #pragma unroll
     for (int i = 0; i < NI; i++) {
       const BandRow w = band_row(a, t0 + R::TPI * i);
-      off[i] = (uint32_t)(w.tok * (int)st[2] + w.head * (int)st[1]) * 2u + 16u * piece(i);
+      off[i] = (uint32_t)(w.tok * (int)st[2] + w.head * (int)st[1]) * 2u + 16u * piece(i) + (uint32_t)(band_bias<NI> - 1024 * i);
     }
   }
   // rows behind `last` repeat it
@@ -155,9 +186,7 @@ struct BandStageRows {
     const int tk = (int)dlt_fastdiv((uint32_t)f0, a.mG, a.sG);
     const char* b = base + (int64_t)tk * st[2] * 2;   // wave-uniform
     if (a.q16 != 0 && r0 + 15 <= last) {
-#pragma unroll
-      for (int i = 0; i < NI; i++)
-        if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(b, off[i], dst + R::TPI * i * R::ROW);
+      band_copy_group<NI, PAD>(b, off, (int)piece(0) < npieces, (int)piece(1) < npieces, dst);
     } else {
       keep_branch();
 #pragma unroll 1
@@ -177,6 +206,10 @@ struct BandBuf {
   static constexpr int BUF = 2 * REG;
   static constexpr int BUF_KV = 2 * REG + 2 * CK * 4;
 };
+
+// chunk buffers of a workgroup: as many as leave a CU two workgroups and more (one more at d = 128, with one block of rows per wave: 155 -> 186 us for the decode
+// step of 64 sequences, 18 -> 29 for 3 x 6 heads of 1111 tokens)
+constexpr int band_nbuf(int buf) { return 4 * buf <= 65536 ? 3 : 2; }
 
 // Accumulators in C layout (lane (n, g): dims 16 d + 4 g .. + 3 of own row n, times mul[p]) -> LDS tile of 16-bit values -> rows.
 // `ptr(row)`: the row's place or NULL.  The tile takes the chunk buffers' LDS.
@@ -244,11 +277,8 @@ DLT_DEV float band_formed(float v) {
   return v;
 }
 
-#ifndef BAND_RD
-#define BAND_RD 1
-#endif
-#ifndef BAND_RD_Q
-#define BAND_RD_Q 1
+#ifndef BAND_RD1
+#define BAND_RD1 1
 #endif
 #ifndef BAND_RD_KV
 #define BAND_RD_KV 3

@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, VB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
-  constexpr int NBUF = 4 * B::BUF <= 65536 ? 3 : 2, AHEAD = NBUF - 1;
+  constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;                              // groups of 16 tokens that a wave copies
   static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
   constexpr int PER_CHUNK = 2 * NG * BandStage<D>::NI;
@@ -195,7 +195,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1 = NKB * 2 * KC, NT = N1 + NKB * VB;
-    constexpr int RD = BAND_RD;
+    constexpr int RD = NP == 1 ? BAND_RD1 : 1;
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;

@@ -12,7 +12,6 @@
 
 namespace {
 constexpr int D = DLT_BAND_D;
-constexpr int band_bufs(int buf) { return 4 * buf <= 65536 ? 3 : 2; }
 constexpr int band_lds(int bufs, int rows) { return bufs > rows * (2 * D + 16) ? bufs : rows * (2 * D + 16); }
 
 template <typename KernT>
@@ -31,7 +30,7 @@ inline bool band_whole(const BandArgs& a) { return a.dk_ == D && a.dv_ == D; }
 template <typename TIO, int NP, int CK, int NW>
 int band_fwd(const BandArgs& a, hipStream_t stream) {
   constexpr bool PG = DLT_BAND_PART == 1;
-  constexpr int lds = band_lds(band_bufs(BandBuf<D, CK>::BUF) * BandBuf<D, CK>::BUF, 16 * NP * NW);
+  constexpr int lds = band_lds(band_nbuf(BandBuf<D, CK>::BUF) * BandBuf<D, CK>::BUF, 16 * NP * NW);
   return band_go(band_whole(a) ? band_fwd_kernel<TIO, D, NP, CK, NW, PG, 0> : band_fwd_kernel<TIO, D, NP, CK, NW, PG, 1>, a,
                  (int64_t)a.B * a.Hkv * a.nblk * a.shares, 64 * NW, lds, DLT_K_FWD, "window forward launch", stream);
 }
@@ -50,7 +49,7 @@ int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int np, 
 #elif DLT_BAND_PART == 2
 template <typename TIO, int NP>
 int band_bwd_q(const BandArgs& a, hipStream_t stream) {
-  constexpr int lds = band_lds(band_bufs(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
+  constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
   return band_go(band_whole(a) ? band_bwd_q_kernel<TIO, D, NP, 64, 4, 0> : band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>, a, (int64_t)a.B * a.Hkv * a.nblk, 256, lds,
                  DLT_K_BWD_Q, "window dQ launch", stream);
 }
@@ -64,7 +63,7 @@ int DLT_BCAT(dlt_band_bwd_q_, DLT_BAND_D)(const BandArgs& a, int dtype, int np, 
 template <typename TIO>
 int band_bwd_kv(const BandArgs& a, hipStream_t stream) {
   constexpr int NP = band_kv_own(D) / 64;
-  constexpr int lds = band_lds(band_bufs(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF_KV, 64 * NP);
+  constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF_KV, 64 * NP);
   return band_go(band_whole(a) ? band_bwd_kv_kernel<TIO, D, NP, 64, 4, 0> : band_bwd_kv_kernel<TIO, D, NP, 64, 4, 1>, a,
                  (int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + a.far * a.far_groups), 256, lds, DLT_K_BWD_KV, "window dK/dV launch", stream);
 }
