@@ -256,12 +256,9 @@ DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {
   return odd;
 }
 
-// maximum of three scores.  fmaxf would first multiply every operand by 1 (to quiet signalling NaNs), one vector instruction in eight of the forward loop
-DLT_DEV float band_max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
+// maximum of three scores.  Written in C++, never in inline asm: the scores come from matrix instructions, and the compiler keeps the waits behind those
+// only for readers that it knows
+DLT_DEV float band_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // Hidden pairs of a chunk at the edge.  Key x + 4 g + c of own row p (c a constant of the unrolled code) is seen iff c <= h && (c > l || c < s).  The
 // bounds are formed here, per chunk, from a value the compiler cannot look through: left to itself it keeps one register for each c, in kernels that have none left.
 struct BandEdge { int h, l, s; };
