@@ -8,66 +8,89 @@
 namespace {
 
 // ---- sums of shares -------------------------------------------------------------------------------------------------------------
-// Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row.  A workgroup joins one row: every wave forms the
-// weights of all shares (a lane each), then adds up every fourth share, and the four sums are added in their order.  (One thread per 4 dims walking all shares:
-// 36 us for 96 rows of 64 shares; this way JOINTIME.)
-template <typename TIO>
+// Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row, joined in the order of the shares.
+// WG: a workgroup to a row; every wave forms the weights of all shares (a lane each), adds up every fourth share, and the four sums are added.  Else (up to 8 shares) a wave to
+// a row.  One thread per 4 dims walking all shares: 36 us for 96 rows of 64 shares, this way 4.8; 8192 rows of 4 shares 14.4 by workgroups, 6.2 by waves.
+DLT_DEV float band_share_weight(const float2& x, float m) {
+  // a share that held no key of the row has (-inf, 0); a sum that is infinite or NaN goes through
+  return x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : fast_exp2(x.x - m);
+}
+template <typename TIO, bool WG>
 __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
-  __shared__ float sum[4][128];
-  const int64_t at = blockIdx.x;
+  __shared__ float sum[WG ? 4 : 1][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = WG ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (!WG && at >= (int64_t)a.B * a.Hkv * a.rows) return;
   const int bh = (int)(at / a.rows), r = (int)(at - (int64_t)bh * a.rows), b = bh / a.Hkv, h = bh - b * a.Hkv;
   const int n_q = a.pg.n_new != nullptr ? dlt_imax(0, dlt_imin(a.pg.n_new[b], a.Lq)) : a.Lq;
   const bool on = r < n_q * a.G;   // the others have no partial results
   const float2* ml = reinterpret_cast<const float2*>(a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_) + (int64_t)bh * a.shares * a.rows + r;
-  float2 x[BAND_SHARES_MAX / 64];
-  float m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int i = 0; i < BAND_SHARES_MAX / 64; i++) {
-    const int s = 64 * i + lane;
-    x[i] = on && s < a.shares ? ml[(int64_t)s * a.rows] : float2{-INFINITY, 0.f};
-    m = fmaxf(m, x[i].x);
-  }
-  m = band_wave_max(m);
-  float wgt[BAND_SHARES_MAX / 64];
-#pragma unroll
-  for (int i = 0; i < BAND_SHARES_MAX / 64; i++) {
-    // a share that held no key of the row has (-inf, 0); a sum that is infinite or NaN goes through
-    wgt[i] = x[i].x == -INFINITY ? (x[i].y == 0.f ? 0.f : 1.f) : fast_exp2(x[i].x - m);
-    l = fmaf(x[i].y, wgt[i], l);
-  }
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k);
-  float o[2] = {0.f, 0.f};
-  if (on && 2 * lane < a.dv_) {
-    const float* part = a.part + ((int64_t)bh * a.shares * a.rows + r) * a.dv_ + 2 * lane;
+  const float* part = a.part + ((int64_t)bh * a.shares * a.rows + r) * a.dv_ + 2 * dlt_imin(lane, a.dv_ / 2 - 1);
+  const int64_t step = (int64_t)a.rows * a.dv_;
+  float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
+  auto add = [&](const float2& v, float f) __attribute__((always_inline)) {
+    if (f != 0.f) {
+      o[0] = fmaf(v.x, f, o[0]);
+      o[1] = fmaf(v.y, f, o[1]);
+    }
+  };
+  if constexpr (WG) {
     static_assert(BAND_SHARES_MAX == 128, "two weights a lane");
-    for (int s0 = wave; s0 < a.shares; s0 += 32) {
-      float2 v[8];
+    float2 x[2];
+    float wgt[2];
 #pragma unroll
-      for (int u = 0; u < 8; u++) v[u] = *reinterpret_cast<const float2*>(part + (int64_t)dlt_imin(s0 + 4 * u, a.shares - 1) * a.rows * a.dv_);
+    for (int i = 0; i < 2; i++) {
+      const int s = 64 * i + lane;
+      x[i] = on && s < a.shares ? ml[(int64_t)s * a.rows] : float2{-INFINITY, 0.f};
+      m = fmaxf(m, x[i].x);
+    }
+    m = band_wave_max(m);
 #pragma unroll
-      for (int u = 0; u < 8; u++) {
-        const int s = s0 + 4 * u;
-        const float f = s < 64 ? band_lane(wgt[0], s) : band_lane(wgt[1], s - 64);
-        if (s < a.shares && f != 0.f) {
-          o[0] = fmaf(v[u].x, f, o[0]);
-          o[1] = fmaf(v[u].y, f, o[1]);
+    for (int i = 0; i < 2; i++) {
+      wgt[i] = band_share_weight(x[i], m);
+      l = fmaf(x[i].y, wgt[i], l);
+    }
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) l += __shfl_xor(l, k);
+    if (on)
+      for (int s0 = wave; s0 < a.shares; s0 += 32) {
+        float2 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) v[u] = *reinterpret_cast<const float2*>(part + dlt_imin(s0 + 4 * u, a.shares - 1) * step);
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+          const int s = s0 + 4 * u;
+          const float f = s < 64 ? band_lane(wgt[0], s) : band_lane(wgt[1], s - 64);
+          if (s < a.shares) add(v[u], f);
         }
       }
+    sum[wave][2 * lane] = o[0];
+    sum[wave][2 * lane + 1] = o[1];
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int j = 0; j < 2; j++) o[j] = ((sum[0][2 * lane + j] + sum[1][2 * lane + j]) + sum[2][2 * lane + j]) + sum[3][2 * lane + j];
+  } else if (on) {
+    float2 x[8], v[8];
+#pragma unroll
+    for (int s = 0; s < 8; s++) {
+      const int c = dlt_imin(s, a.shares - 1);
+      x[s] = ml[(int64_t)c * a.rows];
+      v[s] = *reinterpret_cast<const float2*>(part + c * step);
+    }
+#pragma unroll
+    for (int s = 0; s < 8; s++) m = fmaxf(m, x[s].x);   // the last share again behind it
+#pragma unroll
+    for (int s = 0; s < 8; s++) {
+      if (s >= a.shares) break;
+      const float f = band_share_weight(x[s], m);
+      l = fmaf(x[s].y, f, l);
+      add(v[s], f);
     }
   }
-  if (2 * lane < 128) { sum[wave][2 * lane] = o[0]; sum[wave][2 * lane + 1] = o[1]; }
-  __syncthreads();
-  if (wave != 0) return;
   const float f = l == 0.f ? 0.f : 1.f / l;
   TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r);
-  if (2 * lane < a.dv_) {
-    float y[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) y[j] = ((sum[0][2 * lane + j] + sum[1][2 * lane + j]) + sum[2][2 * lane + j]) + sum[3][2 * lane + j];
-    *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(y[0] * f, y[1] * f);
-  }
+  if (2 * lane < a.dv_) *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(o[0] * f, o[1] * f);
   if (lane == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
@@ -102,14 +125,20 @@ int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
   if (backward ? a.part_keys == 0 : a.shares <= 1) return DLT_OK;
   const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.part_keys : a.rows);
   const int per = dlt_imax(a.dk_, a.dv_) / 4;
-  const dim3 grid((unsigned)(backward ? (rows * per + 255) / 256 : rows), backward ? 2 : 1);
+  const bool wg = a.shares > 8;
+  const dim3 grid((unsigned)(backward ? (rows * per + 255) / 256 : wg ? rows : (rows + 3) / 4), backward ? 2 : 1);
   dlt_timing_before(backward ? DLT_K_BWD_KV : DLT_K_FWD, stream);
   if (backward) {
     if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kv_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL(band_join_kv_kernel<f16_t>, grid, dim3(256), 0, stream, a);
   } else {
-    if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(band_join_kernel<f16_t>, grid, dim3(256), 0, stream, a);
+    if (dtype == DLT_BF16) {
+      if (wg) hipLaunchKernelGGL((band_join_kernel<bf16_t, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((band_join_kernel<bf16_t, false>), grid, dim3(256), 0, stream, a);
+    } else {
+      if (wg) hipLaunchKernelGGL((band_join_kernel<f16_t, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((band_join_kernel<f16_t, false>), grid, dim3(256), 0, stream, a);
+    }
   }
   dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("window sum launch");
@@ -192,23 +221,40 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
 }
 
 // ---- cutting a call into workgroups ---------------------------------------------------------------------------------------------------
-// Rows: 128 a workgroup, 64 where that leaves CUs idle.  Where even those are few, the keys of a block are taken by several workgroups (shares).
-int plan_rows(BandArgs& a, bool shares) {
+// Rows: how many a workgroup has, and how many workgroups share the keys of a block of rows.
+//   BAND_TWO     128 rows, where that makes two workgroups a CU
+//   BAND_ONE     64 rows otherwise
+//   BAND_HALVES  64 rows, their keys over two groups of waves, while one workgroup a CU is all there is and the keys of a block are too few, or the workgroups too many, to be
+//                shared: a wave alone on its SIMD waits out every latency.  8 heads of 2048 queries, d = 64 / 128, us: 2560 keys each 32 -> 25 / 46 -> 35; 640 keys 11.7 -> 11.7 /
+//                16.4 -> 15.2; 4 heads, 640 keys, 10.1 + 6.3 for the sum of 4 shares -> 11.0 / 14.6 + 5.9 -> 14.0; but 12 heads (384 workgroups) 14.6 -> 19.7 / 20 -> 26
+//   BAND_FEW     up to 16 rows (a decode step), few keys: a wave has 32-key chunks of its own.  8 heads on 300 keys, d = 64, 8.4 -> 7.8; memory bound calls lose by it, since a CU
+//                holds one such workgroup (64 sequences of 4096 keys, d = 128: 155 -> 181)
+// Shares: up to two workgroups a CU, at least four chunks each.  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
+// (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).
+int plan_rows(BandArgs& a, bool forward) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv;
-  const int np = a.rows <= 64 || bh * ((a.rows + 127) / 128) < 2 * cus ? 1 : 2;
-  a.nblk = (a.rows + 64 * np - 1) / (64 * np);
+  const bool paged = a.pg.cols != 0;
+  auto blocks = [&](int own) { return (a.rows + own - 1) / own; };
+  auto chunks = [&](int own) { return (int)dlt_imin64((int64_t)a.W + a.S + own / a.G + 1, a.Lk) / 64 + 1; };   // of 64 keys, of a block
+  int kind = a.rows <= 64 || bh * blocks(128) < 2 * cus ? BAND_ONE : BAND_TWO;
+  const int64_t one = bh * blocks(64);
+  const bool uneven = paged && 2 * one > cus && 2 * one <= 3 * cus && chunks(64) > 32;
+  if (forward && kind == BAND_ONE && one <= cus && !uneven) {
+    if (a.rows <= 16 && chunks(16) <= 16) kind = BAND_FEW;
+    else if (chunks(64) <= 12 || 2 * one > cus) kind = BAND_HALVES;
+  }
+  const int own = kind == BAND_TWO ? 128 : kind == BAND_FEW ? 16 : 64;
+  a.nblk = blocks(own);
   a.shares = 1;
-  if (shares) {
-    const int64_t wgs = bh * a.nblk;
-    const int most = (int)dlt_imin64((int64_t)a.W + a.S + 64 * np / a.G + 1, a.Lk) / 64 + 1;   // chunks of a block
-    int64_t n = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
-    n = dlt_imin64(dlt_imin64(n, most / 4), BAND_SHARES_MAX);
+  const int64_t wgs = bh * a.nblk;
+  if (forward && kind == BAND_ONE && wgs > 0 && (wgs < cus || uneven)) {
+    int64_t n = dlt_imin64(dlt_imin64(((uneven ? 4 : 2) * cus + wgs - 1) / wgs, chunks(own) / 4), BAND_SHARES_MAX);
     const int64_t row_bytes = bh * a.rows * (a.dv_ + 2) * 4;
     n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(row_bytes > 0 ? row_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
     a.shares = n < 1 ? 1 : (int)n;
   }
-  return np;
+  return kind;
 }
 int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
 int64_t keys_bytes(const BandArgs& a) { return a.part_keys > 0 ? BandParts(a, band_kv_group(band_class(a.dk_, a.dv_))).floats * 4 : 0; }
@@ -282,13 +328,13 @@ extern "C" int dlt_window_fwd(const void* q, const int64_t q_strides[4], const v
   if ((rc = check_rows(who, "v", v, v_strides, a.Lk == 0, key_span(v_strides))) != DLT_OK) return rc;
   if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
   DLT_REQUIRE(lse2 != nullptr || a.Lq == 0, "%s: lse2 is NULL", who);
-  const int np = plan_rows(a, true);
+  const int kind = plan_rows(a, true);
   if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
   a.q = q; a.k = k; a.v = v; a.out = o; a.lse = lse2; a.part = (float*)ws;
   strides3(a.qs, q_strides); strides3(a.ks, k_strides); strides3(a.vs, v_strides); strides3(a.os, o_strides);
-  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_fwd_64(a, shape->dtype, np, stream) : dlt_band_fwd_128(a, shape->dtype, np, stream);
+  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_fwd_64(a, shape->dtype, kind, stream) : dlt_band_fwd_128(a, shape->dtype, kind, stream);
   return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
 }
 
@@ -311,7 +357,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
   DLT_REQUIRE((lse2 != nullptr && delta != nullptr) || nq, "%s: lse2 or delta is NULL", who);
   BandArgs kv = a;
   plan_keys(kv);
-  const int np = plan_rows(a, false);
+  const int kind = plan_rows(a, false);
   if ((rc = check_ws(who, ws, ws_bytes, keys_bytes(kv))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK || (rc = check_grid(who, kv)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND)) return DLT_OK;
@@ -322,7 +368,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
     strides3(x->dqs, dq_strides); strides3(x->dks, dk_strides); strides3(x->dvs, dv_strides);
   }
   const bool small = band_class(a.dk_, a.dv_) == 64;
-  if (!nq && (rc = small ? dlt_band_bwd_q_64(a, shape->dtype, np, stream) : dlt_band_bwd_q_128(a, shape->dtype, np, stream)) != DLT_OK) return rc;
+  if (!nq && (rc = small ? dlt_band_bwd_q_64(a, shape->dtype, kind, stream) : dlt_band_bwd_q_128(a, shape->dtype, kind, stream)) != DLT_OK) return rc;
   if (nk) return DLT_OK;
   if ((rc = small ? dlt_band_bwd_kv_64(kv, shape->dtype, stream) : dlt_band_bwd_kv_128(kv, shape->dtype, stream)) != DLT_OK) return rc;
   return join(kv, true, shape->dtype, stream);
@@ -352,14 +398,14 @@ extern "C" int dlt_paged_attn(const void* q, const int64_t q_strides[4], const v
   if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
   DLT_REQUIRE(table != nullptr && seq_len != nullptr, "%s: table or seq_len is NULL", who);
   DLT_REQUIRE(table_stride >= 0, "%s: negative table stride", who);
-  const int np = plan_rows(a, true);
+  const int kind = plan_rows(a, true);
   if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
   a.q = q; a.k = k_cache; a.v = v_cache; a.out = o; a.part = (float*)ws;
   strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);
   a.pg.table = table; a.pg.seq = seq_len; a.pg.n_new = n_new; a.pg.ts = table_stride;
-  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged_64(a, shape->dtype, np, stream) : dlt_band_paged_128(a, shape->dtype, np, stream);
+  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged_64(a, shape->dtype, kind, stream) : dlt_band_paged_128(a, shape->dtype, kind, stream);
   return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
 }
 

@@ -125,7 +125,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1H = 2 * KC, N1 = 2 * N1H, NB = N1 + KB, NT = NKB * NB;
-    constexpr int RD = NP == 1 ? BAND_RD1 : 1;
+    constexpr int RD = 1;   // LDS reads ahead of the matrix instruction (2 to 6: no faster)
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   }
   TIO* dqb = reinterpret_cast<TIO*>(a.dq) + b * a.dqs[0] + (int64_t)h * a.G * a.dqs[1];
   constexpr int PT = D * 2 + 16;
-  band_store_rows<D, NP, TIO>(smem, acc, mul, NW, a.dk_, wave, n, g, tid,
+  band_store_rows<D, NP, TIO>(smem, acc, mul, NW, 1, true, a.dk_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(dqb, a.dqs, a, x0 + row) : nullptr; },
                               [&]() {
                                 // rows with an infinite or NaN sum once more, over the keys that they see alone (band_common.h)
@@ -262,10 +262,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 // window.  The rows behind the block's window ("far" rows) are therefore taken by workgroups of their own, a share of the rows each: the 16 NP keys
 // of a far workgroup belong to all its waves, which take 16 of a chunk's 64 rows each, with half-filled second products.  Far workgroups
 // and the blocks with sinks leave partial sums, which a second launch adds in a fixed order.  16 heads on 4, 8192 tokens, window 1024, 4 sinks,
-// d = 128: 876 us with the far rows in the block, FARTIME with 22 shares of them beside it.
+// d = 128: 876 us with the far rows in the block, 187 with workgroups of 1024 far rows, launched first, beside it.
 // ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
 template <typename TIO, int D, int NP, int CK, int NW, int PAD>
-__global__ __launch_bounds__(64 * NW, NP * D > 128 ? 1 : 2) void band_bwd_kv_kernel(const BandArgs a) {
+__global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs a) {
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(64 * NW, NP * D > 128 ? 1 : 2) void band_bwd_kv_ker
     constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NP2 = 2 * KB, NT = N1 + NQB * NP2;
     constexpr int NU = 2 * NP;
     static_assert(NP2 >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
-    constexpr int RD = BAND_RD_KV;
+    constexpr int RD = 3;   // 1: 197 us, 3: 187 for 16 heads on 4, 8192 tokens, window 1024, d = 128; more: spills
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
@@ -622,8 +622,8 @@ __global__ __launch_bounds__(64 * NW, NP * D > 128 ? 1 : 2) void band_bwd_kv_ker
   };
   TIO* dkb = reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1];
   TIO* dvb = reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1];
-  band_store_rows<D, NP, TIO>(smem, dk_acc, mulk, NW, a.dk_, wave, n, g, tid,
+  band_store_rows<D, NP, TIO>(smem, dk_acc, mulk, NW, 1, true, a.dk_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.Lk ? dkb + (x0 + row) * a.dks[2] : nullptr; }, [&]() { again(true); });
-  band_store_rows<D, NP, TIO>(smem, dv_acc, mulv, NW, a.dv_, wave, n, g, tid,
+  band_store_rows<D, NP, TIO>(smem, dv_acc, mulv, NW, 1, true, a.dv_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.Lk ? dvb + (x0 + row) * a.dvs[2] : nullptr; }, [&]() { again(false); });
 }

@@ -209,17 +209,18 @@ struct BandBuf {
 
 // chunk buffers of a workgroup: as many as leave a CU two workgroups and more (one more at d = 128, with one block of rows per wave: 155 -> 186 us for the decode
 // step of 64 sequences, 18 -> 29 for 3 x 6 heads of 1111 tokens)
-constexpr int band_nbuf(int buf) { return 4 * buf <= 65536 ? 3 : 2; }
+constexpr int band_nbuf(int buf, int groups = 1) { return 4 * buf <= 65536 && 3 * groups * buf <= 131072 ? 3 : 2; }
 
 // Accumulators in C layout (lane (n, g): dims 16 d + 4 g .. + 3 of own row n, times mul[p]) -> LDS tile of 16-bit values -> rows.
 // `ptr(row)`: the row's place or NULL.  The tile takes the chunk buffers' LDS.
 // `again()`: the wave writes rows of its own part of the tile once more (see below).
 template <int D, int NP, typename TIO, int NA, typename PtrFn, typename AgainFn>
-DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int dims, int wave, int n, int g, int tid, PtrFn ptr,
+DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int groups, bool write, int dims, int wave, int n, int g, int tid, PtrFn ptr,
                              AgainFn again) {
   constexpr int PT = D * 2 + 16;
+  // `write`: the wave's group writes the tile; the waves of all groups store it
 #pragma unroll
-  for (int p = 0; p < NP; p++) {
+  for (int p = 0; write && p < NP; p++) {
     char* row = sT + (wave * 16 * NP + 16 * p + n) * PT + 8 * g;
 #pragma unroll
     for (int d = 0; d < NA; d++) {
@@ -236,7 +237,7 @@ DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (
   constexpr int CH = D / 8;
   const int c = tw % CH;
   if (8 * c < dims)
-    for (int row = tw / CH; row < 16 * NP * nw; row += 64 * nw / CH) {
+    for (int row = tw / CH; row < 16 * NP * nw; row += 64 * nw * groups / CH) {
       TIO* p = ptr(row);
       if (p == nullptr) continue;
       const u32x4 v = lds_read16(sT + row * PT + 16 * c);
@@ -256,9 +257,6 @@ DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {
   return odd;
 }
 
-// maximum of three scores.  Written in C++, never in inline asm: the scores come from matrix instructions, and the compiler keeps the waits behind those
-// only for readers that it knows
-DLT_DEV float band_max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 // Hidden pairs of a chunk at the edge.  Key x + 4 g + c of own row p (c a constant of the unrolled code) is seen iff c <= h && (c > l || c < s).  The
 // bounds are formed here, per chunk, from a value the compiler cannot look through: left to itself it keeps one register for each c, in kernels that have none left.
 struct BandEdge { int h, l, s; };
@@ -273,13 +271,6 @@ DLT_DEV float band_formed(float v) {
   asm volatile("" : "+v"(v));
   return v;
 }
-
-#ifndef BAND_RD1
-#define BAND_RD1 1
-#endif
-#ifndef BAND_RD_KV
-#define BAND_RD_KV 3
-#endif
 
 // ---- rows whose sums came out infinite or NaN ------------------------------------------------------------------------------------
 // The matrix products of a chunk at the edge of a window multiply hidden pairs by 0, and 0 times an infinity or a NaN is NaN: a hidden key

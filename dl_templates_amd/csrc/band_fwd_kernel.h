@@ -47,7 +47,7 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
 #pragma unroll 1
     for (int x = W.x(i); x < W.x(i) + CK; x += 64) {
       const int j = x + lane;
-      const bool sees = j < n_k && band_sees(pos, j, a.W, a.S);
+      const bool sees = j < n_k && (CK >= 64 || lane < CK) && band_sees(pos, j, a.W, a.S);
       uint64_t todo = __builtin_amdgcn_ballot_w64(sees);
       if (todo == 0) continue;
       const float s = sees ? band_dot(q, kb + band_key_off<PAGED>(a, pages, a.ks, j), a.dk_) * a.scale_log2 : -INFINITY;
@@ -67,19 +67,21 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
     }
 }
 
-template <typename TIO, int D, int NP, int CK, int NW, bool PAGED, int PAD>
-__global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
+// GR groups of NW waves own the same rows and take every GR-th chunk each; their results are joined at the end, through LDS.
+template <typename TIO, int D, int NP, int CK, int NW, int GR, bool PAGED, int PAD>
+__global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, VB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
-  constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
+  constexpr int NBUF = band_nbuf(B::BUF, GR), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;                              // groups of 16 tokens that a wave copies
   static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
   constexpr int PER_CHUNK = 2 * NG * BandStage<D>::NI;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, n = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave_all = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = GR == 1 ? 0 : wave_all / NW, wave = wave_all - grp * NW;   // group of the wave, wave of the group
 
   const int lin = xcd_remap(blockIdx.x, gridDim.x);
   int bh, r_, unit;
@@ -107,11 +109,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   stv.init(lane, a.dv_, a.vs[2]);
   if constexpr (PAD) {
 #pragma unroll
-    for (int i = 0; i < NBUF; i++) {
-      flashd_zero_pads<D>(smem + i * B::BUF, CK, a.dk_ >> 3, tid, 64 * NW);
-      flashd_zero_pads<D>(smem + i * B::BUF + B::REG, CK, a.dv_ >> 3, tid, 64 * NW);
+    for (int i = 0; i < NBUF * GR; i++) {
+      flashd_zero_pads<D>(smem + i * B::BUF, CK, a.dk_ >> 3, tid, 64 * NW * GR);
+      flashd_zero_pads<D>(smem + i * B::BUF + B::REG, CK, a.dv_ >> 3, tid, 64 * NW * GR);
     }
   }
+  char* const bufs = smem + grp * NBUF * B::BUF;   // of the group
   auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
     const int x = W.x(i) + wave * 16 * NG;
 #pragma unroll
@@ -151,7 +154,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   };
 #pragma unroll 1
   for (int i = 0; i < AHEAD; i++)
-    if (i_beg + i < i_end) issue(i_beg + i, smem + i * B::BUF);
+    if (i_beg + i * GR + grp < i_end) issue(i_beg + i * GR + grp, bufs + i * B::BUF);
 
   const int wq0 = x0 + wave * 16 * NP;
   u32x4 qf[NP][KC];
@@ -188,14 +191,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   pin_loaded(qf);
 #pragma unroll
   for (int i = 0; i < AHEAD; i++)
-    if (i_beg + i < i_end) settle(i_beg + i, smem + i * B::BUF);
+    if (i_beg + i * GR + grp < i_end) settle(i_beg + i * GR + grp, bufs + i * B::BUF);
   __syncthreads();
 
   auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1 = NKB * 2 * KC, NT = N1 + NKB * VB;
-    constexpr int RD = NP == 1 ? BAND_RD1 : 1;
+    constexpr int RD = 1;   // LDS reads ahead of the matrix instruction (2 to 6: no faster)
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
@@ -238,14 +241,12 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
         if constexpr (k == N1 - 1) {
 #pragma unroll
           for (int p = 0; p < NP; p++) {
-            float mx[4];
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 4; i++) mx[i] = band_max3(t[p][0][2 * i], t[p][0][2 * i + 1], t[p][0][2 * i]);
+            for (int kb2 = 0; kb2 < NKB; kb2++)
 #pragma unroll
-            for (int kb2 = 1; kb2 < NKB; kb2++)
-#pragma unroll
-              for (int i = 0; i < 4; i++) mx[i] = band_max3(mx[i], t[p][kb2][2 * i], t[p][kb2][2 * i + 1]);
-            const float mloc = wave_max4(band_max3(band_max3(mx[0], mx[1], mx[2]), mx[3], mx[3]));
+              for (int i = 0; i < 4; i++) mx[i] = fmaxf(fmaxf(mx[i], t[p][kb2][2 * i]), t[p][kb2][2 * i + 1]);
+            const float mloc = wave_max4(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
             // the reference maximum moves only when a score exceeds it by more than 2^8 after scaling: P stays below 2^8, its sum in
             // 32 bits below 2^8 times the keys
             if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > 8.f)) {
@@ -287,41 +288,79 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
   W.whole(first, last, a.W, i_beg, i_end, f0, f1);
   // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
   // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
-  int bi = 0, i = i_beg, stop = f0;
-  auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
+  const int rounds = (i_end - i_beg + GR - 1) / GR, r0 = (f0 - i_beg + GR - 1) / GR, r1 = (f1 - i_beg) / GR;
+  int bi = 0, it = 0, stop = dlt_imin(r0, rounds);
+  auto buf_of = [&](int i) { return bufs + (i >= NBUF ? i - NBUF : i) * B::BUF; };
   auto step = [&](auto mask_tag) __attribute__((always_inline)) {
-    const bool more = i + AHEAD < i_end;
-    if (more) issue(i + AHEAD, buf_of(bi + AHEAD));
-    chunk(i, buf_of(bi), mask_tag);
+    const int i = i_beg + it * GR + grp;
+    const bool more = i + AHEAD * GR < i_end;
+    if (more) issue(i + AHEAD * GR, buf_of(bi + AHEAD));
+    if (GR == 1 || !decltype(mask_tag)::value || i < i_end) chunk(i, buf_of(bi), mask_tag);
     if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
     else swa2_wait_copies();
     bi = bi + 1 == NBUF ? 0 : bi + 1;
-    i++;
-    if (i < i_end) settle(i, buf_of(bi));
-    __syncthreads();
+    it++;
+    if (i + GR < i_end) settle(i + GR, buf_of(bi));
+    if constexpr (NW > 1) __syncthreads();   // a group of one wave has its buffers to itself
   };
 #pragma unroll 1
   for (;;) {
 #pragma unroll 1
-    while (i < stop) step(std::true_type{});
-    if (i >= i_end) break;
+    while (it < stop) step(std::true_type{});
+    if (it >= rounds) break;
 #pragma unroll 1
-    while (i < f1) step(std::false_type{});
-    stop = i_end;
+    while (it < r1) step(std::false_type{});
+    stop = rounds;
   }
 
   // ---- epilogue
   float lt[NP], inv[NP];
   unsigned odd[NP];   // rows of the wave to be taken again
 #pragma unroll
+  for (int p = 0; p < NP; p++) lt[p] = wave_sum4(acc_l[p][0]);
+  if constexpr (GR > 1) {
+    // every lane of the other groups leaves its registers for the same lane of group 0
+    constexpr int PER = NP * (VB * 16 + 8) * 64;   // bytes of a wave
+    __syncthreads();
+    char* mine = smem + ((grp - 1) * NW + wave) * PER + 16 * lane;
+    if (grp > 0) {
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+#pragma unroll
+        for (int d = 0; d < VB; d++) *reinterpret_cast<f32x4*>(mine + (p * VB + d) * 1024) = acc[p][d];
+        *reinterpret_cast<float2*>(smem + ((grp - 1) * NW + wave) * PER + NP * VB * 1024 + p * 512 + 8 * lane) = float2{m_run[p], lt[p]};
+      }
+    }
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll 1
+      for (int o = 0; o < GR - 1; o++) {
+        const char* theirs = smem + (o * NW + wave) * PER;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const float2 x = *reinterpret_cast<const float2*>(theirs + NP * VB * 1024 + p * 512 + 8 * lane);
+          float f1, f2;
+          flash_merge(m_run[p], x.x, scale, f1, f2);
+          lt[p] = flash_add(lt[p], f1, x.y, f2);
+#pragma unroll
+          for (int d = 0; d < VB; d++) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(theirs + (p * VB + d) * 1024 + 16 * lane);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[p][d][i] = flash_add(acc[p][d][i], f1, v[i], f2);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
   for (int p = 0; p < NP; p++) {
-    lt[p] = wave_sum4(acc_l[p][0]);
     inv[p] = lt[p] > 0.f && wq0 + 16 * p + n < n_rows ? fast_rcp(lt[p]) : 0.f;   // rows that see nothing, and rows behind the last query: zeros
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < n_rows && (band_odd_row(acc, p) || band_odd(lt[p])));
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(grp == 0 && wq0 + 16 * p + n < n_rows && (band_odd_row(acc, p) || band_odd(lt[p])));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }
   const int64_t row0 = (int64_t)bh * a.rows;
   if (a.shares > 1) {
+    if (grp != 0) return;
     const int64_t at = ((int64_t)bh * a.shares + share) * a.rows;
     float* part = a.part + at * a.dv_;
     float* ml = a.part + (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dv_ + 2 * at;
@@ -345,13 +384,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 ? 2 : 1) void band_fwd_kernel(cons
 #pragma unroll
     for (int p = 0; p < NP; p++) {
       const int r = wq0 + 16 * p + n;
-      if (g == 0 && r < n_rows && (odd[p] >> n & 1) == 0) store_stream4(a.lse + row0 + r, m_run[p] * scale + fast_log2(lt[p]));
+      if (grp == 0 && g == 0 && r < n_rows && (odd[p] >> n & 1) == 0) store_stream4(a.lse + row0 + r, m_run[p] * scale + fast_log2(lt[p]));
     }
   }
   __syncthreads();
   TIO* ob = reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1];
   constexpr int PT = D * 2 + 16;
-  band_store_rows<D, NP, TIO>(smem, acc, inv, NW, a.dv_, wave, n, g, tid,
+  band_store_rows<D, NP, TIO>(smem, acc, inv, NW, GR, grp == 0, a.dv_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(ob, a.os, a, x0 + row) : nullptr; },
                               [&]() {
 #pragma unroll 1

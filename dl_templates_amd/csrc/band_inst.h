@@ -27,24 +27,30 @@ int band_go(KernT kern, const BandArgs& a, int64_t grid, int threads, int lds, i
 inline bool band_whole(const BandArgs& a) { return a.dk_ == D && a.dv_ == D; }
 
 #if DLT_BAND_PART < 2
-template <typename TIO, int NP, int CK, int NW>
+template <typename TIO, int NP, int CK, int NW, int GR>
 int band_fwd(const BandArgs& a, hipStream_t stream) {
   constexpr bool PG = DLT_BAND_PART == 1;
-  constexpr int lds = band_lds(band_nbuf(BandBuf<D, CK>::BUF) * BandBuf<D, CK>::BUF, 16 * NP * NW);
-  return band_go(band_whole(a) ? band_fwd_kernel<TIO, D, NP, CK, NW, PG, 0> : band_fwd_kernel<TIO, D, NP, CK, NW, PG, 1>, a,
-                 (int64_t)a.B * a.Hkv * a.nblk * a.shares, 64 * NW, lds, DLT_K_FWD, "window forward launch", stream);
+  constexpr int join = (GR - 1) * NW * NP * (D + 8) * 64, bufs = GR * band_nbuf(BandBuf<D, CK>::BUF, GR) * BandBuf<D, CK>::BUF;
+  constexpr int lds = band_lds(bufs > join ? bufs : join, 16 * NP * NW);
+  return band_go(band_whole(a) ? band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 0> : band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 1>, a,
+                 (int64_t)a.B * a.Hkv * a.nblk * a.shares, 64 * NW * GR, lds, DLT_K_FWD, "window forward launch", stream);
 }
 template <typename TIO>
-int band_fwd_np(const BandArgs& a, int np, hipStream_t stream) {
-  return np == 1 ? band_fwd<TIO, 1, 64, 4>(a, stream) : band_fwd<TIO, 2, 64, 4>(a, stream);
+int band_fwd_np(const BandArgs& a, int kind, hipStream_t stream) {
+  switch (kind) {
+    case BAND_FEW: return band_fwd<TIO, 1, 32, 1, 4>(a, stream);
+    case BAND_HALVES: return band_fwd<TIO, 1, 64, 4, 2>(a, stream);
+    case BAND_ONE: return band_fwd<TIO, 1, 64, 4, 1>(a, stream);
+    default: return band_fwd<TIO, 2, 64, 4, 1>(a, stream);
+  }
 }
 }  // namespace
 #if DLT_BAND_PART == 0
-int DLT_BCAT(dlt_band_fwd_, DLT_BAND_D)(const BandArgs& a, int dtype, int np, hipStream_t stream) {
+int DLT_BCAT(dlt_band_fwd_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind, hipStream_t stream) {
 #else
-int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int np, hipStream_t stream) {
+int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind, hipStream_t stream) {
 #endif
-  return dtype == DLT_BF16 ? band_fwd_np<bf16_t>(a, np, stream) : band_fwd_np<f16_t>(a, np, stream);
+  return dtype == DLT_BF16 ? band_fwd_np<bf16_t>(a, kind, stream) : band_fwd_np<f16_t>(a, kind, stream);
 }
 #elif DLT_BAND_PART == 2
 template <typename TIO, int NP>
@@ -54,10 +60,10 @@ int band_bwd_q(const BandArgs& a, hipStream_t stream) {
                  DLT_K_BWD_Q, "window dQ launch", stream);
 }
 template <typename TIO>
-int band_bwd_q_np(const BandArgs& a, int np, hipStream_t stream) { return np == 1 ? band_bwd_q<TIO, 1>(a, stream) : band_bwd_q<TIO, 2>(a, stream); }
+int band_bwd_q_np(const BandArgs& a, int kind, hipStream_t stream) { return kind != BAND_TWO ? band_bwd_q<TIO, 1>(a, stream) : band_bwd_q<TIO, 2>(a, stream); }
 }  // namespace
-int DLT_BCAT(dlt_band_bwd_q_, DLT_BAND_D)(const BandArgs& a, int dtype, int np, hipStream_t stream) {
-  return dtype == DLT_BF16 ? band_bwd_q_np<bf16_t>(a, np, stream) : band_bwd_q_np<f16_t>(a, np, stream);
+int DLT_BCAT(dlt_band_bwd_q_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind, hipStream_t stream) {
+  return dtype == DLT_BF16 ? band_bwd_q_np<bf16_t>(a, kind, stream) : band_bwd_q_np<f16_t>(a, kind, stream);
 }
 #else
 template <typename TIO>
