@@ -13,8 +13,10 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <torch/csrc/Exceptions.h>
@@ -215,20 +217,25 @@ Spec window_spec(const Tensor& q, const Tensor& k, const Tensor& v, const int64_
   check_assert(q.size(3) == k.size(3), "q and k must have one head dim");
   check_assert(q.size(0) == k.size(0) && k.sizes().slice(0, 3) == v.sizes().slice(0, 3), "k and v must match q");
   check_assert(q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type(), "q, k and v must have one dtype");
+  for (const Tensor* x : {&q, &k, &v})
+    for (int64_t n : x->sizes()) require(n <= INT32_MAX, PyExc_ValueError, "a dim of q, k or v does not fit 32 bits");
   Spec s;
   s.op = Op::Window;
   s.window = {(int32_t)q.size(0), (int32_t)q.size(1), (int32_t)k.size(1), (int32_t)q.size(2), (int32_t)k.size(2), (int32_t)q.size(3), (int32_t)v.size(3),
               (int32_t)dims[0], (int32_t)dims[1], (float)scale, dtype_code(q)};
   return s;
 }
-// The window and paged kernels read rows in 16-byte pieces; anything else is copied first.
-bool rows16(const Tensor& x) {
+// The window and paged kernels read rows in 16-byte pieces, those of 16 tokens and the heads of a group (`G`; keys: 0) at 32-bit offsets.  Anything else is
+// copied first, the heads of a token side by side.
+bool rows16(const Tensor& x, int64_t G = 0) {
   if (x.dim() != 4 || x.numel() == 0) return true;
   bool ok = (x.stride(3) == 1 || x.size(3) == 1) && (uintptr_t)x.const_data_ptr() % 16 == 0;
   for (int i = 0; i < 3; i++) ok = ok && (x.size(i) == 1 || (x.stride(i) % 8 == 0 && x.stride(i) >= 0));
-  return ok;
+  auto span = [&](int i, int64_t n) { return x.size(i) == 1 ? 0 : x.stride(i) > ((int64_t)1 << 30) / n ? (int64_t)1 << 30 : n * x.stride(i); };
+  return ok && span(2, 17) + (G > 0 ? span(1, G) : 0) < (int64_t)1 << 30;
 }
-Tensor as_rows16(const Tensor& x) { return rows16(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
+Tensor as_rows16(const Tensor& x, int64_t G = 0) { return rows16(x, G) ? x : x.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2); }
+int64_t group_of(const Tensor& q, const Tensor& k) { return k.dim() == 4 && k.size(1) > 0 ? q.size(1) / k.size(1) : 0; }
 // strides of a [.., .., .., D] tensor as the C ABI takes them: those of dims of one element do not matter
 std::array<int64_t, 4> st16(const Tensor& x) {
   std::array<int64_t, 4> s;
@@ -323,7 +330,7 @@ std::array<Tensor, 3> run_backward(const Spec& s, const Tensor& q, const Tensor&
     const Workspace ws = window_workspace(s.window, 1, q);
     Tensor dq = empty(q.sizes(), q.scalar_type(), q), dk = empty(k.sizes(), k.scalar_type(), k), dv = empty(v.sizes(), v.scalar_type(), v);
     Tensor delta = empty(lse.sizes(), at::kFloat, lse);
-    const Tensor g = as_rows16(d_o);
+    const Tensor g = as_rows16(d_o, group_of(q, k));
     check_rc(dlt_window_bwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), o.const_data_ptr(),
                             st16(o).data(), g.const_data_ptr(), st16(g).data(), (const float*)lse.const_data_ptr(), (float*)delta.mutable_data_ptr(),
                             dq.mutable_data_ptr(), st16(dq).data(), dk.mutable_data_ptr(), st16(dk).data(), dv.mutable_data_ptr(), st16(dv).data(), &s.window,
@@ -387,6 +394,27 @@ Tensor pad_last(const Tensor& x, int64_t d) { return x.size(-1) == d ? x : at::c
 Tensor cut_last(const Tensor& x, int64_t d) { return x.size(-1) == d ? x : x.narrow(-1, 0, d).contiguous(); }
 
 // ---- autograd ---------------------------------------------------------------------------------------
+// A leaf keeps one accumulation node while any graph of it lives, with the stream that was current when the node was made.  A backward pass that is being captured
+// cannot pass a gradient to one of the default stream: the engine would make the two streams wait for each other, which ends the capture, and on ROCm the process.
+void check_capture(Node& node) {
+  bool on_default = false;
+  for (const torch::autograd::Edge& e : node.next_edges()) {
+    const std::optional<c10::Stream> s = e.is_valid() ? e.function->stream() : std::nullopt;
+    on_default = on_default || (s.has_value() && s->id() == 0);
+  }
+  if (C10_UNLIKELY(on_default && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None))
+    raise_py(PyExc_RuntimeError, "a captured backward pass reaches a leaf that belongs to a graph of the default stream: release that graph (the tensors made from the "
+                                 "leaf outside the capture), or make it on another stream");
+}
+// first derivatives only: a second one raises where it is asked for (without a graph it would be dropped in silence)
+void differentiable_once(variable_list& grads) {
+  if (C10_LIKELY(!at::GradMode::is_enabled())) return;
+  std::shared_ptr<torch::autograd::DelayedError> once(
+      new torch::autograd::DelayedError("trying to differentiate twice a function that was marked with @once_differentiable", (int64_t)grads.size()), torch::autograd::deleteNode);
+  for (Tensor& g : grads) g = g.detach().requires_grad_(true);
+  grads = (*once)(std::move(grads));
+}
+
 struct AttnBackward : public Node {
   Spec spec;
   bool has_rope = false, rotated = false;
@@ -400,23 +428,36 @@ struct AttnBackward : public Node {
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    if (spec.op == Op::Window) check_capture(*this);
     if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();   // as torch.autograd.Function does
     // Unpacked with autograd as it is: an unpack hook may run the forward pass again (activation checkpointing), and what it runs
     // has to be recorded.
-    const Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), o_ = o.unpack(shared_from_this()), lse_ = lse.unpack();
+    Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), o_ = o.unpack(shared_from_this()), lse_ = lse.unpack();
     Tensor idx_, row_, col_;
     if (has_rope) {
       idx_ = idx.unpack();
       row_ = row.unpack();
       col_ = col.unpack();
     }
-    at::AutoDispatchBelowADInplaceOrView below;
-    Rope rope;
-    if (has_rope) rope = make_rope_for(idx_, row_, col_, q_, q_.size(2));
-    Tensor d_o = pad_last(grads[0], v_.size(-1));
-    if (spec.narrow && !rows_of_pieces(d_o)) d_o = d_o.contiguous();
-    auto g = run_backward(spec, q_, k_, v_, o_, lse_, d_o, has_rope ? &rope : nullptr, rotated);
-    return {cut_last(g[0], dk), cut_last(g[1], dk), cut_last(g[2], dv)};
+    variable_list out;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      Rope rope;
+      if (has_rope) rope = make_rope_for(idx_, row_, col_, q_, q_.size(2));
+      Tensor d_o = pad_last(grads[0], v_.size(-1));
+      if (spec.narrow && !rows_of_pieces(d_o)) d_o = d_o.contiguous();
+      if (spec.op == Op::Window) {   // what an unpack hook gives need not lie as what was packed
+        q_ = as_rows16(q_, group_of(q_, k_));
+        k_ = as_rows16(k_);
+        v_ = as_rows16(v_);
+        o_ = as_rows16(o_);
+        lse_ = lse_.contiguous();
+      }
+      auto g = run_backward(spec, q_, k_, v_, o_, lse_, d_o, has_rope ? &rope : nullptr, rotated);
+      out = {cut_last(g[0], dk), cut_last(g[1], dk), cut_last(g[2], dv)};
+    }
+    if (spec.op == Op::Window) differentiable_once(out);
+    return out;
   }
 };
 
@@ -462,7 +503,7 @@ Tensor attention(Op op, const Tensor& q, const Tensor& k, const Tensor& v, const
     if (op == Op::Window) {
       check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
       require_gpu(q, k, v);
-      pq = as_rows16(pq);
+      pq = as_rows16(pq, group_of(pq, pk));
       pk = as_rows16(pk);
       pv = as_rows16(pv);
     }
@@ -578,6 +619,14 @@ void rope_apply(const Tensor& x, const Rows& r, const Tensor& idx, const Tensor&
 }
 
 // ---- rotation with several axes -------------------------------------------------------------------------
+// tensors that a call writes: no element twice
+void check_written(const Tensor& x, const char* name) {
+  if (C10_UNLIKELY(at::has_internal_overlap(x) == at::MemOverlap::Yes)) raise_py(PyExc_RuntimeError, std::string(name) + " has elements that share memory (an expanded tensor): it cannot be written in place");
+}
+void check_two(const Tensor& x, const Tensor& y, const char* names) {
+  if (C10_UNLIKELY(x.numel() > 0 && y.numel() > 0 && x.const_data_ptr() == y.const_data_ptr())) raise_py(PyExc_RuntimeError, std::string(names) + " must be two tensors");
+}
+
 struct Axes {
   Tensor pos;                   // int32 [axes, N] or [axes, B, N]
   std::vector<Tensor> tables;   // fp32 [len, R, 2]
@@ -620,6 +669,9 @@ void run_axes(const Tensor& q, const Tensor& k, const Tensor& q_out, const Tenso
   check_assert(!k.defined() || (k.size(0) == q.size(0) && k.size(2) == q.size(2) && k.size(3) == q.size(3) && k.scalar_type() == q.scalar_type()),
                "q and k must have one batch, token count, head dim and dtype");
   check_assert(t.pos.defined(), "pos is needed");
+  for (const Tensor* x : {&q, &k})
+    if (x->defined())
+      for (int64_t n : x->sizes()) require(n <= INT32_MAX, PyExc_ValueError, "a dim of q or k does not fit 32 bits");
   if (k.defined()) require_gpu(q, k);
   else require_gpu(q);
   dlt_rope_axes_t d;
@@ -654,6 +706,7 @@ struct RopeAxesBackward : public Node {
   // The backward pass of a rotation is the inverse one: the same operator, which records its own graph where one is wanted.
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
+    check_capture(*this);
     Axes t;
     t.pos = pos.unpack();
     for (SavedVariable& s : tables) t.tables.push_back(s.unpack());
@@ -923,7 +976,8 @@ PyObject* py_window_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]);
   const int64_t dims[2] = {window_arg(a[3]), int_arg(a[4])};
   require_gpu(q, k, v);
-  const Tensor q_ = as_rows16(q), k_ = as_rows16(k), v_ = as_rows16(v);
+  check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
+  const Tensor q_ = as_rows16(q, group_of(q, k)), k_ = as_rows16(k), v_ = as_rows16(v);
   const Forward f = run_forward(window_spec(q_, k_, v_, dims, float_arg(a[5])), q_, k_, v_, nullptr, false);
   return Py_BuildValue("(NN)", THPVariable_Wrap(f.o), THPVariable_Wrap(f.lse));
   END_HANDLE_TH_ERRORS
@@ -936,7 +990,8 @@ PyObject* py_window_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &o = tensor_arg(a[3]), &lse = tensor_arg(a[4]), &d_o = tensor_arg(a[5]);
   const int64_t dims[2] = {window_arg(a[6]), int_arg(a[7])};
   require_gpu(q, k, v, o, lse, d_o);
-  const Tensor q_ = as_rows16(q), k_ = as_rows16(k), v_ = as_rows16(v), o_ = as_rows16(o);
+  check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
+  const Tensor q_ = as_rows16(q, group_of(q, k)), k_ = as_rows16(k), v_ = as_rows16(v), o_ = as_rows16(o);
   auto g = run_backward(window_spec(q_, k_, v_, dims, float_arg(a[8])), q_, k_, v_, o_, lse.contiguous(), d_o, nullptr, false);
   return Py_BuildValue("(NNN)", THPVariable_Wrap(g[0]), THPVariable_Wrap(g[1]), THPVariable_Wrap(g[2]));
   END_HANDLE_TH_ERRORS
@@ -982,6 +1037,13 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return wrap_pair(out[0], out[1]);
   }
   if (mode == 2) {
+    require_gpu(q);
+    check_written(q, "q");
+    if (k.defined()) {
+      require_gpu(q, k);
+      check_written(k, "k");
+      check_two(q, k, "q and k");
+    }
     torch::autograd::check_inplace(q, torch::autograd::compute_requires_grad(q));
     if (k.defined()) torch::autograd::check_inplace(k, torch::autograd::compute_requires_grad(k));
     {
@@ -1015,6 +1077,9 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, k.size(0), k.size(2), q.defined() ? q.size(1) : 0);
   require_gpu(kc, k, v);
   if (q.defined()) require_gpu(kc, q);
+  check_written(kc, "k_cache");
+  check_written(vc, "v_cache");
+  check_two(kc, vc, "k_cache and v_cache");
   for (const Tensor* c : {&kc, &vc}) torch::autograd::check_inplace(*c, torch::autograd::compute_requires_grad(*c));
   Tensor q_out;
   if (p.s.B > 0) {
@@ -1053,7 +1118,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c10::DeviceGuard guard(kc.device());
   Tensor o = empty({q0.size(0), q0.size(1), q0.size(2), vc.size(3)}, q0.scalar_type(), q0);
   if (o.numel() == 0) return THPVariable_Wrap(o);
-  const Tensor q = as_rows16(q0);
+  const Tensor q = as_rows16(q0, group_of(q0, kc));
   Workspace ws;
   check_rc(dlt_paged_workspace(&p.s, &ws.bytes));
   if (ws.bytes > 0) {

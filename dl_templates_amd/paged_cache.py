@@ -22,7 +22,8 @@ def paged_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor,
 
     ``rope``: None or ``(pos, tables, layout)`` as ``rope_axes_qk`` takes them; ``pos`` None: a token's place in its sequence on every axis.
     With ``q`` [B, H, T, Dk] rotated queries come back in a new tensor (padded rows as they were), else None.  Padding, positions outside the
-    table and page numbers outside the cache write nothing.  No two tokens of a call may have the same place.  bfloat16, float16 and
+    table and page numbers outside the cache write nothing.  No two tokens of a call may have the same place, and q, k and v must not lie in
+    the caches.  bfloat16, float16 and
     float32, any strides and page size."""
     pos, tables, layout = rope if rope is not None else (None, None, "blocks")
     return _lib.native.paged_append(k_cache, v_cache, k, v, page_table, seq_len, n_new, pos, None if rope is None else tuple(tables), _layout(layout), q)

@@ -1,0 +1,663 @@
+"""The long-sequence operators where they can go wrong (GPU): infinities and NaN, empty sides, layouts, streams, graphs, large offsets, and a run of them together."""
+import math
+
+import pytest
+import torch
+
+from dl_templates_amd.paged_cache import paged_append_, paged_attention
+from dl_templates_amd.rope_axes import RotaryPositionEncodingAxes, rope_axes_qk, rope_axes_qk_
+from dl_templates_amd.window_attn import window_attention
+from tests import long_oracle as orc
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+NAN, INF = float("nan"), float("inf")
+name_of = lambda c: "-".join(str(x).replace("torch.", "").replace(" ", "") for x in c)  # noqa: E731
+
+
+def make(seed, B, Hq, Hkv, Lq, Lk, dk, dv, dtype):
+    gen = torch.Generator().manual_seed(seed)
+    mk = lambda *s: torch.randn(s, generator=gen).to(dtype).cuda()  # noqa: E731
+    return mk(B, Hq, Lq, dk), mk(B, Hkv, Lk, dk), mk(B, Hkv, Lk, dv), mk(B, Hq, Lq, dv)
+
+
+def run(q, k, v, do, *args):
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    o = window_attention(q, k, v, *args)
+    return dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, (q, k, v), do)))
+
+
+def against(q, k, v, do, *args):
+    got = run(q, k, v, do, *args)
+    for name, want in orc.window(q, k, v, *args, do).items():
+        orc.check(got[name], want, name)
+    return got
+
+
+# one block of rows and few keys, halves of the keys, shares of them, 64 and 128 rows a workgroup, far rows behind sinks
+SHAPES = [
+    # B, Hq, Hkv, Lq, Lk, dk, dv, window, sinks, dtype
+    (1, 4, 2, 3, 300, 64, 64, None, 0, BF),
+    (1, 4, 1, 40, 500, 128, 128, 200, 3, HF),
+    (1, 2, 1, 1, 3000, 64, 64, None, 0, HF),
+    (1, 2, 1, 5, 3000, 128, 128, 2500, 20, BF),
+    (1, 4, 2, 260, 260, 80, 80, 64, 4, BF),
+    (2, 16, 16, 1100, 1100, 64, 64, 100, 5, HF),
+    (2, 20, 10, 900, 900, 128, 128, 64, 1, BF),
+    (1, 2, 1, 1500, 1500, 128, 128, 33, 17, BF),
+]
+
+
+@pytest.mark.parametrize("where", ["key", "value", "query", "grad"])
+@pytest.mark.parametrize("case", SHAPES, ids=name_of)
+def test_nan_reaches_what_sees_it_and_nothing_else(case, where):
+    B, Hq, Hkv, Lq, Lk, dk, dv, window, n_sink, dtype = case
+    q, k, v, do = make(7, B, Hq, Hkv, Lq, Lk, dk, dv, dtype)
+    scale, G = 1.0 / math.sqrt(dk), Hq // Hkv
+    want = orc.window(q, k, v, window, n_sink, scale, do)
+    vis = orc.seen(torch.arange(Lq, device="cuda") + Lk - Lq, Lk, window, n_sink)
+    row, key = min(Lq - 1, Lq * 2 // 3), max(0, Lk - max(1, min(window or Lk, Lk) // 2) - 1)
+    none_q, none_k = torch.zeros(B, Hq, Lq, dtype=torch.bool, device="cuda"), torch.zeros(B, Hkv, Lk, dtype=torch.bool, device="cuda")
+    bq, bk, bv, bd = none_q.clone(), none_k.clone(), none_k.clone(), none_q.clone()
+    if where == "key":
+        k[0, 0, key, 3], bk[0, 0, key] = NAN, True
+    elif where == "value":
+        v[0, 0, key], bv[0, 0, key] = NAN, True
+    elif where == "query":
+        q[0, 0, row, 5], bq[0, 0, row] = NAN, True
+    else:
+        do[0, 0, row], bd[0, 0, row] = NAN, True
+    got = run(q, k, v, do, window, n_sink, scale)
+    sees = lambda bad: (bad.repeat_interleave(G, 1).float() @ vis.float().t()) > 0  # noqa: E731
+    p_bad = bq | sees(bk)
+    o_bad = p_bad | sees(bv)
+    row_bad = o_bad | bd
+    reach = lambda bad: (bad.float() @ vis.float()).reshape(B, Hkv, G, Lk).sum(2) > 0  # noqa: E731
+    bad = {"o": o_bad, "dq": row_bad, "dv": reach(p_bad | bd), "dk": reach(row_bad)}
+    assert bad["dk"].any() and not (Lq > 500 and bad["dk"].all())
+    for name, (value, bound) in want.items():
+        x, b = got[name], bad[name]
+        assert x[b].isnan().all(), f"{name}: a NaN is lost"
+        # the formula's values hold where no NaN is seen: a key with NaN is seen by some row, so that its own gradients are NaN as well
+        orc.check(x[~b], (value[~b], bound[~b]), name)
+
+
+@pytest.mark.parametrize("case", SHAPES, ids=name_of)
+def test_infinite_values(case):
+    """An infinite value is infinite in every output that sees it, however small its weight; other dims and rows are as they were."""
+    B, Hq, Hkv, Lq, Lk, dk, dv, window, n_sink, dtype = case
+    q, k, v, do = make(8, B, Hq, Hkv, Lq, Lk, dk, dv, dtype)
+    scale, G = 1.0 / math.sqrt(dk), Hq // Hkv
+    key = max(0, Lk - max(1, min(window or Lk, Lk) // 2) - 1)
+    k[0, 0, key] = -q[0, 0, -1] * 2   # a weight of e^(-2 |q|^2 scale): fp16 holds no such number at d = 64
+    value, bound = orc.window(q, k, v, window, n_sink, scale)["o"]
+    v[0, 0, key, 1] = INF
+    o = window_attention(q, k, v, window, n_sink, scale)
+    vis = orc.seen(torch.arange(Lq, device="cuda") + Lk - Lq, Lk, window, n_sink)
+    hit = torch.zeros(B, Hq, Lq, dv, dtype=torch.bool, device="cuda")
+    hit[0, :G, :, 1] = vis[:, key]
+    assert hit.any() and (o[hit] == INF).all()
+    orc.check(o[~hit], (value[~hit], bound[~hit]), "o")
+
+
+def test_scores_beyond_the_type():
+    """Scores of 2^17 and -2^17 (no 16-bit score could hold the first in fp16): weights of keys with one score are equal."""
+    for dtype in (BF, HF):
+        v = torch.randn(1, 1, 200, 64, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+        k = torch.full_like(v, 32.0)
+        for sign in (1, -1):
+            q = torch.full((1, 2, 200, 64), 64.0 * sign, dtype=dtype, device="cuda")
+            o = window_attention(q, k, v, 50, 2, 1.0)
+            vis = orc.seen(torch.arange(200, device="cuda"), 200, 50, 2).double()
+            p = vis / vis.sum(-1, keepdim=True)
+            mean, mag = p @ v.double(), p @ v.double().abs()
+            u = torch.finfo(dtype).eps / 2
+            orc.check(o, (mean.expand(1, 2, -1, -1), (u * (mag + 2 * mean.abs()) + orc.SLACK * mag).expand(1, 2, -1, -1)), "o")
+
+
+@pytest.mark.parametrize("Lq, Lk", [(0, 0), (0, 50), (50, 0), (1, 1), (3, 1), (1, 64)])
+def test_empty_and_single(Lq, Lk):
+    q, k, v, do = make(2, 2, 4, 2, Lq, Lk, 64, 32, BF)
+    got = against(q, k, v, do, 16, 2, 0.125)
+    assert got["o"].shape == (2, 4, Lq, 32) and got["dk"].shape == (2, 2, Lk, 64)
+    if Lk == 0:
+        assert (got["o"] == 0).all() and (got["dq"] == 0).all()
+    if Lq == 0:
+        assert (got["dk"] == 0).all() and (got["dv"] == 0).all()
+
+
+@pytest.mark.parametrize("dk, dv", [(20, 33), (64, 7), (1, 1), (127, 90), (100, 64)])
+def test_head_dims_between_multiples_of_8(dk, dv):
+    q, k, v, do = make(3, 1, 4, 2, 70, 90, dk, dv, HF)
+    against(q, k, v, do, 30, 3, 1.0 / math.sqrt(dk))
+
+
+def test_layouts():
+    """Tokens outside heads, rows that start anywhere, heads and batches that share memory, a gradient that is one number."""
+    q, k, v, do = make(4, 2, 4, 2, 100, 120, 64, 64, BF)
+    scale, args = 0.125, (40, 2, 0.125)
+    base = run(q, k, v, do, *args)
+    same = lambda got: all(torch.equal(got[n], base[n]) for n in base)  # noqa: E731
+    swap = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    assert same(run(swap(q), swap(k), swap(v), swap(do), *args))
+    apart = lambda x, off: torch.zeros(x.numel() * 2 + 64, dtype=x.dtype, device="cuda")[off:off + 2 * x.numel()].reshape(*x.shape[:-1], -1)[..., :x.shape[-1]].copy_(x)  # noqa: E731
+    assert same(run(apart(q, 8), apart(k, 16), apart(v, 0), apart(do, 8), *args))
+    assert same(run(apart(q, 1), apart(k, 3), apart(v, 5), apart(do, 7), *args))
+    last = lambda x: x.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+    assert same(run(last(q), last(k), last(v), last(do), *args))
+    # packed q, k and v: one tensor, gradients into it
+    pack = torch.randn(2, 50, 3, 4, 64, generator=torch.Generator().manual_seed(5)).to(BF).cuda().requires_grad_(True)
+    x = [pack[:, :, i].transpose(1, 2) for i in range(3)]
+    g = torch.autograd.grad(window_attention(*x, *args).sum(), pack)[0]
+    one = torch.ones(2, 4, 50, 64, dtype=BF, device="cuda")
+    want = orc.window(*(y.detach() for y in x), *args, one)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        orc.check(g[:, :, i].transpose(1, 2), want[n], n)
+    # one k and v for all batches and heads: their gradients are sums over both, in the type (a rounding each of 2 x 4 terms)
+    k1 = k[:1, :1].clone().requires_grad_(True)
+    v1 = v[:1, :1].clone().requires_grad_(True)
+    o = window_attention(q, k1.expand(2, 4, -1, -1), v1.expand(2, 4, -1, -1), *args)
+    dk, dv = torch.autograd.grad(o, (k1, v1), do)
+    want = orc.window(q, k1.detach().expand(2, 4, -1, -1), v1.detach().expand(2, 4, -1, -1), *args, do)
+    for x, n in ((dk, "dk"), (dv, "dv")):
+        value, bound = (y.sum((0, 1), keepdim=True) for y in want[n])
+        orc.check(x, (value, bound + 8 * torch.finfo(BF).eps * want[n][0].abs().sum((0, 1), keepdim=True)), n)
+
+
+def test_heads_far_apart():
+    """Heads of a group 2^30 elements and more apart are copied first; batches and kv heads may be any distance apart."""
+    big = torch.zeros((1 << 30) + 100 * 64, dtype=BF, device="cuda")
+    q, k, v, do = make(6, 1, 2, 1, 100, 100, 64, 64, BF)
+    far = lambda x: big.as_strided((1, 2, 100, 64), (0, 1 << 30, 64, 1)).copy_(x)  # noqa: E731
+    base = run(q, k, v, do, 30, 1, 0.125)
+    assert torch.equal(window_attention(far(q), k, v, 30, 1, 0.125), base["o"])
+    got = run(q, k, v, far(do), 30, 1, 0.125)
+    assert all(torch.equal(got[n], base[n]) for n in base)
+    k2, v2 = torch.cat([k, k.flip(2)], 1), torch.cat([v, v.flip(2)], 1)
+    assert torch.equal(window_attention(q, far(k2), v2, 30, 1, 0.125), window_attention(q, k2, v2, 30, 1, 0.125))
+
+
+@pytest.mark.parametrize("case", SHAPES, ids=name_of)
+def test_repeats_are_equal_on_any_stream(case):
+    B, Hq, Hkv, Lq, Lk, dk, dv, window, n_sink, dtype = case
+    q, k, v, do = make(9, B, Hq, Hkv, Lq, Lk, dk, dv, dtype)
+    base = run(q, k, v, do, window, n_sink, 0.1)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):   # two calls at once, on streams of their own
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(run(q, k, v, do, window, n_sink, 0.1))
+    torch.cuda.synchronize()
+    for got in outs:
+        assert all(torch.equal(got[n], base[n]) for n in base)
+
+
+def test_directional_differences():
+    """(L(x + h e) - L(x - h e)) / 2h of L = sum(o dO) against <grad, e>: off by what the outputs are (twice sum |dO| tol / 2h), by what the gradients
+    are, and by the remainder, which the 64-bit form has as well."""
+    q, k, v, do = make(10, 1, 4, 2, 60, 80, 64, 64, HF)
+    args, h = (25, 2, 0.125), 2.0 ** -4
+    got, want = run(q, k, v, do, *args), orc.window(q, k, v, *args, do)
+    for i, n in enumerate(("dq", "dk", "dv")):
+        x = [q, k, v]
+        e = torch.randn(x[i].shape, generator=torch.Generator().manual_seed(i)).cuda()
+        up, down = (x[i].float() + h * e).half(), (x[i].float() - h * e).half()
+        step = (up.double() - down.double())   # what the call really differs by
+        val, tol, exact = [], 0.0, []
+        for y in (up, down):
+            z = list(x)
+            z[i] = y
+            o = window_attention(*z, *args)
+            value, bound = orc.window(*z, *args)["o"]
+            val.append((o.double() * do.double()).sum())
+            exact.append((value * do.double()).sum())
+            tol += ((bound + orc.tiny(HF)) * do.double().abs()).sum()
+        grad, grad_tol = want[n]
+        remainder = (exact[0] - exact[1] - (grad * step).sum()).abs()
+        along = (got[n].double() * step).sum()
+        assert (val[0] - val[1] - along).abs() <= tol + ((grad_tol + orc.tiny(HF)) * step.abs()).sum() + remainder
+
+
+def test_derivatives_of_derivatives():
+    q, k, v, do = make(11, 1, 2, 1, 30, 30, 64, 64, BF)
+    q.requires_grad_(True)
+    g = torch.autograd.grad(window_attention(q, k, v, 8).float().pow(2).sum(), q, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        g.float().sum().backward()
+    # the rotation is linear: the derivative of its gradient by the output's gradient is the rotation
+    pos = RotaryPositionEncodingAxes.encode_pos(3, 10).cuda()
+    tables = [orc.table(3, 8).cuda(), orc.table(10, 16).cuda()]
+    x = torch.randn(1, 2, 30, 64, device="cuda", requires_grad=True)
+    w = torch.randn(1, 2, 30, 64, device="cuda", requires_grad=True)
+    y = rope_axes_qk(x, None, pos, tables)[0]
+    g = torch.autograd.grad(y, x, w, create_graph=True)[0]
+    assert torch.equal(g, rope_axes_qk(w, None, pos, tables, inverse=True)[0])
+    c = torch.randn_like(x)
+    assert torch.equal(torch.autograd.grad(g, w, c)[0], rope_axes_qk(c, None, pos, tables)[0])
+
+
+@pytest.mark.parametrize("layout, sections, C, dtype", [("blocks", (8, 16), 64, F32), ("halves", (5, 6), 30, HF), ("blocks", (6, 11, 11), 64, BF)])
+def test_rope_gradients(layout, sections, C, dtype):
+    """Against the formula (the inverse rotation), with q or k alone, shared (expanded) inputs, and differences: the rotation is linear, so that
+    <R x, w> = <x, R^T w> up to the roundings of both."""
+    gen = torch.Generator().manual_seed(12)
+    lens = (3, 5, 2)[:len(sections)]
+    pos = RotaryPositionEncodingAxes.encode_pos(*lens).cuda()
+    N = pos.shape[1]
+    tables = [orc.table(n, r).cuda() for n, r in zip(lens, sections)]
+    mk = lambda h: torch.randn(2, h, N, C, generator=gen).to(dtype).cuda()  # noqa: E731
+    q, k, wq, wk = mk(4), mk(2), mk(4), mk(2)
+    q.requires_grad_(True), k.requires_grad_(True)
+    yq, yk = rope_axes_qk(q, k, pos, tables, layout)
+    dq, dk = torch.autograd.grad((yq, yk), (q, k), (wq, wk), retain_graph=True)
+    for g, w, x, y in ((dq, wq, q, yq), (dk, wk, k, yk)):
+        orc.check(g, orc.rotate(w, pos, tables, layout, inverse=True), "gradient")
+        tol = (orc.rotate(x.detach(), pos, tables, layout)[1] * w.double().abs()).sum() + (orc.rotate(w, pos, tables, layout, True)[1] * x.detach().double().abs()).sum()
+        assert ((y.detach().double() * w.double()).sum() - (x.detach().double() * g.double()).sum()).abs() <= tol + 1e-3 * (dtype == HF) + 1e-9
+    assert torch.equal(torch.autograd.grad(yk, k, wk, retain_graph=True)[0], dk)
+    assert torch.equal(torch.autograd.grad(yq, q, wq, retain_graph=True)[0], dq)
+    assert torch.equal(torch.autograd.grad(rope_axes_qk(q, None, pos, tables, layout)[0], q, wq)[0], dq)
+    one = k[:1, :1].detach().clone().requires_grad_(True)
+    wide = rope_axes_qk(one.expand(2, 4, -1, -1), None, pos, tables, layout)[0]
+    g = torch.autograd.grad(wide, one, wq)[0]
+    value, bound = (x.sum((0, 1), keepdim=True) for x in orc.rotate(wq, pos, tables, layout, inverse=True))
+    orc.check(g, (value, bound + 8 * torch.finfo(dtype).eps * orc.rotate(wq, pos, tables, layout, True)[0].abs().sum((0, 1), keepdim=True)), "shared")
+
+
+def test_rope_special_values_and_sides():
+    """A NaN stays within its pair, dims that are not rotated keep their bits, empty tensors pass."""
+    pos = torch.tensor([[0, 1, -1, 3]], dtype=torch.int32, device="cuda")
+    tables = [orc.table(5, 4).cuda()]
+    x = torch.randn(1, 2, 4, 16, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+    clean = rope_axes_qk(x, None, pos, tables)[0]
+    y = x.clone()
+    y[0, 0, 1, 2], y[0, 1, 2, 0], y[0, 1, 3, 12] = NAN, NAN, INF
+    got = rope_axes_qk(y, None, pos, tables)[0]
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[0, 0, 1, [2, 6]] = bad[0, 1, 2, 0] = True
+    assert got[bad].isnan().all() and got[0, 1, 3, 12] == INF
+    bad[0, 1, 3, 12] = True
+    assert torch.equal(got[~bad], clean[~bad])
+    assert torch.equal(got[..., 8:][~bad[..., 8:]], x[..., 8:][~bad[..., 8:]])
+    for shape in ((0, 2, 4, 16), (1, 0, 4, 16), (1, 2, 0, 16)):
+        e = torch.zeros(shape, dtype=BF, device="cuda")
+        p = pos[:, :0] if shape[2] == 0 else pos
+        assert rope_axes_qk(e, None, p, tables)[0].shape == shape and rope_axes_qk_(e, e.clone(), p, tables)[0] is e
+
+
+def test_rope_layouts_and_refusals():
+    case = torch.Generator().manual_seed(2)
+    pos = RotaryPositionEncodingAxes.encode_pos(4, 6).cuda()
+    tables = [orc.table(4, 8).cuda(), orc.table(6, 12).cuda()]
+    q, k = (torch.randn(2, h, 24, 64, generator=case).to(HF).cuda() for h in (3, 2))
+    for layout in ("blocks", "halves"):
+        want = rope_axes_qk(q, k, pos, tables, layout)
+        swap = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+        last = lambda x: x.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+        odd = lambda x: torch.zeros(x.numel() + 7, dtype=x.dtype, device="cuda")[3:3 + x.numel()].reshape(x.shape).copy_(x)  # noqa: E731
+        for f in (swap, last, odd):
+            assert all(torch.equal(a, b) for a, b in zip(rope_axes_qk(f(q), f(k), pos, tables, layout), want))
+            a, b = f(q), f(k)
+            rope_axes_qk_(a, b, pos, tables, layout)
+            assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+        # positions and tables of other strides and types
+        p2 = pos.t().contiguous().t()
+        t2 = [t.double() for t in tables]
+        t3 = [torch.cat([t, t], 1)[:, :t.shape[1]] for t in tables]
+        for p, t in ((p2, tables), (pos, t2), (pos, t3), (pos[:, None].expand(-1, 2, -1), tables)):
+            assert all(torch.equal(a, b) for a, b in zip(rope_axes_qk(q, k, p, t, layout), want))
+        # q and k as parts of one tensor, rotated in place
+        pack = torch.cat([q, k], 1)
+        rope_axes_qk_(pack[:, :3], pack[:, 3:], pos, tables, layout)
+        assert torch.equal(pack, torch.cat(want, 1))
+    with pytest.raises(RuntimeError, match="two tensors"):
+        rope_axes_qk_(q, q, pos, tables)
+    with pytest.raises(RuntimeError, match="share memory"):
+        rope_axes_qk_(q[:, :1].expand(-1, 3, -1, -1), None, pos, tables)
+    with pytest.raises(TypeError):
+        rope_axes_qk(q, k, pos.long(), tables)
+    with pytest.raises(ValueError, match="every axis"):
+        rope_axes_qk(q, k, pos[:1], tables)
+    with pytest.raises(RuntimeError, match="on one device|ROCm GPU only"):
+        rope_axes_qk(q, k, pos.cpu(), tables)
+    with pytest.raises(AssertionError):
+        rope_axes_qk(q, k.float(), pos, tables)
+    # written in place after it was saved
+    x = q.clone().requires_grad_(True)
+    y = rope_axes_qk(x * 1, None, pos, tables)[0]
+    z = y * y
+    rope_axes_qk_(y.detach(), None, pos, tables)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.sum().backward()
+
+
+def test_other_paths_of_autograd():
+    """Dispatch modes take the classes, hooks and checkpoints the compiled nodes: all give the same bits."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from torch.utils.checkpoint import checkpoint
+
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    q, k, v, do = make(13, 1, 4, 2, 60, 70, 40, 36, BF)
+    pos = RotaryPositionEncodingAxes.encode_pos(6, 10).cuda()
+    tables = [orc.table(6, 8).cuda(), orc.table(10, 12).cuda()]
+
+    def step(wrap=lambda f, *a: f(*a)):
+        a, b, c = (x.detach().requires_grad_(True) for x in (q, k, v))
+
+        def f(a, b, c):
+            r = rope_axes_qk(a, None, pos, tables)[0]
+            return window_attention(r, b, c, 20, 2)
+        return torch.autograd.grad(wrap(f, a, b, c), (a, b, c), do)
+    base = step()
+    with Seen():
+        modes = step()
+    with torch.autograd.graph.save_on_cpu():
+        hooks = step()
+    again = step(lambda f, *a: checkpoint(f, *a, use_reentrant=False))
+    for other in (modes, hooks, again):
+        assert all(torch.equal(x, y) for x, y in zip(base, other))
+
+
+# ---- the cache -----------------------------------------------------------------------------------------------------------------------
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def test_cache_refusals():
+    cache = torch.zeros(4, 2, 16, 64, dtype=BF, device="cuda")
+    x = torch.zeros(1, 2, 3, 64, dtype=BF, device="cuda")
+    table, seq = ints(0, 1)[None], ints(3)
+    with pytest.raises(RuntimeError, match="two tensors"):
+        paged_append_(cache, cache, x, x, table, seq)
+    with pytest.raises(RuntimeError, match="share memory"):
+        paged_append_(cache[:1].expand(4, -1, -1, -1), cache, x, x, table, seq)
+    with pytest.raises(RuntimeError, match="leaf Variable"):
+        paged_append_(cache.clone().requires_grad_(True), cache, x, x, table, seq)
+    with pytest.raises(RuntimeError, match="on one device|ROCm GPU only"):
+        paged_append_(cache, cache.clone(), x, x, table.cpu(), seq)
+    with pytest.raises(RuntimeError, match="on one device|ROCm GPU only"):
+        paged_attention(x, cache, cache, table, seq.cpu())
+    with pytest.raises(ValueError, match="16 bytes"):
+        paged_attention(x, cache.transpose(2, 3).contiguous().transpose(2, 3), cache, table, seq)
+    with pytest.raises(Exception, match="multiple of 16"):
+        paged_attention(x, cache[:, :, :8].contiguous(), cache[:, :, :8].contiguous(), table, seq)
+    with pytest.raises(Exception, match="fp32"):
+        paged_attention(x.float(), cache.float(), cache.float(), table, seq)
+    with pytest.raises(Exception, match="evenly"):
+        paged_attention(x[:, :1], cache, cache, table, seq)
+
+
+def test_append_writes_nothing_it_should_not():
+    """Page numbers outside the cache, positions outside the table or before its start, padding: the rest of the cache keeps its bits."""
+    gen = torch.Generator().manual_seed(20)
+    for dtype, D, page in ((BF, 64, 16), (F32, 20, 5)):
+        kc, vc = (torch.randn(6, 2, page, D, generator=gen).to(dtype).cuda() for _ in range(2))
+        k, v, q = (torch.randn(5, h, 4, D, generator=gen).to(dtype).cuda() for h in (2, 2, 3))
+        # -1 and 6: not pages of the cache; sequence 2 ends behind its table, 3 has more new tokens than tokens, 4 says more new tokens than there are
+        table = ints(0, -1, 6, 1, 2, 3, 4, 0, 5, 0).reshape(5, 2)
+        seq, new = ints(page + 2, page + 2, 2 * page + 2, 2, 4), ints(4, 4, 4, 4, 9)
+        for with_pos in (False, True):
+            for rope in (False, True):
+                a, b = kc.clone(), vc.clone()
+                tables = [orc.table(64, D // 2).cuda()]
+                places = [[min(max(int(seq[i]) - min(int(new[i]), 4) + t, -1), 63) for t in range(4)] for i in range(5)]
+                pos = torch.tensor(places, dtype=torch.int32, device="cuda")[None]
+                out = paged_append_(a, b, k, v, table, seq, new, (pos if with_pos else None, tables, "halves") if rope else None, q)
+                want_k = orc.rotate(k, pos, tables, "halves") if rope else (k.double(), torch.zeros_like(k, dtype=torch.float64))
+                wk, tk, wv = kc.double(), torch.zeros_like(kc, dtype=torch.float64), vc.clone()
+                for i in range(5):
+                    for t in range(4):
+                        p = int(seq[i]) - min(int(new[i]), 4) + t
+                        if not 0 <= p < 2 * page:
+                            continue
+                        at = int(table[i, p // page])
+                        if not 0 <= at < 6:
+                            continue
+                        wk[at, :, p % page], tk[at, :, p % page], wv[at, :, p % page] = want_k[0][i, :, t], want_k[1][i, :, t], v[i, :, t]
+                orc.check(a, (wk, tk), "keys")
+                assert torch.equal(b, wv)
+                if not rope:
+                    assert torch.equal(out, q)
+                else:
+                    seen = pos[0] >= 0
+                    orc.check(out.transpose(1, 2)[seen], tuple(x.transpose(1, 2)[seen] for x in orc.rotate(q, pos, tables, "halves")), "queries")
+
+
+def dense_of(cache, table, n):
+    return cache[table.long()].transpose(1, 2).reshape(table.shape[0], cache.shape[1], -1, cache.shape[3])[:, :, :n]
+
+
+@pytest.mark.parametrize("H, Hkv, D, lens, window, dtype", [(4, 2, 64, (300, 40), None, BF), (8, 1, 128, (3000, 2000), 1000, HF), (2, 2, 64, (6000, 1), None, HF), (8, 8, 80, (500, 499), 100, BF)])
+def test_special_values_in_the_cache(H, Hkv, D, lens, window, dtype):
+    gen = torch.Generator().manual_seed(21)
+    cols = -(-max(lens) // 16)
+    table = torch.randperm(2 * cols, generator=gen).reshape(2, cols).to(torch.int32).cuda()
+    kc, vc = (torch.randn(2 * cols, Hkv, 16, D, generator=gen).to(dtype).cuda() for _ in range(2))
+    q = torch.randn(2, H, 2, D, generator=gen).to(dtype).cuda()
+    seq, scale, G = ints(*lens), 1.0 / math.sqrt(D), H // Hkv
+    base = paged_attention(q, kc, vc, table, seq, window, 3, scale)
+    n = lens[0]
+    place = lambda c, b, p: c[int(table[b, p // 16]), 0, p % 16]  # noqa: E731
+    k2, v2 = kc.clone(), vc.clone()
+    at = n - 1 - min(window or n, n) // 2
+    place(v2, 0, at)[5] = INF
+    o = paged_attention(q, kc, v2, table, seq, window, 3, scale)
+    assert (o[0, :G, :, 5] == INF).all()
+    o[0, :G, :, 5] = base[0, :G, :, 5]
+    want = orc.window(q[:1], dense_of(kc, table[:1], n), dense_of(vc, table[:1], n), window, 3, scale)["o"]
+    orc.check(o[:1], want, "o")
+    assert torch.equal(o[1], base[1])
+    place(k2, 0, at)[0] = NAN
+    o = paged_attention(q, k2, vc, table, seq, window, 3, scale)
+    assert o[0, :G].isnan().all() and torch.equal(o[0, G:], base[0, G:]) and torch.equal(o[1], base[1])
+    if window is not None and n > window + 10:   # a key nobody sees any more
+        k2, v2 = kc.clone(), vc.clone()
+        place(k2, 0, 5)[:] = NAN
+        place(v2, 0, 6)[:] = INF
+        # rows that meet an infinity in a masked place are summed once more, with weights of 32 bits: other roundings than before, within the same bound
+        o = paged_attention(q, k2, v2, table, seq, window, 3, scale)
+        orc.check(o[:1], want, "o")
+        assert torch.equal(o[1], base[1])
+
+
+def test_lengths_out_of_range_and_empty_calls():
+    gen = torch.Generator().manual_seed(22)
+    kc, vc = (torch.randn(8, 2, 16, 64, generator=gen).to(BF).cuda() for _ in range(2))
+    table = torch.arange(8, dtype=torch.int32, device="cuda").reshape(4, 2)
+    q = torch.randn(4, 4, 3, 64, generator=gen).to(BF).cuda()
+    # a negative length, none, fewer tokens than new ones, more than the table holds (taken as all it holds)
+    o = paged_attention(q, kc, vc, table, ints(-5, 0, 2, 1000), None, 0, None, ints(3, 2, 3, -1))
+    assert (o[0] == 0).all() and (o[1] == 0).all() and (o[2, :, 0] == 0).all() and (o[3] == 0).all()
+    want = orc.window(q[2:3, :, 1:], dense_of(kc, table[2:3], 2), dense_of(vc, table[2:3], 2), None, 0, 0.125)["o"]
+    orc.check(o[2:3, :, 1:], want, "o")
+    o = paged_attention(q, kc, vc, table, ints(32, 32, 32, 1000))
+    orc.check(o[3:], orc.window(q[3:], dense_of(kc, table[3:], 32), dense_of(vc, table[3:], 32), None, 0, 0.125)["o"], "o")
+    assert paged_attention(q[:, :, :0], kc, vc, table, ints(1, 2, 3, 4)).shape == (4, 4, 0, 64)
+    assert paged_attention(q[:0], kc, vc, table[:0], ints()).shape == (0, 4, 3, 64)
+    before = kc.clone()
+    assert paged_append_(kc, vc, q[:, :2, :0], q[:, :2, :0], table, ints(1, 2, 3, 4)) is None
+    assert paged_append_(kc, vc, q[:0, :2], q[:0, :2], table[:0], ints(), q=q[:0]).shape == (0, 4, 3, 64)
+    assert torch.equal(kc, before)
+
+
+def test_cache_offsets_beyond_32_bits():
+    """Pages whose bytes and elements lie behind 2^32, keys of one sequence at both ends."""
+    pages = (1 << 32) // (2 * 16 * 128) + 40
+    kc, vc = (torch.empty(pages, 2, 16, 128, dtype=BF, device="cuda") for _ in range(2))
+    gen = torch.Generator().manual_seed(23)
+    q, k, v = (torch.randn(2, h, 200, 128, generator=gen).to(BF).cuda() for h in (4, 2, 2))
+    cols = 13
+    table = torch.stack([torch.arange(cols) * 2 % 26, pages - 1 - torch.arange(cols) * 2]).to(torch.int32).cuda()
+    table[0, 3], table[1, 5] = pages - 30, 35
+    seq = ints(200, 200)
+    assert paged_append_(kc, vc, k, v, table, seq, None, (None, [orc.table(200, 64).cuda()], "halves")) is None
+    pos = torch.arange(200, dtype=torch.int32, device="cuda")[None]
+    rk = rope_axes_qk(k, None, pos, [orc.table(200, 64).cuda()], "halves")[0]
+    assert torch.equal(dense_of(kc, table, 200), rk) and torch.equal(dense_of(vc, table, 200), v)
+    o = paged_attention(q[:, :, -3:], kc, vc, table, seq)
+    orc.check(o, orc.window(q[:, :, -3:], rk, v, None, 0, 1.0 / math.sqrt(128))["o"], "o")
+    o = paged_attention(q, kc, vc, table, seq, 64, 4)
+    orc.check(o, orc.window(q, rk, v, 64, 4, 1.0 / math.sqrt(128))["o"], "o")
+
+
+def test_cache_views():
+    """Keys and values in one tensor, heads outside pages, tables with longer rows, queries in any layout."""
+    gen = torch.Generator().manual_seed(24)
+    both = torch.zeros(20, 2, 2, 32, 64, dtype=HF, device="cuda")
+    kc, vc = both[:, 0], both[:, 1]
+    outer = torch.zeros(2, 2, 20, 32, 64, dtype=HF, device="cuda")
+    kc2, vc2 = outer[0].transpose(0, 1), outer[1].transpose(0, 1)
+    wide = torch.randperm(20, generator=gen).reshape(2, 10).to(torch.int32).cuda()
+    table = wide[:, :4]
+    k, v, q = (torch.randn(2, h, 100, 64, generator=gen).to(HF).cuda() for h in (2, 2, 4))
+    seq = ints(100, 128)
+    for a, b in ((kc, vc), (kc2, vc2)):
+        paged_append_(a, b, k, v, table, seq)
+    o = paged_attention(q, kc, vc, table, seq, 50, 1)
+    assert torch.equal(o, paged_attention(q, kc2, vc2, table, seq, 50, 1))
+    assert torch.equal(o, paged_attention(q.transpose(1, 2).contiguous().transpose(1, 2), kc, vc, table, seq, 50, 1))
+    assert torch.equal(o, paged_attention(q.transpose(2, 3).contiguous().transpose(2, 3), kc, vc, table, seq, 50, 1))
+    orc.check(o[:1], orc.window(q[:1], k[:1], v[:1], 50, 1, 0.125)["o"], "o")
+
+
+# ---- graphs --------------------------------------------------------------------------------------------------------------------------
+def captured(f):
+    """(graph, outputs): `f` recorded after a warm call on another stream."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        f()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = f()
+    return g, out
+
+
+def test_a_decode_loop_in_a_graph():
+    """Append with the rotation and attention, recorded once: every replay works on what the lengths and tensors hold then."""
+    gen = torch.Generator().manual_seed(30)
+    B, H, Hkv, D, page, cols = 3, 8, 2, 64, 16, 160
+    tables = [orc.table(cols * page, D // 2).cuda()]
+    table = torch.randperm(B * cols, generator=gen).reshape(B, cols).to(torch.int32).cuda()
+    start = [torch.randn(B * cols, Hkv, page, D, generator=gen).to(BF).cuda() for _ in range(2)]
+    caches, plain = [x.clone() for x in start], [x.clone() for x in start]
+    q, k, v = (torch.zeros(B, h, 1, D, dtype=BF, device="cuda") for h in (H, Hkv, Hkv))
+    seq = ints(1, 1, 1)
+
+    def step(kc, vc):
+        r = paged_append_(kc, vc, k, v, table, seq, None, (None, tables, "halves"), q)
+        return paged_attention(r, kc, vc, table, seq, 900, 4)
+    g, out = captured(lambda: step(*caches))
+    for x, y in zip(caches, start):
+        x.copy_(y)
+    lens = torch.tensor([20, 2000, 0], dtype=torch.int32)
+    for i in range(6):
+        lens += 1
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=gen))
+        seq.copy_(lens)
+        torch.cuda.synchronize()
+        g.replay()
+        got = out.clone()
+        want = step(*plain)
+        assert torch.equal(got, want) and torch.equal(caches[0], plain[0]) and torch.equal(caches[1], plain[1])
+
+
+def test_training_step_in_a_graph():
+    """Rotation and window attention forward and backward; two graphs with one pool, replayed in turn, give the eager bits every time."""
+    gen = torch.Generator().manual_seed(31)
+    pos = RotaryPositionEncodingAxes.encode_pos(3, 20, 25).cuda()
+    tables = [orc.table(n, r).cuda() for n, r in zip((3, 20, 25), (8, 12, 12))]
+    shapes = [(2, 4, 1500, 64), (2, 2, 1500, 64), (2, 2, 1500, 64)]
+
+    def step(leaves, window):
+        q, k = rope_axes_qk(leaves[0], leaves[1], pos, tables)
+        o = window_attention(q, k, leaves[2], window, 3)
+        return (o.detach(),) + torch.autograd.grad(o, leaves, o.detach())
+    leaves = [torch.zeros(s, dtype=BF, device="cuda", requires_grad=True) for s in shapes]
+    pool = torch.cuda.graph_pool_handle()
+    graphs = []
+    for window in (100, 700):
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            step(leaves, window)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            graphs.append((g, step(leaves, window), window))
+    for i in range(4):
+        with torch.no_grad():
+            for x in leaves:
+                x.copy_(torch.randn(x.shape, generator=gen))
+        got = []
+        for g, out, _ in graphs:
+            g.replay()
+            got.append([x.clone() for x in out])
+        torch.cuda.synchronize()
+        for (_, _, window), x in zip(graphs, got):
+            want = step([y.detach().clone().requires_grad_(True) for y in leaves], window)
+            assert all(torch.equal(a, b) for a, b in zip(x, want))
+
+
+def test_a_captured_backward_pass_refuses_leaves_of_a_live_graph():
+    """The gradient of such a leaf belongs to the default stream, which a capture may not wait for: refused before the engine passes it on."""
+    q, k, v, _ = make(32, 1, 2, 2, 40, 40, 64, 64, BF)
+    q.requires_grad_(True)
+    pos = RotaryPositionEncodingAxes.encode_pos(40).cuda()
+    tables = [orc.table(40, 32).cuda()]
+    for f in (lambda: window_attention(q, k, v, 8), lambda: rope_axes_qk(q, None, pos, tables)[0]):
+        eager = f()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = f()
+            with pytest.raises(RuntimeError, match="graph of the default stream"):
+                torch.autograd.grad(o, q, o.detach())
+        torch.cuda.synchronize()
+        assert torch.autograd.grad(eager, q, eager.detach())[0].isfinite().all()
+        del eager, o
+
+
+# ---- together ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("H, Hkv, D, page, window, n_sink, layout, dtype", [(8, 2, 64, 16, None, 0, "halves", BF), (6, 6, 128, 48, 100, 4, "blocks", HF), (4, 1, 80, 32, 33, 1, "halves", BF)])
+def test_prompts_and_steps_through_the_cache_match_the_dense_window(H, Hkv, D, page, window, n_sink, layout, dtype):
+    """Three sequences of other lengths: a padded batch of prompts, then single tokens.  What the cache holds are the bits of the rotated keys, and
+    its attention is the window's over the whole sequence, both within the bounds of the 64-bit form."""
+    gen = torch.Generator().manual_seed(40)
+    prompt, steps, B = (150, 1, 77), 12, 3
+    total = [n + steps for n in prompt]
+    cols = -(-max(total) // page)
+    table = torch.randperm(B * cols, generator=gen).reshape(B, cols).to(torch.int32).cuda()
+    kc, vc = (torch.full((B * cols, Hkv, page, D), NAN, dtype=dtype, device="cuda") for _ in range(2))
+    mk = lambda h: torch.randn(B, h, max(total), D, generator=gen).to(dtype).cuda()  # noqa: E731
+    q, k, v = mk(H), mk(Hkv), mk(Hkv)
+    tables = [orc.table(max(total), D // 2).cuda()]
+    pos = torch.arange(max(total), dtype=torch.int32, device="cuda")[None]
+    rq, rk = rope_axes_qk(q, k, pos, tables, layout)
+    outs = [[] for _ in range(B)]
+    T = max(prompt)
+    seq, new = ints(*prompt), ints(*prompt)
+    r = paged_append_(kc, vc, k[:, :, :T], v[:, :, :T], table, seq, new, (None, tables, layout), q[:, :, :T])
+    o = paged_attention(r, kc, vc, table, seq, window, n_sink, None, new)
+    for b in range(B):
+        outs[b].append(o[b, :, :prompt[b]])
+        assert (o[b, :, prompt[b]:] == 0).all() and torch.equal(r[b, :, prompt[b]:], q[b, :, prompt[b]:T])
+    for s in range(steps):
+        at = [n + s for n in prompt]
+        one = lambda x: torch.stack([x[b, :, at[b]:at[b] + 1] for b in range(B)])  # noqa: E731
+        seq += 1
+        r = paged_append_(kc, vc, one(k), one(v), table, seq, None, (None, tables, layout), one(q))
+        assert torch.equal(r, one(rq))
+        o = paged_attention(r, kc, vc, table, seq, window, n_sink)
+        for b in range(B):
+            outs[b].append(o[b])
+    for b in range(B):
+        n = total[b]
+        assert torch.equal(dense_of(kc, table[b:b + 1], n)[0], rk[b, :, :n]) and torch.equal(dense_of(vc, table[b:b + 1], n)[0], v[b, :, :n])
+        want = orc.window(rq[b:b + 1, :, :n], rk[b:b + 1, :, :n], v[b:b + 1, :, :n], window, n_sink, 1.0 / math.sqrt(D))["o"]
+        orc.check(torch.cat(outs[b], 1)[None], want, f"sequence {b} through the cache")
+        orc.check(window_attention(rq[b:b + 1, :, :n], rk[b:b + 1, :, :n], v[b:b + 1, :, :n], window, n_sink), want, f"sequence {b}, dense")
