@@ -94,27 +94,46 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
   if (lane == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
-// dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares
+// dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares.  Keys with far sums, of which there are up to hundreds,
+// come first, a workgroup to a key, where 8 runs of threads take every eighth sum (one run: 9 us for 16 keys of 112 sums on 4 heads, this way 5.5).
 template <typename TIO>
 __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
+  __shared__ f32x4 run[8][32];
   const bool keys = blockIdx.y == 0;
   const int dims = keys ? a.dk_ : a.dv_, per = dims / 4;
-  const BandParts P(a, band_kv_group(band_class(a.dk_, a.dv_)));
+  const BandParts P(a);
   const float *part = a.part + (keys ? 0 : P.v_at), *fpart = a.part + (keys ? P.far_at : P.v_at + P.v_far_at);
-  const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t at = gid / per;
-  const int d = 4 * (int)(gid - at * per);
-  if (at >= (int64_t)a.B * a.Hkv * P.keys) return;
-  const int bh = (int)(at / P.keys), j = (int)(at - (int64_t)bh * P.keys), b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const int n_far = (int)dlt_imin64(P.far_keys, P.keys), far_blocks = a.B * a.Hkv * n_far;
+  const bool far = (int)blockIdx.x < far_blocks;
+  int bh, j, d;
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (far) {
+    bh = blockIdx.x / n_far;
+    j = blockIdx.x - bh * n_far;
+    const int c = threadIdx.x & 31, r = threadIdx.x >> 5, n = 4 * a.far;
+    d = 4 * c;
+    if (c < per) {
+      const float* p = fpart + ((int64_t)bh * n * P.far_keys + j) * dims + d;
+#pragma unroll 4
+      for (int i = r; i < n; i += 8) s += *reinterpret_cast<const f32x4*>(p + (int64_t)i * P.far_keys * dims);
+    }
+    run[r][c] = s;
+    __syncthreads();
+    if (r != 0 || c >= per) return;
+    for (int i = 1; i < 8; i++) s += run[i][c];
+  } else {
+    const int64_t gid = (int64_t)(blockIdx.x - far_blocks) * 256 + threadIdx.x, at = gid / per, n = P.keys - n_far;
+    d = 4 * (int)(gid - at * per);
+    if (at >= (int64_t)a.B * a.Hkv * n) return;
+    bh = (int)(at / n);
+    j = n_far + (int)(at - bh * n);
+  }
 #pragma unroll 4
   for (int i = 0; i < a.shares; i++) s += *reinterpret_cast<const f32x4*>(part + (((int64_t)bh * a.shares + i) * P.keys + j) * dims + d);
-  if (j < P.far_keys) {
-#pragma unroll 8
-    for (int i = 0; i < 4 * a.far; i++) s += *reinterpret_cast<const f32x4*>(fpart + (((int64_t)bh * a.far * 4 + i) * P.far_keys + j) * dims + d);
-  }
   if (keys) s *= a.sm_scale;
-  TIO* p = keys ? reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1] + j * a.dks[2] : reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1] + j * a.dvs[2];
+  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  TIO* p = keys ? reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1] + j * a.dks[2]
+                : reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1] + j * a.dvs[2];
   u32x2 w;
   w.x = pack2<TIO>(s[0], s[1]);
   w.y = pack2<TIO>(s[2], s[3]);
@@ -123,10 +142,10 @@ __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
 
 int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
   if (backward ? a.part_keys == 0 : a.shares <= 1) return DLT_OK;
-  const int64_t rows = (int64_t)a.B * a.Hkv * (backward ? a.part_keys : a.rows);
+  const int64_t bh = (int64_t)a.B * a.Hkv, rows = bh * a.rows, far = backward ? bh * dlt_imin64(BandParts(a).far_keys, a.part_keys) : 0;
   const int per = dlt_imax(a.dk_, a.dv_) / 4;
   const bool wg = a.shares > 8;
-  const dim3 grid((unsigned)(backward ? (rows * per + 255) / 256 : wg ? rows : (rows + 3) / 4), backward ? 2 : 1);
+  const dim3 grid((unsigned)(backward ? far + ((bh * a.part_keys - far) * per + 255) / 256 : wg ? rows : (rows + 3) / 4), backward ? 2 : 1);
   dlt_timing_before(backward ? DLT_K_BWD_KV : DLT_K_FWD, stream);
   if (backward) {
     if (dtype == DLT_BF16) hipLaunchKernelGGL(band_join_kv_kernel<bf16_t>, grid, dim3(256), 0, stream, a);
@@ -222,8 +241,9 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
 
 // ---- cutting a call into workgroups ---------------------------------------------------------------------------------------------------
 // Rows: how many a workgroup has, and how many workgroups share the keys of a block of rows.
-//   BAND_TWO     128 rows, where that makes two workgroups a CU
-//   BAND_ONE     64 rows otherwise
+//   BAND_TWO     128 rows, where that makes two workgroups a CU (8 kv heads of 6000 tokens, d = 64, one and a half a CU: forward 29 us by 64 rows, 37 by 128; dQ 33, 42)
+//   BAND_ONE     64 rows otherwise, and in a forward pass over few keys at d <= 64, whose set-up weighs more than its reads of LDS (64 kv heads of 4444 rows, window 300, d = 64: 78 ->
+//                72 us; window 500 78 -> 76; window 1024 69 -> 70; at d = 128 107 -> 114; dQ 74 -> 82)
 //   BAND_HALVES  64 rows, their keys over two groups of waves, while one workgroup a CU is all there is and the keys of a block are too few, or the workgroups too many, to be
 //                shared: a wave alone on its SIMD waits out every latency.  8 heads of 2048 queries, d = 64 / 128, us: 2560 keys each 32 -> 25 / 46 -> 35; 640 keys 11.7 -> 11.7 /
 //                16.4 -> 15.2; 4 heads, 640 keys, 10.1 + 6.3 for the sum of 4 shares -> 11.0 / 14.6 + 5.9 -> 14.0; but 12 heads (384 workgroups) 14.6 -> 19.7 / 20 -> 26
@@ -238,6 +258,7 @@ int plan_rows(BandArgs& a, bool forward) {
   auto blocks = [&](int own) { return (a.rows + own - 1) / own; };
   auto chunks = [&](int own) { return (int)dlt_imin64((int64_t)a.W + a.S + own / a.G + 1, a.Lk) / 64 + 1; };   // of 64 keys, of a block
   int kind = a.rows <= 64 || bh * blocks(128) < 2 * cus ? BAND_ONE : BAND_TWO;
+  if (forward && band_class(a.dk_, a.dv_) == 64 && chunks(128) <= 12) kind = BAND_ONE;
   const int64_t one = bh * blocks(64);
   const bool uneven = paged && 2 * one > cus && 2 * one <= 3 * cus && chunks(64) > 32;
   if (forward && kind == BAND_ONE && one <= cus && !uneven) {
@@ -257,15 +278,16 @@ int plan_rows(BandArgs& a, bool forward) {
   return kind;
 }
 int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
-int64_t keys_bytes(const BandArgs& a) { return a.part_keys > 0 ? BandParts(a, band_kv_group(band_class(a.dk_, a.dv_))).floats * 4 : 0; }
+int64_t keys_bytes(const BandArgs& a) { return a.part_keys > 0 ? BandParts(a).floats * 4 : 0; }
 // Keys: the rows that see a block of keys taken by several workgroups where blocks are few, the far rows of sinks always
 void plan_keys(BandArgs& a) {
   const int cus = dlt_device_cus();
-  const int cls = band_class(a.dk_, a.dv_), own = band_kv_own(cls), group = band_kv_group(cls);
+  const int64_t bh = (int64_t)a.B * a.Hkv;
+  constexpr int own = BAND_KV_OWN, group = 16;
   a.nblk = (a.Lk + own - 1) / own;
   a.shares = 1;
   a.far = a.far_groups = a.part_keys = 0;
-  const int64_t bh = (int64_t)a.B * a.Hkv, wgs = bh * a.nblk;
+  const int64_t wgs = bh * a.nblk;
   const int64_t near_chunks = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;   // of a block without sinks
   const int64_t want = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
   const int64_t key_bytes = dlt_imax64(bh * a.Lk * (a.dk_ + a.dv_) * 4, 1);

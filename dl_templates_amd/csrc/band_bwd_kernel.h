@@ -259,13 +259,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 }
 
 // Sinks are seen by every later row, so a block of keys with sinks would have the rows of the whole sequence where others have those of a
-// window.  The rows behind the block's window ("far" rows) are therefore taken by workgroups of their own, a share of the rows each: the 16 NP keys
+// window.  The rows behind the block's window ("far" rows) are therefore taken by workgroups of their own, a share of the rows each: the 16 keys
 // of a far workgroup belong to all its waves, which take 16 of a chunk's 64 rows each, with half-filled second products.  Far workgroups
 // and the blocks with sinks leave partial sums, which a second launch adds in a fixed order.  16 heads on 4, 8192 tokens, window 1024, 4 sinks,
 // d = 128: 876 us with the far rows in the block, 187 with workgroups of 1024 far rows, launched first, beside it.
 // ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
-template <typename TIO, int D, int NP, int CK, int NW, int PAD>
-__global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs a) {
+template <typename TIO, int D, int PAD>
+__global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
+  constexpr int NP = 1, CK = 64, NW = 4;   // blocks of 16 keys a wave, rows of a chunk, waves
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(64 * NW, 2) void band_bwd_kv_kernel(const BandArgs 
     }
   };
   if (far || a.shares > 1 || (a.far != 0 && x0 < a.S)) {
-    const BandParts P(a, 16 * NP);
+    const BandParts P(a);
     float* pk = a.part + (far ? P.far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dk_ : ((int64_t)bh * a.shares + share) * P.keys * a.dk_);
     float* pv = a.part + P.v_at + (far ? P.v_far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dv_ : ((int64_t)bh * a.shares + share) * P.keys * a.dv_);
     const int len = far ? (int)P.far_keys : a.Lk;

@@ -42,10 +42,10 @@ DLT_HD int64_t dlt_imax64(int64_t a, int64_t b) { return a > b ? a : b; }
 // Partial sums of the dK / dV kernel in `part`: dK rows [bh][share][keys], far dK rows [bh][far share, wave][far_keys], then the same of dV
 struct BandParts {
   int64_t keys, far_keys, far_at, v_at, v_far_at, floats;   // far_at from the start, v_far_at from v_at on
-  DLT_HD BandParts(const BandArgs& a, int group) {
+  DLT_HD BandParts(const BandArgs& a) {
     const int64_t bh = (int64_t)a.B * a.Hkv;
     keys = a.part_keys;
-    far_keys = (int64_t)a.far_groups * group;
+    far_keys = (int64_t)a.far_groups * 16;
     far_at = bh * a.shares * keys * a.dk_;
     v_at = far_at + bh * a.far * 4 * far_keys * a.dk_;
     v_far_at = bh * a.shares * keys * a.dv_;

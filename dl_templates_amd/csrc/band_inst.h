@@ -68,9 +68,8 @@ int DLT_BCAT(dlt_band_bwd_q_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind
 #else
 template <typename TIO>
 int band_bwd_kv(const BandArgs& a, hipStream_t stream) {
-  constexpr int NP = band_kv_own(D) / 64;
-  constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF_KV, 64 * NP);
-  return band_go(band_whole(a) ? band_bwd_kv_kernel<TIO, D, NP, 64, 4, 0> : band_bwd_kv_kernel<TIO, D, NP, 64, 4, 1>, a,
+  constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF_KV, 64);
+  return band_go(band_whole(a) ? band_bwd_kv_kernel<TIO, D, 0> : band_bwd_kv_kernel<TIO, D, 1>, a,
                  (int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + a.far * a.far_groups), 256, lds, DLT_K_BWD_KV, "window dK/dV launch", stream);
 }
 }  // namespace

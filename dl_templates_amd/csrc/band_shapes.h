@@ -16,8 +16,7 @@ int dlt_band_bwd_q_128(const BandArgs& a, int dtype, int kind, hipStream_t strea
 int dlt_band_bwd_kv_64(const BandArgs& a, int dtype, hipStream_t stream);
 int dlt_band_bwd_kv_128(const BandArgs& a, int dtype, hipStream_t stream);
 constexpr int BAND_SHARES_MAX = 128;   // workgroups that share the keys of a block of rows (forward)
-// keys of a workgroup of the dK / dV kernel
-// (128 at d = 128 leave one wave a SIMD: 187 -> 198 us for 16 heads on 4, 8192 tokens, window 1024)
-constexpr int band_kv_own(int d) { return d <= 64 ? 128 : 64; }
-// ... and of one of its workgroups for far rows
-constexpr int band_kv_group(int d) { return band_kv_own(d) / 4; }
+// Keys of a dK / dV workgroup, 16 a wave.  128 (32 a wave) read half as much from LDS for a product, and that is not what these kernels lack: with as many workgroups on a CU,
+// 8 x 8 kv heads of 4 query heads, 1111 tokens, window 300, d = 64: 112 us against 81; 4 x 8, 2048 tokens, window 500: 101 / 99; 4 heads, 8192 tokens, window 1024: 131 / 100,
+// d = 128: 198 / 187.  So did 128 keys on 8 waves with the values in LDS, d = 128: 189.
+constexpr int BAND_KV_OWN = 64;
