@@ -295,9 +295,9 @@ void plan_keys(BandArgs& a) {
   const int64_t near_end = dlt_imin64((int64_t)dlt_imax(dlt_imin(own, a.Lk) - 1 - a.off + a.W, 0) * a.G, a.rows);
   const int64_t far_chunks = (a.rows - near_end + 63) / 64;
   if (a.S > 0 && far_chunks > 4) {
-    // 16 chunks each: short beside the near workgroups, which start as these end
+    // 16 chunks each, and no more than a near workgroup has: short beside those, which start as these end
     a.far_groups = (a.S + group - 1) / group;
-    const int64_t most = 16;
+    const int64_t most = dlt_imin64(16, dlt_imax64(4, near_chunks / a.shares));
     const int64_t far_bytes = bh * 4 * a.far_groups * group * (a.dk_ + a.dv_) * 4;
     a.far = (int)dlt_imax64(1, dlt_imin64((far_chunks + most - 1) / most, DLT_WINDOW_WORKSPACE_MAX / 4 / far_bytes));
     a.part_keys = dlt_imin((a.S + own - 1) / own * own, a.Lk);

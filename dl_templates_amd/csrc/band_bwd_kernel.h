@@ -13,7 +13,7 @@ template <typename TIO, int D, int NP, int CK, int NW, int PAD>
 __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_q_kernel(const BandArgs a) {
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
-  constexpr int KC = D / 32, KB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int KC = band_kc(D, PAD), KB = 2 * KC, NKB = CK / 32, OWN = 16 * NP * NW;
   constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;
   static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");
@@ -269,7 +269,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   constexpr int NP = 1, CK = 64, NW = 4;   // blocks of 16 keys a wave, rows of a chunk, waves
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
-  constexpr int KC = D / 32, KB = D / 16, NQB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int KC = band_kc(D, PAD), KB = 2 * KC, NQB = CK / 32, OWN = 16 * NP * NW;
   constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;
   static_assert(NG >= 1 && NG * NW * 16 == CK && CK == 64, "whole groups of 16 rows per wave; one copy of scalars a chunk");

@@ -87,6 +87,10 @@ struct BandWalk {
   }
 };
 
+// Blocks of 32 head dims that take part.  PAD 0: both tensors have D dims; 1: fewer; 2 (D = 128): at most 96 (2 x 8 kv heads of 4 query heads, 4096 tokens,
+// window 500, forward / dQ / dK and dV, us: d = 96 105 / 127 / 143, d = 112, where all blocks take part, 124 / 172 / 165)
+constexpr int band_kc(int d, int pad) { return pad == 2 ? 3 : d / 32; }
+
 // Own rows as B operands: lane (n, g) holds head dims 32 c + 8 g .. + 7 of row n; r < 0: no row
 template <int KC, typename TIO>
 DLT_DEV void band_load_own(u32x4 (&f)[KC], const TIO* row, bool on, int dims, int g) {

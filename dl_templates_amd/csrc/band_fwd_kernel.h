@@ -72,7 +72,7 @@ template <typename TIO, int D, int NP, int CK, int NW, int GR, bool PAGED, int P
 __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
-  constexpr int KC = D / 32, VB = D / 16, NKB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int KC = band_kc(D, PAD), VB = 2 * KC, NKB = CK / 32, OWN = 16 * NP * NW;
   constexpr int NBUF = band_nbuf(B::BUF, GR), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;                              // groups of 16 tokens that a wave copies
   static_assert(NG >= 1 && NG * NW * 16 == CK, "whole groups of 16 tokens per wave");

@@ -24,7 +24,10 @@ int band_go(KernT kern, const BandArgs& a, int64_t grid, int threads, int lds, i
   DLT_CHECK_LAUNCH(who);
   return DLT_OK;
 }
-inline bool band_whole(const BandArgs& a) { return a.dk_ == D && a.dv_ == D; }
+constexpr int FEWER = D == 128 ? 2 : 1;
+inline int band_pad(const BandArgs& a) { return a.dk_ == D && a.dv_ == D ? 0 : dlt_imax(a.dk_, a.dv_) <= 96 ? FEWER : 1; }
+template <typename KernT>
+KernT band_pick(const BandArgs& a, KernT whole, KernT fewer, KernT less) { const int pad = band_pad(a); return pad == 0 ? whole : pad == FEWER ? fewer : less; }
 
 #if DLT_BAND_PART < 2
 template <typename TIO, int NP, int CK, int NW, int GR>
@@ -32,7 +35,7 @@ int band_fwd(const BandArgs& a, hipStream_t stream) {
   constexpr bool PG = DLT_BAND_PART == 1;
   constexpr int join = (GR - 1) * NW * NP * (D + 8) * 64, bufs = GR * band_nbuf(BandBuf<D, CK>::BUF, GR) * BandBuf<D, CK>::BUF;
   constexpr int lds = band_lds(bufs > join ? bufs : join, 16 * NP * NW);
-  return band_go(band_whole(a) ? band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 0> : band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 1>, a,
+  return band_go(band_pick(a, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 0>, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, FEWER>, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 1>), a,
                  (int64_t)a.B * a.Hkv * a.nblk * a.shares, 64 * NW * GR, lds, DLT_K_FWD, "window forward launch", stream);
 }
 template <typename TIO>
@@ -56,7 +59,7 @@ int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind
 template <typename TIO, int NP>
 int band_bwd_q(const BandArgs& a, hipStream_t stream) {
   constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
-  return band_go(band_whole(a) ? band_bwd_q_kernel<TIO, D, NP, 64, 4, 0> : band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>, a, (int64_t)a.B * a.Hkv * a.nblk, 256, lds,
+  return band_go(band_pick(a, band_bwd_q_kernel<TIO, D, NP, 64, 4, 0>, band_bwd_q_kernel<TIO, D, NP, 64, 4, FEWER>, band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>), a, (int64_t)a.B * a.Hkv * a.nblk, 256, lds,
                  DLT_K_BWD_Q, "window dQ launch", stream);
 }
 template <typename TIO>
@@ -69,7 +72,7 @@ int DLT_BCAT(dlt_band_bwd_q_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind
 template <typename TIO>
 int band_bwd_kv(const BandArgs& a, hipStream_t stream) {
   constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF_KV, 64);
-  return band_go(band_whole(a) ? band_bwd_kv_kernel<TIO, D, 0> : band_bwd_kv_kernel<TIO, D, 1>, a,
+  return band_go(band_pick(a, band_bwd_kv_kernel<TIO, D, 0>, band_bwd_kv_kernel<TIO, D, FEWER>, band_bwd_kv_kernel<TIO, D, 1>), a,
                  (int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + a.far * a.far_groups), 256, lds, DLT_K_BWD_KV, "window dK/dV launch", stream);
 }
 }  // namespace
