@@ -17,6 +17,7 @@ DLT_DEV float band_share_weight(const float2& x, float m) {
 }
 template <typename TIO, bool WG>
 __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
   __shared__ float sum[WG ? 4 : 1][128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t at = WG ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
@@ -98,6 +99,7 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
 // come first, a workgroup to a key, where 8 runs of threads take every eighth sum (one run: 9 us for 16 keys of 112 sums on 4 heads, this way 5.5).
 template <typename TIO>
 __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
   __shared__ f32x4 run[8][32];
   const bool keys = blockIdx.y == 0;
   const int dims = keys ? a.dk_ : a.dv_, per = dims / 4;
@@ -239,6 +241,15 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
   return DLT_OK;
 }
 
+void set_map(BandArgs& a) {
+  auto div = [](int64_t d) { BandDiv x; dlt_fastdiv_make((uint32_t)dlt_imin64(dlt_imax64(d, 1), 0x7fffffff), x.m, x.s); return x; };   // (more workgroups than that are refused)
+  a.units = (int)dlt_imin64((int64_t)a.nblk * a.shares, 0x7fffffff);
+  a.by_group_units = div((int64_t)a.group * a.units);
+  a.by_group = div(a.group);
+  a.by_last = div((int64_t)a.B * a.Hkv % a.group);
+  a.by_shares = div(a.shares);
+  a.by_heads = div(a.Hkv);
+}
 // ---- cutting a call into workgroups ---------------------------------------------------------------------------------------------------
 // Rows: how many a workgroup has, and how many workgroups share the keys of a block of rows.
 //   BAND_TWO     128 rows, where that makes two workgroups a CU (8 kv heads of 6000 tokens, d = 64, one and a half a CU: forward 29 us by 64 rows, 37 by 128; dQ 33, 42)
@@ -247,8 +258,10 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
 //   BAND_HALVES  64 rows, their keys over two groups of waves, while one workgroup a CU is all there is and the keys of a block are too few, or the workgroups too many, to be
 //                shared: a wave alone on its SIMD waits out every latency.  8 heads of 2048 queries, d = 64 / 128, us: 2560 keys each 32 -> 25 / 46 -> 35; 640 keys 11.7 -> 11.7 /
 //                16.4 -> 15.2; 4 heads, 640 keys, 10.1 + 6.3 for the sum of 4 shares -> 11.0 / 14.6 + 5.9 -> 14.0; but 12 heads (384 workgroups) 14.6 -> 19.7 / 20 -> 26
-//   BAND_FEW     up to 16 rows (a decode step), few keys: a wave has 32-key chunks of its own.  8 heads on 300 keys, d = 64, 8.4 -> 7.8; memory bound calls lose by it, since a CU
-//                holds one such workgroup (64 sequences of 4096 keys, d = 128: 155 -> 181)
+//   BAND_FEW     16 rows, where that makes no more than a workgroup a CU, few keys: a wave has 32-key chunks of its own, a quarter of the dependent work.  us, against HALVES: 4 heads of
+//                200 tokens, window 64, d = 64, 6.7 -> 5.2; of 1000 tokens, window 300, 9.4 -> 7.0, d = 128 11.8 -> 8.6; 8 heads of 500, window 200, d = 128, 10.4 -> 7.8; one token on 300 keys,
+//                8 heads, 8.2 -> 7.6.  With two workgroups a CU 7.7 -> 10.2 (8 heads of 1000, window 100, d = 64); with more keys the shares win: 8 tokens of 8 heads on 900 keys, d = 128,
+//                15.2 -> 8.4 + 3.8
 // Shares: up to two workgroups a CU, at least four chunks each.  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
 // (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).
 int plan_rows(BandArgs& a, bool forward) {
@@ -262,7 +275,7 @@ int plan_rows(BandArgs& a, bool forward) {
   const int64_t one = bh * blocks(64);
   const bool uneven = paged && 2 * one > cus && 2 * one <= 3 * cus && chunks(64) > 32;
   if (forward && kind == BAND_ONE && one <= cus && !uneven) {
-    if (a.rows <= 16 && chunks(16) <= 16) kind = BAND_FEW;
+    if (bh * blocks(16) <= cus && chunks(16) <= (band_class(a.dk_, a.dv_) == 64 ? 16 : 10)) kind = BAND_FEW;
     else if (chunks(64) <= 12 || 2 * one > cus) kind = BAND_HALVES;
   }
   const int own = kind == BAND_TWO ? 128 : kind == BAND_FEW ? 16 : 64;
@@ -275,6 +288,7 @@ int plan_rows(BandArgs& a, bool forward) {
     n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(row_bytes > 0 ? row_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
     a.shares = n < 1 ? 1 : (int)n;
   }
+  set_map(a);
   return kind;
 }
 int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
@@ -307,6 +321,7 @@ void plan_keys(BandArgs& a) {
     a.far = a.far_groups = 0;
     a.part_keys = a.shares > 1 ? a.Lk : 0;
   }
+  set_map(a);
 }
 
 int check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
@@ -349,7 +364,6 @@ extern "C" int dlt_window_fwd(const void* q, const int64_t q_strides[4], const v
   if ((rc = check_rows(who, "k", k, k_strides, a.Lk == 0, key_span(k_strides))) != DLT_OK) return rc;
   if ((rc = check_rows(who, "v", v, v_strides, a.Lk == 0, key_span(v_strides))) != DLT_OK) return rc;
   if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
-  DLT_REQUIRE(lse2 != nullptr || a.Lq == 0, "%s: lse2 is NULL", who);
   const int kind = plan_rows(a, true);
   if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK) return rc;

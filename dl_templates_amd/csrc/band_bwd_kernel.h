@@ -11,6 +11,7 @@
 // ---- dQ ---------------------------------------------------------------------------------------------------------------------------
 template <typename TIO, int D, int NP, int CK, int NW, int PAD>
 __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_q_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = band_kc(D, PAD), KB = 2 * KC, NKB = CK / 32, OWN = 16 * NP * NW;
@@ -24,10 +25,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  int bh, r_, blk;
-  flash_block_causal(lin, a.nblk, a.B * a.Hkv, a.group, 1, true, bh, r_, blk);
-  const int x0 = blk * OWN;
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  int b, h, blk, share_;
+  band_block(a, lin, true, b, h, blk, share_);
+  const int x0 = blk * OWN, bh = b * a.Hkv + h;
   const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];
   const TIO* dob = reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1];
   const TIO* ob = reinterpret_cast<const TIO*>(a.o) + b * a.os[0] + (int64_t)h * a.G * a.os[1];
@@ -266,6 +266,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 // ---- dK / dV -------------------------------------------------------------------------------------------------------------------------
 template <typename TIO, int D, int PAD>
 __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
   constexpr int NP = 1, CK = 64, NW = 4;   // blocks of 16 keys a wave, rows of a chunk, waves
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
@@ -283,21 +284,21 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   const int n_far = a.far * a.far_groups, all_far = a.B * a.Hkv * n_far;
   const bool far = (int)blockIdx.x < all_far;
   const int lin = far ? xcd_remap(blockIdx.x, all_far) : xcd_remap((int)blockIdx.x - all_far, (int)gridDim.x - all_far);
-  int bh, share, x0;
+  int b, h, share, x0;
   if (far) {
-    bh = lin / n_far;
+    const int bh = lin / n_far;
     const int rest = lin - bh * n_far, grp = rest / a.far;
     share = rest - grp * a.far;
     x0 = grp * 16 * NP;
+    b = band_div(bh, a.by_heads);
+    h = bh - b * a.Hkv;
   } else {
-    int r_, unit;
-    flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, false, bh, r_, unit);
-    const int blk = unit / a.shares;
-    share = unit - blk * a.shares;
+    int blk;
+    band_block(a, lin, false, b, h, blk, share);
     x0 = blk * OWN;
   }
+  const int bh = b * a.Hkv + h;
   const int xe = dlt_imin(x0 + (far ? 16 * NP : OWN), a.Lk);
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   const char* qb = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1]);
   const char* dob = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1]);
   const TIO* kh = reinterpret_cast<const TIO*>(a.k) + b * a.ks[0] + h * a.ks[1];

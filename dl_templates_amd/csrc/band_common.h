@@ -8,6 +8,7 @@
 // lse2 and delta are contiguous [B, Hkv, Lq G] in that row order.
 #pragma once
 #include "flash_dma_kernel.hpp"
+#include "kernargs.h"
 
 struct BandPages {          // keys and values in pages (paged calls); strides in elements
   const int32_t* table;     // [B, cols] page numbers
@@ -19,6 +20,7 @@ struct BandPages {          // keys and values in pages (paged calls); strides i
   uint32_t m16, s16;        // division by p16
 };
 
+struct BandDiv { uint32_t m, s; };   // division of 31-bit numbers (dlt_fastdiv)
 struct BandArgs {
   const void *q, *k, *v, *o, *d_o;
   void *out, *dq, *dk, *dv;
@@ -27,7 +29,9 @@ struct BandArgs {
   int32_t B, Hkv, G, Lq, Lk, dk_, dv_;
   uint32_t mG, sG;          // division by G
   int32_t W, S, off, rows;  // W <= Lk; rows = Lq G
-  int32_t nblk, group;      // own blocks of a (batch, kv head); heads interleaved at launch (flash_block_causal)
+  int32_t nblk, group;      // own blocks of a (batch, kv head); heads interleaved at launch (band_block)
+  int32_t units;            // nblk * shares
+  BandDiv by_group_units, by_group, by_last, by_shares, by_heads;   // workgroups of a group of heads; heads of a group, of the last one; shares; kv heads
   int32_t shares;           // workgroups that share the keys (forward) or rows (dK / dV) of an own block
   int32_t far, far_groups;  // dK / dV: workgroups that share the far rows of a group of sinks, such groups (band_bwd_kernel.h); 0: none
   int32_t part_keys;        // keys of a (batch, kv head) with partial sums
@@ -52,6 +56,22 @@ struct BandParts {
     floats = v_at + v_far_at + bh * a.far * 4 * far_keys * a.dv_;
   }
 };
+
+// Workgroup -> (batch, kv head), own block and share of it: `group` heads at a time are interleaved, as flash_block_causal has it, the blocks from the last on (`rev`: own =
+// queries, whose first blocks may see less) or from the first.  Divisions are products: four divisions were a third of the instructions in front of the first copy.
+DLT_DEV int band_div(int n, const BandDiv& d) { return (int)dlt_fastdiv((uint32_t)n, d.m, d.s); }
+DLT_DEV void band_block(const BandArgs& a, int lin, bool rev, int& b, int& h, int& blk, int& share) {
+  const int grp = band_div(lin, a.by_group_units), rem = lin - grp * (a.group * a.units);
+  const int left = a.B * a.Hkv - grp * a.group;
+  const bool last = left < a.group;
+  const int gc = last ? left : a.group, rank = band_div(rem, last ? a.by_last : a.by_group);
+  const int bh = grp * a.group + (rem - rank * gc);
+  const int unit = rev ? a.units - 1 - rank : rank;
+  blk = band_div(unit, a.by_shares);
+  share = unit - blk * a.shares;
+  b = band_div(bh, a.by_heads);
+  h = bh - b * a.Hkv;
+}
 
 // Of the rows of a tile: token and head in the group
 struct BandRow { int tok, head; };

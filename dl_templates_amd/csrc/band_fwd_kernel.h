@@ -70,6 +70,7 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
 // GR groups of NW waves own the same rows and take every GR-th chunk each; their results are joined at the end, through LDS.
 template <typename TIO, int D, int NP, int CK, int NW, int GR, bool PAGED, int PAD>
 __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = band_kc(D, PAD), VB = 2 * KC, NKB = CK / 32, OWN = 16 * NP * NW;
@@ -84,11 +85,9 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   const int grp = GR == 1 ? 0 : wave_all / NW, wave = wave_all - grp * NW;   // group of the wave, wave of the group
 
   const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  int bh, r_, unit;
-  flash_block_causal(lin, a.nblk * a.shares, a.B * a.Hkv, a.group, 1, true, bh, r_, unit);
-  const int blk = unit / a.shares, share = unit - blk * a.shares;
-  const int x0 = blk * OWN;
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+  int b, h, blk, share;
+  band_block(a, lin, true, b, h, blk, share);
+  const int x0 = blk * OWN, bh = b * a.Hkv + h;
   const BandSeq sq = band_seq<PAGED>(a, b);
   const int n_rows = sq.n_q * a.G;                              // rows with a query; those behind get zeros
   const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];

@@ -7,6 +7,7 @@
 // element, and parts of fewer than 8 pairs move in pieces of 4, 2 and 1.  Rows with other strides than 1 take a kernel of one pair per thread.
 // Rotated values are formed in 32 bits, each product rounded before the sum as in the 2D rotation, and rounded once.
 // 16 + 16 heads of 49152 tokens, d = 128, bf16: 149 us, 5.4 TB/s (a large copy: 5.15).  Memory bound; small calls take the launch.
+#include "kernargs.h"
 #include "rope_axes.h"
 
 namespace {
@@ -219,6 +220,7 @@ constexpr int ROT_BLOCKS = 2048;   // workgroups that a large call aims for
 // WHOLE: every part has 8 dims or pairs (the others cost branches in front of every access)
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(256) void rotate_rows_kernel(RotArgs a, int parts) {
+  dlt_kernargs_in<sizeof(RotArgs)>();
   const int C = a.s[0].C;
   const uint64_t first = (uint64_t)blockIdx.x * 256 / (unsigned)parts;   // the workgroup's first token
   const unsigned rest = (unsigned)((uint64_t)blockIdx.x * 256 - first * parts) + threadIdx.x;
@@ -303,6 +305,7 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(RotArgs a, int parts) 
 // tokens, d = 64, sections of 6, 11 and 11 pairs, fp16: 32 -> 12.6 us).
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_rows_lds_kernel(RotArgs a, int parts) {
+  dlt_kernargs_in<sizeof(RotArgs)>();
   __shared__ __align__(16) T sm[4][UNR][64 * 8];
   const int P = a.r.pairs;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -401,6 +404,7 @@ __global__ __launch_bounds__(256) void rotate_rows_lds_kernel(RotArgs a, int par
 // any strides, one thread per (token, pair or dim that is not rotated)
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_single_kernel(RotArgs a) {
+  dlt_kernargs_in<sizeof(RotArgs)>();
   const int P = a.r.pairs;
   int dims = P;
   for (int z = 0; z < a.n; z++) dims = dlt_imax(dims, a.s[z].rot ? a.s[z].C - P : a.s[z].C);

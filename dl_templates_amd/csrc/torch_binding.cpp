@@ -272,7 +272,7 @@ Workspace window_workspace(const dlt_window_shape_t& shape, int backward, const 
 struct Forward { Tensor o, lse, q_rot, k_rot; };
 
 // keep_rot: the rotated q and k are stored as well (for the backward pass)
-Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tensor& v, const Rope* rope, bool keep_rot) {
+Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tensor& v, const Rope* rope, bool keep_rot, bool want_lse = true /* Window */) {
   require_gpu(q, k, v);
   c10::DeviceGuard guard(q.device());
   Forward f;
@@ -289,9 +289,9 @@ Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tenso
   if (s.op == Op::Window) {
     const Workspace ws = window_workspace(s.window, 0, q);
     f.o = empty({q.size(0), q.size(1), q.size(2), v.size(3)}, dt, q);
-    f.lse = empty({q.size(0), k.size(1), q.size(2), q.size(1) / k.size(1)}, at::kFloat, q);
+    if (want_lse) f.lse = empty({q.size(0), k.size(1), q.size(2), q.size(1) / k.size(1)}, at::kFloat, q);
     check_rc(dlt_window_fwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), f.o.mutable_data_ptr(),
-                            st16(f.o).data(), (float*)f.lse.mutable_data_ptr(), &s.window, ws.ptr, ws.bytes, stream));
+                            st16(f.o).data(), want_lse ? (float*)f.lse.mutable_data_ptr() : nullptr, &s.window, ws.ptr, ws.bytes, stream));
     return f;
   }
   if (s.op == Op::Image) {
@@ -516,7 +516,7 @@ Tensor attention(Op op, const Tensor& q, const Tensor& k, const Tensor& v, const
       require_gpu(pq, pk, pv);
       rope = make_rope_for(rope_t[0], rope_t[1], rope_t[2], pq, pq.size(2));
     }
-    f = run_forward(spec, pq, pk, pv, rope_t ? &rope : nullptr, keep_rot);
+    f = run_forward(spec, pq, pk, pv, rope_t ? &rope : nullptr, keep_rot, grad);
     out = cut_last(f.o, dv);
   }
   // saved with autograd as it is: pack hooks are the caller's code

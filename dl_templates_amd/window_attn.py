@@ -47,4 +47,6 @@ class WindowAttention(torch.autograd.Function):
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = None, n_sink: int = 0, sm_scale: float = None) -> torch.Tensor:
     """o [B, H, Lq, Dv]; ``sm_scale`` None: ``1 / sqrt(Dk)``."""
-    return WindowAttention.apply(q, k, v, window, n_sink, 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale)
+    args = (q, k, v, window, n_sink, 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale)
+    o = _lib.native.window(*args)
+    return WindowAttention.apply(*args) if o is NotImplemented else o

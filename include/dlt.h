@@ -305,8 +305,8 @@ int dlt_rope_axes(const void* q, const int64_t q_strides[4], void* q_out, const 
 /* ---- attention over a 1D window with sinks ---------------------------------------------------
  * q [B, H, Lq, dk], k [B, Hkv, Lk, dk], v [B, Hkv, Lk, dv], o [B, H, Lq, dv]; head h of q reads head h / (H / Hkv) of k and v.  Query i
  * stands at position p = Lk - Lq + i and sees key j iff j <= p and (p - j < window or j < n_sink): the last `window` keys up to its own
- * and the first n_sink ones.  A query that sees nothing (p < 0) gives zeros and lse2 = -inf.  lse2 and delta are fp32, contiguous
- * [B, Hkv, Lq, H / Hkv].  DLT_BF16 and DLT_FP16; dk and dv multiples of 8 up to 128, rows of unit last stride in multiples of 16
+ * and the first n_sink ones.  A query that sees nothing (p < 0) gives zeros and lse2 = -inf.  lse2 (NULL in a forward pass that no
+ * backward pass follows) and delta are fp32, contiguous [B, Hkv, Lq, H / Hkv].  DLT_BF16 and DLT_FP16; dk and dv multiples of 8 up to 128, rows of unit last stride in multiples of 16
  * bytes; sm_scale > 0. */
 typedef struct {
   int32_t B, H, Hkv, Lq, Lk, dk, dv;

@@ -52,7 +52,7 @@ def window(L, backward=False, ptr=None, st=None, ws=ONE, ws_bytes=1 << 40, **kw)
     (dict(B=0), 1, "positive"), (dict(Hkv=0), 1, "positive"), (dict(H=5), 1, "evenly"), (dict(window=0), 1, "window"), (dict(window=-3), 1, "window"),
     (dict(n_sink=-1), 1, "n_sink"), (dict(sm_scale=0.0), 1, "sm_scale"), (dict(sm_scale=-1.0), 1, "sm_scale"), (dict(sm_scale=float("nan")), 1, "sm_scale"),
     (dict(sm_scale=float("inf")), 1, "sm_scale"), (dict(Lq=-1), 1, "length"), (dict(Lk=1 << 30), 2, "tokens"), (dict(Lq=1 << 29), 2, "tokens"),
-    (dict(ptr={"k": None}), 1, "k is NULL"), (dict(ptr={"lse2": None}), 1, "lse2"), (dict(ptr={"q": ctypes.c_void_p(264)}), 1, "16 bytes"),
+    (dict(ptr={"k": None}), 1, "k is NULL"), (dict(ptr={"q": ctypes.c_void_p(264)}), 1, "16 bytes"),
     (dict(st={"v": I64(8192, 4096, 68, 1)}), 1, "16 bytes"), (dict(st={"q": I64(16384, 4096, 64, 2)}), 1, "contiguous"), (dict(st={"k": I64(8192, -4096, 64, 1)}), 1, "negative"),
     (dict(st={"k": I64(8192, 4096, 1 << 27, 1)}), 2, "too large"), (dict(st={"q": I64(8192, 1 << 29, 64, 1)}), 2, "too large"),
     (dict(B=MAX, Lk=4096, Lq=4096), 2, "workgroups"),
@@ -67,6 +67,8 @@ def test_window_accepts(L, kw):
     for backward in (False, True):
         assert window(L, backward, **kw) == 0, err(L)
         assert lib.dlt_last_kernel_family() == L.KERNEL_FAMILIES.index("band")
+    assert window(L, ptr={"lse2": None}, **kw) == 0, err(L)   # a forward pass alone needs no sums
+    assert kw.get("Lq") == 0 or (window(L, True, ptr={"lse2": None}, **kw) == 1 and "lse2" in err(L))
     if kw.get("Lq") == 0:   # a tensor without elements may be NULL
         assert window(L, ptr={"q": None, "o": None, "lse2": None}, **kw) == 0, err(L)
 
