@@ -29,7 +29,7 @@ EXPORTS = (
     "dlt_timing_enable", "dlt_timing_collect", "dlt_debug_copy",
     "dlt_swa_fwd_image", "dlt_swa_bwd_image", "dlt_swa_image_offsets", "dlt_swa_fwd_rot", "dlt_swa_bwd_rot",
     "dlt_swa_bwd_noalloc", "dlt_dry_run", "dlt_last_kernel_family",
-    "dlt_rope_axes", "dlt_window_workspace", "dlt_window_fwd", "dlt_window_bwd", "dlt_paged_append", "dlt_paged_workspace", "dlt_paged_attn",
+    "dlt_rope_axes", "dlt_window_workspace", "dlt_window_low_tokens", "dlt_window_fwd", "dlt_window_bwd", "dlt_paged_append", "dlt_paged_workspace", "dlt_paged_attn",
 )
 KERNEL_FAMILIES = ("none", "marching", "streaming", "tile", "flash", "generic", "band")   # DLT_FAMILY_* of include/dlt.h
 NOALLOC_MAX_DELTA = 1 << 20  # DLT_NOALLOC_MAX_DELTA of include/dlt.h
@@ -167,9 +167,11 @@ def _declare(lib) -> None:
     lib.dlt_window_workspace.restype = c_int
     lib.dlt_window_workspace.argtypes = [POINTER(WindowShape), c_int, P64]
     lib.dlt_window_fwd.restype = c_int
-    lib.dlt_window_fwd.argtypes = tensor * 4 + [c_void_p, POINTER(WindowShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_window_fwd.argtypes = tensor * 4 + [c_void_p, c_void_p, POINTER(WindowShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_window_low_tokens.restype = c_int
+    lib.dlt_window_low_tokens.argtypes = [POINTER(WindowShape), POINTER(c_int32)]
     lib.dlt_window_bwd.restype = c_int
-    lib.dlt_window_bwd.argtypes = tensor * 5 + [c_void_p, c_void_p] + tensor * 3 + [POINTER(WindowShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_window_bwd.argtypes = tensor * 4 + [c_void_p] + tensor + [c_void_p, c_void_p] + tensor * 3 + [POINTER(WindowShape), c_void_p, c_int64, c_void_p]
     lib.dlt_paged_append.restype = c_int
     lib.dlt_paged_append.argtypes = tensor * 6 + [c_void_p, c_int64, c_void_p, c_void_p, POINTER(RopeAxesDesc), POINTER(PagedShape), c_void_p]
     lib.dlt_paged_workspace.restype = c_int

@@ -92,6 +92,8 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
   const float f = l == 0.f ? 0.f : 1.f / l;
   TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r);
   if (2 * lane < a.dv_) *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(o[0] * f, o[1] * f);
+  TIO* low = a.low != nullptr ? band_low<TIO>(a, b, h, r) : nullptr;
+  if (low != nullptr && 2 * lane < a.dv_) *reinterpret_cast<unsigned*>(low + 2 * lane) = pack2<TIO>(band_dropped<TIO>(o[0] * f), band_dropped<TIO>(o[1] * f));
   if (lane == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
   }
 #pragma unroll 4
   for (int i = 0; i < a.shares; i++) s += *reinterpret_cast<const f32x4*>(part + (((int64_t)bh * a.shares + i) * P.keys + j) * dims + d);
-  if (keys) s *= a.sm_scale;
+  if (keys) s *= a.grad_scale;
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   TIO* p = keys ? reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1] + j * a.dks[2]
                 : reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1] + j * a.dvs[2];
@@ -199,6 +201,7 @@ void set_scalars(BandArgs& a, float sm_scale, int Hkv, int G) {
   a.q16 = 16 % G == 0;
 }
 
+constexpr int LOW_KEYS = 16;
 int window_problem(const char* who, const dlt_window_shape_t* s, BandArgs& a) {
   DLT_REQUIRE(s != nullptr, "%s: shape is NULL", who);
   const int rc = check_common(who, s->B, s->H, s->Hkv, s->dk, s->dv, s->window, s->n_sink, s->sm_scale, s->dtype);
@@ -214,6 +217,9 @@ int window_problem(const char* who, const dlt_window_shape_t* s, BandArgs& a) {
   a.rows = s->Lq * G;
   a.shares = 1;
   set_scalars(a, s->sm_scale, s->Hkv, G);
+  a.grad_scale = (a.W == 1 && a.S == 0) || a.Lk == 1 ? 0.f : s->sm_scale;
+  // rows with low parts (band_low): all of a short window, else those of the first positions
+  a.low_rows = G * (a.W + a.S <= LOW_KEYS ? a.Lq : dlt_imax(0, dlt_imin(LOW_KEYS - a.off, a.Lq)));
   a.group = flash_causal_group(dlt_imax(s->Lk, 1), s->dk, s->dv);
   return DLT_OK;
 }
@@ -353,8 +359,17 @@ extern "C" int dlt_window_workspace(const dlt_window_shape_t* shape, int backwar
   return DLT_OK;
 }
 
+extern "C" int dlt_window_low_tokens(const dlt_window_shape_t* shape, int32_t* tokens) {
+  DLT_REQUIRE(tokens != nullptr, "window_low_tokens: tokens is NULL");
+  BandArgs a;
+  const int rc = window_problem("window_low_tokens", shape, a);
+  if (rc != DLT_OK) return rc;
+  *tokens = a.low_rows / a.G;
+  return DLT_OK;
+}
+
 extern "C" int dlt_window_fwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
-                              void* o, const int64_t o_strides[4], float* lse2, const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
+                              void* o, const int64_t o_strides[4], void* o_low, float* lse2, const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
   const char* who = "window_fwd";
   hipStream_t stream = (hipStream_t)stream_;
   BandArgs a;
@@ -364,18 +379,19 @@ extern "C" int dlt_window_fwd(const void* q, const int64_t q_strides[4], const v
   if ((rc = check_rows(who, "k", k, k_strides, a.Lk == 0, key_span(k_strides))) != DLT_OK) return rc;
   if ((rc = check_rows(who, "v", v, v_strides, a.Lk == 0, key_span(v_strides))) != DLT_OK) return rc;
   if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
+  DLT_REQUIRE((uintptr_t)o_low % 16 == 0, "%s: o_low must start at a multiple of 16 bytes", who);
   const int kind = plan_rows(a, true);
   if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
-  a.q = q; a.k = k; a.v = v; a.out = o; a.lse = lse2; a.part = (float*)ws;
+  a.q = q; a.k = k; a.v = v; a.out = o; a.low = o_low; a.lse = lse2; a.part = (float*)ws;
   strides3(a.qs, q_strides); strides3(a.ks, k_strides); strides3(a.vs, v_strides); strides3(a.os, o_strides);
   rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_fwd_64(a, shape->dtype, kind, stream) : dlt_band_fwd_128(a, shape->dtype, kind, stream);
   return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
 }
 
 extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
-                              const void* o, const int64_t o_strides[4], const void* d_o, const int64_t do_strides[4], const float* lse2, float* delta,
+                              const void* o, const int64_t o_strides[4], const void* o_low, const void* d_o, const int64_t do_strides[4], const float* lse2, float* delta,
                               void* dq, const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4], void* dv, const int64_t dv_strides[4],
                               const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
   const char* who = "window_bwd";
@@ -391,6 +407,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
   for (const auto& t : ts)
     if ((rc = check_rows(who, t.name, t.p, t.st, t.none, t.span)) != DLT_OK) return rc;
   DLT_REQUIRE((lse2 != nullptr && delta != nullptr) || nq, "%s: lse2 or delta is NULL", who);
+  DLT_REQUIRE((uintptr_t)o_low % 16 == 0, "%s: o_low must start at a multiple of 16 bytes", who);
   BandArgs kv = a;
   plan_keys(kv);
   const int kind = plan_rows(a, false);
@@ -399,7 +416,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
   if (dlt_route_note(DLT_FAMILY_BAND)) return DLT_OK;
   for (BandArgs* x : {&a, &kv}) {
     x->q = q; x->k = k; x->v = v; x->o = o; x->d_o = d_o; x->dq = dq; x->dk = dk; x->dv = dv;
-    x->lse = const_cast<float*>(lse2); x->delta = delta; x->part = (float*)ws;
+    x->low = const_cast<void*>(o_low); x->lse = const_cast<float*>(lse2); x->delta = delta; x->part = (float*)ws;
     strides3(x->qs, q_strides); strides3(x->ks, k_strides); strides3(x->vs, v_strides); strides3(x->os, o_strides); strides3(x->dos, do_strides);
     strides3(x->dqs, dq_strides); strides3(x->dks, dk_strides); strides3(x->dvs, dv_strides);
   }

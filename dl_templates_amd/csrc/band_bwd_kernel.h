@@ -95,6 +95,18 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 #pragma unroll
       for (int j = 0; j < 8; j++) sum += fo[j] * fd[j];
     }
+    const TIO* low = on && a.low != nullptr ? band_low<TIO>(a, b, h, r) : nullptr;
+    if (low != nullptr) {
+      band_load_own<KC>(of, low, true, a.dv_, g);
+#pragma unroll
+      for (int c = 0; c < KC; c++) {
+        float fo[8], fd[8];
+        unpack8<TIO>(of[c], fo);
+        unpack8<TIO>(dof[p][c], fd);
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum += fo[j] * fd[j];
+      }
+    }
     del[p] = wave_sum4(sum);
     if (g == 0 && on) store_stream4(a.delta + row0 + r, del[p]);
   }
@@ -220,7 +232,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   unsigned odd[NP];
 #pragma unroll
   for (int p = 0; p < NP; p++) {
-    mul[p] = a.sm_scale;
+    mul[p] = hi[p] == 0 ? 0.f : a.grad_scale;   // a row at position 0 sees one key
     const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < a.rows && band_odd_row(acc, p));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }
@@ -253,7 +265,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
                                         }
                                       }
                                     if (2 * lane < D)
-                                      *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * a.sm_scale, sum[1] * a.sm_scale);
+                                      *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * (pos == 0 ? 0.f : a.grad_scale), sum[1] * (pos == 0 ? 0.f : a.grad_scale));
                                   }
                               });
 }
@@ -563,7 +575,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   float mulk[NP], mulv[NP];
 #pragma unroll
   for (int p = 0; p < NP; p++) {
-    mulk[p] = a.sm_scale;
+    mulk[p] = a.grad_scale;
     mulv[p] = 1.f;
     const uint64_t bad = __builtin_amdgcn_ballot_w64(wk0 + 16 * p + n < a.Lk && (band_odd_row(dk_acc, p) || band_odd_row(dv_acc, p)));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
@@ -618,7 +630,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
         const int w = 16 * p + __builtin_ctz(todo);
         float sk[2], sv[2];
         exact(wk0 + w, sk, sv);
-        const float f = keys ? a.sm_scale : 1.f;
+        const float f = keys ? a.grad_scale : 1.f;
         if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>((keys ? sk[0] : sv[0]) * f, (keys ? sk[1] : sv[1]) * f);
       }
   };

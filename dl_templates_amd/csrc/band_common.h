@@ -25,6 +25,7 @@ struct BandArgs {
   const void *q, *k, *v, *o, *d_o;
   void *out, *dq, *dk, *dv;
   float *lse, *delta, *part;
+  void* low;                // what the rounding of o left, [B, H, low tokens, dv] (see band_low)
   int64_t qs[3], ks[3], vs[3], os[3], dos[3], dqs[3], dks[3], dvs[3];   // batch (pages: page), head, token; head dims are contiguous
   int32_t B, Hkv, G, Lq, Lk, dk_, dv_;
   uint32_t mG, sG;          // division by G
@@ -35,8 +36,9 @@ struct BandArgs {
   int32_t shares;           // workgroups that share the keys (forward) or rows (dK / dV) of an own block
   int32_t far, far_groups;  // dK / dV: workgroups that share the far rows of a group of sinks, such groups (band_bwd_kernel.h); 0: none
   int32_t part_keys;        // keys of a (batch, kv head) with partial sums
+  int32_t low_rows;         // rows of a (batch, kv head) with low parts
   int32_t q16;              // 16 is a multiple of G: 16 rows are whole tokens
-  float scale_log2, sm_scale;
+  float scale_log2, sm_scale, grad_scale;   // grad_scale: of dQ and dK; 0 where every row sees one key, whose dS are zero but for roundings
   BandPages pg;
 };
 
@@ -79,6 +81,23 @@ DLT_DEV BandRow band_row(const BandArgs& a, int r) {
   const int t = (int)dlt_fastdiv((uint32_t)r, a.mG, a.sG);
   return BandRow{t, r - t * a.G};
 }
+// delta = dO . o is subtracted from every dP of a row; where a row sees few keys these cancel, and the rounding of o is what is left of it: with two keys dQ and dK are off by 2.3
+// times what their own rounding is, with 16 by 1.5, at most 1.5 in any case with o unrounded (the roundings of dS remain).  Rows that see up to 16 keys, those of short windows and of the
+// first 16 positions, therefore keep the part of o that its rounding drops.
+template <typename TIO>
+DLT_DEV TIO* band_low(const BandArgs& a, int b, int h, int r) {
+  if (r >= a.low_rows) return nullptr;
+  const BandRow w = band_row(a, r);
+  const int tokens = a.low_rows / a.G;
+  return reinterpret_cast<TIO*>(a.low) + (((int64_t)b * a.Hkv + h) * a.G + w.head) * tokens * a.dv_ + (int64_t)w.tok * a.dv_;
+}
+// v less its rounding (0 where that is no number)
+template <typename TIO>
+DLT_DEV float band_dropped(float v) {
+  const float d = v - (float)(TIO)v;
+  return fabsf(d) < INFINITY ? d : 0.f;
+}
+
 template <typename T>
 DLT_DEV T* band_row_ptr(T* base, const int64_t (&st)[3], const BandArgs& a, int r) {
   const BandRow w = band_row(a, r);
@@ -237,8 +256,8 @@ constexpr int band_nbuf(int buf, int groups = 1) { return 4 * buf <= 65536 && 3 
 
 // Accumulators in C layout (lane (n, g): dims 16 d + 4 g .. + 3 of own row n, times mul[p]) -> LDS tile of 16-bit values -> rows.
 // `ptr(row)`: the row's place or NULL.  The tile takes the chunk buffers' LDS.
-// `again()`: the wave writes rows of its own part of the tile once more (see below).
-template <int D, int NP, typename TIO, int NA, typename PtrFn, typename AgainFn>
+// `again()`: the wave writes rows of its own part of the tile once more (see below).  LOW: what the rounding drops instead of what it leaves.
+template <int D, int NP, typename TIO, bool LOW = false, int NA, typename PtrFn, typename AgainFn>
 DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int groups, bool write, int dims, int wave, int n, int g, int tid, PtrFn ptr,
                              AgainFn again) {
   constexpr int PT = D * 2 + 16;
@@ -248,9 +267,12 @@ DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (
     char* row = sT + (wave * 16 * NP + 16 * p + n) * PT + 8 * g;
 #pragma unroll
     for (int d = 0; d < NA; d++) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] = LOW ? band_dropped<TIO>(acc[p][d][i] * mul[p]) : acc[p][d][i] * mul[p];
       u32x2 w;
-      w.x = pack2<TIO>(acc[p][d][0] * mul[p], acc[p][d][1] * mul[p]);
-      w.y = pack2<TIO>(acc[p][d][2] * mul[p], acc[p][d][3] * mul[p]);
+      w.x = pack2<TIO>(v[0], v[1]);
+      w.y = pack2<TIO>(v[2], v[3]);
       *reinterpret_cast<u32x2*>(row + 32 * d) = w;
     }
   }

@@ -404,4 +404,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
                                     if (lane == 0 && a.lse != nullptr) a.lse[row0 + r] = m + fast_log2(l);
                                   }
                               });
+  if (!PAGED && a.low != nullptr && x0 < a.low_rows)
+    band_store_rows<D, NP, TIO, true>(smem, acc, inv, NW, GR, grp == 0, a.dv_, wave, n, g, tid,
+                                      [&](int row) -> TIO* { return x0 + row < a.rows ? band_low<TIO>(a, b, h, x0 + row) : nullptr; }, []() {});
 }

@@ -269,7 +269,7 @@ Workspace window_workspace(const dlt_window_shape_t& shape, int backward, const 
   return w;
 }
 
-struct Forward { Tensor o, lse, q_rot, k_rot; };
+struct Forward { Tensor o, lse, q_rot, k_rot, low; };
 
 // keep_rot: the rotated q and k are stored as well (for the backward pass)
 Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tensor& v, const Rope* rope, bool keep_rot, bool want_lse = true /* Window */) {
@@ -289,9 +289,14 @@ Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tenso
   if (s.op == Op::Window) {
     const Workspace ws = window_workspace(s.window, 0, q);
     f.o = empty({q.size(0), q.size(1), q.size(2), v.size(3)}, dt, q);
-    if (want_lse) f.lse = empty({q.size(0), k.size(1), q.size(2), q.size(1) / k.size(1)}, at::kFloat, q);
+    if (want_lse) {
+      f.lse = empty({q.size(0), k.size(1), q.size(2), q.size(1) / k.size(1)}, at::kFloat, q);
+      int32_t tokens = 0;
+      check_rc(dlt_window_low_tokens(&s.window, &tokens));
+      if (tokens > 0) f.low = empty({q.size(0), q.size(1), tokens, v.size(3)}, dt, q);
+    }
     check_rc(dlt_window_fwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), f.o.mutable_data_ptr(),
-                            st16(f.o).data(), want_lse ? (float*)f.lse.mutable_data_ptr() : nullptr, &s.window, ws.ptr, ws.bytes, stream));
+                            st16(f.o).data(), f.low.defined() ? f.low.mutable_data_ptr() : nullptr, want_lse ? (float*)f.lse.mutable_data_ptr() : nullptr, &s.window, ws.ptr, ws.bytes, stream));
     return f;
   }
   if (s.op == Op::Image) {
@@ -322,7 +327,7 @@ Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tenso
 
 // rotated: q and k are the rotated tensors that the forward pass kept
 std::array<Tensor, 3> run_backward(const Spec& s, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& lse,
-                                   const Tensor& d_o, const Rope* rope, bool rotated) {
+                                   const Tensor& d_o, const Rope* rope, bool rotated, const Tensor& low = Tensor() /* Window */) {
   require_gpu(q, k, v, o, lse, d_o);
   c10::DeviceGuard guard(q.device());
   void* stream = stream_of(q);
@@ -332,7 +337,7 @@ std::array<Tensor, 3> run_backward(const Spec& s, const Tensor& q, const Tensor&
     Tensor delta = empty(lse.sizes(), at::kFloat, lse);
     const Tensor g = as_rows16(d_o, group_of(q, k));
     check_rc(dlt_window_bwd(q.const_data_ptr(), st16(q).data(), k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), o.const_data_ptr(),
-                            st16(o).data(), g.const_data_ptr(), st16(g).data(), (const float*)lse.const_data_ptr(), (float*)delta.mutable_data_ptr(),
+                            st16(o).data(), low.defined() ? low.const_data_ptr() : nullptr, g.const_data_ptr(), st16(g).data(), (const float*)lse.const_data_ptr(), (float*)delta.mutable_data_ptr(),
                             dq.mutable_data_ptr(), st16(dq).data(), dk.mutable_data_ptr(), st16(dk).data(), dv.mutable_data_ptr(), st16(dv).data(), &s.window,
                             ws.ptr, ws.bytes, stream));
     return {dq, dk, dv};
@@ -419,12 +424,12 @@ struct AttnBackward : public Node {
   Spec spec;
   bool has_rope = false, rotated = false;
   int64_t dk = 0, dv = 0;   // head dims of the caller's tensors
-  SavedVariable q, k, v, o, lse, idx, row, col;
+  SavedVariable q, k, v, o, lse, idx, row, col, low;
 
   std::string name() const override { return "DltAttentionBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* s : {&q, &k, &v, &o, &lse, &idx, &row, &col}) s->reset_data();
+    for (SavedVariable* s : {&q, &k, &v, &o, &lse, &idx, &row, &col, &low}) s->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -433,7 +438,8 @@ struct AttnBackward : public Node {
     // Unpacked with autograd as it is: an unpack hook may run the forward pass again (activation checkpointing), and what it runs
     // has to be recorded.
     Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack(), o_ = o.unpack(shared_from_this()), lse_ = lse.unpack();
-    Tensor idx_, row_, col_;
+    Tensor idx_, row_, col_, low_;
+    if (spec.op == Op::Window) low_ = low.unpack();
     if (has_rope) {
       idx_ = idx.unpack();
       row_ = row.unpack();
@@ -452,8 +458,9 @@ struct AttnBackward : public Node {
         v_ = as_rows16(v_);
         o_ = as_rows16(o_);
         lse_ = lse_.contiguous();
+        if (low_.defined()) low_ = low_.contiguous();
       }
-      auto g = run_backward(spec, q_, k_, v_, o_, lse_, d_o, has_rope ? &rope : nullptr, rotated);
+      auto g = run_backward(spec, q_, k_, v_, o_, lse_, d_o, has_rope ? &rope : nullptr, rotated, low_);
       out = {cut_last(g[0], dk), cut_last(g[1], dk), cut_last(g[2], dv)};
     }
     if (spec.op == Op::Window) differentiable_once(out);
@@ -528,6 +535,7 @@ Tensor attention(Op op, const Tensor& q, const Tensor& k, const Tensor& v, const
     node->k = SavedVariable(keep_rot ? f.k_rot : pk, false);
     node->v = SavedVariable(pv, false);
     node->lse = SavedVariable(f.lse, false);
+    node->low = SavedVariable(f.low, false);
     if (rope_t != nullptr) {
       node->has_rope = true;
       node->rotated = keep_rot;
@@ -968,7 +976,7 @@ PyObject* py_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// the same -> (o, lse2) and (q, k, v, o, lse2, do, the same 3 numbers) -> (dq, dk, dv): no graph, no padding
+// the same -> (o, lse2, o's low part or None) and (q, k, v, o, lse2, low part, do, the same 3 numbers) -> (dq, dk, dv): no graph, no padding
 PyObject* py_window_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 6, 6);
@@ -979,20 +987,21 @@ PyObject* py_window_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
   const Tensor q_ = as_rows16(q, group_of(q, k)), k_ = as_rows16(k), v_ = as_rows16(v);
   const Forward f = run_forward(window_spec(q_, k_, v_, dims, float_arg(a[5])), q_, k_, v_, nullptr, false);
-  return Py_BuildValue("(NN)", THPVariable_Wrap(f.o), THPVariable_Wrap(f.lse));
+  return Py_BuildValue("(NNN)", THPVariable_Wrap(f.o), THPVariable_Wrap(f.lse), THPVariable_Wrap(f.low));
   END_HANDLE_TH_ERRORS
 }
 
 PyObject* py_window_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 9, 9);
+  count(n, 10, 10);
   at::AutoDispatchBelowADInplaceOrView below;
-  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &o = tensor_arg(a[3]), &lse = tensor_arg(a[4]), &d_o = tensor_arg(a[5]);
-  const int64_t dims[2] = {window_arg(a[6]), int_arg(a[7])};
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &o = tensor_arg(a[3]), &lse = tensor_arg(a[4]), &d_o = tensor_arg(a[6]);
+  const Tensor low = a[5] == Py_None ? Tensor() : tensor_arg(a[5]).contiguous();
+  const int64_t dims[2] = {window_arg(a[7]), int_arg(a[8])};
   require_gpu(q, k, v, o, lse, d_o);
   check_assert(q.dim() == 4, "q, k and v must have shape [B, heads, L, D]");
   const Tensor q_ = as_rows16(q, group_of(q, k)), k_ = as_rows16(k), v_ = as_rows16(v), o_ = as_rows16(o);
-  auto g = run_backward(window_spec(q_, k_, v_, dims, float_arg(a[8])), q_, k_, v_, o_, lse.contiguous(), d_o, nullptr, false);
+  auto g = run_backward(window_spec(q_, k_, v_, dims, float_arg(a[9])), q_, k_, v_, o_, lse.contiguous(), d_o, nullptr, false, low);
   return Py_BuildValue("(NNN)", THPVariable_Wrap(g[0]), THPVariable_Wrap(g[1]), THPVariable_Wrap(g[2]));
   END_HANDLE_TH_ERRORS
 }

@@ -33,15 +33,15 @@ class WindowAttention(torch.autograd.Function):
         if plan is not None:
             q, k, v = _pad_last(q, plan[0]), _pad_last(k, plan[0]), _pad_last(v, plan[1])
         ctx.scalars = (window, n_sink, sm_scale)
-        o, lse2 = _lib.native.window_forward(q, k, v, *ctx.scalars)
-        ctx.save_for_backward(q, k, v, o, lse2)
+        o, lse2, low = _lib.native.window_forward(q, k, v, *ctx.scalars)
+        ctx.save_for_backward(q, k, v, o, lse2, low)
         return _cut_last(o, ctx.dims[1])
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse2 = ctx.saved_tensors
-        dq, dk, dv = _lib.native.window_backward(q, k, v, o, lse2, _pad_last(do, v.shape[-1]), *ctx.scalars)
+        q, k, v, o, lse2, low = ctx.saved_tensors
+        dq, dk, dv = _lib.native.window_backward(q, k, v, o, lse2, low, _pad_last(do, v.shape[-1]), *ctx.scalars)
         return _cut_last(dq, ctx.dims[0]), _cut_last(dk, ctx.dims[0]), _cut_last(dv, ctx.dims[1]), None, None, None
 
 

@@ -319,12 +319,16 @@ typedef struct {
  * DLT_WINDOW_WORKSPACE_MAX.  The workspace is 16-byte aligned device memory that belongs to the call until its kernels have run. */
 #define DLT_WINDOW_WORKSPACE_MAX (256 << 20)
 int dlt_window_workspace(const dlt_window_shape_t* shape, int backward, int64_t* bytes);
+/* Tokens whose output's low part a backward pass wants: rows that see few keys (all of a window of at most 16 keys with its sinks, else those of the first 16 positions),
+ * whose gradients would suffer from the rounding of o.  o_low [B, H, tokens, dv], contiguous and 16-byte aligned, of o's type: what the forward pass's rounding
+ * of these rows of o dropped.  NULL (in either pass): not wanted. */
+int dlt_window_low_tokens(const dlt_window_shape_t* shape, int32_t* tokens);
 int dlt_window_fwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
-                   const void* v, const int64_t v_strides[4], void* o, const int64_t o_strides[4], float* lse2,
+                   const void* v, const int64_t v_strides[4], void* o, const int64_t o_strides[4], void* o_low, float* lse2,
                    const dlt_window_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
 /* delta: scratch of the size of lse2.  dk and dv are summed over the heads that share a key in a fixed order. */
 int dlt_window_bwd(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
-                   const void* v, const int64_t v_strides[4], const void* o, const int64_t o_strides[4],
+                   const void* v, const int64_t v_strides[4], const void* o, const int64_t o_strides[4], const void* o_low,
                    const void* d_o, const int64_t do_strides[4], const float* lse2, float* delta,
                    void* dq, const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4],
                    void* dv, const int64_t dv_strides[4],

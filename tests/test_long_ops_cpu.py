@@ -41,9 +41,9 @@ def window(L, backward=False, ptr=None, st=None, ws=ONE, ws_bytes=1 << 40, **kw)
     arg = lambda n: [ptr.get(n, ONE), st.get(n, dense(*t[n]))]  # noqa: E731
     lib = L.load()
     if backward:
-        args = sum((arg(n) for n in ("q", "k", "v", "o", "d_o")), []) + [ptr.get("lse2", ONE), ptr.get("delta", ONE)] + sum((arg(n) for n in ("dq", "dk", "dv")), [])
+        args = sum((arg(n) for n in ("q", "k", "v", "o")), []) + [ptr.get("low")] + arg("d_o") + [ptr.get("lse2", ONE), ptr.get("delta", ONE)] + sum((arg(n) for n in ("dq", "dk", "dv")), [])
         return lib.dlt_window_bwd(*args, s, ws, ws_bytes, None)
-    return lib.dlt_window_fwd(*sum((arg(n) for n in "qkvo"), []), ptr.get("lse2", ONE), s, ws, ws_bytes, None)
+    return lib.dlt_window_fwd(*sum((arg(n) for n in "qkvo"), []), ptr.get("low"), ptr.get("lse2", ONE), s, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("backward", [False, True])
@@ -52,7 +52,7 @@ def window(L, backward=False, ptr=None, st=None, ws=ONE, ws_bytes=1 << 40, **kw)
     (dict(B=0), 1, "positive"), (dict(Hkv=0), 1, "positive"), (dict(H=5), 1, "evenly"), (dict(window=0), 1, "window"), (dict(window=-3), 1, "window"),
     (dict(n_sink=-1), 1, "n_sink"), (dict(sm_scale=0.0), 1, "sm_scale"), (dict(sm_scale=-1.0), 1, "sm_scale"), (dict(sm_scale=float("nan")), 1, "sm_scale"),
     (dict(sm_scale=float("inf")), 1, "sm_scale"), (dict(Lq=-1), 1, "length"), (dict(Lk=1 << 30), 2, "tokens"), (dict(Lq=1 << 29), 2, "tokens"),
-    (dict(ptr={"k": None}), 1, "k is NULL"), (dict(ptr={"q": ctypes.c_void_p(264)}), 1, "16 bytes"),
+    (dict(ptr={"k": None}), 1, "k is NULL"), (dict(ptr={"q": ctypes.c_void_p(264)}), 1, "16 bytes"), (dict(ptr={"low": ctypes.c_void_p(264)}), 1, "o_low"),
     (dict(st={"v": I64(8192, 4096, 68, 1)}), 1, "16 bytes"), (dict(st={"q": I64(16384, 4096, 64, 2)}), 1, "contiguous"), (dict(st={"k": I64(8192, -4096, 64, 1)}), 1, "negative"),
     (dict(st={"k": I64(8192, 4096, 1 << 27, 1)}), 2, "too large"), (dict(st={"q": I64(8192, 1 << 29, 64, 1)}), 2, "too large"),
     (dict(B=MAX, Lk=4096, Lq=4096), 2, "workgroups"),
@@ -96,6 +96,18 @@ def test_window_workspace(L):
     for kw in (dict(B=300, H=32, Hkv=32, Lq=2000, Lk=2000, n_sink=2000, dk=128, dv=128), dict(Lq=1 << 20, Lk=1 << 20, n_sink=1 << 20), dict(Lq=1 << 24, Lk=(1 << 30) - 1, window=MAX),
                dict(H=MAX // 2, Hkv=1, Lq=1, Lk=1 << 20), dict(B=1 << 16, H=64, Hkv=64, Lq=1 << 14, Lk=1 << 14, n_sink=4)):
         assert need(0, **kw) <= 256 << 20 and need(1, **kw) <= 256 << 20, kw
+
+
+def test_window_low_tokens(L):
+    lib, n = L.load(), ctypes.c_int32(-1)
+
+    def tokens(**kw):
+        assert lib.dlt_window_low_tokens(L.WindowShape(**{**WINDOW, **kw}), ctypes.byref(n)) == 0, err(L)
+        return n.value
+    assert lib.dlt_window_low_tokens(L.WindowShape(**WINDOW), None) == 1 and "NULL" in err(L)
+    # all rows of a window of up to 16 keys, sinks counted; else those of positions below 16, the queries before the first key among them
+    assert tokens() == 64 and tokens(window=15, n_sink=1) == 64 and tokens(window=17) == 16 and tokens(window=16, n_sink=1) == 16 and tokens(window=MAX, n_sink=MAX) == 16
+    assert tokens(window=100, Lk=70) == 10 and tokens(window=100, Lk=200) == 0 and tokens(window=40, Lk=54) == 26 and tokens(window=100, Lq=3) == 0 and tokens(window=100, Lq=3, Lk=5) == 3
 
 
 PAGED = dict(B=2, H=4, Hkv=2, T=1, dk=64, dv=64, page=16, n_pages=100, cols=10, window=MAX, n_sink=0, sm_scale=0.125, dtype=BF16)

@@ -68,3 +68,28 @@ FAR = [
 def test_rows_far_behind_the_sinks(case):
     """Gradients of first keys that the rows of the whole sequence see."""
     test_against_64_bits(case)
+
+
+@pytest.mark.parametrize("Hq, Hkv, L, dk, dtype", [(2, 2, 70, 64, BF), (6, 2, 300, 128, HF), (4, 1, 1000, 96, BF)])
+def test_a_single_key_has_no_gradient_of_scores(Hq, Hkv, L, dk, dtype):
+    """The softmax of one score is 1 whatever the score is: dq and dk are zero, not the rest of a cancellation."""
+    q, k, v, do = make(2, 1, Hq, Hkv, L, L, dk, dk, dtype)
+    got = run(q, k, v, do, 1, 0, 0.3)
+    assert torch.equal(got["o"], v.repeat_interleave(Hq // Hkv, 1)) and not got["dq"].any() and not got["dk"].any() and got["dv"].any()
+    got = run(q[:, :, :1], k[:, :, :1], v[:, :, :1], do[:, :, :1], None, 3, 0.3)
+    assert not got["dq"].any() and not got["dk"].any()
+    got = run(q, k, v, do, None, 0, 0.3)
+    assert not got["dq"][:, :, 0].any() and got["dq"][:, :, 1].any()   # the query at position 0 sees one key
+
+
+@pytest.mark.parametrize("window, n_sink, dtype", [(2, 0, BF), (2, 0, HF), (3, 1, HF), (1, 2, BF), (8, 0, BF), (500, 0, HF)])
+def test_gradients_of_few_keys(window, n_sink, dtype):
+    """Where a row sees few keys, dP and delta nearly cancel, and delta must not suffer from the rounding of o.  The errors of dq and dk, as norms, against those that
+    their own rounding makes (1): the rounding of dS makes as much, sqrt(2) together, and P, from sums of rounded exponentials, a third of it: sqrt(2 + 1 / 9) < 1.46, with two keys,
+    whose dS are opposite, up to 1.6.  With delta from the rounded o two keys gave 2.3, eight 1.6."""
+    q, k, v, do = make(3, 1, 4, 4, 400, 400, 64, 64, dtype)
+    got, want = run(q, k, v, do, window, n_sink, 0.125), orc.window(q, k, v, window, n_sink, 0.125, do)
+    for name in ("dq", "dk"):
+        value = want[name][0]
+        own = (value.to(dtype).double() - value).norm()
+        assert (got[name].double() - value).norm() <= 1.7 * own, name
