@@ -309,6 +309,7 @@ void plan_keys(BandArgs& a) {
   a.far = a.far_groups = a.part_keys = 0;
   const int64_t wgs = bh * a.nblk;
   const int64_t near_chunks = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;   // of a block without sinks
+  a.cycle = (int)near_chunks;
   const int64_t want = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
   const int64_t key_bytes = dlt_imax64(bh * a.Lk * (a.dk_ + a.dv_) * 4, 1);
   a.shares = (int)dlt_imax64(1, dlt_imin64(dlt_imin64(want, near_chunks / 4), DLT_WINDOW_WORKSPACE_MAX / 2 / key_bytes));

@@ -36,6 +36,7 @@ struct BandArgs {
   int32_t shares;           // workgroups that share the keys (forward) or rows (dK / dV) of an own block
   int32_t far, far_groups;  // dK / dV: workgroups that share the far rows of a group of sinks, such groups (band_bwd_kernel.h); 0: none
   int32_t part_keys;        // keys of a (batch, kv head) with partial sums
+  int32_t cycle;            // dK / dV: chunks of rows that see a block of keys
   int32_t low_rows;         // rows of a (batch, kv head) with low parts
   int32_t q16;              // 16 is a multiple of G: 16 rows are whole tokens
   float scale_log2, sm_scale, grad_scale;   // grad_scale: of dQ and dK; 0 where every row sees one key, whose dS are zero but for roundings
