@@ -410,6 +410,10 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     // issued in pieces behind the matrix instructions of the following segment
     constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NP2 = 2 * KB, NT = N1 + NQB * NP2;
     constexpr int NU = 2 * NP;
+    // Each sum is a chain of products that wait for each other: at d = 128 S and dP take turns (8192 tokens, window 1024, 16 heads on 4 179 -> 173 us; 8 x 8 kv heads of 4 query
+    // heads, 1111 tokens, 138 -> 129), at d = 64, where three workgroups share a CU, one follows the other (98 against 100, 76 against 76)
+    constexpr auto score = [](int r) { return D > 64 ? r % 2 == 0 : r < KC; };
+    constexpr auto dims = [](int r) { return D > 64 ? r / 2 : r % KC; };
     static_assert(NP2 >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
     constexpr int RD = 3;   // 1: 197 us, 3: 187 for 16 heads on 4, 8192 tokens, window 1024, d = 128; more: spills
     u32x4 ring[RD + 1];
@@ -417,8 +421,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
       constexpr int k = decltype(kc)::value;
       if constexpr (k < N1) {
         constexpr int hh = k / N1H, r = k % N1H, T0 = 16 * hh;
-        if constexpr (r < KC) ring[k % (RD + 1)] = swa2_lds16(sQ + T0 * FlashDRow<D>::ROW + L.a[r]);
-        else ring[k % (RD + 1)] = swa2_lds16(sDO + T0 * FlashDRow<D>::ROW + L.a[r - KC]);
+        ring[k % (RD + 1)] = swa2_lds16((score(r) ? sQ : sDO) + T0 * FlashDRow<D>::ROW + L.a[dims(r)]);
       } else {
         constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
         if constexpr (d < KB) ring[k % (RD + 1)] = flashd_read_tr<D, 32 * qb_>(sDO, L, d);
@@ -478,8 +481,8 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
         constexpr int hh = k / N1H, r = k % N1H;
 #pragma unroll
         for (int p = 0; p < NP; p++) {
-          if constexpr (r < KC) sv[hh & 1][p] = Mma<TIO>::mfma(op, kf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[hh & 1][p]);
-          else dp[hh & 1][p] = Mma<TIO>::mfma(op, vf[p][r - KC], r == KC ? dl[hh & 1] : dp[hh & 1][p]);
+          if constexpr (score(r)) sv[hh & 1][p] = Mma<TIO>::mfma(op, kf[p][dims(r)], dims(r) == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[hh & 1][p]);
+          else dp[hh & 1][p] = Mma<TIO>::mfma(op, vf[p][dims(r)], dims(r) == 0 ? dl[hh & 1] : dp[hh & 1][p]);
         }
         if constexpr (hh >= 1 && r < NU) {
           ew(std::integral_constant<int, hh - 1>{}, std::integral_constant<int, r>{});
