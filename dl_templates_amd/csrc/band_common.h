@@ -293,6 +293,8 @@ DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (
   __syncthreads();
 }
 
+// 1 / sum of a row at position `pos` (< 0: it sees nothing, and gives zeros).  A sum of 0 otherwise means that every score that the row sees is -inf: the softmax of those is NaN.
+DLT_DEV float band_inverse(float sum, int pos) { return sum != 0.f ? fast_rcp(sum) : pos < 0 ? 0.f : NAN; }
 DLT_DEV bool band_odd(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }   // infinite or NaN
 template <int NP, int NA>
 DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {

@@ -353,7 +353,8 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   }
 #pragma unroll
   for (int p = 0; p < NP; p++) {
-    inv[p] = lt[p] > 0.f && wq0 + 16 * p + n < n_rows ? fast_rcp(lt[p]) : 0.f;   // rows that see nothing, and rows behind the last query: zeros
+    const int r = wq0 + 16 * p + n;   // rows behind the last query: zeros
+    inv[p] = band_inverse(lt[p], r < n_rows ? sq.off + band_row(a, r).tok : -1);
     const uint64_t bad = __builtin_amdgcn_ballot_w64(grp == 0 && wq0 + 16 * p + n < n_rows && (band_odd_row(acc, p) || band_odd(lt[p])));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
                                     float m, l, o2[2];
                                     band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok,
                                                                    sq.n_k, lane, m, l, o2);
-                                    const float f = l == 0.f ? 0.f : 1.f / l;
+                                    const float f = band_inverse(l, sq.off + band_row(a, r).tok);
                                     if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(o2[0] * f, o2[1] * f);
                                     if (lane == 0 && a.lse != nullptr) a.lse[row0 + r] = m + fast_log2(l);
                                   }

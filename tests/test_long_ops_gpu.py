@@ -100,6 +100,28 @@ def test_infinite_values(case):
     orc.check(o[~hit], (value[~hit], bound[~hit]), "o")
 
 
+@pytest.mark.parametrize("Lq, Lk, window, n_sink", [(70, 70, 1, 0), (300, 300, 1, 0), (1, 2000, 1, 0), (3, 3000, None, 0), (90, 40, 1, 0)])
+def test_scores_of_minus_infinity(Lq, Lk, window, n_sink):
+    """A row all of whose scores are -inf is NaN, as the formula's softmax is; next to a finite score they weigh nothing; rows that see nothing are zeros."""
+    q, k, v, do = make(14, 1, 4, 2, Lq, Lk, 64, 64, BF)
+    q = q.abs() + 0.1
+    k[0, 0] = -INF
+    o = window_attention(q, k, v, window, n_sink, 0.125)
+    sees = torch.arange(Lq, device="cuda") + Lk - Lq >= 0
+    assert o[0, :2][:, sees].isnan().all() and (o[0, :2][:, ~sees] == 0).all()
+    orc.check(o[:, 2:], tuple(x[:, 2:] for x in orc.window(q, k.nan_to_num(0, 0, 0), v, window, n_sink, 0.125)["o"]), "the other head")
+    k[0, 0, Lk - 1] = 0.5
+    o = window_attention(q[:, :2, -1:], k[:, :1], v[:, :1], None, 0, 0.125)
+    assert torch.equal(o, v[:, :1, -1:].expand(1, 2, 1, 64))
+    kc, vc = (x[0].transpose(0, 1).reshape(-1, 2, 64).transpose(0, 1).reshape(2, -1, 64) for x in (k, v))
+    if Lk % 16 == 0:   # the same through pages
+        pages = lambda x: x.reshape(2, Lk // 16, 16, 64).transpose(0, 1).contiguous()  # noqa: E731
+        kc[0] = -INF
+        table = torch.arange(Lk // 16, dtype=torch.int32, device="cuda")[None]
+        o = paged_attention(q, pages(kc), pages(vc), table, ints(Lk), window, n_sink, 0.125)
+        assert o[0, :2].isnan().all() and not o[0, 2:].isnan().any()
+
+
 def test_scores_beyond_the_type():
     """Scores of 2^17 and -2^17 (no 16-bit score could hold the first in fp16): weights of keys with one score are equal."""
     for dtype in (BF, HF):
