@@ -311,9 +311,12 @@ void plan_keys(BandArgs& a) {
   const int64_t wgs = bh * a.nblk;
   const int64_t near_chunks = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;   // of a block without sinks
   a.cycle = (int)near_chunks;
+  // at least 4 chunks a share, 8 at d = 128, whose partial sums weigh more (us with the sum of the parts, 4 / 8 chunks: 2 kv heads of 2000 tokens, 4 query heads each, window 500, 29.8 / 27.6;
+  // 4 of 1500, window 300, 37.4 / 30.0; at d = 64 one of 600, window 200, 13.8 / 17.1)
+  const int64_t least = band_class(a.dk_, a.dv_) == 64 ? 4 : 8;
   const int64_t want = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
   const int64_t key_bytes = dlt_imax64(bh * a.Lk * (a.dk_ + a.dv_) * 4, 1);
-  a.shares = (int)dlt_imax64(1, dlt_imin64(dlt_imin64(want, near_chunks / 4), DLT_WINDOW_WORKSPACE_MAX / 2 / key_bytes));
+  a.shares = (int)dlt_imax64(1, dlt_imin64(dlt_imin64(want, near_chunks / least), DLT_WINDOW_WORKSPACE_MAX / 2 / key_bytes));
   const int64_t near_end = dlt_imin64((int64_t)dlt_imax(dlt_imin(own, a.Lk) - 1 - a.off + a.W, 0) * a.G, a.rows);
   const int64_t far_chunks = (a.rows - near_end + 63) / 64;
   if (a.S > 0 && far_chunks > 4) {
