@@ -98,6 +98,36 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
   if (lane == 0 && a.lse != nullptr) a.lse[at] = m + fast_log2(l);
 }
 
+// dQ: partial rows [bh][share][row][dk], added in the order of the shares (WG: every wave every fourth one, then the four)
+template <typename TIO, bool WG>
+__global__ __launch_bounds__(256) void band_join_q_kernel(const BandArgs a) {
+  dlt_kernargs_in<sizeof(BandArgs)>();
+  __shared__ float2 sum[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = WG ? (int64_t)blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+  if (!WG && at >= (int64_t)a.B * a.Hkv * a.rows) return;
+  const int bh = (int)(at / a.rows), r = (int)(at - (int64_t)bh * a.rows), b = bh / a.Hkv, h = bh - b * a.Hkv;
+  const bool on = 2 * lane < a.dk_;
+  const int64_t step = (int64_t)a.rows * a.dk_;
+  const float* part = a.part + ((int64_t)bh * a.shares * a.rows + r) * a.dk_ + (on ? 2 * lane : 0);
+  float2 s = {0.f, 0.f};
+#pragma unroll 8
+  for (int i = WG ? wave : 0; i < a.shares; i += WG ? 4 : 1) {
+    const float2 v = *reinterpret_cast<const float2*>(part + i * step);
+    s.x += v.x;
+    s.y += v.y;
+  }
+  if constexpr (WG) {
+    sum[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0) return;
+    for (int i = 1; i < 4; i++) { s.x += sum[i][lane].x; s.y += sum[i][lane].y; }
+  }
+  const float f = a.off + band_row(a, r).tok == 0 ? 0.f : a.grad_scale;   // a row at position 0 sees one key
+  TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.dq) + b * a.dqs[0] + (int64_t)h * a.G * a.dqs[1], a.dqs, a, r);
+  if (on) *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(s.x * f, s.y * f);
+}
+
 // dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares.  Keys with far sums, of which there are up to hundreds,
 // come first, a workgroup to a key, where 8 runs of threads take every eighth sum (one run: 9 us for 16 keys of 112 sums on 4 heads, this way 5.5).
 template <typename TIO>
@@ -143,6 +173,24 @@ __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
   w.x = pack2<TIO>(s[0], s[1]);
   w.y = pack2<TIO>(s[2], s[3]);
   store_stream8(p + d, w);
+}
+
+int join_q(const BandArgs& a, int dtype, hipStream_t stream) {
+  if (a.shares <= 1) return DLT_OK;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.rows;
+  const bool wg = a.shares > 8;
+  const dim3 grid((unsigned)(wg ? rows : (rows + 3) / 4));
+  dlt_timing_before(DLT_K_BWD_Q, stream);
+  if (dtype == DLT_BF16) {
+    if (wg) hipLaunchKernelGGL((band_join_q_kernel<bf16_t, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((band_join_q_kernel<bf16_t, false>), grid, dim3(256), 0, stream, a);
+  } else {
+    if (wg) hipLaunchKernelGGL((band_join_q_kernel<f16_t, true>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((band_join_q_kernel<f16_t, false>), grid, dim3(256), 0, stream, a);
+  }
+  dlt_timing_after(stream);
+  DLT_CHECK_LAUNCH("window dQ sum launch");
+  return DLT_OK;
 }
 
 int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
@@ -269,7 +317,9 @@ void set_map(BandArgs& a) {
 //                200 tokens, window 64, d = 64, 6.7 -> 5.2; of 1000 tokens, window 300, 9.4 -> 7.0, d = 128 11.8 -> 8.6; 8 heads of 500, window 200, d = 128, 10.4 -> 7.8; one token on 300 keys,
 //                8 heads, 8.2 -> 7.6.  With two workgroups a CU 7.7 -> 10.2 (8 heads of 1000, window 100, d = 64); with more keys the shares win: 8 tokens of 8 heads on 900 keys, d = 128,
 //                15.2 -> 8.4 + 3.8
-// Shares: up to two workgroups a CU, at least four chunks each.  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
+// Shares: up to two workgroups a CU (one round of them: 4 kv heads, 200 queries of two heads on 8000 keys, d = 128, 19 shares of 28
+// blocks 24 us, 18 shares 18), at least four chunks each; dQ: while its blocks fill half of the CUs (us with the sum of the parts: 4 kv heads, 200 queries of two heads on
+// 8000 keys, d = 128, 132 -> 28; 2 heads, 10 queries of 4 heads on 2000, d = 64, 27 -> 12; but 1000 queries of 8 heads on 1000 keys, 250 blocks, 18 -> 20).  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
 // (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).
 int plan_rows(BandArgs& a, bool forward) {
   const int cus = dlt_device_cus();
@@ -289,9 +339,9 @@ int plan_rows(BandArgs& a, bool forward) {
   a.nblk = blocks(own);
   a.shares = 1;
   const int64_t wgs = bh * a.nblk;
-  if (forward && kind == BAND_ONE && wgs > 0 && (wgs < cus || uneven)) {
-    int64_t n = dlt_imin64(dlt_imin64(((uneven ? 4 : 2) * cus + wgs - 1) / wgs, chunks(own) / 4), BAND_SHARES_MAX);
-    const int64_t row_bytes = bh * a.rows * (a.dv_ + 2) * 4;
+  if (kind == BAND_ONE && wgs > 0 && (forward ? wgs < cus || uneven : 2 * wgs <= cus)) {
+    int64_t n = dlt_imin64(dlt_imin64((uneven ? 4 : 2) * cus / wgs, chunks(own) / 4), BAND_SHARES_MAX);
+    const int64_t row_bytes = bh * a.rows * (forward ? a.dv_ + 2 : a.dk_) * 4;
     n = dlt_imin64(n, DLT_WINDOW_WORKSPACE_MAX / dlt_imin64(row_bytes > 0 ? row_bytes : 1, DLT_WINDOW_WORKSPACE_MAX));
     a.shares = n < 1 ? 1 : (int)n;
   }
@@ -299,6 +349,7 @@ int plan_rows(BandArgs& a, bool forward) {
   return kind;
 }
 int64_t rows_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * (a.dv_ + 2) * 4 : 0; }
+int64_t q_bytes(const BandArgs& a) { return a.shares > 1 ? (int64_t)a.B * a.Hkv * a.shares * a.rows * a.dk_ * 4 : 0; }
 int64_t keys_bytes(const BandArgs& a) { return a.part_keys > 0 ? BandParts(a).floats * 4 : 0; }
 // Keys: the rows that see a block of keys taken by several workgroups where blocks are few, the far rows of sinks always
 void plan_keys(BandArgs& a) {
@@ -358,9 +409,15 @@ extern "C" int dlt_window_workspace(const dlt_window_shape_t* shape, int backwar
   BandArgs a;
   const int rc = window_problem("window_workspace", shape, a);
   if (rc != DLT_OK) return rc;
-  if (backward) plan_keys(a);
-  else plan_rows(a, true);
-  *bytes = backward ? keys_bytes(a) : rows_bytes(a);
+  if (backward) {   // the passes use the workspace one after the other
+    plan_rows(a, false);
+    *bytes = q_bytes(a);
+    plan_keys(a);
+    *bytes = dlt_imax64(*bytes, keys_bytes(a));
+  } else {
+    plan_rows(a, true);
+    *bytes = rows_bytes(a);
+  }
   return DLT_OK;
 }
 
@@ -416,7 +473,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
   BandArgs kv = a;
   plan_keys(kv);
   const int kind = plan_rows(a, false);
-  if ((rc = check_ws(who, ws, ws_bytes, keys_bytes(kv))) != DLT_OK) return rc;
+  if ((rc = check_ws(who, ws, ws_bytes, dlt_imax64(q_bytes(a), keys_bytes(kv)))) != DLT_OK) return rc;
   if ((rc = check_grid(who, a)) != DLT_OK || (rc = check_grid(who, kv)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND)) return DLT_OK;
   for (BandArgs* x : {&a, &kv}) {
@@ -427,6 +484,7 @@ extern "C" int dlt_window_bwd(const void* q, const int64_t q_strides[4], const v
   }
   const bool small = band_class(a.dk_, a.dv_) == 64;
   if (!nq && (rc = small ? dlt_band_bwd_q_64(a, shape->dtype, kind, stream) : dlt_band_bwd_q_128(a, shape->dtype, kind, stream)) != DLT_OK) return rc;
+  if (!nq && (rc = join_q(a, shape->dtype, stream)) != DLT_OK) return rc;
   if (nk) return DLT_OK;
   if ((rc = small ? dlt_band_bwd_kv_64(kv, shape->dtype, stream) : dlt_band_bwd_kv_128(kv, shape->dtype, stream)) != DLT_OK) return rc;
   return join(kv, true, shape->dtype, stream);

@@ -25,8 +25,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   const int lin = xcd_remap(blockIdx.x, gridDim.x);
-  int b, h, blk, share_;
-  band_block(a, lin, true, b, h, blk, share_);
+  int b, h, blk, share;
+  band_block(a, lin, true, b, h, blk, share);
   const int x0 = blk * OWN, bh = b * a.Hkv + h;
   const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];
   const TIO* dob = reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1];
@@ -38,6 +38,9 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   const int xl = dlt_imin(x0 + OWN, a.rows) - 1;
   const int first = a.off + band_row(a, x0).tok, last = a.off + band_row(a, xl).tok;
   W.init(first, last, a.W, a.S);
+  // chunks of this share: few rows on many keys (BAND_ONE) are split over workgroups, whose partial sums a second launch adds
+  const int per = NP == 1 ? (W.n + a.shares - 1) / a.shares : W.n;
+  const int i_beg = NP == 1 ? dlt_imin(share * per, W.n) : 0, i_end = NP == 1 ? dlt_imin(i_beg + per, W.n) : W.n;
 
   BandStage<D> stk, stv;
   stk.init(lane, a.dk_, a.ks[2]);
@@ -67,7 +70,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   };
 #pragma unroll 1
   for (int i = 0; i < AHEAD; i++)
-    if (i < W.n) issue(i, smem + i * B::BUF);
+    if (i_beg + i < i_end) issue(i_beg + i, smem + i * B::BUF);
 
   const int wq0 = x0 + wave * 16 * NP;
   u32x4 qf[NP][KC], dof[NP][KC];
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
       }
     }
     del[p] = wave_sum4(sum);
-    if (g == 0 && on) store_stream4(a.delta + row0 + r, del[p]);
+    if (g == 0 && on && share == 0) store_stream4(a.delta + row0 + r, del[p]);
   }
   const int wl = dlt_imin(wq0 + 16 * NP, a.rows) - 1;
   const int pa = wl >= wq0 ? a.off + band_row(a, wq0).tok : 0, pb = wl >= wq0 ? a.off + band_row(a, wl).tok : -1;
@@ -203,13 +206,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     consume(x, (Swa2Lds)buf, mask_tag);
   };
   int f0, f1;
-  W.whole(first, last, a.W, 0, W.n, f0, f1);
+  W.whole(first, last, a.W, i_beg, i_end, f0, f1);
   // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
   // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
-  int bi = 0, i = 0, stop = f0;
+  int bi = 0, i = i_beg, stop = f0;
   auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
   auto step = [&](auto mask_tag) __attribute__((always_inline)) {
-    const bool more = i + AHEAD < W.n;
+    const bool more = i + AHEAD < i_end;
     if (more) issue(i + AHEAD, buf_of(bi + AHEAD));
     chunk(i, buf_of(bi), mask_tag);
     if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
@@ -222,10 +225,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   for (;;) {
 #pragma unroll 1
     while (i < stop) step(std::true_type{});
-    if (i >= W.n) break;
+    if (i >= i_end) break;
 #pragma unroll 1
     while (i < f1) step(std::false_type{});
-    stop = W.n;
+    stop = i_end;
   }
   __syncthreads();
   float mul[NP];
@@ -236,36 +239,52 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < a.rows && band_odd_row(acc, p));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }
+  // a row with an infinite or NaN sum once more, over the keys of the share that it sees alone (band_common.h): two dims, without the factor
+  auto exact = [&](int r, float (&sum)[2]) __attribute__((always_inline)) {
+    const int pos = a.off + band_row(a, r).tok;
+    const TIO *q = band_row_ptr(qb, a.qs, a, r), *d_o = band_row_ptr(dob, a.dos, a, r);
+    const float lse = a.lse[row0 + r], delta = band_dot(band_row_ptr(ob, a.os, a, r), d_o, a.dv_);
+    sum[0] = sum[1] = 0.f;
+#pragma unroll 1
+    for (int c = i_beg; c < i_end; c++)
+#pragma unroll 1
+      for (int x = W.x(c); x < W.x(c) + CK; x += 64) {
+        const int j = x + lane;
+        const bool sees = j < a.Lk && band_sees(pos, j, a.W, a.S);
+        uint64_t left = __builtin_amdgcn_ballot_w64(sees);
+        float ds = 0.f;
+        if (sees) ds = fast_exp2(band_dot(q, kh + j * a.ks[2], a.dk_) * scale - lse) * (band_dot(d_o, vh + j * a.vs[2], a.dv_) - delta);
+        for (; left != 0; left &= left - 1) {
+          const int u = __builtin_ctzll(left);
+          band_axpy(sum, band_lane(ds, u), kh + (x + u) * a.ks[2], a.dk_, lane);
+        }
+      }
+  };
+  if (NP == 1 && a.shares > 1) {
+    float* part = a.part + ((int64_t)bh * a.shares + share) * a.rows * a.dk_;
+    flash_share_put<NP>(part, acc, a.dk_, wq0 + n, a.rows, g);
+    for (unsigned todo = odd[0]; todo != 0; todo &= todo - 1) {
+      const int r = wq0 + __builtin_ctz(todo);
+      float sum[2];
+      exact(r, sum);
+      __threadfence();   // behind the wave's own stores of the row
+      if (2 * lane < a.dk_) *reinterpret_cast<float2*>(part + (int64_t)r * a.dk_ + 2 * lane) = float2{sum[0], sum[1]};
+    }
+    return;
+  }
   TIO* dqb = reinterpret_cast<TIO*>(a.dq) + b * a.dqs[0] + (int64_t)h * a.G * a.dqs[1];
   constexpr int PT = D * 2 + 16;
   band_store_rows<D, NP, TIO>(smem, acc, mul, NW, 1, true, a.dk_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(dqb, a.dqs, a, x0 + row) : nullptr; },
                               [&]() {
-                                // rows with an infinite or NaN sum once more, over the keys that they see alone (band_common.h)
 #pragma unroll 1
                                 for (int p = 0; p < NP; p++)
                                   for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
-                                    const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w, pos = a.off + band_row(a, r).tok;
-                                    const TIO *q = band_row_ptr(qb, a.qs, a, r), *d_o = band_row_ptr(dob, a.dos, a, r);
-                                    const float lse = a.lse[row0 + r], delta = band_dot(band_row_ptr(ob, a.os, a, r), d_o, a.dv_);
-                                    float sum[2] = {0.f, 0.f};
-#pragma unroll 1
-                                    for (int c = 0; c < W.n; c++)
-#pragma unroll 1
-                                      for (int x = W.x(c); x < W.x(c) + CK; x += 64) {
-                                        const int j = x + lane;
-                                        const bool sees = j < a.Lk && band_sees(pos, j, a.W, a.S);
-                                        uint64_t left = __builtin_amdgcn_ballot_w64(sees);
-                                        float ds = 0.f;
-                                        if (sees)
-                                          ds = fast_exp2(band_dot(q, kh + j * a.ks[2], a.dk_) * scale - lse) * (band_dot(d_o, vh + j * a.vs[2], a.dv_) - delta);
-                                        for (; left != 0; left &= left - 1) {
-                                          const int u = __builtin_ctzll(left);
-                                          band_axpy(sum, band_lane(ds, u), kh + (x + u) * a.ks[2], a.dk_, lane);
-                                        }
-                                      }
-                                    if (2 * lane < D)
-                                      *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * (pos == 0 ? 0.f : a.grad_scale), sum[1] * (pos == 0 ? 0.f : a.grad_scale));
+                                    const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w;
+                                    float sum[2];
+                                    exact(r, sum);
+                                    const float f = a.off + band_row(a, r).tok == 0 ? 0.f : a.grad_scale;
+                                    if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * f, sum[1] * f);
                                   }
                               });
 }

@@ -59,7 +59,7 @@ int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind
 template <typename TIO, int NP>
 int band_bwd_q(const BandArgs& a, hipStream_t stream) {
   constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
-  return band_go(band_pick(a, band_bwd_q_kernel<TIO, D, NP, 64, 4, 0>, band_bwd_q_kernel<TIO, D, NP, 64, 4, FEWER>, band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>), a, (int64_t)a.B * a.Hkv * a.nblk, 256, lds,
+  return band_go(band_pick(a, band_bwd_q_kernel<TIO, D, NP, 64, 4, 0>, band_bwd_q_kernel<TIO, D, NP, 64, 4, FEWER>, band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>), a, (int64_t)a.B * a.Hkv * a.nblk * a.shares, 256, lds,
                  DLT_K_BWD_Q, "window dQ launch", stream);
 }
 template <typename TIO>

@@ -70,6 +70,21 @@ def test_rows_far_behind_the_sinks(case):
     test_against_64_bits(case)
 
 
+SHARED = [
+    (1, 4, 2, 20, 3000, 64, 64, None, 4, BF),
+    (1, 2, 1, 10, 5000, 128, 128, None, 0, HF),
+    (2, 2, 2, 100, 2100, 80, 72, 2000, 9, BF),
+    (1, 3, 1, 130, 4000, 128, 40, 3000, 70, HF),
+    (1, 1, 1, 1, 9000, 64, 64, None, 0, BF),
+]
+
+
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_few_queries_on_many_keys(case):
+    """Keys shared by workgroups, in the forward pass and for dq."""
+    test_against_64_bits(case)
+
+
 @pytest.mark.parametrize("Hq, Hkv, L, dk, dtype", [(2, 2, 70, 64, BF), (6, 2, 300, 128, HF), (4, 1, 1000, 96, BF)])
 def test_a_single_key_has_no_gradient_of_scores(Hq, Hkv, L, dk, dtype):
     """The softmax of one score is 1 whatever the score is: dq and dk are zero, not the rest of a cancellation."""
