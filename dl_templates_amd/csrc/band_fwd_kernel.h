@@ -247,8 +247,8 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
               for (int i = 0; i < 4; i++) mx[i] = fmaxf(fmaxf(mx[i], t[p][kb2][2 * i]), t[p][kb2][2 * i + 1]);
             const float mloc = wave_max4(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
             // the reference maximum moves only when a score exceeds it by more than 2^8 after scaling: P stays below 2^8, its sum in
-            // 32 bits below 2^8 times the keys
-            if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > 8.f)) {
+            // 32 bits below 2^8 times the keys.  In masked chunks, where rows of few keys lie, it moves with the maximum: the largest P is then 1, and not rounded
+            if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > (MASK ? 0.f : 8.f))) {
               keep_branch();
               const float m_new = fmaxf(m_run[p], mloc);
               const float alpha = fast_exp2((m_run[p] - m_new) * scale);
@@ -263,6 +263,12 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
             for (int kb2 = 0; kb2 < NKB; kb2++) {
 #pragma unroll
               for (int i = 0; i < 8; i++) t[p][kb2][i] = fast_exp2(fmaf(t[p][kb2][i], scale, neg_m2));
+              if constexpr (MASK) {   // rows of few keys lie in masked chunks: the sum of what is rounded afterwards, in 32 bits
+                float l[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) l[i] = t[p][kb2][i] + t[p][kb2][4 + i];
+                acc_l[p][0] += (l[0] + l[1]) + (l[2] + l[3]);
+              }
               pb_[p][kb2] = pack8<TIO>(t[p][kb2]);
             }
           }
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
         constexpr int kb = (k - N1) / VB, d = (k - N1) % VB;
 #pragma unroll
         for (int p = 0; p < NP; p++) acc[p][d] = Mma<TIO>::mfma(op, pb_[p][kb], acc[p][d]);
-        if constexpr (d == VB - 1) {
+        if constexpr (d == VB - 1 && !MASK) {   // elsewhere the sum of the rounded P, a row of ones in the matrix product
 #pragma unroll
           for (int p = 0; p < NP; p++) acc_l[p] = Mma<TIO>::mfma(ones, pb_[p][kb], acc_l[p]);
         }
