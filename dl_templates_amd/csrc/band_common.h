@@ -154,9 +154,9 @@ DLT_DEV void band_copy2(const char* base, uint32_t va, uint32_t vb, char* lds) {
 DLT_DEV void band_copy4(const char* base, const uint32_t (&v)[4], char* lds) {
   const uint32_t m = (uint32_t)(uintptr_t)(DLT_LDS char*)lds;
   uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:1024\n\t"
-               "global_load_lds_dwordx4 %4, %1 offset:2048\n\tglobal_load_lds_dwordx4 %5, %1 offset:3072\n\ts_mov_b32 m0, %0"
-               : "=&s"(saved) : "s"(base), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(m) : "memory");
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %6\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1\n\tglobal_load_lds_dwordx4 %3, %1 offset:%7\n\t"
+               "global_load_lds_dwordx4 %4, %1 offset:%8\n\tglobal_load_lds_dwordx4 %5, %1 offset:%9\n\ts_mov_b32 m0, %0"
+               : "=&s"(saved) : "s"(base), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(m), "n"(1024), "n"(2 * 1024), "n"(3 * 1024) : "memory");
 }
 // All copies of a group of 16 tokens: copy i goes to `lds` + 1024 i; v[i] = the lane's offset + band_bias - 1024 i, taken from base - band_bias.  Under PAD lanes of pieces that
 // do not exist copy nothing; copies two apart move the same piece (8 tokens apart).
@@ -170,8 +170,8 @@ DLT_DEV void band_copy_group(const char* base, const uint32_t (&v)[NI], bool on0
   } else if constexpr (!PAD) {
     band_copy4(b, v, lds);
   } else {
-    if (on0) band_copy2<0, 2048>(b, v[0], v[2], lds);
-    if (on1) band_copy2<1024, 3072>(b, v[1], v[3], lds);
+    if (on0) band_copy2<0, 2 * 1024>(b, v[0], v[2], lds);
+    if (on1) band_copy2<1024, 3 * 1024>(b, v[1], v[3], lds);
   }
 }
 

@@ -545,6 +545,24 @@ def test_cache_views():
     orc.check(o[:1], orc.window(q[:1], k[:1], v[:1], 50, 1, 0.125)["o"], "o")
 
 
+def test_inference_mode():
+    """Tensors made in inference mode: caches written there, attention over them, the dense operator and the rotation."""
+    gen = torch.Generator().manual_seed(25)
+    raw = [torch.randn(2, h, 40, 64, generator=gen).to(BF).cuda() for h in (4, 2, 2)]
+    tables, pos = [orc.table(64, 32).cuda()], torch.arange(40, dtype=torch.int32, device="cuda")[None]
+
+    def work():
+        q, k, v = (x.clone() for x in raw)
+        kc, vc = (torch.zeros(6, 2, 16, 64, dtype=BF, device="cuda") for _ in range(2))
+        table, seq = torch.arange(6, dtype=torch.int32, device="cuda").reshape(2, 3), ints(40, 40)
+        r = paged_append_(kc, vc, k, v, table, seq, None, (None, tables, "halves"), q)
+        return kc, vc, paged_attention(r, kc, vc, table, seq, 16, 1), window_attention(q, k, v, 16, 1), *rope_axes_qk(q, k, pos, tables), *rope_axes_qk_(q, k, pos, tables)
+    want = work()
+    with torch.inference_mode():
+        got = work()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---- graphs --------------------------------------------------------------------------------------------------------------------------
 def captured(f):
     """(graph, outputs): `f` recorded after a warm call on another stream."""
