@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
     }
   }
   const int n_k = a.pg.seq != nullptr ? dlt_imax(0, dlt_imin(a.pg.seq[b], a.Lk)) : a.Lk;
-  const float f = band_inverse(l, on ? n_k - n_q + band_row(a, r).tok : -1);
+  const float f = on ? band_inverse(l, n_k - n_q + band_row(a, r).tok) : 0.f;
   TIO* p = band_row_ptr(reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1], a.os, a, r);
   if (2 * lane < a.dv_) *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(o[0] * f, o[1] * f);
   TIO* low = a.low != nullptr ? band_low<TIO>(a, b, h, r) : nullptr;

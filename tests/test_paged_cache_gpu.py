@@ -38,6 +38,11 @@ ATTN = [
     (1, 64, 1, 3, 16, [77], None, 32, 32, 16, 1, HF),
     (1, 2, 1, 200, 128, [3000], None, 96, 96, 700, 9, BF),
     (1, 8, 8, 1, 16, [4000], None, 64, 64, None, 0, HF),
+    # padded rows beside rows that see whole chunks
+    (5, 8, 1, 2, 16, [317, 326, 356, 352, 293], [1, 0, 2, 1, 2], 104, 104, None, 0, BF),
+    (6, 32, 8, 185, 96, [54, 217, 627, 366, 183, 569], [48, 149, 73, 127, 143, 44], 112, 16, 582, 0, BF),
+    (2, 4, 2, 30, 32, [6000, 5000], [3, 30], 64, 64, None, 4, HF),
+    (3, 4, 4, 300, 64, [1500, 900, 300], [20, 300, 0], 128, 128, 700, 2, BF),
 ]
 
 
