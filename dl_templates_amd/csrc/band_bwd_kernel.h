@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NG; u++) {
-      const int t0 = W.x(i) + wave * 16 * NG + 16 * u;
+      const int t0 = W.tok(CK * i + wave * 16 * NG + 16 * u);
       char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
       if (t0 + 16 <= a.Lk) {
         stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (int64_t)t0 * a.ks[2]), dst);
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     const int r = wq0 + 16 * p + n;
     const bool on = r < a.rows;
     const int rc = on ? r : 0, pos = a.off + band_row(a, rc).tok;
-    hi[p] = on ? pos : -1;
-    lo[p] = pos - a.W;
+    hi[p] = on ? pos - W.jump : -1;   // the row sees places lo < y <= hi, and the sinks
+    lo[p] = pos - a.W - W.jump;
     band_load_own<KC>(qf[p], band_row_ptr(qb, a.qs, a, rc), on, a.dk_, g);
     band_load_own<KC>(dof[p], band_row_ptr(dob, a.dos, a, rc), on, a.dv_, g);
     nlse[p] = on ? -a.lse[row0 + r] : 0.f;
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     if (g == 0 && on && share == 0) store_stream4(a.delta + row0 + r, del[p]);
   }
   const int wl = dlt_imin(wq0 + 16 * NP, a.rows) - 1;
-  const int pa = wl >= wq0 ? a.off + band_row(a, wq0).tok : 0, pb = wl >= wq0 ? a.off + band_row(a, wl).tok : -1;
+  const int pa = wl >= wq0 ? a.off + band_row(a, wq0).tok - W.jump : 0, pb = wl >= wq0 ? a.off + band_row(a, wl).tok - W.jump : -1;
 
   f32x4 acc[NP][KB];
 #pragma unroll
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
     });
   };
   auto chunk = [&](int i, char* buf, auto mask_tag) __attribute__((always_inline)) {
-    const int x = W.x(i);
+    const int x = CK * i;
     if (decltype(mask_tag)::value && (x > pb || (x + CK - 1 <= pa - a.W && x >= a.S))) return;
     consume(x, (Swa2Lds)buf, mask_tag);
   };
@@ -235,7 +235,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   unsigned odd[NP];
 #pragma unroll
   for (int p = 0; p < NP; p++) {
-    mul[p] = hi[p] == 0 ? 0.f : a.grad_scale;   // a row at position 0 sees one key
+    mul[p] = hi[p] + W.jump == 0 ? 0.f : a.grad_scale;   // a row at position 0 sees one key
     const uint64_t bad = __builtin_amdgcn_ballot_w64(wq0 + 16 * p + n < a.rows && band_odd_row(acc, p));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }
@@ -248,15 +248,15 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 #pragma unroll 1
     for (int c = i_beg; c < i_end; c++)
 #pragma unroll 1
-      for (int x = W.x(c); x < W.x(c) + CK; x += 64) {
-        const int j = x + lane;
+      for (int x = CK * c; x < CK * c + CK; x += 64) {
+        const int j = W.tok(x + lane);
         const bool sees = j < a.Lk && band_sees(pos, j, a.W, a.S);
         uint64_t left = __builtin_amdgcn_ballot_w64(sees);
         float ds = 0.f;
         if (sees) ds = fast_exp2(band_dot(q, kh + j * a.ks[2], a.dk_) * scale - lse) * (band_dot(d_o, vh + j * a.vs[2], a.dv_) - delta);
         for (; left != 0; left &= left - 1) {
           const int u = __builtin_ctzll(left);
-          band_axpy(sum, band_lane(ds, u), kh + (x + u) * a.ks[2], a.dk_, lane);
+          band_axpy(sum, band_lane(ds, u), kh + W.tok(x + u) * a.ks[2], a.dk_, lane);
         }
       }
   };

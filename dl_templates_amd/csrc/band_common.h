@@ -105,25 +105,30 @@ DLT_DEV T* band_row_ptr(T* base, const int64_t (&st)[3], const BandArgs& a, int 
   return base + (w.tok * st[2] + w.head * st[1]);
 }
 
-// Chunks of CK keys that the rows of a block at positions [first, last] see: those with sinks, then those of the window.
+// Keys that the rows of a block at positions [first, last] see, in groups of 16: those with sinks, then those of the window.  Places y count them without the gap between
+// (token y, from 16 sink groups on token y + jump); chunk i holds places CK i .. + CK - 1, so sinks share a chunk with the window's first keys.  With
+// bounds less the jump a row's rule is the same for places as for tokens: no token below the window's first group is in any row's window, and none behind the sinks' groups is
+// a sink.  us, against sinks in chunks of their own and a window that starts at a multiple
+// of CK: 8 x 8 kv heads of 4 query heads, 1111 tokens, window 300, 5 sinks, forward / dQ, d = 64 69 / 70 -> 60 / 62, d = 128 109 / 149 -> 96 / 137; 4 of 8192, window 1024, d = 128
+// 111 / 138 -> 106 / 136.  Without sinks a start at multiples of 16 changes nothing or loses up to 3 %: neighbouring blocks' chunks then are not the same.
 template <int CK>
 struct BandWalk {
-  int ns, c0, n;
+  int sinks, jump, n;   // places with sinks, when there is a gap behind them; tokens left out; chunks
   DLT_DEV void init(int first, int last, int W, int S) {
-    ns = c0 = n = 0;
+    sinks = jump = n = 0;
     if (last < 0) return;
-    first = dlt_imax(first, 0);
-    c0 = first >= W ? (first - W + 1) / CK : 0;
-    ns = dlt_imin((dlt_imin(S, last + 1) + CK - 1) / CK, c0);
-    n = ns + last / CK + 1 - c0;
+    const int w0 = dlt_imax(first - W + 1, 0) & (S > 0 ? ~15 : ~(CK - 1)), end = (dlt_imin(S, last + 1) + 15) & ~15;
+    if (w0 > end) { sinks = end; jump = w0 - end; }
+    n = (last - jump) / CK + 1;
   }
-  DLT_DEV int x(int i) const { return CK * (i < ns ? i : c0 + i - ns); }
-  // of chunks [beg, end) those that every one of the rows sees whole (chunks of sinks not counted): [f0, f1)
+  DLT_DEV int tok(int y) const { return y + (y >= sinks ? jump : 0); }
+  // of chunks [beg, end) those that every one of the rows sees whole (sinks not counted): [f0, f1)
   DLT_DEV void whole(int first, int last, int W, int beg, int end, int& f0, int& f1) const {
-    const int lo = last >= W ? (last - W) / CK + 1 : 0;       // first chunk behind the last row's window start
-    const int hi = first >= 0 ? (first + 1) / CK : 0;         // first chunk that ends behind the first row
-    f0 = dlt_imin(dlt_imax(beg, ns + dlt_imax(lo - c0, 0)), end);
-    f1 = dlt_imax(f0, dlt_imin(end, ns + hi - c0));
+    const int behind = last - jump - W + 1;                   // the last row's window starts there
+    const int lo = behind > 0 ? (behind + CK - 1) / CK : 0;
+    const int hi = first - jump >= 0 ? (first - jump + 1) / CK : 0;
+    f0 = dlt_imin(dlt_imax(beg, lo), end);
+    f1 = dlt_imax(f0, dlt_imin(end, hi));
   }
 };
 

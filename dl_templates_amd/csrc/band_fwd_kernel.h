@@ -45,8 +45,8 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
 #pragma unroll 1
   for (int i = i0; i < i1; i++)
 #pragma unroll 1
-    for (int x = W.x(i); x < W.x(i) + CK; x += 64) {
-      const int j = x + lane;
+    for (int x = CK * i; x < CK * i + CK; x += 64) {
+      const int j = W.tok(x + lane);
       const bool sees = j < n_k && (CK >= 64 || lane < CK) && band_sees(pos, j, a.W, a.S);
       uint64_t todo = __builtin_amdgcn_ballot_w64(sees);
       if (todo == 0) continue;
@@ -62,7 +62,7 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
         todo &= todo - 1;
         const float w = band_lane(p, u);
         l += w;
-        band_axpy(acc, w, vb + band_key_off<PAGED>(a, pages, a.vs, x + u), a.dv_, lane);
+        band_axpy(acc, w, vb + band_key_off<PAGED>(a, pages, a.vs, W.tok(x + u)), a.dv_, lane);
       }
     }
 }
@@ -115,18 +115,17 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   }
   char* const bufs = smem + grp * NBUF * B::BUF;   // of the group
   auto issue = [&](int i, char* buf) __attribute__((always_inline)) {
-    const int x = W.x(i) + wave * 16 * NG;
 #pragma unroll
     for (int u = 0; u < NG; u++) {
+      const int t0 = W.tok(CK * i + wave * 16 * NG + 16 * u);
       char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
       if constexpr (PAGED) {
         int in16;
-        const int page = band_page(a.pg, pages, dlt_imin(x / 16 + u, (sq.n_k - 1) >> 4), in16);
+        const int page = band_page(a.pg, pages, dlt_imin(t0 >> 4, (sq.n_k - 1) >> 4), in16);
         const int64_t row = 16 * in16;
         stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (page * a.ks[0] + row * a.ks[2])), dst);
         stv.template issue<PAD>(reinterpret_cast<const char*>(vh + (page * a.vs[0] + row * a.vs[2])), dst + B::REG);
       } else {
-        const int t0 = x + 16 * u;
         if (t0 + 16 <= a.Lk) {
           stk.template issue<PAD>(reinterpret_cast<const char*>(kh + (int64_t)t0 * a.ks[2]), dst);
           stv.template issue<PAD>(reinterpret_cast<const char*>(vh + (int64_t)t0 * a.vs[2]), dst + B::REG);
@@ -142,12 +141,15 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   // Pages hold anything behind the last key: those value rows, which no row sees, are cleared by the wave that copied them
   auto settle = [&](int i, char* buf) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-      const int x = W.x(i) + wave * 16 * NG;
-      if (x + 16 * NG > sq.n_k) {
-        keep_branch();
-        char* v = buf + B::REG + wave * 16 * NG * 2 * D;
-        for (int s = lane; s < 16 * NG * D / 8; s += 64)
-          if (x + s / (D / 8) >= sq.n_k) lds_write16(v + 16 * s, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+      for (int u = 0; u < NG; u++) {
+        const int t0 = W.tok(CK * i + wave * 16 * NG + 16 * u);
+        if (t0 + 16 > sq.n_k) {
+          keep_branch();
+          char* v = buf + B::REG + (wave * 16 * NG + 16 * u) * 2 * D;
+          for (int s = lane; s < 16 * D / 8; s += 64)
+            if (t0 + s / (D / 8) >= sq.n_k) lds_write16(v + 16 * s, u32x4{0u, 0u, 0u, 0u});
+        }
       }
     }
   };
@@ -157,19 +159,19 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
 
   const int wq0 = x0 + wave * 16 * NP;
   u32x4 qf[NP][KC];
-  int hi[NP], lo[NP];   // the row sees keys lo < j <= hi, and the sinks
+  int hi[NP], lo[NP];   // the row sees places lo < y <= hi, and the sinks
 #pragma unroll
   for (int p = 0; p < NP; p++) {
     const int r = wq0 + 16 * p + n;
     const bool on = r < n_rows;
     const int pos = sq.off + band_row(a, on ? r : 0).tok;
-    hi[p] = on ? dlt_imin(pos, sq.n_k - 1) : -1;
-    lo[p] = pos - a.W;
+    hi[p] = on ? dlt_imin(pos, sq.n_k - 1) - W.jump : -1;
+    lo[p] = pos - a.W - W.jump;
     band_load_own<KC>(qf[p], band_row_ptr(qb, a.qs, a, on ? r : 0), on, a.dk_, g);
   }
-  // positions of the wave's first and last row
+  // places of the wave's first and last row
   const int wl = dlt_imin(wq0 + 16 * NP, n_rows) - 1;
-  const int pa = wl >= wq0 ? sq.off + band_row(a, wq0).tok : 0, pb = wl >= wq0 ? sq.off + band_row(a, wl).tok : -1;
+  const int pa = wl >= wq0 ? sq.off + band_row(a, wq0).tok - W.jump : 0, pb = wl >= wq0 ? sq.off + band_row(a, wl).tok - W.jump : -1;
 
   float m_run[NP];
   f32x4 acc[NP][VB], acc_l[NP];
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
     });
   };
   auto chunk = [&](int i, char* buf, auto mask_tag) __attribute__((always_inline)) {
-    const int x = W.x(i);
+    const int x = CK * i;
     if (decltype(mask_tag)::value && (x > pb || (x + CK - 1 <= pa - a.W && x >= a.S))) return;   // no row of the wave sees any of it
     consume(x, (Swa2Lds)buf, mask_tag);
   };
