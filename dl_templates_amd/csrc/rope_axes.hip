@@ -215,7 +215,9 @@ __device__ inline void store_part(T* p, const Vec8<T>& v, int n) {
 
 // heads in flight
 constexpr int UNR = 4;
-constexpr int ROT_BLOCKS = 2048;   // workgroups that a large call aims for
+// Workgroups that a large call aims for: two a CU, since a thread that walks more heads fetches its cos and sin less often (us, by 512 / 2048 / 256: prompts of 7 sequences of 2047 tokens,
+// 16 + 8 + 8 heads, d = 64, 20.4 / 24.0 / 19.5; 6 of 1500, 32 + 8 + 8, d = 128, 41 / 46 / 45; 2 x 8192 tokens, 16 + 16, d = 64, 29 / 32 / 28; 4096 tokens, 16 + 4, d = 128, 8.8 / 8.7 / 9.3)
+constexpr int ROT_BLOCKS = 512;
 
 // WHOLE: every part has 8 dims or pairs (the others cost branches in front of every access)
 template <typename T, bool WHOLE>
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(RotArgs a, int parts) 
 
 // The same with 8 dims of whole, 16-byte aligned rows to a lane; partners, at any distance, come through the row in LDS, which belongs to the wave.  For sections
 // whose parts would be short or whose second dims start between 16-byte pieces (2 x 10 heads of 7755
-// tokens, d = 64, sections of 6, 11 and 11 pairs, fp16: 32 -> 12.6 us).
+// tokens, d = 64, sections of 6, 11 and 11 pairs, fp16: 32 -> 11 us).
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_rows_lds_kernel(RotArgs a, int parts) {
   dlt_kernargs_in<sizeof(RotArgs)>();
