@@ -384,6 +384,12 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   for (int p = 0; p < NP; p++) {
     const int r = wq0 + 16 * p + n;   // rows behind the last query: zeros
     inv[p] = r < n_rows ? band_inverse(lt[p], sq.off + band_row(a, r).tok) : 0.f;
+    // these (pages) went through the products with P = 0 or 1: what an infinite or NaN key or value left there a factor of 0 would not clear
+    if constexpr (PAGED)
+#pragma unroll
+      for (int d = 0; d < VB; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[p][d][i] = r < n_rows ? acc[p][d][i] : 0.f;
     const uint64_t bad = __builtin_amdgcn_ballot_w64(grp == 0 && wq0 + 16 * p + n < n_rows && (band_odd_row(acc, p) || band_odd(lt[p])));
     odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
   }

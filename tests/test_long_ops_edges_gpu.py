@@ -1,0 +1,59 @@
+"""Edges of the long-sequence operators that a plan, a padded batch or an unusual caller reaches (GPU)."""
+import math
+
+import pytest
+import torch
+
+from dl_templates_amd.paged_cache import paged_attention
+from tests import long_oracle as orc
+from tests.test_paged_cache_gpu import gathered, pool
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+NAN, INF = float("nan"), float("inf")
+name_of = lambda c: "-".join(str(x).replace("torch.", "").replace(" ", "") for x in c)  # noqa: E731
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ---- padded batches ------------------------------------------------------------------------------------------------------------------
+# workgroups of 16 rows, of 64 with the keys over two groups of waves, of 64, of 128, and keys shared by workgroups
+PADDED = [
+    # B, H, Hkv, T, lens, n_new, D, window, sinks, dtype
+    (3, 4, 2, 6, (100, 37, 64), (2, 6, 0), 64, None, 0, BF),
+    (3, 4, 2, 6, (100, 37, 64), (3, 5, 1), 64, 20, 2, HF),
+    (3, 16, 4, 150, (400, 260, 300), (18, 150, 90), 64, None, 0, BF),
+    (4, 32, 8, 150, (400, 260, 300, 150), (18, 150, 90, 1), 64, 100, 3, HF),
+    (8, 64, 16, 150, (400, 260, 300, 150, 200, 201, 202, 203), (20, 150, 90, 1, 2, 3, 4, 5), 128, 100, 3, BF),
+    (1, 2, 1, 30, (3000,), (3,), 64, None, 0, BF),
+]
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("where", ["a value that is seen", "a hidden value", "a key that is seen", "a hidden key", "the first value", "the first key"])
+@pytest.mark.parametrize("case", PADDED, ids=name_of)
+def test_padded_rows_are_zeros_beside_special_values(case, where, bad):
+    """Padded rows have no keys: an infinity or a NaN among those of the sequence does not reach them, nor the rows that do not see it."""
+    B, H, Hkv, T, lens, new, D, window, n_sink, dtype = case
+    kc, vc, table = (x.cuda() for x in pool(torch.Generator().manual_seed(50), B, Hkv, 16, lens, D, D, dtype))
+    q = torch.randn(B, H, T, D, generator=torch.Generator().manual_seed(51)).to(dtype).cuda()
+    scale, G, n, first = 1.0 / math.sqrt(D), H // Hkv, lens[0], lens[0] - new[0]
+    # seen by every new token of sequence 0; hidden: just outside of the first one's window, or ahead of all but the last one
+    j = first if "seen" in where else 0 if "first" in where else first - window if window is not None else n - 1
+    vis = orc.seen(torch.arange(new[0], device="cuda") + first, n, window, n_sink)[:, j]
+    assert vis.all() if "seen" in where else "first" in where or not vis[0]
+    keys, values = (gathered(c, table, 0, n)[None] for c in (kc, vc))
+    (vc if "value" in where else kc)[int(table[0, j // 16]), 0, j % 16] = bad
+    o = paged_attention(q, kc, vc, table, ints(*lens), window, n_sink, scale, ints(*new))
+    for b in range(B):
+        assert (o[b, :, new[b]:] == 0).all()
+        assert b == 0 or o[b].isfinite().all()
+    value, bound = orc.window(q[:1, :, :new[0]], keys, values, window, n_sink, scale)["o"]
+    clean = torch.ones(1, H, new[0], dtype=torch.bool, device="cuda")
+    clean[0, :G] = ~vis
+    got = o[:1, :, :new[0]]
+    orc.check(got[clean], (value[clean], bound[clean]), "rows that do not see it")
+    if bad != bad:
+        assert got[~clean].isnan().all()
