@@ -29,11 +29,10 @@ __global__ __launch_bounds__(256) void band_join_kernel(const BandArgs a) {
   const float* part = a.part + ((int64_t)bh * a.shares * a.rows + r) * a.dv_ + 2 * dlt_imin(lane, a.dv_ / 2 - 1);
   const int64_t step = (int64_t)a.rows * a.dv_;
   float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
+  // with a weight of 0 too: an infinite or NaN part holds such a value of a key that the row sees, and 0 times it is NaN
   auto add = [&](const float2& v, float f) __attribute__((always_inline)) {
-    if (f != 0.f) {
-      o[0] = fmaf(v.x, f, o[0]);
-      o[1] = fmaf(v.y, f, o[1]);
-    }
+    o[0] = fmaf(v.x, f, o[0]);
+    o[1] = fmaf(v.y, f, o[1]);
   };
   if constexpr (WG) {
     static_assert(BAND_SHARES_MAX == 128, "two weights a lane");

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from dl_templates_amd.paged_cache import paged_attention
+from dl_templates_amd.window_attn import window_attention
 from tests import long_oracle as orc
 from tests.test_paged_cache_gpu import gathered, pool
 
@@ -57,3 +58,26 @@ def test_padded_rows_are_zeros_beside_special_values(case, where, bad):
     orc.check(got[clean], (value[clean], bound[clean]), "rows that do not see it")
     if bad != bad:
         assert got[~clean].isnan().all()
+
+
+# ---- shares of keys --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("low", [-400.0, -INF])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("H, Hkv, Lq, Lk", [(2, 1, 1, 300), (8, 8, 64, 500), (2, 1, 1, 1600), (4, 2, 3, 3008), (4, 1, 20, 8000), (64, 64, 400, 800)])
+def test_a_nan_of_no_weight_is_not_lost(H, Hkv, Lq, Lk, dtype, low):
+    """The first half of the keys has scores so low that their weights are 0, and one value there is NaN: 0 times NaN is NaN in the formula, however the keys are shared."""
+    gen = torch.Generator().manual_seed(52)
+    q = torch.rand(1, H, Lq, 64, generator=gen).add(0.1).to(dtype).cuda()
+    k, v = (torch.randn(1, Hkv, Lk, 64, generator=gen).to(dtype).cuda() for _ in range(2))
+    k[:, :, :Lk // 2] = low
+    v[:, :, 5, 3] = NAN
+    value, bound = orc.window(q, k, v, None, 0, 0.125)["o"]
+    assert value[..., 3].isnan().all() and value[..., :3].isfinite().all()
+    outs = {"dense": window_attention(q, k, v, None, 0, 0.125)}
+    if Lk % 16 == 0:
+        pages = lambda x: x[0].reshape(Hkv, Lk // 16, 16, 64).transpose(0, 1).contiguous()  # noqa: E731
+        outs["paged"] = paged_attention(q, pages(k), pages(v), torch.arange(Lk // 16, dtype=torch.int32, device="cuda")[None], ints(Lk), None, 0, 0.125)
+    for name, o in outs.items():
+        assert o[..., 3].isnan().all(), f"{name}: the NaN is lost"
+        keep = [d for d in range(64) if d != 3]
+        orc.check(o[..., keep], (value[..., keep], bound[..., keep]), name)
