@@ -425,22 +425,24 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   __syncthreads();
   TIO* ob = reinterpret_cast<TIO*>(a.out) + b * a.os[0] + (int64_t)h * a.G * a.os[1];
   constexpr int PT = D * 2 + 16;
-  band_store_rows<D, NP, TIO>(smem, acc, inv, NW, GR, grp == 0, a.dv_, wave, n, g, tid,
-                              [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(ob, a.os, a, x0 + row) : nullptr; },
-                              [&]() {
+  // odd rows of the wave once more: o, or (`low`) what its rounding drops
+  auto again = [&](bool low) __attribute__((always_inline)) {
 #pragma unroll 1
-                                for (int p = 0; p < NP; p++)
-                                  for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
-                                    const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w;
-                                    float m, l, o2[2];
-                                    band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok,
-                                                                   sq.n_k, lane, m, l, o2);
-                                    const float f = band_inverse(l, sq.off + band_row(a, r).tok);
-                                    if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(o2[0] * f, o2[1] * f);
-                                    if (lane == 0 && a.lse != nullptr) a.lse[row0 + r] = m + fast_log2(l);
-                                  }
-                              });
+    for (int p = 0; p < NP; p++)
+      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
+        const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w;
+        float m, l, o2[2];
+        band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
+        const float f = band_inverse(l, sq.off + band_row(a, r).tok);
+#pragma unroll
+        for (int j = 0; j < 2; j++) o2[j] = low ? band_dropped<TIO>(o2[j] * f) : o2[j] * f;
+        if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(o2[0], o2[1]);
+        if (lane == 0 && !low && a.lse != nullptr) a.lse[row0 + r] = m + fast_log2(l);
+      }
+  };
+  band_store_rows<D, NP, TIO>(smem, acc, inv, NW, GR, grp == 0, a.dv_, wave, n, g, tid,
+                              [&](int row) -> TIO* { return x0 + row < a.rows ? band_row_ptr(ob, a.os, a, x0 + row) : nullptr; }, [&]() { again(false); });
   if (!PAGED && a.low != nullptr && x0 < a.low_rows)
     band_store_rows<D, NP, TIO, true>(smem, acc, inv, NW, GR, grp == 0, a.dv_, wave, n, g, tid,
-                                      [&](int row) -> TIO* { return x0 + row < a.rows ? band_low<TIO>(a, b, h, x0 + row) : nullptr; }, []() {});
+                                      [&](int row) -> TIO* { return x0 + row < a.rows ? band_low<TIO>(a, b, h, x0 + row) : nullptr; }, [&]() { again(true); });
 }

@@ -4,6 +4,7 @@ import math
 import pytest
 import torch
 
+from dl_templates_amd import _lib
 from dl_templates_amd.paged_cache import paged_attention
 from dl_templates_amd.window_attn import window_attention
 from tests import long_oracle as orc
@@ -81,3 +82,23 @@ def test_a_nan_of_no_weight_is_not_lost(H, Hkv, Lq, Lk, dtype, low):
         assert o[..., 3].isnan().all(), f"{name}: the NaN is lost"
         keep = [d for d in range(64) if d != 3]
         orc.check(o[..., keep], (value[..., keep], bound[..., keep]), name)
+
+
+# ---- rows taken again --------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_low_parts_of_rows_taken_again(dtype):
+    """Rows that meet a hidden NaN are formed once more; o and its low part together are then the value in 32 bits: the low part's own rounding is u^2 |o|, 8 terms and
+    scores of 64 products of a sum of magnitudes below 12 are off by 2 (8 + 64 12) 2^-24 < 2^-13 of the terms' magnitude."""
+    gen = torch.Generator().manual_seed(53)
+    q, k, v = (torch.randn(1, h, 64, 64, generator=gen).to(dtype).cuda() for h in (4, 2, 2))
+    value, _ = orc.window(q, k, v, 8, 0, 0.125)["o"]
+    mag, _ = orc.window(q, k, v.abs(), 8, 0, 0.125)["o"]
+    scores = (q.double().abs() @ k.double().abs().repeat_interleave(2, 1).transpose(-1, -2) * 0.125).amax()
+    assert scores < 12
+    v[:, :, 20, :32] = NAN   # hidden from tokens 16 to 19, which meet it in their chunk
+    o, _, low = _lib.native.window_forward(q, k, v, 8, 0, 0.125)
+    at = (slice(None), slice(None), slice(16, 20))
+    u = torch.finfo(dtype).eps / 2
+    orc.check(o[at], (value[at], u * value[at].abs() + 2.0 ** -13 * mag[at]), "o")
+    off = (o[at].double() + low[at].double() - value[at]).abs()
+    assert (off <= u * u * value[at].abs() + 2.0 ** -13 * mag[at] + orc.tiny(dtype)).all()
