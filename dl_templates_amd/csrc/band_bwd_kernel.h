@@ -243,7 +243,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   auto exact = [&](int r, float (&sum)[2]) __attribute__((always_inline)) {
     const int pos = a.off + band_row(a, r).tok;
     const TIO *q = band_row_ptr(qb, a.qs, a, r), *d_o = band_row_ptr(dob, a.dos, a, r);
-    const float lse = a.lse[row0 + r], delta = band_dot(band_row_ptr(ob, a.os, a, r), d_o, a.dv_);
+    const TIO* low = a.low != nullptr ? band_low<TIO>(a, b, h, r) : nullptr;
+    const float lse = a.lse[row0 + r], delta = band_dot(band_row_ptr(ob, a.os, a, r), d_o, a.dv_) + (low != nullptr ? band_dot(low, d_o, a.dv_) : 0.f);
     sum[0] = sum[1] = 0.f;
 #pragma unroll 1
     for (int c = i_beg; c < i_end; c++)
