@@ -124,6 +124,10 @@ bool plain(const T&... ts) {
   return plain_keys(c10::impl::tls_local_dispatch_key_set().included_, MODES) && (one(ts) && ...);
 }
 
+// of those that are there
+template <typename... T>
+bool plain_each(const T&... ts) { return ((!ts.defined() || plain(ts)) && ...); }
+
 // ---- rotary operands --------------------------------------------------------------------------
 struct Rope {
   Tensor idx, row, col;   // row, col: fp32 [len, R, 2] with a contiguous [R, 2] tail
@@ -1024,12 +1028,18 @@ Axes axes_arg(PyObject* pos, PyObject* tables, PyObject* layout) {
   t.layout = (int)int_arg(layout);
   return t;
 }
+bool plain_axes(const Axes& t) {
+  bool ok = plain_each(t.pos);
+  for (const Tensor& x : t.tables) ok = ok && plain(x);
+  return ok;
+}
 PyObject* wrap_pair(const Tensor& q, const Tensor& k) {
   if (!k.defined()) return Py_BuildValue("(NO)", THPVariable_Wrap(q), Py_None);
   return Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(k));
 }
 
-// (q, k or None, pos, tables, layout number, inverse, mode): mode 0: new tensors, with a graph; 1: new tensors, no graph; 2: in place, no graph
+// (q, k or None, pos, tables, layout number, inverse, mode): mode 0: new tensors, with a graph; 1: new tensors, no graph; 2: in place, no graph; 3: the same
+// for any call (0 and 2 take plain ones)
 PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   count(n, 7, 7);
@@ -1038,14 +1048,12 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Axes t = axes_arg(a[2], a[3], a[4]);
   const bool inverse = bool_arg(a[5]);
   const int64_t mode = int_arg(a[6]);
+  if ((mode == 0 || mode == 2) && !(plain_each(q, k) && plain_axes(t))) Py_RETURN_NOTIMPLEMENTED;
   if (mode == 0) {
-    bool ordinary = plain(q) && (!k.defined() || plain(k)) && (!t.pos.defined() || plain(t.pos));
-    for (const Tensor& x : t.tables) ordinary = ordinary && plain(x);
-    if (!ordinary) Py_RETURN_NOTIMPLEMENTED;
     const auto out = rope_axes(q, k, t, inverse);
     return wrap_pair(out[0], out[1]);
   }
-  if (mode == 2) {
+  if (mode >= 2) {
     require_gpu(q);
     check_written(q, "q");
     if (k.defined()) {
@@ -1069,15 +1077,17 @@ PyObject* py_rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (k_cache, v_cache, k, v, page_table, seq_len, n_new or None, pos or None, tables or None, layout number, q or None) -> rotated q or None
+// (k_cache, v_cache, k, v, page_table, seq_len, n_new or None, pos or None, tables or None, layout number, q or None, any call or plain ones only) -> rotated q or None
 PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 11, 11);
+  count(n, 12, 12);
   const Tensor &kc = tensor_arg(a[0]), &vc = tensor_arg(a[1]), &k = tensor_arg(a[2]), &v = tensor_arg(a[3]), &table = tensor_arg(a[4]), &seq = tensor_arg(a[5]);
   const Tensor n_new = a[6] == Py_None ? Tensor() : tensor_arg(a[6]), q = a[10] == Py_None ? Tensor() : tensor_arg(a[10]);
   const bool rope = a[8] != Py_None;
   Axes t;
   if (rope) t = axes_arg(a[7], a[8], a[9]);
+  for (const Tensor* c : {&kc, &vc}) torch::autograd::check_inplace(*c, torch::autograd::compute_requires_grad(*c));
+  if (!bool_arg(a[11]) && !(plain(kc, vc, k, v, table, seq) && plain_each(n_new, q) && plain_axes(t))) Py_RETURN_NOTIMPLEMENTED;
   check_assert(k.dim() == 4 && v.dim() == 4 && k.sizes().slice(0, 3) == v.sizes().slice(0, 3), "k and v must have shape [B, heads, T, D], all but D alike");
   check_assert(k.size(1) == kc.size(1) && k.size(3) == kc.size(3) && v.size(3) == vc.size(3), "k and v must match their caches");
   check_assert(k.scalar_type() == kc.scalar_type() && v.scalar_type() == kc.scalar_type(), "k, v and the caches must have one dtype");
@@ -1089,7 +1099,6 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   check_written(kc, "k_cache");
   check_written(vc, "v_cache");
   check_two(kc, vc, "k_cache and v_cache");
-  for (const Tensor* c : {&kc, &vc}) torch::autograd::check_inplace(*c, torch::autograd::compute_requires_grad(*c));
   Tensor q_out;
   if (p.s.B > 0) {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -1110,13 +1119,14 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, k_cache, v_cache, page_table, seq_len, window or None, n_sink, scale, n_new or None) -> o, no graph
+// (q, k_cache, v_cache, page_table, seq_len, window or None, n_sink, scale, n_new or None, any call or plain ones only) -> o, no graph
 PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 9, 9);
-  at::AutoDispatchBelowADInplaceOrView below;
+  count(n, 10, 10);
   const Tensor &q0 = tensor_arg(a[0]), &kc = tensor_arg(a[1]), &vc = tensor_arg(a[2]), &table = tensor_arg(a[3]), &seq = tensor_arg(a[4]);
   const Tensor n_new = a[8] == Py_None ? Tensor() : tensor_arg(a[8]);
+  if (!bool_arg(a[9]) && !(plain(q0, kc, vc, table, seq) && plain_each(n_new))) Py_RETURN_NOTIMPLEMENTED;
+  at::AutoDispatchBelowADInplaceOrView below;
   check_assert(q0.dim() == 4 && q0.size(3) == kc.size(-1) && q0.scalar_type() == kc.scalar_type(), "q must have shape [B, heads, T, D] and match the cache");
   Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, q0.size(0), q0.size(2), q0.size(1));
   p.s.window = window_arg(a[5]);

@@ -57,11 +57,33 @@ def rope_axes_qk(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, tables, la
     return RopeAxes.apply(q, k, pos, code, inverse, *tables) if out is NotImplemented else out
 
 
+class RopeAxesInPlace(torch.autograd.Function):
+    """``apply(q, k, pos, layout number, inverse, *tables)`` -> None, q and k rotated in place: what calls of ``rope_axes_qk_`` that are not plain eager ones (trace,
+    transform, dispatch mode) run through, without a graph.  It does not return what it writes: a trace could not run that."""
+
+    @staticmethod
+    def forward(ctx, q, k, pos, layout, inverse, *tables):
+        _lib.native.rope_axes(q, k, pos, tables, layout, inverse, 3)
+
+
+def _refuse_tangents(name: str, *tensors) -> None:
+    """A call that writes in place, or records no graph, would leave a forward-mode tangent behind."""
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no derivative in forward mode")
+
+
 def rope_axes_qk_(q: torch.Tensor, k: torch.Tensor, pos: torch.Tensor, tables, layout: str = "blocks", inverse: bool = False):
-    """The same in place and without a graph; tensors that need a gradient are refused."""
+    """The same in place and without a graph; tensors that need a gradient, and forward-mode tangents, are refused."""
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         raise RuntimeError("rope_axes_qk_ records no graph: use rope_axes_qk for tensors that need a gradient")
-    return _lib.native.rope_axes(q, k, pos, tuple(tables), _layout(layout), inverse, 2)
+    code, tables = _layout(layout), tuple(tables)
+    out = _lib.native.rope_axes(q, k, pos, tables, code, inverse, 2)
+    if out is NotImplemented:
+        _refuse_tangents("rope_axes_qk_", q, k, pos, *tables)
+        with torch.no_grad():
+            RopeAxesInPlace.apply(q, k, pos, code, inverse, *tables)
+        out = q, k
+    return out
 
 
 class RotaryPositionEncodingAxes(torch.nn.Module):

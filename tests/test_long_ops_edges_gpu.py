@@ -3,9 +3,12 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd_ad
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from dl_templates_amd import _lib
-from dl_templates_amd.paged_cache import paged_attention
+from dl_templates_amd.paged_cache import paged_append_, paged_attention
+from dl_templates_amd.rope_axes import rope_axes_qk_
 from dl_templates_amd.window_attn import window_attention
 from tests import long_oracle as orc
 from tests.test_paged_cache_gpu import gathered, pool
@@ -119,3 +122,108 @@ def test_query_gradients_of_rows_taken_again(window, n_sink, dtype):
     got, want = dq[:, :, clean].double(), value[:, :, clean]
     assert dq[:, :, ~clean].isnan().all() and got.isfinite().all()
     assert (got - want).norm() <= 1.7 * (want.to(dtype).double() - want).norm()
+
+
+# ---- traces, modes and tangents -------------------------------------------------------------------------------------------------------
+def small_cache(seed=55, dtype=BF):
+    gen = torch.Generator().manual_seed(seed)
+    kc, vc = (torch.randn(6, 2, 16, 64, generator=gen).to(dtype).cuda() for _ in range(2))
+    q, k, v = (torch.randn(2, h, 3, 64, generator=gen).to(dtype).cuda() for h in (4, 2, 2))
+    return kc, vc, q, k, v, torch.arange(6, dtype=torch.int32, device="cuda").reshape(2, 3), ints(40, 20 + seed % 7)
+
+
+def test_traced_paged_calls_depend_on_their_inputs():
+    tables = [orc.table(64, 32).cuda()]
+
+    def step(kc, vc, q, k, v, pages, seq):
+        r = paged_append_(kc, vc, k, v, pages, seq, None, (None, tables, "halves"), q)
+        return paged_attention(r, kc, vc, pages, seq, 20, 2)
+
+    def fill(kc, vc, q, k, v, pages, seq):
+        before = kc + 0
+        assert paged_append_(kc, vc, k, v, pages, seq) is None
+        return paged_attention(q, kc, vc, pages, seq), before, kc + 0
+
+    def attend(kc, vc, q, k, v, pages, seq):
+        return paged_attention(q, kc, vc, pages, seq, 20, 2, None, seq - 18)
+    for f in (step, fill, attend):
+        traced = torch.jit.trace(f, small_cache(55), check_trace=False)
+        for seed in (56, 57, 58, 59):   # the executor rearranges a graph after its first runs
+            a, b = small_cache(seed), small_cache(seed)
+            got, want = traced(*a), f(*b)
+            got, want = (x if isinstance(x, tuple) else (x,) for x in (got, want))
+            assert all(torch.equal(x, y) for x, y in zip(got + a, want + b))
+
+
+def test_a_traced_rotation_in_place_depends_on_its_inputs():
+    tables = [orc.table(64, 32).cuda()]
+
+    def turn(q, k, pos):
+        before = q + k
+        q, k = rope_axes_qk_(q, k, pos, tables)
+        return before, q + k
+
+    def one(q, k, pos):
+        return rope_axes_qk_(q, None, pos, tables)[0] * k
+    mk = lambda s: tuple(torch.randn(1, 2, 40, 64, generator=torch.Generator().manual_seed(s + i)).cuda() for i in range(2)) + (torch.arange(s, s + 40, dtype=torch.int32, device="cuda")[None],)  # noqa: E731
+    for f in (turn, one):
+        traced = torch.jit.trace(f, mk(1), check_trace=False)
+        for seed in (5, 7, 9, 11):
+            a, b = mk(seed), mk(seed)
+            got, want = traced(*a), f(*b)
+            got, want = (x if isinstance(x, tuple) else (x,) for x in (got, want))
+            assert all(torch.equal(x, y) for x, y in zip(got + a, want + b))
+
+
+def test_tangents_are_refused():
+    """No derivative in forward mode: a tangent on any tensor raises before anything is written, as for the operators beside these."""
+    kc, vc, q, k, v, pages, seq = small_cache()
+    pos, tables = torch.arange(3, dtype=torch.int32, device="cuda")[None], [orc.table(64, 32).cuda()]
+    start = [x.clone() for x in (kc, vc, q, k)]
+    dual = lambda x: fwd_ad.make_dual(x, torch.ones_like(x))  # noqa: E731
+    with fwd_ad.dual_level():
+        for call in (lambda: rope_axes_qk_(dual(q), None, pos, tables), lambda: rope_axes_qk_(q, dual(k), pos, tables), lambda: rope_axes_qk_(q, k, pos, [dual(tables[0])]),
+                     lambda: paged_attention(dual(q), kc, vc, pages, seq), lambda: paged_attention(q, dual(kc), vc, pages, seq), lambda: paged_attention(q, kc, dual(vc), pages, seq),
+                     lambda: paged_append_(kc, vc, dual(k), v, pages, seq), lambda: paged_append_(kc, vc, k, dual(v), pages, seq), lambda: paged_append_(dual(kc), vc, k, v, pages, seq),
+                     lambda: paged_append_(kc, dual(vc), k, v, pages, seq), lambda: paged_append_(kc, vc, k, v, pages, seq, None, (None, tables, "halves"), dual(q)),
+                     lambda: paged_append_(kc, vc, k, v, pages, seq, None, (None, [dual(tables[0])], "halves"), q)):
+            with pytest.raises(NotImplementedError):
+                call()
+    assert all(torch.equal(x, y) for x, y in zip((kc, vc, q, k), start))
+
+
+def test_transforms_are_refused():
+    kc, vc, q, k, v, pages, seq = small_cache()
+    pos, tables = torch.arange(3, dtype=torch.int32, device="cuda")[None], [orc.table(64, 32).cuda()]
+    many = lambda x: torch.stack([x, x])  # noqa: E731
+    for f, x in ((lambda q: paged_attention(q, kc, vc, pages, seq), many(q)), (lambda k: paged_append_(kc, vc, k, v, pages, seq, q=q), many(k)),
+                 (lambda q: rope_axes_qk_(q, None, pos, tables)[0], many(q))):
+        with pytest.raises(RuntimeError, match="setup_context"):
+            torch.func.vmap(f)(x)
+
+
+def test_paged_calls_and_rotation_in_place_under_a_mode():
+    """A dispatch mode takes the classes: the same bits, no graph, and written tensors that count as written."""
+    class Seen(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    pos, tables = torch.arange(3, dtype=torch.int32, device="cuda")[None], [orc.table(64, 32).cuda()]
+
+    def work():
+        kc, vc, q, k, v, pages, seq = small_cache()
+        count = [x._version for x in (kc, vc, q)]
+        q.requires_grad_(True)
+        r = paged_append_(kc, vc, k, v, pages, seq, None, (None, tables, "halves"), q)
+        o = paged_attention(r, kc, vc, pages, seq)
+        assert paged_append_(kc, vc, k, v, pages, seq) is None
+        with torch.no_grad():
+            turned = rope_axes_qk_(q, k, pos, tables)
+        assert turned[0] is q and turned[1] is k and not o.requires_grad and not r.requires_grad
+        assert all(x._version > n for x, n in zip((kc, vc, q), count))
+        with pytest.raises(RuntimeError, match="leaf Variable"):
+            paged_append_(kc.clone().requires_grad_(True), vc, k, v, pages, seq)
+        return kc, vc, r, o, q.detach(), k
+    want = work()
+    with Seen():
+        got = work()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
