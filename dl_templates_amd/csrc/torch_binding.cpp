@@ -273,6 +273,13 @@ Workspace window_workspace(const dlt_window_shape_t& shape, int backward, const 
   return w;
 }
 
+// The C ABI takes one sequence or more; what else is wrong with a call of none is refused as it would be with one.
+void empty_batch(dlt_window_shape_t shape) {
+  int64_t bytes;
+  shape.B = 1;
+  check_rc(dlt_window_workspace(&shape, 0, &bytes));
+}
+
 struct Forward { Tensor o, lse, q_rot, k_rot, low; };
 
 // keep_rot: the rotated q and k are stored as well (for the backward pass)
@@ -288,6 +295,12 @@ Forward run_forward(const Spec& s, const Tensor& q, const Tensor& k, const Tenso
     const Workspace ws = flash_workspace(s.flash, 0, q);
     check_rc(dlt_flash_fwd_ws(q.const_data_ptr(), st(q), k.const_data_ptr(), st(k), v.const_data_ptr(), st(v), f.o.mutable_data_ptr(), st(f.o),
                               (float*)f.lse.mutable_data_ptr(), st(f.lse), &s.flash, ws.ptr, ws.bytes, stream));
+    return f;
+  }
+  if (s.op == Op::Window && s.window.B == 0) {
+    empty_batch(s.window);
+    f.o = empty({0, q.size(1), q.size(2), v.size(3)}, dt, q);
+    f.lse = empty({0}, at::kFloat, q);
     return f;
   }
   if (s.op == Op::Window) {
@@ -335,6 +348,7 @@ std::array<Tensor, 3> run_backward(const Spec& s, const Tensor& q, const Tensor&
   require_gpu(q, k, v, o, lse, d_o);
   c10::DeviceGuard guard(q.device());
   void* stream = stream_of(q);
+  if (s.op == Op::Window && s.window.B == 0) return {empty(q.sizes(), q.scalar_type(), q), empty(k.sizes(), k.scalar_type(), k), empty(v.sizes(), v.scalar_type(), v)};
   if (s.op == Op::Window) {
     const Workspace ws = window_workspace(s.window, 1, q);
     Tensor dq = empty(q.sizes(), q.scalar_type(), q), dk = empty(k.sizes(), k.scalar_type(), k), dv = empty(v.sizes(), v.scalar_type(), v);

@@ -7,6 +7,7 @@ import torch.autograd.forward_ad as fwd_ad
 from torch.utils._python_dispatch import TorchDispatchMode
 
 from dl_templates_amd import _lib
+from dl_templates_amd._lib import DltError
 from dl_templates_amd.paged_cache import paged_append_, paged_attention
 from dl_templates_amd.rope_axes import rope_axes_qk_
 from dl_templates_amd.window_attn import window_attention
@@ -227,3 +228,19 @@ def test_paged_calls_and_rotation_in_place_under_a_mode():
     with Seen():
         got = work()
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+# ---- empty batches ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("D", [64, 40])
+def test_window_attention_of_no_sequence(D):
+    """As paged attention has it: empty outputs and gradients; what is wrong with the other arguments is still refused."""
+    q, k, v = (torch.zeros(0, h, n, D, dtype=BF, device="cuda", requires_grad=True) for h, n in ((4, 5), (2, 9), (2, 9)))
+    o = window_attention(q, k, v, 4, 1)
+    assert o.shape == (0, 4, 5, D) and o.dtype == BF
+    got = torch.autograd.grad(o, (q, k, v), torch.zeros_like(o))
+    assert [g.shape for g in got] == [x.shape for x in (q, k, v)]
+    with torch.no_grad():
+        assert window_attention(q, k, v).shape == o.shape
+    for bad in (lambda: window_attention(q, k, v, 0), lambda: window_attention(q[:, :3], k, v, 4), lambda: window_attention(q, k, v, 4, 0, -1.0), lambda: window_attention(q.float(), k.float(), v.float(), 4)):
+        with pytest.raises(DltError):
+            bad()
