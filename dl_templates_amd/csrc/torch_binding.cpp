@@ -27,6 +27,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <mutex>
 #include <string>
@@ -649,8 +650,55 @@ void rope_apply(const Tensor& x, const Rows& r, const Tensor& idx, const Tensor&
 void check_written(const Tensor& x, const char* name) {
   if (C10_UNLIKELY(at::has_internal_overlap(x) == at::MemOverlap::Yes)) raise_py(PyExc_RuntimeError, std::string(name) + " has elements that share memory (an expanded tensor): it cannot be written in place");
 }
+// Is some element of x one of y?  With x[i] at sum i_d s_d and y[j] at D + sum j_d s'_d that asks for whole numbers with sum i_d s_d - sum j_d s'_d = D.  Strides from the
+// largest on; a number is tried only where the strides behind it can make up the rest, which leaves one or two for dims that lie inside each other.  Layouts that need
+// more than a few thousand tries are taken as apart.
+struct Meeting {
+  struct Dim { int64_t stride, lo, hi; };   // the sum of the dims of both tensors with this stride
+  Dim d[8];
+  int n = 0, tries = 4096;
+  void add(const Tensor& x, bool second) {
+    for (int64_t i = 0; i < x.dim() && i < 4; i++) {
+      const int64_t s = x.stride(i), m = x.size(i) - 1;
+      if (s == 0 || m == 0) continue;
+      int k = 0;
+      while (k < n && d[k].stride != s) k++;
+      if (k == n) d[n++] = {s, 0, 0};
+      (second ? d[k].lo : d[k].hi) += second ? -m : m;
+    }
+  }
+  bool solve(int k, int64_t rest) {
+    if (k == n) return rest == 0;
+    if (--tries < 0) return false;
+    int64_t lo = 0, hi = 0;   // what the dims behind this one can add
+    for (int i = k + 1; i < n; i++) { lo += d[i].stride * d[i].lo; hi += d[i].stride * d[i].hi; }
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t t0 = std::max(d[k].lo, -floor_div(hi - rest, d[k].stride)), t1 = std::min(d[k].hi, floor_div(rest - lo, d[k].stride));
+    for (int64_t t = t0; t <= t1 && tries >= 0; t++)
+      if (solve(k + 1, rest - t * d[k].stride)) return true;
+    return false;
+  }
+};
+bool meet(const Tensor& x, const Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto bytes = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); i++) n += (t.size(i) - 1) * t.stride(i);
+    return n * (int64_t)t.element_size();
+  };
+  const char *px = (const char*)x.const_data_ptr(), *py = (const char*)y.const_data_ptr();
+  if (px + bytes(x) <= py || py + bytes(y) <= px) return false;
+  const int64_t es = (int64_t)x.element_size();   // one dtype
+  if ((py - px) % es != 0) return true;
+  Meeting m;
+  m.add(x, false);
+  m.add(y, true);
+  std::sort(m.d, m.d + m.n, [](const Meeting::Dim& a, const Meeting::Dim& b) { return a.stride > b.stride; });
+  return m.solve(0, (py - px) / es);
+}
 void check_two(const Tensor& x, const Tensor& y, const char* names) {
   if (C10_UNLIKELY(x.numel() > 0 && y.numel() > 0 && x.const_data_ptr() == y.const_data_ptr())) raise_py(PyExc_RuntimeError, std::string(names) + " must be two tensors");
+  if (C10_UNLIKELY(meet(x, y))) raise_py(PyExc_RuntimeError, std::string(names) + " share memory: they cannot be written in one call");
 }
 
 struct Axes {

@@ -9,7 +9,7 @@ from torch.utils._python_dispatch import TorchDispatchMode
 from dl_templates_amd import _lib
 from dl_templates_amd._lib import DltError
 from dl_templates_amd.paged_cache import paged_append_, paged_attention
-from dl_templates_amd.rope_axes import rope_axes_qk_
+from dl_templates_amd.rope_axes import rope_axes_qk, rope_axes_qk_
 from dl_templates_amd.window_attn import window_attention
 from tests import long_oracle as orc
 from tests.test_paged_cache_gpu import gathered, pool
@@ -244,3 +244,32 @@ def test_window_attention_of_no_sequence(D):
     for bad in (lambda: window_attention(q, k, v, 0), lambda: window_attention(q[:, :3], k, v, 4), lambda: window_attention(q, k, v, 4, 0, -1.0), lambda: window_attention(q.float(), k.float(), v.float(), 4)):
         with pytest.raises(DltError):
             bad()
+
+
+# ---- tensors that share memory ------------------------------------------------------------------------------------------------------------
+def test_written_tensors_that_overlap_are_refused():
+    """Tensors that a call writes share no memory: parts of one tensor that meet are refused, parts beside each other are taken."""
+    pos, tables = torch.arange(5, dtype=torch.int32, device="cuda")[None], [orc.table(8, 32).cuda()]
+    for dtype in (BF, F32):
+        pack = torch.randn(2, 6, 5, 64, generator=torch.Generator().manual_seed(60)).to(dtype).cuda()
+        tokens = pack.transpose(1, 2).contiguous().transpose(1, 2)   # tokens outside heads
+        for x in (pack, tokens):
+            before = x.clone()
+            for a, b in ((x[:, :4], x[:, 3:]), (x[:, 2:], x[:, :3]), (x[:1], x[:1, 1:4]), (x[:, ::2], x[:, 2:3])):
+                with pytest.raises(RuntimeError, match="share memory|two tensors"):
+                    rope_axes_qk_(a, b, pos, tables)
+            assert torch.equal(x, before)
+            want = rope_axes_qk(x, None, pos, tables)[0]
+            rope_axes_qk_(x[:, :4], x[:, 4:], pos, tables)
+            assert torch.equal(x, want)
+            want = rope_axes_qk(x, None, pos, tables)[0]
+            rope_axes_qk_(x[:, ::2], x[:, 1::2], pos, tables)
+            assert torch.equal(x, want)
+    both = torch.zeros(9, 2, 2, 16, 64, dtype=BF, device="cuda")
+    k, seq, pages = torch.zeros(1, 2, 3, 64, dtype=BF, device="cuda"), ints(3), ints(0, 1)[None]
+    flat = both.reshape(36, 16, 64)
+    for a, b in ((both[:8, 0], both[1:, 0]), (both[:, 0], both[:, 0]), (flat[:16].reshape(8, 2, 16, 64), flat[2:18].reshape(8, 2, 16, 64))):
+        with pytest.raises(RuntimeError, match="share memory|two tensors"):
+            paged_append_(a, b, k, k, pages, seq)
+    assert paged_append_(both[:, 0], both[:, 1], k, k, pages, seq) is None
+    assert paged_append_(both[:4, 0], both[4:8, 0], k, k, pages, seq) is None
