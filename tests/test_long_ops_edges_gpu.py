@@ -273,3 +273,42 @@ def test_written_tensors_that_overlap_are_refused():
             paged_append_(a, b, k, k, pages, seq)
     assert paged_append_(both[:, 0], both[:, 1], k, k, pages, seq) is None
     assert paged_append_(both[:4, 0], both[4:8, 0], k, k, pages, seq) is None
+
+
+# ---- bounds by the number of terms -----------------------------------------------------------------------------------------------------------
+TERMS = [
+    # B, Hq, Hkv, Lq, Lk, dk, dv, window, sinks, dtype
+    (1, 1, 1, 64, 64, 64, 64, None, 0, HF),
+    (2, 4, 2, 200, 200, 64, 64, 64, 4, HF),
+    (1, 6, 2, 257, 301, 80, 80, 100, 5, HF),
+    (1, 1, 1, 513, 513, 128, 128, 128, 64, HF),
+    (1, 2, 1, 10, 5000, 128, 128, None, 0, HF),
+    (1, 1, 1, 1, 9000, 64, 64, None, 0, BF),
+    (1, 4, 1, 3000, 3000, 64, 64, 33, 4, BF),
+    (1, 1, 1, 4000, 4000, 64, 64, 17, 128, HF),
+]
+
+
+@pytest.mark.parametrize("case", TERMS, ids=name_of)
+def test_against_64_bits_with_bounds_of_the_terms(case, monkeypatch):
+    """The bounds of long_oracle with its flat slack replaced by what the case's own sums can be off by, relative to the sum of the terms' magnitudes.
+    A sum of n products in 32 bits: n 2^-24.  A score is a sum of dk products, so that a probability is off by dk 2^-24 times the largest sum of |q k| (scaled); its exponential, logarithm
+    and the softmax's own sum, of up to Lk terms, add (64 + Lk) 2^-24.  Second-order products of up to four roundings of u: 8 u^2.  o and dq sum Lk terms, dk and dv Lq times the
+    heads of a group."""
+    B, Hq, Hkv, Lq, Lk, dk, dv, window, n_sink, dtype = case
+    gen = torch.Generator().manual_seed(61)
+    mk = lambda *s: torch.randn(s, generator=gen).to(dtype).cuda()  # noqa: E731
+    q, k, v, do = mk(B, Hq, Lq, dk), mk(B, Hkv, Lk, dk), mk(B, Hkv, Lk, dv), mk(B, Hq, Lq, dv)
+    scale, G, u = 1.0 / math.sqrt(dk), Hq // Hkv, torch.finfo(dtype).eps / 2
+    reach = float((q.double().abs() @ k.double().abs().repeat_interleave(G, 1).transpose(-1, -2)).amax()) * scale
+    common = (dk * reach + 64 + Lk + dv) * 2.0 ** -24 + 8 * u * u
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    o = window_attention(q, k, v, window, n_sink, scale)
+    got = dict(zip(("o", "dq", "dk", "dv"), (o.detach(),) + torch.autograd.grad(o, (q, k, v), do)))
+    q, k, v = (x.detach() for x in (q, k, v))
+    for names, terms in ((("o", "dq"), Lk), (("dk", "dv"), Lq * G)):
+        monkeypatch.setattr(orc, "SLACK", common + terms * 2.0 ** -24)
+        want = orc.window(q, k, v, window, n_sink, scale, do)
+        for name in names:
+            orc.check(got[name], want[name], name)
