@@ -422,8 +422,9 @@ Tensor cut_last(const Tensor& x, int64_t d) { return x.size(-1) == d ? x : x.nar
 // cannot pass a gradient to one of the default stream: the engine would make the two streams wait for each other, which ends the capture, and on ROCm the process.
 void check_capture(Node& node) {
   bool on_default = false;
-  for (const torch::autograd::Edge& e : node.next_edges()) {
-    const std::optional<c10::Stream> s = e.is_valid() ? e.function->stream() : std::nullopt;
+  for (size_t i = 0; i < node.num_outputs(); i++) {
+    if (!node.task_should_compute_output(i)) continue;   // this pass asks for no gradient behind that input: the engine passes none on
+    const std::optional<c10::Stream> s = node.next_edge(i).function->stream();
     on_default = on_default || (s.has_value() && s->id() == 0);
   }
   if (C10_UNLIKELY(on_default && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None))

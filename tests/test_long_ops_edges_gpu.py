@@ -312,3 +312,26 @@ def test_against_64_bits_with_bounds_of_the_terms(case, monkeypatch):
         want = orc.window(q, k, v, window, n_sink, scale, do)
         for name in names:
             orc.check(got[name], want[name], name)
+
+
+# ---- captured backward passes ------------------------------------------------------------------------------------------------------------------
+def test_a_captured_backward_pass_that_asks_for_other_leaves_is_taken():
+    """A leaf of a live graph of the default stream is in the way only where its gradient is asked for."""
+    gen = torch.Generator().manual_seed(62)
+    q, k, v = (torch.randn(1, 2, 40, 64, generator=gen).to(BF).cuda().requires_grad_(True) for _ in range(3))
+    side = torch.cuda.Stream()
+    eager = window_attention(q, k.detach(), v.detach(), 8)   # holds q alone
+    with torch.cuda.stream(side):
+        want = torch.autograd.grad(window_attention(q.detach(), k, v, 8), (k, v), eager.detach())
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        o = window_attention(q, k, v, 8)
+        with pytest.raises(RuntimeError, match="graph of the default stream"):
+            torch.autograd.grad(o, (q, k), eager.detach(), retain_graph=True)
+        got = torch.autograd.grad(o, (k, v), eager.detach())
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+    assert torch.autograd.grad(eager, q, eager.detach())[0].isfinite().all()
