@@ -215,9 +215,10 @@ __device__ inline void store_part(T* p, const Vec8<T>& v, int n) {
 
 // heads in flight
 constexpr int UNR = 4;
-// Workgroups that a large call aims for: two a CU, since a thread that walks more heads fetches its cos and sin less often (us, by 512 / 2048 / 256: prompts of 7 sequences of 2047 tokens,
-// 16 + 8 + 8 heads, d = 64, 20.4 / 24.0 / 19.5; 6 of 1500, 32 + 8 + 8, d = 128, 41 / 46 / 45; 2 x 8192 tokens, 16 + 16, d = 64, 29 / 32 / 28; 4096 tokens, 16 + 4, d = 128, 8.8 / 8.7 / 9.3)
-constexpr int ROT_BLOCKS = 512;
+// A large call aims for two workgroups a CU, since a thread that walks more heads fetches its cos and sin less often (us on 256 CUs, by 512 / 2048 / 256 workgroups: prompts of 7
+// sequences of 2047 tokens, 16 + 8 + 8 heads, d = 64, 20.4 / 24.0 / 19.5; 6 of 1500, 32 + 8 + 8, d = 128, 41 / 46 / 45; 2 x 8192 tokens, 16 + 16, d = 64, 29 / 32 / 28; 4096 tokens,
+// 16 + 4, d = 128, 8.8 / 8.7 / 9.3)
+constexpr int ROT_BLOCKS_CU = 2;
 
 // WHOLE: every part has 8 dims or pairs (the others cost branches in front of every access)
 template <typename T, bool WHOLE>
@@ -469,10 +470,11 @@ int launch(RotArgs& a, bool vec, bool vec16, const char* who, hipStream_t stream
   for (int z = 0; z < a.n; z++) dims = dlt_imax(dims, a.s[z].rot ? a.s[z].C - r.pairs : a.s[z].C);
   const int64_t gx = rows ? (tokens + 4 * (64 / parts) - 1) / (4 * (64 / parts)) : (tokens * (vec ? parts : dims) + 255) / 256;
   if (gx > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too much work for one launch (%lld tokens)", who, (long long)tokens);
-  // heads of a thread: all of them while that leaves ROT_BLOCKS workgroups, else fewer, in groups as they are in flight together
+  // heads of a thread: all of them while that leaves ROT_BLOCKS_CU workgroups a CU, else fewer, in groups as they are in flight together, and fewer than those while CUs are idle
+  const int64_t cus = dlt_device_cus();
   a.hb = (a.heads + UNR - 1) / UNR * UNR;
-  while (a.hb > UNR && gx * ((a.heads + a.hb - 1) / a.hb) < ROT_BLOCKS) a.hb = (a.hb / 2 + UNR - 1) / UNR * UNR;
-  while (a.hb > 1 && gx * ((a.heads + a.hb - 1) / a.hb) < 256) a.hb = (a.hb + 1) / 2;
+  while (a.hb > UNR && gx * ((a.heads + a.hb - 1) / a.hb) < ROT_BLOCKS_CU * cus) a.hb = (a.hb / 2 + UNR - 1) / UNR * UNR;
+  while (a.hb > 1 && gx * ((a.heads + a.hb - 1) / a.hb) < cus) a.hb = (a.hb + 1) / 2;
   if ((a.heads + a.hb - 1) / a.hb > 65535) a.hb = (a.heads + 65534) / 65535;
   const dim3 grid((unsigned)gx, (unsigned)((a.heads + a.hb - 1) / a.hb)), block(256);
   dlt_timing_before(DLT_K_ROPE, stream);
