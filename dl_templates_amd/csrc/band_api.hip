@@ -241,7 +241,6 @@ int check_common(const char* who, int B, int H, int Hkv, int dk, int dv, int win
 }
 
 void set_scalars(BandArgs& a, float sm_scale, int Hkv, int G) {
-  a.sm_scale = sm_scale;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
   a.Hkv = Hkv;
   a.G = G;

@@ -207,8 +207,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
   };
   int f0, f1;
   W.whole(first, last, a.W, i_beg, i_end, f0, f1);
-  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
-  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
+  // loops of their own: BandWalk::whole
   int bi = 0, i = i_beg, stop = f0;
   auto buf_of = [&](int i) { return smem + (i >= NBUF ? i - NBUF : i) * B::BUF; };
   auto step = [&](auto mask_tag) __attribute__((always_inline)) {
@@ -299,10 +298,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
 template <typename TIO, int D, int PAD>
 __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   dlt_kernargs_in<sizeof(BandArgs)>();
-  constexpr int NP = 1, CK = 64, NW = 4;   // blocks of 16 keys a wave, rows of a chunk, waves
+  constexpr int CK = 64, NW = 4;   // rows of a chunk; waves, of 16 keys each
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
-  constexpr int KC = band_kc(D, PAD), KB = 2 * KC, NQB = CK / 32, OWN = 16 * NP * NW;
+  constexpr int KC = band_kc(D, PAD), KB = 2 * KC, NQB = CK / 32, OWN = 16 * NW;
   constexpr int NBUF = band_nbuf(B::BUF), AHEAD = NBUF - 1;
   constexpr int NG = CK / NW / 16;
   static_assert(NG >= 1 && NG * NW * 16 == CK && CK == 64, "whole groups of 16 rows per wave; one copy of scalars a chunk");
@@ -321,7 +320,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     const int bh = lin / n_far;
     const int rest = lin - bh * n_far, grp = rest / a.far;
     share = rest - grp * a.far;
-    x0 = grp * 16 * NP;
+    x0 = grp * 16;
     b = band_div(bh, a.by_heads);
     h = bh - b * a.Hkv;
   } else {
@@ -330,7 +329,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     x0 = blk * OWN;
   }
   const int bh = b * a.Hkv + h;
-  const int xe = dlt_imin(x0 + (far ? 16 * NP : OWN), a.Lk);
+  const int xe = dlt_imin(x0 + (far ? 16 : OWN), a.Lk);
   const char* qb = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1]);
   const char* dob = reinterpret_cast<const char*>(reinterpret_cast<const TIO*>(a.d_o) + b * a.dos[0] + (int64_t)h * a.G * a.dos[1]);
   const TIO* kh = reinterpret_cast<const TIO*>(a.k) + b * a.ks[0] + h * a.ks[1];
@@ -384,28 +383,21 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   for (int i = 0; i < AHEAD; i++)
     if (i < n_ch) issue(at(i), smem + i * B::BUF_KV);
 
-  const int wk0 = far ? x0 : x0 + wave * 16 * NP;
-  u32x4 kf[NP][KC], vf[NP][KC];
-  int rlo[NP], rhi[NP];
-#pragma unroll
-  for (int p = 0; p < NP; p++) {
-    const int xk = wk0 + 16 * p + n;
-    const bool on = xk < a.Lk;
-    rlo[p] = on ? rlo_of(xk) : a.rows;
-    rhi[p] = on ? rhi_of(xk) : 0;
-    band_load_own<KC>(kf[p], kh + (on ? xk : 0) * a.ks[2], on, a.dk_, g);
-    band_load_own<KC>(vf[p], vh + (on ? xk : 0) * a.vs[2], on, a.dv_, g);
-  }
+  const int wk0 = far ? x0 : x0 + wave * 16;
+  u32x4 kf[KC], vf[KC];
+  const int own = wk0 + n;
+  const bool on = own < a.Lk;
+  const int rlo = on ? rlo_of(own) : a.rows, rhi = on ? rhi_of(own) : 0;
+  band_load_own<KC>(kf, kh + (on ? own : 0) * a.ks[2], on, a.dk_, g);
+  band_load_own<KC>(vf, vh + (on ? own : 0) * a.vs[2], on, a.dv_, g);
   // rows that see some key of the wave: [wlo, whi)
-  const int wk1 = dlt_imin(wk0 + 16 * NP, xe) - 1;
+  const int wk1 = dlt_imin(wk0 + 16, xe) - 1;
   const bool wave_on = wk1 >= wk0;
   const int wlo = wave_on ? rlo_of(wk0) : 0, whi = !wave_on ? 0 : wk0 < a.S ? r_end : rhi_of(wk1);
 
-  f32x4 dk_acc[NP][KB], dv_acc[NP][KB];
+  f32x4 dk_acc[1][KB], dv_acc[1][KB];   // as the helpers of several blocks a wave take them
 #pragma unroll
-  for (int p = 0; p < NP; p++)
-#pragma unroll
-    for (int d = 0; d < KB; d++) dk_acc[p][d] = dv_acc[p][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < KB; d++) dk_acc[0][d] = dv_acc[0][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   const float scale = a.scale_log2;
   FlashDLane<D> L;
   flashd_lane_init(L, n, g);
@@ -415,11 +407,9 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   pin_loaded(vf);
   // the own values are negated and the dP products start from the rows' delta: the matrix pipe delivers -(dP - delta)
 #pragma unroll
-  for (int p = 0; p < NP; p++)
-#pragma unroll
-    for (int c = 0; c < KC; c++) {
-      vf[p][c].x ^= 0x80008000u; vf[p][c].y ^= 0x80008000u; vf[p][c].z ^= 0x80008000u; vf[p][c].w ^= 0x80008000u;
-    }
+  for (int c = 0; c < KC; c++) {
+    vf[c].x ^= 0x80008000u; vf[c].y ^= 0x80008000u; vf[c].z ^= 0x80008000u; vf[c].w ^= 0x80008000u;
+  }
   __syncthreads();
 
   auto consume = [&](const int q0, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
@@ -428,13 +418,13 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     Swa2Lds sLse = cur + 2 * B::REG + 16 * g, sDel = sLse + CK * 4;
     // the first products (S, dP) of every 16-row half, then the second ones (dV, dK) block by block; the element-wise work of a half is
     // issued in pieces behind the matrix instructions of the following segment
-    constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NP2 = 2 * KB, NT = N1 + NQB * NP2;
-    constexpr int NU = 2 * NP;
+    constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NSEG = 2 * KB, NT = N1 + NQB * NSEG;
+    constexpr int NU = 2;   // element-wise pieces of a half
     // Each sum is a chain of products that wait for each other: at d = 128 S and dP take turns (8192 tokens, window 1024, 16 heads on 4 179 -> 173 us; 8 x 8 kv heads of 4 query
     // heads, 1111 tokens, 138 -> 129), at d = 64, where three workgroups share a CU, one follows the other (98 against 100, 76 against 76)
     constexpr auto score = [](int r) { return D > 64 ? r % 2 == 0 : r < KC; };
     constexpr auto dims = [](int r) { return D > 64 ? r / 2 : r % KC; };
-    static_assert(NP2 >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
+    static_assert(NSEG >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
     constexpr int RD = 3;   // 1: 197 us, 3: 187 for 16 heads on 4, 8192 tokens, window 1024, d = 128; more: spills
     u32x4 ring[RD + 1];
     auto rd = [&](auto kc) __attribute__((always_inline)) {
@@ -443,33 +433,33 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
         constexpr int hh = k / N1H, r = k % N1H, T0 = 16 * hh;
         ring[k % (RD + 1)] = swa2_lds16((score(r) ? sQ : sDO) + T0 * FlashDRow<D>::ROW + L.a[dims(r)]);
       } else {
-        constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
+        constexpr int qb_ = (k - N1) / NSEG, d = (k - N1) % NSEG;
         if constexpr (d < KB) ring[k % (RD + 1)] = flashd_read_tr<D, 32 * qb_>(sDO, L, d);
         else ring[k % (RD + 1)] = flashd_read_tr<D, 32 * qb_>(sQ, L, d - KB);
       }
     };
-    int elo[NP], ehi[NP];   // row 16 hh + 4 g + i of the chunk is seen iff elo <= 16 hh + i < ehi (see band_edge)
+    int elo, ehi;   // row 16 hh + 4 g + i of the chunk is seen iff elo <= 16 hh + i < ehi (see band_edge)
     if constexpr (MASK) {
       int at = q0 + 4 * g;
       asm volatile("" : "+v"(at));
-#pragma unroll
-      for (int p = 0; p < NP; p++) { elo[p] = rlo[p] - at; ehi[p] = rhi[p] - at; }
+      elo = rlo - at;
+      ehi = rhi - at;
     }
     swa2_for<0, RD>([&](auto kc) __attribute__((always_inline)) { rd(kc); });
-    f32x4 sv[2][NP], dp[2][NP], lq[2], dl[2];   // by the parity of the half
+    f32x4 sv[2], dp[2], lq[2], dl[2];   // by the parity of the half
     dl[0] = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
-    u32x4 pb[NQB][NP], dsb[NQB][NP];
+    u32x4 pb[NQB], dsb[NQB];
     auto ew = [&](auto hhc, auto uc) __attribute__((always_inline)) {
       constexpr int hh = decltype(hhc)::value, u = decltype(uc)::value;
-      constexpr int qb_ = hh / 2, mb = hh % 2, p = u / 2, i0_ = 2 * (u % 2);
+      constexpr int qb_ = hh / 2, mb = hh % 2, i0_ = 2 * u;
       float pr[2], ds[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         const int i = i0_ + t;
-        float pv = fast_exp2(fmaf(sv[hh & 1][p][i], scale, -lq[hh & 1][i]));
-        float dv = -pv * dp[hh & 1][p][i];
+        float pv = fast_exp2(fmaf(sv[hh & 1][i], scale, -lq[hh & 1][i]));
+        float dv = -pv * dp[hh & 1][i];
         if constexpr (MASK) {
-          const bool sees = 16 * hh + i >= elo[p] && 16 * hh + i < ehi[p];
+          const bool sees = 16 * hh + i >= elo && 16 * hh + i < ehi;
           pv = band_formed(pv);
           dv = band_formed(dv);
           pv = sees ? pv : 0.f;
@@ -479,10 +469,10 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
         ds[t] = dv;
       }
       const unsigned pw = pack2<TIO>(pr[0], pr[1]), dw = pack2<TIO>(ds[0], ds[1]);
-      if constexpr (mb == 0 && i0_ == 0) { pb[qb_][p].x = pw; dsb[qb_][p].x = dw; }
-      if constexpr (mb == 0 && i0_ == 2) { pb[qb_][p].y = pw; dsb[qb_][p].y = dw; }
-      if constexpr (mb == 1 && i0_ == 0) { pb[qb_][p].z = pw; dsb[qb_][p].z = dw; }
-      if constexpr (mb == 1 && i0_ == 2) { pb[qb_][p].w = pw; dsb[qb_][p].w = dw; }
+      if constexpr (mb == 0 && i0_ == 0) { pb[qb_].x = pw; dsb[qb_].x = dw; }
+      if constexpr (mb == 0 && i0_ == 2) { pb[qb_].y = pw; dsb[qb_].y = dw; }
+      if constexpr (mb == 1 && i0_ == 0) { pb[qb_].z = pw; dsb[qb_].z = dw; }
+      if constexpr (mb == 1 && i0_ == 2) { pb[qb_].w = pw; dsb[qb_].w = dw; }
     };
     swa2_for<0, NT>([&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
@@ -499,25 +489,19 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
       const u32x4 op = ring[k % (RD + 1)];
       if constexpr (k < N1) {
         constexpr int hh = k / N1H, r = k % N1H;
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-          if constexpr (score(r)) sv[hh & 1][p] = Mma<TIO>::mfma(op, kf[p][dims(r)], dims(r) == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[hh & 1][p]);
-          else dp[hh & 1][p] = Mma<TIO>::mfma(op, vf[p][dims(r)], dims(r) == 0 ? dl[hh & 1] : dp[hh & 1][p]);
-        }
+        if constexpr (score(r)) sv[hh & 1] = Mma<TIO>::mfma(op, kf[dims(r)], dims(r) == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[hh & 1]);
+        else dp[hh & 1] = Mma<TIO>::mfma(op, vf[dims(r)], dims(r) == 0 ? dl[hh & 1] : dp[hh & 1]);
         if constexpr (hh >= 1 && r < NU) {
           ew(std::integral_constant<int, hh - 1>{}, std::integral_constant<int, r>{});
-          SWA2_MIX(NP, 12 / NP)
+          SWA2_MIX(1, 12)
         }
       } else {
-        constexpr int qb_ = (k - N1) / NP2, d = (k - N1) % NP2;
-#pragma unroll
-        for (int p = 0; p < NP; p++) {
-          if constexpr (d < KB) dv_acc[p][d] = Mma<TIO>::mfma(op, pb[qb_][p], dv_acc[p][d]);
-          else dk_acc[p][d - KB] = Mma<TIO>::mfma(op, dsb[qb_][p], dk_acc[p][d - KB]);
-        }
+        constexpr int qb_ = (k - N1) / NSEG, d = (k - N1) % NSEG;
+        if constexpr (d < KB) dv_acc[0][d] = Mma<TIO>::mfma(op, pb[qb_], dv_acc[0][d]);
+        else dk_acc[0][d - KB] = Mma<TIO>::mfma(op, dsb[qb_], dk_acc[0][d - KB]);
         if constexpr (qb_ == 0 && d < NU) {
           ew(std::integral_constant<int, NH - 1>{}, std::integral_constant<int, d>{});
-          SWA2_MIX(NP, 12 / NP)
+          SWA2_MIX(1, 12)
         }
       }
     });
@@ -527,39 +511,28 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     Swa2Lds sQ = cur + 16 * wave * FlashDRow<D>::ROW, sDO = sQ + B::REG;
     Swa2Lds sLse = cur + 2 * B::REG + 16 * g + 64 * wave, sDel = sLse + CK * 4;
     const f32x4 lq = __builtin_bit_cast(f32x4, swa2_lds16(sLse)), dl = __builtin_bit_cast(f32x4, swa2_lds16(sDel));
-    f32x4 sv[NP], dp[NP];
+    f32x4 sv, dp;
 #pragma unroll
     for (int r = 0; r < KC; r++) {
       const u32x4 x = swa2_lds16(sQ + L.a[r]), y = swa2_lds16(sDO + L.a[r]);
-#pragma unroll
-      for (int p = 0; p < NP; p++) {
-        sv[p] = Mma<TIO>::mfma(x, kf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv[p]);
-        dp[p] = Mma<TIO>::mfma(y, vf[p][r], r == 0 ? dl : dp[p]);
-      }
+      sv = Mma<TIO>::mfma(x, kf[r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : sv);
+      dp = Mma<TIO>::mfma(y, vf[r], r == 0 ? dl : dp);
     }
-    u32x4 pb[NP], dsb[NP];
+    float pr[4], ds[4];
 #pragma unroll
-    for (int p = 0; p < NP; p++) {
-      float pr[4], ds[4];
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int r = q0 + 16 * wave + 4 * g + i;
-        const bool sees = r >= rlo[p] && r < rhi[p];
-        const float pv = fast_exp2(fmaf(sv[p][i], scale, -lq[i]));
-        pr[i] = sees ? pv : 0.f;
-        ds[i] = sees ? -pv * dp[p][i] : 0.f;
-      }
-      pb[p] = u32x4{pack2<TIO>(pr[0], pr[1]), pack2<TIO>(pr[2], pr[3]), 0u, 0u};
-      dsb[p] = u32x4{pack2<TIO>(ds[0], ds[1]), pack2<TIO>(ds[2], ds[3]), 0u, 0u};
+    for (int i = 0; i < 4; i++) {
+      const int r = q0 + 16 * wave + 4 * g + i;
+      const bool sees = r >= rlo && r < rhi;
+      const float pv = fast_exp2(fmaf(sv[i], scale, -lq[i]));
+      pr[i] = sees ? pv : 0.f;
+      ds[i] = sees ? -pv * dp[i] : 0.f;
     }
+    const u32x4 pb = {pack2<TIO>(pr[0], pr[1]), pack2<TIO>(pr[2], pr[3]), 0u, 0u}, dsb = {pack2<TIO>(ds[0], ds[1]), pack2<TIO>(ds[2], ds[3]), 0u, 0u};
 #pragma unroll
     for (int d = 0; d < KB; d++) {
       const u32x2 x = swa2_lds_tr(sDO + L.tr[d]), y = swa2_lds_tr(sQ + L.tr[d]);
-#pragma unroll
-      for (int p = 0; p < NP; p++) {
-        dv_acc[p][d] = Mma<TIO>::mfma(u32x4{x.x, x.y, 0u, 0u}, pb[p], dv_acc[p][d]);
-        dk_acc[p][d] = Mma<TIO>::mfma(u32x4{y.x, y.y, 0u, 0u}, dsb[p], dk_acc[p][d]);
-      }
+      dv_acc[0][d] = Mma<TIO>::mfma(u32x4{x.x, x.y, 0u, 0u}, pb, dv_acc[0][d]);
+      dk_acc[0][d] = Mma<TIO>::mfma(u32x4{y.x, y.y, 0u, 0u}, dsb, dk_acc[0][d]);
     }
   };
   struct Far {};
@@ -574,9 +547,7 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   // chunks whose rows see all keys of the workgroup: rows [rlo of the last key, rhi of the first one without sinks)
   const int all_lo = rlo_of(xe - 1), all_hi = x0 >= a.S ? rhi_of(x0) : xe <= a.S ? r_end : rhi_of(a.S);
   const int f0 = dlt_imin(dlt_imax(i_beg, (all_lo - r_beg + CK - 1) / CK), i_end), f1 = dlt_imax(f0, dlt_imin(i_end, all_hi > r_beg ? (all_hi - r_beg) / CK : 0));
-  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
-  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
-  // Counted from `start`: masked chunks up to `stop`, whole ones up to `whole`, masked ones up to m1, whole ones
+  // loops of their own (BandWalk::whole), counted from `start`: masked chunks up to `stop`, whole ones up to `whole`, masked ones up to m1, whole ones
   const int g0 = f0 - i_beg, g1 = f1 - i_beg;   // whole chunks
   int bi = 0, i = 0;
   int stop = start < g0 ? g0 - start : start < g1 ? 0 : n_ch - start + g0, whole = start < g1 ? g1 - start : n_ch - start + g1;
@@ -609,15 +580,9 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   __syncthreads();
 
   // ---- epilogue
-  unsigned odd[NP];
-  float mulk[NP], mulv[NP];
-#pragma unroll
-  for (int p = 0; p < NP; p++) {
-    mulk[p] = a.grad_scale;
-    mulv[p] = 1.f;
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(wk0 + 16 * p + n < a.Lk && (band_odd_row(dk_acc, p) || band_odd_row(dv_acc, p)));
-    odd[p] = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);
-  }
+  const float mulk[1] = {a.grad_scale}, mulv[1] = {1.f};
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(own < a.Lk && (band_odd_row(dk_acc, 0) || band_odd_row(dv_acc, 0)));
+  const unsigned odd = (unsigned)((bad | bad >> 16 | bad >> 32 | bad >> 48) & 0xffff);   // keys of the wave to be taken again
   // one own key once more over the rows of chunks [i_beg, i_end) that see it: two dims of dK (without sm_scale) and dV
   auto exact = [&](int xk, float (&sk)[2], float (&sv)[2]) __attribute__((always_inline)) {
     const TIO *k = kh + xk * a.ks[2], *v = vh + xk * a.vs[2];
@@ -646,36 +611,32 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     float* pk = a.part + (far ? P.far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dk_ : ((int64_t)bh * a.shares + share) * P.keys * a.dk_);
     float* pv = a.part + P.v_at + (far ? P.v_far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dv_ : ((int64_t)bh * a.shares + share) * P.keys * a.dv_);
     const int len = far ? (int)P.far_keys : a.Lk;
-    flash_share_put<NP>(pk, dk_acc, a.dk_, wk0 + n, len, g);
-    flash_share_put<NP>(pv, dv_acc, a.dv_, wk0 + n, len, g);
-#pragma unroll 1
-    for (int p = 0; p < NP; p++)
-      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
-        const int xk = wk0 + 16 * p + __builtin_ctz(todo);
-        float sk[2], sv[2];
-        exact(xk, sk, sv);
-        __threadfence();   // behind the wave's own stores of the row
-        if (2 * lane < a.dk_) *reinterpret_cast<float2*>(pk + (int64_t)xk * a.dk_ + 2 * lane) = float2{sk[0], sk[1]};
-        if (2 * lane < a.dv_) *reinterpret_cast<float2*>(pv + (int64_t)xk * a.dv_ + 2 * lane) = float2{sv[0], sv[1]};
-      }
+    flash_share_put<1>(pk, dk_acc, a.dk_, wk0 + n, len, g);
+    flash_share_put<1>(pv, dv_acc, a.dv_, wk0 + n, len, g);
+    for (unsigned todo = odd; todo != 0; todo &= todo - 1) {
+      const int xk = wk0 + __builtin_ctz(todo);
+      float sk[2], sv[2];
+      exact(xk, sk, sv);
+      __threadfence();   // behind the wave's own stores of the row
+      if (2 * lane < a.dk_) *reinterpret_cast<float2*>(pk + (int64_t)xk * a.dk_ + 2 * lane) = float2{sk[0], sk[1]};
+      if (2 * lane < a.dv_) *reinterpret_cast<float2*>(pv + (int64_t)xk * a.dv_ + 2 * lane) = float2{sv[0], sv[1]};
+    }
     return;
   }
   constexpr int PT = D * 2 + 16;
   auto again = [&](bool keys) __attribute__((always_inline)) {
-#pragma unroll 1
-    for (int p = 0; p < NP; p++)
-      for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
-        const int w = 16 * p + __builtin_ctz(todo);
-        float sk[2], sv[2];
-        exact(wk0 + w, sk, sv);
-        const float f = keys ? a.grad_scale : 1.f;
-        if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>((keys ? sk[0] : sv[0]) * f, (keys ? sk[1] : sv[1]) * f);
-      }
+    for (unsigned todo = odd; todo != 0; todo &= todo - 1) {
+      const int w = __builtin_ctz(todo);
+      float sk[2], sv[2];
+      exact(wk0 + w, sk, sv);
+      const float f = keys ? a.grad_scale : 1.f;
+      if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 + w) * PT + 4 * lane) = pack2<TIO>((keys ? sk[0] : sv[0]) * f, (keys ? sk[1] : sv[1]) * f);
+    }
   };
   TIO* dkb = reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1];
   TIO* dvb = reinterpret_cast<TIO*>(a.dv) + b * a.dvs[0] + h * a.dvs[1];
-  band_store_rows<D, NP, TIO>(smem, dk_acc, mulk, NW, 1, true, a.dk_, wave, n, g, tid,
+  band_store_rows<D, 1, TIO>(smem, dk_acc, mulk, NW, 1, true, a.dk_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.Lk ? dkb + (x0 + row) * a.dks[2] : nullptr; }, [&]() { again(true); });
-  band_store_rows<D, NP, TIO>(smem, dv_acc, mulv, NW, 1, true, a.dv_, wave, n, g, tid,
+  band_store_rows<D, 1, TIO>(smem, dv_acc, mulv, NW, 1, true, a.dv_, wave, n, g, tid,
                               [&](int row) -> TIO* { return x0 + row < a.Lk ? dvb + (x0 + row) * a.dvs[2] : nullptr; }, [&]() { again(false); });
 }

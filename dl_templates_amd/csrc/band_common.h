@@ -39,7 +39,7 @@ struct BandArgs {
   int32_t cycle;            // dK / dV: chunks of rows that see a block of keys
   int32_t low_rows;         // rows of a (batch, kv head) with low parts
   int32_t q16;              // 16 is a multiple of G: 16 rows are whole tokens
-  float scale_log2, sm_scale, grad_scale;   // grad_scale: of dQ and dK; 0 where every row sees one key, whose dS are zero but for roundings
+  float scale_log2, grad_scale;   // grad_scale: of dQ and dK; 0 where every row sees one key, whose dS are zero but for roundings
   BandPages pg;
 };
 
@@ -122,7 +122,8 @@ struct BandWalk {
     n = (last - jump) / CK + 1;
   }
   DLT_DEV int tok(int y) const { return y + (y >= sinks ? jump : 0); }
-  // of chunks [beg, end) those that every one of the rows sees whole (sinks not counted): [f0, f1)
+  // Of chunks [beg, end) those that every one of the rows sees whole (sinks not counted): [f0, f1).  These and the others, at an edge of the window, run in loops of their own:
+  // with both bodies in one loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210).
   DLT_DEV void whole(int first, int last, int W, int beg, int end, int& f0, int& f1) const {
     const int behind = last - jump - W + 1;                   // the last row's window starts there
     const int lo = behind > 0 ? (behind + CK - 1) / CK : 0;

@@ -314,8 +314,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   };
   int f0, f1;
   W.whole(first, last, a.W, i_beg, i_end, f0, f1);
-  // Chunks at an edge of the window and chunks that every row of the workgroup sees whole run in loops of their own: with both bodies in one
-  // loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210)
+  // loops of their own: BandWalk::whole
   const int rounds = (i_end - i_beg + GR - 1) / GR, r0 = (f0 - i_beg + GR - 1) / GR, r1 = (f1 - i_beg) / GR;
   int bi = 0, it = 0, stop = dlt_imin(r0, rounds);
   auto buf_of = [&](int i) { return bufs + (i >= NBUF ? i - NBUF : i) * B::BUF; };
