@@ -318,7 +318,10 @@ void set_map(BandArgs& a) {
 // Shares: up to two workgroups a CU (one round of them: 4 kv heads, 200 queries of two heads on 8000 keys, d = 128, 19 shares of 28
 // blocks 24 us, 18 shares 18), at least four chunks each; dQ: while its blocks fill half of the CUs (us with the sum of the parts: 4 kv heads, 200 queries of two heads on
 // 8000 keys, d = 128, 132 -> 28; 2 heads, 10 queries of 4 heads on 2000, d = 64, 27 -> 12; but 1000 queries of 8 heads on 1000 keys, 250 blocks, 18 -> 20).  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
-// (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).
+// (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).  Above one and a half workgroups a CU
+// they lose: 64 sequences, 8 kv heads, d = 128, us without / with shares and their sum: of 5000 keys 212 / 219, of 590 to 5000 165 / 169, 8 of 20000 and 56 of 2500 573 / 579; 56 of 600
+// to 5000 154 / 160.  They would win, and not by much, where one context is far longer than the rest (65536 among 63 of 500: 1170 / 600, its bytes take 77).  Both rules go by the table's
+// width, since lengths stay on the device: 300 keys in a table for 8192 are planned as 8192 (9.4 us; 6.8 in a table for 300).
 int plan_rows(BandArgs& a, bool forward) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv;

@@ -3,7 +3,8 @@
 A cache is a tensor [pages, Hkv, page, D]; row b of ``page_table`` (int32 [B, columns]) names the pages of sequence b in order, so that position
 p lies in row ``p % page`` of page ``page_table[b, p // page]``.  ``seq_len`` (int32 [B]) counts the tokens of every sequence, its newest
 ones included; of T new tokens in a call sequence b has the first ``n_new[b]`` (None: all T), at positions ``seq_len[b] - n_new[b] ..
-seq_len[b] - 1``; those behind are padding.  Both calls take the same ``seq_len`` and ``n_new``, which stay on the device: no call waits for
+seq_len[b] - 1``; those behind are padding.  A ``seq_len`` beyond the table's row is a mistake: the append leaves out what does not fit, attention
+takes what the row holds.  Both calls take the same ``seq_len`` and ``n_new``, which stay on the device: no call waits for
 the host, and a captured graph sees what they hold when it is replayed.  Neither records a graph for autograd, and forward-mode tangents are
 refused.
 """
@@ -56,7 +57,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     n_sink: int = 0, sm_scale: float = None, n_new: torch.Tensor = None) -> torch.Tensor:
     """``window_attention`` of the newest tokens q [B, H, T, Dk] over the cached keys and values: o [B, H, T, Dv].
 
-    Padded rows, and rows of sequences without a key, give zeros.  bfloat16 and float16, head dims in multiples of 8 up to 128, pages of a
+    Padded rows, and rows of sequences without a key, give zeros, whatever the keys and values beside them hold.  bfloat16 and float16, head dims in multiples of 8 up to 128, pages of a
     multiple of 16 tokens, cache rows contiguous and 16-byte aligned.  What a page holds behind a sequence's last token does not matter; a
     page number outside the cache is a mistake that is not looked for (some page of the cache is read)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale

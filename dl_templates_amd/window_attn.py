@@ -3,7 +3,8 @@
 The window of ``tiled_swa`` along a sequence: with ``q`` [B, H, Lq, Dk], ``k`` [B, Hkv, Lk, Dk] and ``v`` [B, Hkv, Lk, Dv], query ``i``
 stands at position ``p = Lk - Lq + i`` (the queries are the newest tokens) and sees key ``j`` iff ``j <= p`` and ``p - j < window`` or
 ``j < n_sink``.  A query that sees nothing (``p < 0``) gives zeros.  bfloat16 and float16, head dims up to 128; head dims that are
-no multiples of 8 are zero-padded around the kernels, rows that cannot be read in 16-byte pieces are copied first.  The serving form
+no multiples of 8 are zero-padded around the kernels, rows that cannot be read in 16-byte pieces are copied first.  Infinities and NaN
+reach the rows and keys that see them and no others, at a price: those are summed by one wave each.  The serving form
 of it, keys and values in pages, is ``paged_cache.paged_attention``.
 """
 from __future__ import annotations

@@ -337,8 +337,9 @@ int dlt_window_bwd(const void* q, const int64_t q_strides[4], const void* k, con
 /* ---- keys and values in pages -----------------------------------------------------------------
  * A cache is [n_pages, Hkv, page, d] by element strides (page, head, row, dim).  Row b of `table` (int32, `cols` pages, element stride
  * table_stride) names the pages of sequence b in order: position p lies in row p % page of page table[b][p / page].  seq_len[b] counts the
- * tokens of sequence b with its n_new[b] newest ones (n_new NULL: T of every sequence; n_new[b] is taken within 0 .. T, seq_len[b] within
- * 0 .. cols * page); new token t < n_new[b] stands at position seq_len[b] - n_new[b] + t, tokens t >= n_new[b] are padding. */
+ * tokens of sequence b with its n_new[b] newest ones (n_new NULL: T of every sequence; n_new[b] is taken within 0 .. T); new token
+ * t < n_new[b] stands at position seq_len[b] - n_new[b] + t, tokens t >= n_new[b] are padding.  A seq_len[b] outside 0 .. cols * page is a
+ * mistake: attention takes it as the nearest of those numbers, the append takes it as it is and leaves out positions outside the table. */
 typedef struct {
   int32_t B, H, Hkv, T, dk, dv;
   int32_t page, n_pages, cols;
@@ -357,7 +358,7 @@ int dlt_paged_append(const void* k, const int64_t k_strides[4], const void* v, c
                      const dlt_rope_axes_t* rope, const dlt_paged_shape_t* shape, void* stream);
 
 /* The window attention above for the T newest tokens of every sequence, keys and values in pages (page a multiple of 16).  Padded rows and rows
- * that see nothing give zeros.  What pages hold behind a sequence's last token does not matter.  A page number outside the pool reads
+ * that see nothing give zeros, whatever keys and values beside them hold.  What pages hold behind a sequence's last token does not matter.  A page number outside the pool reads
  * another page of it. */
 int dlt_paged_workspace(const dlt_paged_shape_t* shape, int64_t* bytes);
 int dlt_paged_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4],
@@ -388,7 +389,7 @@ int dlt_debug_copy(void* dst, const void* src, int64_t bytes, void* stream);
  * autotuning, src/tiled_swa.py:570-573); here the host routes every call by shape, element type, strides and
  * alignment, and a C caller cannot see from the outside that, say, head dim 80 or a 9-token tile at head dim 96 lands on the
  * generic kernels (several times slower than the tuned ones).  dlt_last_kernel_family() returns the family the calling
- * thread's latest forward / backward call (dlt_swa_*, dlt_flash_*) was routed to.  With dlt_dry_run(1) (per thread) those
+ * thread's latest forward / backward call (dlt_swa_*, dlt_flash_*, dlt_window_*, dlt_paged_attn) was routed to.  With dlt_dry_run(1) (per thread) those
  * calls validate their arguments and route, but launch nothing and touch no memory: pointers only need the alignment
  * of the real ones, so the query also works in a process without a GPU.
  *   MARCHING  token grids (b_size 1), head dim 32, windows up to 21 x 21, and 64, up to 13 x 13 (rotation: head dim 64, 8 rotary pairs, in
