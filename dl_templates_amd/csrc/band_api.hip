@@ -9,8 +9,9 @@ namespace {
 
 // ---- sums of shares -------------------------------------------------------------------------------------------------------------
 // Forward: partial outputs [bh][share][row][dv] and, behind them, {maximum in log2 units, sum} of each row, joined in the order of the shares.
-// WG: a workgroup to a row; every wave forms the weights of all shares (a lane each), adds up every fourth share, and the four sums are added.  Else (up to 8 shares) a wave to
-// a row.  One thread per 4 dims walking all shares: 36 us for 96 rows of 64 shares, this way 4.8; 8192 rows of 4 shares 14.4 by workgroups, 6.2 by waves.
+// WG: a workgroup to a row; every wave forms the weights of all shares (a lane each), adds up every fourth share, and the four sums are added.  Else (up to 8
+// shares) a wave to a row.  One thread per 4 dims walking all shares: 36 us for 96 rows of 64 shares, this way 4.8; 8192 rows of 4 shares 14.4 by workgroups,
+// 6.2 by waves.
 DLT_DEV float band_share_weight(const float2& x, float m) {
   // a share that held no key of the row has (-inf, 0); a sum that is infinite or NaN goes through
   return x.x == -INFINITY ? (x.y == 0.f ? 0.f : 1.f) : fast_exp2(x.x - m);
@@ -127,8 +128,9 @@ __global__ __launch_bounds__(256) void band_join_q_kernel(const BandArgs a) {
   if (on) *reinterpret_cast<unsigned*>(p + 2 * lane) = pack2<TIO>(s.x * f, s.y * f);
 }
 
-// dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares.  Keys with far sums, of which there are up to hundreds,
-// come first, a workgroup to a key, where 8 runs of threads take every eighth sum (one run: 9 us for 16 keys of 112 sums on 4 heads, this way 5.5).
+// dK (times sm_scale) or dV: partial sums of the keys that have any (BandParts), added in the order of the shares.  Keys with far sums, of which there are up
+// to hundreds, come first, a workgroup to a key, where 8 runs of threads take every eighth sum (one run: 9 us for 16 keys of 112 sums on 4 heads, this way
+// 5.5).
 template <typename TIO>
 __global__ __launch_bounds__(256) void band_join_kv_kernel(const BandArgs a) {
   dlt_kernargs_in<sizeof(BandArgs)>();
@@ -217,7 +219,8 @@ int join(const BandArgs& a, bool backward, int dtype, hipStream_t stream) {
 }
 
 // ---- checks ------------------------------------------------------------------------------------------------------------------------
-int check_rows(const char* who, const char* name, const void* p, const int64_t* st, bool empty, int64_t span /* largest offset inside a slab that must fit 32 bits, elements */) {
+// span: largest offset inside a slab that must fit 32 bits, elements
+int check_rows(const char* who, const char* name, const void* p, const int64_t* st, bool empty, int64_t span) {
   DLT_REQUIRE(st != nullptr && (p != nullptr || empty), "%s: %s is NULL", who, name);
   if (empty) return DLT_OK;
   DLT_REQUIRE(st[3] == 1 && (uintptr_t)p % 16 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0,
@@ -295,7 +298,11 @@ int paged_problem(const char* who, const dlt_paged_shape_t* s, BandArgs& a) {
 }
 
 void set_map(BandArgs& a) {
-  auto div = [](int64_t d) { BandDiv x; dlt_fastdiv_make((uint32_t)dlt_imin64(dlt_imax64(d, 1), 0x7fffffff), x.m, x.s); return x; };   // (more workgroups than that are refused)
+  auto div = [](int64_t d) {
+    BandDiv x;
+    dlt_fastdiv_make((uint32_t)dlt_imin64(dlt_imax64(d, 1), 0x7fffffff), x.m, x.s);   // (more workgroups than that are refused)
+    return x;
+  };
   a.units = (int)dlt_imin64((int64_t)a.nblk * a.shares, 0x7fffffff);
   a.by_group_units = div((int64_t)a.group * a.units);
   a.by_group = div(a.group);
@@ -305,23 +312,27 @@ void set_map(BandArgs& a) {
 }
 // ---- cutting a call into workgroups ---------------------------------------------------------------------------------------------------
 // Rows: how many a workgroup has, and how many workgroups share the keys of a block of rows.
-//   BAND_TWO     128 rows, where that makes two workgroups a CU (8 kv heads of 6000 tokens, d = 64, one and a half a CU: forward 29 us by 64 rows, 37 by 128; dQ 33, 42)
-//   BAND_ONE     64 rows otherwise, and in a forward pass over few keys at d <= 64, whose set-up weighs more than its reads of LDS (64 kv heads of 4444 rows, window 300, d = 64: 78 ->
-//                72 us; window 500 78 -> 76; window 1024 69 -> 70; at d = 128 107 -> 114; dQ 74 -> 82)
-//   BAND_HALVES  64 rows, their keys over two groups of waves, while one workgroup a CU is all there is and the keys of a block are too few, or the workgroups too many, to be
-//                shared: a wave alone on its SIMD waits out every latency.  8 heads of 2048 queries, d = 64 / 128, us: 2560 keys each 32 -> 25 / 46 -> 35; 640 keys 11.7 -> 11.7 /
-//                16.4 -> 15.2; 4 heads, 640 keys, 10.1 + 6.3 for the sum of 4 shares -> 11.0 / 14.6 + 5.9 -> 14.0; but 12 heads (384 workgroups) 14.6 -> 19.7 / 20 -> 26
-//   BAND_FEW     16 rows, where that makes no more than a workgroup a CU, few keys: a wave has 32-key chunks of its own, a quarter of the dependent work.  us, against HALVES: 4 heads of
-//                200 tokens, window 64, d = 64, 6.7 -> 5.2; of 1000 tokens, window 300, 9.4 -> 7.0, d = 128 11.8 -> 8.6; 8 heads of 500, window 200, d = 128, 10.4 -> 7.8; one token on 300 keys,
-//                8 heads, 8.2 -> 7.6.  With two workgroups a CU 7.7 -> 10.2 (8 heads of 1000, window 100, d = 64); with more keys the shares win: 8 tokens of 8 heads on 900 keys, d = 128,
-//                15.2 -> 8.4 + 3.8
+//   BAND_TWO     128 rows, where that makes two workgroups a CU (8 kv heads of 6000 tokens, d = 64, one and a half a CU: forward 29 us by 64 rows, 37 by 128;
+//                dQ 33, 42)
+//   BAND_ONE     64 rows otherwise, and in a forward pass over few keys at d <= 64, whose set-up weighs more than its reads of LDS (64 kv heads of 4444 rows,
+//                window 300, d = 64: 78 -> 72 us; window 500 78 -> 76; window 1024 69 -> 70; at d = 128 107 -> 114; dQ 74 -> 82)
+//   BAND_HALVES  64 rows, their keys over two groups of waves, while one workgroup a CU is all there is and the keys of a block are too few, or the workgroups
+//                too many, to be shared: a wave alone on its SIMD waits out every latency.  8 heads of 2048 queries, d = 64 / 128, us: 2560 keys each 32 -> 25
+//                / 46 -> 35; 640 keys 11.7 -> 11.7 / 16.4 -> 15.2; 4 heads, 640 keys, 10.1 + 6.3 for the sum of 4 shares -> 11.0 / 14.6 + 5.9 -> 14.0; but 12
+//                heads (384 workgroups) 14.6 -> 19.7 / 20 -> 26
+//   BAND_FEW     16 rows, where that makes no more than a workgroup a CU, few keys: a wave has 32-key chunks of its own, a quarter of the dependent work.  us,
+//                against HALVES: 4 heads of 200 tokens, window 64, d = 64, 6.7 -> 5.2; of 1000 tokens, window 300, 9.4 -> 7.0, d = 128 11.8 -> 8.6; 8 heads of
+//                500, window 200, d = 128, 10.4 -> 7.8; one token on 300 keys, 8 heads, 8.2 -> 7.6.  With two workgroups a CU 7.7 -> 10.2 (8 heads of 1000,
+//                window 100, d = 64); with more keys the shares win: 8 tokens of 8 heads on 900 keys, d = 128, 15.2 -> 8.4 + 3.8
 // Shares: up to two workgroups a CU (one round of them: 4 kv heads, 200 queries of two heads on 8000 keys, d = 128, 19 shares of 28
-// blocks 24 us, 18 shares 18), at least four chunks each; dQ: while its blocks fill half of the CUs (us with the sum of the parts: 4 kv heads, 200 queries of two heads on
-// 8000 keys, d = 128, 132 -> 28; 2 heads, 10 queries of 4 heads on 2000, d = 64, 27 -> 12; but 1000 queries of 8 heads on 1000 keys, 250 blocks, 18 -> 20).  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then
-// (32 sequences of up to 5000 keys, 8 kv heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).  Above one and a half workgroups a CU
-// they lose: 64 sequences, 8 kv heads, d = 128, us without / with shares and their sum: of 5000 keys 212 / 219, of 590 to 5000 165 / 169, 8 of 20000 and 56 of 2500 573 / 579; 56 of 600
-// to 5000 154 / 160.  They would win, and not by much, where one context is far longer than the rest (65536 among 63 of 500: 1170 / 600, its bytes take 77).  Both rules go by the table's
-// width, since lengths stay on the device: 300 keys in a table for 8192 are planned as 8192 (9.4 us; 6.8 in a table for 300).
+// blocks 24 us, 18 shares 18), at least four chunks each; dQ: while its blocks fill half of the CUs (us with the sum of the parts: 4 kv heads, 200 queries of
+// two heads on 8000 keys, d = 128, 132 -> 28; 2 heads, 10 queries of 4 heads on 2000, d = 64, 27 -> 12; but 1000 queries of 8 heads on 1000 keys, 250 blocks,
+// 18 -> 20).  Contexts in pages differ in length, and a workgroup does not know its own before it runs: four a CU then (32 sequences of up to 5000 keys, 8 kv
+// heads, d = 64 / 128: 47 -> 31 + 5 us / 88 -> 74 + 5; of up to 10000 keys 101 -> 71 + 5 / 169 -> 129 + 5).  Above one and a half workgroups a CU they lose: 64
+// sequences, 8 kv heads, d = 128, us without / with shares and their sum: of 5000 keys 212 / 219, of 590 to 5000 165 / 169, 8 of 20000 and 56 of 2500 573 /
+// 579; 56 of 600 to 5000 154 / 160.  They would win, and not by much, where one context is far longer than the rest (65536 among 63 of 500: 1170 / 600, its
+// bytes take 77).  Both rules go by the table's width, since lengths stay on the device: 300 keys in a table for 8192 are planned as 8192 (9.4 us; 6.8 in a
+// table for 300).
 int plan_rows(BandArgs& a, bool forward) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv;
@@ -363,8 +374,8 @@ void plan_keys(BandArgs& a) {
   const int64_t wgs = bh * a.nblk;
   const int64_t near_chunks = dlt_imin64((int64_t)(a.W + own) * a.G, a.rows) / 64 + 1;   // of a block without sinks
   a.cycle = (int)near_chunks;
-  // at least 4 chunks a share, 8 at d = 128, whose partial sums weigh more (us with the sum of the parts, 4 / 8 chunks: 2 kv heads of 2000 tokens, 4 query heads each, window 500, 29.8 / 27.6;
-  // 4 of 1500, window 300, 37.4 / 30.0; at d = 64 one of 600, window 200, 13.8 / 17.1)
+  // at least 4 chunks a share, 8 at d = 128, whose partial sums weigh more (us with the sum of the parts, 4 / 8 chunks: 2 kv heads of 2000 tokens, 4 query
+  // heads each, window 500, 29.8 / 27.6; 4 of 1500, window 300, 37.4 / 30.0; at d = 64 one of 600, window 200, 13.8 / 17.1)
   const int64_t least = band_class(a.dk_, a.dv_) == 64 ? 4 : 8;
   const int64_t want = wgs > 0 && wgs < cus ? (2 * cus + wgs - 1) / wgs : 1;
   const int64_t key_bytes = dlt_imax64(bh * a.Lk * (a.dk_ + a.dv_) * 4, 1);
@@ -393,7 +404,8 @@ int check_ws(const char* who, const void* ws, int64_t have, int64_t need) {
   return DLT_OK;
 }
 int check_grid(const char* who, const BandArgs& a) {
-  if ((int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + (int64_t)a.far * a.far_groups) > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  if ((int64_t)a.B * a.Hkv * ((int64_t)a.nblk * a.shares + (int64_t)a.far * a.far_groups) > 0x7fffffff)
+    return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
   return DLT_OK;
 }
 void strides3(int64_t (&to)[3], const int64_t* st) {

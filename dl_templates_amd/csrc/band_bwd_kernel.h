@@ -284,7 +284,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 && D <= 64 ? 3 : 2) void band_bwd_
                                     float sum[2];
                                     exact(r, sum);
                                     const float f = a.off + band_row(a, r).tok == 0 ? 0.f : a.grad_scale;
-                                    if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * f, sum[1] * f);
+                                    if (2 * lane < D)
+                                      *reinterpret_cast<unsigned*>(smem + (wave * 16 * NP + w) * PT + 4 * lane) = pack2<TIO>(sum[0] * f, sum[1] * f);
                                   }
                               });
 }
@@ -367,11 +368,12 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
       stq.template issue<PAD>(a, qb, a.qs, r0 + at, a.rows - 1, buf + at * 2 * D);
       std_.template issue<PAD>(a, dob, a.dos, r0 + at, a.rows - 1, buf + B::REG + at * 2 * D);
     }
-    if (wave < 2) dlt_copy4_to_lds(reinterpret_cast<const char*>(scal + r0), (uint32_t)dlt_imin(lane, a.rows - 1 - r0) * 4u, buf + 2 * B::REG + wave * (CK * 4));
+    if (wave < 2)
+      dlt_copy4_to_lds(reinterpret_cast<const char*>(scal + r0), (uint32_t)dlt_imin(lane, a.rows - 1 - r0) * 4u, buf + 2 * B::REG + wave * (CK * 4));
   };
-  // Chunks are taken cyclically from one whose place is a multiple of `cycle` on: a block's rows overlap those of its neighbours, which then ask for the same chunk at the same time.
-  // Each from its own first one, the workgroups of an XCD would spread over more rows than its L2 holds (8192 tokens, window 1024, 16 heads on 4, d = 128: 860 MB fetched for 84, now 144;
-  // 188 -> 184 us; 4 sequences, window 512, 32 heads on 8, 665 -> 632)
+  // Chunks are taken cyclically from one whose place is a multiple of `cycle` on: a block's rows overlap those of its neighbours, which then ask for the same
+  // chunk at the same time. Each from its own first one, the workgroups of an XCD would spread over more rows than its L2 holds (8192 tokens, window 1024, 16
+  // heads on 4, d = 128: 860 MB fetched for 84, now 144; 188 -> 184 us; 4 sequences, window 512, 32 heads on 8, 665 -> 632)
   const int n_ch = i_end - i_beg;
   int start = 0;
   if (!far) {
@@ -420,8 +422,8 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
     // issued in pieces behind the matrix instructions of the following segment
     constexpr int N1H = 2 * KC, NH = 2 * NQB, N1 = NH * N1H, NSEG = 2 * KB, NT = N1 + NQB * NSEG;
     constexpr int NU = 2;   // element-wise pieces of a half
-    // Each sum is a chain of products that wait for each other: at d = 128 S and dP take turns (8192 tokens, window 1024, 16 heads on 4 179 -> 173 us; 8 x 8 kv heads of 4 query
-    // heads, 1111 tokens, 138 -> 129), at d = 64, where three workgroups share a CU, one follows the other (98 against 100, 76 against 76)
+    // Each sum is a chain of products that wait for each other: at d = 128 S and dP take turns (8192 tokens, window 1024, 16 heads on 4 179 -> 173 us; 8 x 8 kv
+    // heads of 4 query heads, 1111 tokens, 138 -> 129), at d = 64, where three workgroups share a CU, one follows the other (98 against 100, 76 against 76)
     constexpr auto score = [](int r) { return D > 64 ? r % 2 == 0 : r < KC; };
     constexpr auto dims = [](int r) { return D > 64 ? r / 2 : r % KC; };
     static_assert(NSEG >= NU && N1H >= NU, "a segment must have room for the element-wise pieces of a half");
@@ -546,7 +548,8 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   };
   // chunks whose rows see all keys of the workgroup: rows [rlo of the last key, rhi of the first one without sinks)
   const int all_lo = rlo_of(xe - 1), all_hi = x0 >= a.S ? rhi_of(x0) : xe <= a.S ? r_end : rhi_of(a.S);
-  const int f0 = dlt_imin(dlt_imax(i_beg, (all_lo - r_beg + CK - 1) / CK), i_end), f1 = dlt_imax(f0, dlt_imin(i_end, all_hi > r_beg ? (all_hi - r_beg) / CK : 0));
+  const int f0 = dlt_imin(dlt_imax(i_beg, (all_lo - r_beg + CK - 1) / CK), i_end);
+  const int f1 = dlt_imax(f0, dlt_imin(i_end, all_hi > r_beg ? (all_hi - r_beg) / CK : 0));
   // loops of their own (BandWalk::whole), counted from `start`: masked chunks up to `stop`, whole ones up to `whole`, masked ones up to m1, whole ones
   const int g0 = f0 - i_beg, g1 = f1 - i_beg;   // whole chunks
   int bi = 0, i = 0;
@@ -608,8 +611,9 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
   };
   if (far || a.shares > 1 || (a.far != 0 && x0 < a.S)) {
     const BandParts P(a);
-    float* pk = a.part + (far ? P.far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dk_ : ((int64_t)bh * a.shares + share) * P.keys * a.dk_);
-    float* pv = a.part + P.v_at + (far ? P.v_far_at + (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys * a.dv_ : ((int64_t)bh * a.shares + share) * P.keys * a.dv_);
+    const int64_t row = far ? (((int64_t)bh * a.far + share) * 4 + wave) * P.far_keys : ((int64_t)bh * a.shares + share) * P.keys;
+    float* pk = a.part + (far ? P.far_at : 0) + row * a.dk_;
+    float* pv = a.part + P.v_at + (far ? P.v_far_at : 0) + row * a.dv_;
     const int len = far ? (int)P.far_keys : a.Lk;
     flash_share_put<1>(pk, dk_acc, a.dk_, wk0 + n, len, g);
     flash_share_put<1>(pv, dv_acc, a.dv_, wk0 + n, len, g);
@@ -630,7 +634,8 @@ __global__ __launch_bounds__(256, 2) void band_bwd_kv_kernel(const BandArgs a) {
       float sk[2], sv[2];
       exact(wk0 + w, sk, sv);
       const float f = keys ? a.grad_scale : 1.f;
-      if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 + w) * PT + 4 * lane) = pack2<TIO>((keys ? sk[0] : sv[0]) * f, (keys ? sk[1] : sv[1]) * f);
+      const float x = (keys ? sk[0] : sv[0]) * f, y = (keys ? sk[1] : sv[1]) * f;
+      if (2 * lane < D) *reinterpret_cast<unsigned*>(smem + (wave * 16 + w) * PT + 4 * lane) = pack2<TIO>(x, y);
     }
   };
   TIO* dkb = reinterpret_cast<TIO*>(a.dk) + b * a.dks[0] + h * a.dks[1];

@@ -60,8 +60,9 @@ struct BandParts {
   }
 };
 
-// Workgroup -> (batch, kv head), own block and share of it: `group` heads at a time are interleaved, as flash_block_causal has it, the blocks from the last on (`rev`: own =
-// queries, whose first blocks may see less) or from the first.  Divisions are products: four divisions were a third of the instructions in front of the first copy.
+// Workgroup -> (batch, kv head), own block and share of it: `group` heads at a time are interleaved, as flash_block_causal has it, the blocks from the last on
+// (`rev`: own = queries, whose first blocks may see less) or from the first.  Divisions are products: four divisions were a third of the instructions in front
+// of the first copy.
 DLT_DEV int band_div(int n, const BandDiv& d) { return (int)dlt_fastdiv((uint32_t)n, d.m, d.s); }
 DLT_DEV void band_block(const BandArgs& a, int lin, bool rev, int& b, int& h, int& blk, int& share) {
   const int grp = band_div(lin, a.by_group_units), rem = lin - grp * (a.group * a.units);
@@ -82,9 +83,9 @@ DLT_DEV BandRow band_row(const BandArgs& a, int r) {
   const int t = (int)dlt_fastdiv((uint32_t)r, a.mG, a.sG);
   return BandRow{t, r - t * a.G};
 }
-// delta = dO . o is subtracted from every dP of a row; where a row sees few keys these cancel, and the rounding of o is what is left of it: with two keys dQ and dK are off by 2.3
-// times what their own rounding is, with 16 by 1.5, at most 1.5 in any case with o unrounded (the roundings of dS remain).  Rows that see up to 16 keys, those of short windows and of the
-// first 16 positions, therefore keep the part of o that its rounding drops.
+// delta = dO . o is subtracted from every dP of a row; where a row sees few keys these cancel, and the rounding of o is what is left of it: with two keys dQ
+// and dK are off by 2.3 times what their own rounding is, with 16 by 1.5, at most 1.5 in any case with o unrounded (the roundings of dS remain).  Rows that see
+// up to 16 keys, those of short windows and of the first 16 positions, therefore keep the part of o that its rounding drops.
 template <typename TIO>
 DLT_DEV TIO* band_low(const BandArgs& a, int b, int h, int r) {
   if (r >= a.low_rows) return nullptr;
@@ -105,12 +106,13 @@ DLT_DEV T* band_row_ptr(T* base, const int64_t (&st)[3], const BandArgs& a, int 
   return base + (w.tok * st[2] + w.head * st[1]);
 }
 
-// Keys that the rows of a block at positions [first, last] see, in groups of 16: those with sinks, then those of the window.  Places y count them without the gap between
-// (token y, from 16 sink groups on token y + jump); chunk i holds places CK i .. + CK - 1, so sinks share a chunk with the window's first keys.  With
-// bounds less the jump a row's rule is the same for places as for tokens: no token below the window's first group is in any row's window, and none behind the sinks' groups is
-// a sink.  us, against sinks in chunks of their own and a window that starts at a multiple
-// of CK: 8 x 8 kv heads of 4 query heads, 1111 tokens, window 300, 5 sinks, forward / dQ, d = 64 69 / 70 -> 60 / 62, d = 128 109 / 149 -> 96 / 137; 4 of 8192, window 1024, d = 128
-// 111 / 138 -> 106 / 136.  Without sinks a start at multiples of 16 changes nothing or loses up to 3 %: neighbouring blocks' chunks then are not the same.
+// Keys that the rows of a block at positions [first, last] see, in groups of 16: those with sinks, then those of the window.  Places y count them without the
+// gap between (token y, from 16 sink groups on token y + jump); chunk i holds places CK i .. + CK - 1, so sinks share a chunk with the window's first keys.
+// With bounds less the jump a row's rule is the same for places as for tokens: no token below the window's first group is in any row's window, and none behind
+// the sinks' groups is a sink.  us, against sinks in chunks of their own and a window that starts at a multiple
+// of CK: 8 x 8 kv heads of 4 query heads, 1111 tokens, window 300, 5 sinks, forward / dQ, d = 64 69 / 70 -> 60 / 62, d = 128 109 / 149 -> 96 / 137; 4 of 8192,
+// window 1024, d = 128 111 / 138 -> 106 / 136.  Without sinks a start at multiples of 16 changes nothing or loses up to 3 %: neighbouring blocks' chunks then
+// are not the same.
 template <int CK>
 struct BandWalk {
   int sinks, jump, n;   // places with sinks, when there is a gap behind them; tokens left out; chunks
@@ -122,8 +124,9 @@ struct BandWalk {
     n = (last - jump) / CK + 1;
   }
   DLT_DEV int tok(int y) const { return y + (y >= sinks ? jump : 0); }
-  // Of chunks [beg, end) those that every one of the rows sees whole (sinks not counted): [f0, f1).  These and the others, at an edge of the window, run in loops of their own:
-  // with both bodies in one loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector instructions next to 210).
+  // Of chunks [beg, end) those that every one of the rows sees whole (sinks not counted): [f0, f1).  These and the others, at an edge of the window, run in
+  // loops of their own: with both bodies in one loop the compiler copies the accumulators from one set of registers to another, twice a chunk (72 vector
+  // instructions next to 210).
   DLT_DEV void whole(int first, int last, int W, int beg, int end, int& f0, int& f1) const {
     const int behind = last - jump - W + 1;                   // the last row's window starts there
     const int lo = behind > 0 ? (behind + CK - 1) / CK : 0;
@@ -147,14 +150,15 @@ DLT_DEV void band_load_own(u32x4 (&f)[KC], const TIO* row, bool on, int dims, in
   }
 }
 
-// Copies of 16 bytes a lane to `lds` + OA, + OB (and + OC, + OD) + 16 lane, as dlt_copy16_to_lds (swa2_common.hpp) with one set-up of M0 for all: the offset field of
-// the instruction counts for the memory address too, so `voff` of a copy is its lane's offset less that.  (A set-up for each copy was a sixth of a
+// Copies of 16 bytes a lane to `lds` + OA, + OB (and + OC, + OD) + 16 lane, as dlt_copy16_to_lds (swa2_common.hpp) with one set-up of M0 for all: the offset
+// field of the instruction counts for the memory address too, so `voff` of a copy is its lane's offset less that.  (A set-up for each copy was a sixth of a
 // chunk's instructions.)
 template <int OA, int OB>
 DLT_DEV void band_copy2(const char* base, uint32_t va, uint32_t vb, char* lds) {
   const uint32_t m = (uint32_t)(uintptr_t)(DLT_LDS char*)lds;
   uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1 offset:%5\n\tglobal_load_lds_dwordx4 %3, %1 offset:%6\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %1 offset:%5\n\t"
+               "global_load_lds_dwordx4 %3, %1 offset:%6\n\ts_mov_b32 m0, %0"
                : "=&s"(saved) : "s"(base), "v"(va), "v"(vb), "s"(m), "n"(OA), "n"(OB) : "memory");
 }
 DLT_DEV void band_copy4(const char* base, const uint32_t (&v)[4], char* lds) {
@@ -164,8 +168,8 @@ DLT_DEV void band_copy4(const char* base, const uint32_t (&v)[4], char* lds) {
                "global_load_lds_dwordx4 %4, %1 offset:%8\n\tglobal_load_lds_dwordx4 %5, %1 offset:%9\n\ts_mov_b32 m0, %0"
                : "=&s"(saved) : "s"(base), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]), "s"(m), "n"(1024), "n"(2 * 1024), "n"(3 * 1024) : "memory");
 }
-// All copies of a group of 16 tokens: copy i goes to `lds` + 1024 i; v[i] = the lane's offset + band_bias - 1024 i, taken from base - band_bias.  Under PAD lanes of pieces that
-// do not exist copy nothing; copies two apart move the same piece (8 tokens apart).
+// All copies of a group of 16 tokens: copy i goes to `lds` + 1024 i; v[i] = the lane's offset + band_bias - 1024 i, taken from base - band_bias.  Under PAD
+// lanes of pieces that do not exist copy nothing; copies two apart move the same piece (8 tokens apart).
 template <int NI> constexpr int band_bias = 1024 * (NI - 1);
 template <int NI, int PAD>
 DLT_DEV void band_copy_group(const char* base, const uint32_t (&v)[NI], bool on0, bool on1, char* lds) {
@@ -257,16 +261,16 @@ struct BandBuf {
   static constexpr int BUF_KV = 2 * REG + 2 * CK * 4;
 };
 
-// chunk buffers of a workgroup: as many as leave a CU two workgroups and more (one more at d = 128, with one block of rows per wave: 155 -> 186 us for the decode
-// step of 64 sequences, 18 -> 29 for 3 x 6 heads of 1111 tokens)
+// chunk buffers of a workgroup: as many as leave a CU two workgroups and more (one more at d = 128, with one block of rows per wave: 155 -> 186 us for the
+// decode step of 64 sequences, 18 -> 29 for 3 x 6 heads of 1111 tokens)
 constexpr int band_nbuf(int buf, int groups = 1) { return 4 * buf <= 65536 && 3 * groups * buf <= 131072 ? 3 : 2; }
 
 // Accumulators in C layout (lane (n, g): dims 16 d + 4 g .. + 3 of own row n, times mul[p]) -> LDS tile of 16-bit values -> rows.
 // `ptr(row)`: the row's place or NULL.  The tile takes the chunk buffers' LDS.
 // `again()`: the wave writes rows of its own part of the tile once more (see below).  LOW: what the rounding drops instead of what it leaves.
 template <int D, int NP, typename TIO, bool LOW = false, int NA, typename PtrFn, typename AgainFn>
-DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int groups, bool write, int dims, int wave, int n, int g, int tid, PtrFn ptr,
-                             AgainFn again) {
+DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (&mul)[NP], int nw, int groups, bool write, int dims, int wave, int n, int g,
+                             int tid, PtrFn ptr, AgainFn again) {
   constexpr int PT = D * 2 + 16;
   // `write`: the wave's group writes the tile; the waves of all groups store it
 #pragma unroll
@@ -299,7 +303,8 @@ DLT_DEV void band_store_rows(char* sT, const f32x4 (&acc)[NP][NA], const float (
   __syncthreads();
 }
 
-// 1 / sum of a row at position `pos` (< 0: it sees nothing, and gives zeros).  A sum of 0 otherwise means that every score that the row sees is -inf: the softmax of those is NaN.
+// 1 / sum of a row at position `pos` (< 0: it sees nothing, and gives zeros).  A sum of 0 otherwise means that every score that the row sees is -inf: the
+// softmax of those is NaN.
 DLT_DEV float band_inverse(float sum, int pos) { return sum != 0.f ? fast_rcp(sum) : pos < 0 ? 0.f : NAN; }
 DLT_DEV bool band_odd(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }   // infinite or NaN
 template <int NP, int NA>
@@ -313,7 +318,8 @@ DLT_DEV bool band_odd_row(const f32x4 (&acc)[NP][NA], int p) {
 }
 
 // Hidden pairs of a chunk at the edge.  Key x + 4 g + c of own row p (c a constant of the unrolled code) is seen iff c <= h && (c > l || c < s).  The
-// bounds are formed here, per chunk, from a value the compiler cannot look through: left to itself it keeps one register for each c, in kernels that have none left.
+// bounds are formed here, per chunk, from a value the compiler cannot look through: left to itself it keeps one register for each c, in kernels that have none
+// left.
 struct BandEdge { int h, l, s; };
 DLT_DEV BandEdge band_edge(int hi, int lo, int S, int x, int g) {
   int at = x + 4 * g;

@@ -163,8 +163,8 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       }
     }
   };
-  // Pages of the first chunks are looked up together: one trip to memory, not one a chunk (a token each of 8 sequences of up to 900, d = 64: 10.7 -> 10.1 us; one
-  // sequence of 5000, d = 128: 10.1 -> 8.7; large grids alike).  Looked up behind the last chunk too: the table has a column for position 0.
+  // Pages of the first chunks are looked up together: one trip to memory, not one a chunk (a token each of 8 sequences of up to 900, d = 64: 10.7 -> 10.1 us;
+  // one sequence of 5000, d = 128: 10.1 -> 8.7; large grids alike).  Looked up behind the last chunk too: the table has a column for position 0.
   if constexpr (PAGED) {
     Groups x[AHEAD];
 #pragma unroll
@@ -270,7 +270,8 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
               for (int i = 0; i < 4; i++) mx[i] = fmaxf(fmaxf(mx[i], t[p][kb2][2 * i]), t[p][kb2][2 * i + 1]);
             const float mloc = wave_max4(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
             // the reference maximum moves only when a score exceeds it by more than 2^8 after scaling: P stays below 2^8, its sum in
-            // 32 bits below 2^8 times the keys.  In masked chunks, where rows of few keys lie, it moves with the maximum: the largest P is then 1, and not rounded
+            // 32 bits below 2^8 times the keys.  In masked chunks, where rows of few keys lie, it moves with the maximum: the largest P is then 1, and not
+            // rounded
             if (__builtin_amdgcn_ballot_w64((mloc - m_run[p]) * scale > (MASK ? 0.f : 8.f))) {
               keep_branch();
               const float m_new = fmaxf(m_run[p], mloc);

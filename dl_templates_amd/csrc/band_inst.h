@@ -35,8 +35,9 @@ int band_fwd(const BandArgs& a, hipStream_t stream) {
   constexpr bool PG = DLT_BAND_PART == 1;
   constexpr int join = (GR - 1) * NW * NP * (D + 8) * 64, bufs = GR * band_nbuf(BandBuf<D, CK>::BUF, GR) * BandBuf<D, CK>::BUF;
   constexpr int lds = band_lds(bufs > join ? bufs : join, 16 * NP * NW);
-  return band_go(band_pick(a, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 0>, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, FEWER>, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 1>), a,
-                 (int64_t)a.B * a.Hkv * a.nblk * a.shares, 64 * NW * GR, lds, DLT_K_FWD, "window forward launch", stream);
+  return band_go(band_pick(a, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 0>, band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, FEWER>,
+                           band_fwd_kernel<TIO, D, NP, CK, NW, GR, PG, 1>), a, (int64_t)a.B * a.Hkv * a.nblk * a.shares,
+                 64 * NW * GR, lds, DLT_K_FWD, "window forward launch", stream);
 }
 template <typename TIO>
 int band_fwd_np(const BandArgs& a, int kind, hipStream_t stream) {
@@ -59,8 +60,8 @@ int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind
 template <typename TIO, int NP>
 int band_bwd_q(const BandArgs& a, hipStream_t stream) {
   constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
-  return band_go(band_pick(a, band_bwd_q_kernel<TIO, D, NP, 64, 4, 0>, band_bwd_q_kernel<TIO, D, NP, 64, 4, FEWER>, band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>), a, (int64_t)a.B * a.Hkv * a.nblk * a.shares, 256, lds,
-                 DLT_K_BWD_Q, "window dQ launch", stream);
+  return band_go(band_pick(a, band_bwd_q_kernel<TIO, D, NP, 64, 4, 0>, band_bwd_q_kernel<TIO, D, NP, 64, 4, FEWER>, band_bwd_q_kernel<TIO, D, NP, 64, 4, 1>), a,
+                 (int64_t)a.B * a.Hkv * a.nblk * a.shares, 256, lds, DLT_K_BWD_Q, "window dQ launch", stream);
 }
 template <typename TIO>
 int band_bwd_q_np(const BandArgs& a, int kind, hipStream_t stream) { return kind != BAND_TWO ? band_bwd_q<TIO, 1>(a, stream) : band_bwd_q<TIO, 2>(a, stream); }

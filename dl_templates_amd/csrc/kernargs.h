@@ -2,8 +2,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
-// The compiler loads each argument where it is first used; every first touch of a cache line is then a trip to memory of its own, one after the other, before the kernel has
-// asked for any data.  Here one word of each line is loaded, all at once.  Rotation of 256 tokens 7.1 -> 6.4 us, append of one token to 64
+// The compiler loads each argument where it is first used; every first touch of a cache line is then a trip to memory of its own, one after the other, before
+// the kernel has asked for any data.  Here one word of each line is loaded, all at once.  Rotation of 256 tokens 7.1 -> 6.4 us, append of one token to 64
 // sequences 6.6 -> 6.0, decode step on 300 keys 7.8 -> 7.4.
 template <int BYTES>
 __device__ __attribute__((always_inline)) inline void dlt_kernargs_in() {

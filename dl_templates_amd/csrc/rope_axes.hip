@@ -3,8 +3,8 @@
 // Pure streaming: every element is read once and written once.  A thread owns one (token, part of a row): up to 8 pairs of one axis, or up to 8 dims
 // that are not rotated.  Its (cos, sin) pairs are fetched once and stay in registers while it walks the heads of q, k and v, so table traffic is
 // shared by the heads; the first heads' elements are asked for before them, since nothing about them depends on positions or pages.
-// A part's two runs of dims start wherever the sections put them: accesses are as wide as the part (16 bytes of a 2-byte type for 8 dims), at any alignment of the
-// element, and parts of fewer than 8 pairs move in pieces of 4, 2 and 1.  Rows with other strides than 1 take a kernel of one pair per thread.
+// A part's two runs of dims start wherever the sections put them: accesses are as wide as the part (16 bytes of a 2-byte type for 8 dims), at any alignment of
+// the element, and parts of fewer than 8 pairs move in pieces of 4, 2 and 1.  Rows with other strides than 1 take a kernel of one pair per thread.
 // Rotated values are formed in 32 bits, each product rounded before the sum as in the 2D rotation, and rounded once.
 // 16 + 16 heads of 49152 tokens, d = 128, bf16: 149 us, 5.4 TB/s (a large copy: 5.15).  Memory bound; small calls take the launch.
 #include "kernargs.h"
@@ -215,9 +215,9 @@ __device__ inline void store_part(T* p, const Vec8<T>& v, int n) {
 
 // heads in flight
 constexpr int UNR = 4;
-// A large call aims for two workgroups a CU, since a thread that walks more heads fetches its cos and sin less often (us on 256 CUs, by 512 / 2048 / 256 workgroups: prompts of 7
-// sequences of 2047 tokens, 16 + 8 + 8 heads, d = 64, 20.4 / 24.0 / 19.5; 6 of 1500, 32 + 8 + 8, d = 128, 41 / 46 / 45; 2 x 8192 tokens, 16 + 16, d = 64, 29 / 32 / 28; 4096 tokens,
-// 16 + 4, d = 128, 8.8 / 8.7 / 9.3)
+// A large call aims for two workgroups a CU, since a thread that walks more heads fetches its cos and sin less often (us on 256 CUs, by 512 / 2048 / 256
+// workgroups: prompts of 7 sequences of 2047 tokens, 16 + 8 + 8 heads, d = 64, 20.4 / 24.0 / 19.5; 6 of 1500, 32 + 8 + 8, d = 128, 41 / 46 / 45; 2 x 8192
+// tokens, 16 + 16, d = 64, 29 / 32 / 28; 4096 tokens, 16 + 4, d = 128, 8.8 / 8.7 / 9.3)
 constexpr int ROT_BLOCKS_CU = 2;
 
 // WHOLE: every part has 8 dims or pairs (the others cost branches in front of every access)
@@ -303,8 +303,8 @@ __global__ __launch_bounds__(256) void rotate_rows_kernel(RotArgs a, int parts) 
   }
 }
 
-// The same with 8 dims of whole, 16-byte aligned rows to a lane; partners, at any distance, come through the row in LDS, which belongs to the wave.  For sections
-// whose parts would be short or whose second dims start between 16-byte pieces (2 x 10 heads of 7755
+// The same with 8 dims of whole, 16-byte aligned rows to a lane; partners, at any distance, come through the row in LDS, which belongs to the wave.  For
+// sections whose parts would be short or whose second dims start between 16-byte pieces (2 x 10 heads of 7755
 // tokens, d = 64, sections of 6, 11 and 11 pairs, fp16: 32 -> 11 us).
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_rows_lds_kernel(RotArgs a, int parts) {
@@ -470,7 +470,8 @@ int launch(RotArgs& a, bool vec, bool vec16, const char* who, hipStream_t stream
   for (int z = 0; z < a.n; z++) dims = dlt_imax(dims, a.s[z].rot ? a.s[z].C - r.pairs : a.s[z].C);
   const int64_t gx = rows ? (tokens + 4 * (64 / parts) - 1) / (4 * (64 / parts)) : (tokens * (vec ? parts : dims) + 255) / 256;
   if (gx > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too much work for one launch (%lld tokens)", who, (long long)tokens);
-  // heads of a thread: all of them while that leaves ROT_BLOCKS_CU workgroups a CU, else fewer, in groups as they are in flight together, and fewer than those while CUs are idle
+  // heads of a thread: all of them while that leaves ROT_BLOCKS_CU workgroups a CU, else fewer, in groups as they are in flight together, and fewer than those
+  // while CUs are idle
   const int64_t cus = dlt_device_cus();
   a.hb = (a.heads + UNR - 1) / UNR * UNR;
   while (a.hb > UNR && gx * ((a.heads + a.hb - 1) / a.hb) < ROT_BLOCKS_CU * cus) a.hb = (a.hb / 2 + UNR - 1) / UNR * UNR;
