@@ -57,9 +57,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     n_sink: int = 0, sm_scale: float = None, n_new: torch.Tensor = None) -> torch.Tensor:
     """``window_attention`` of the newest tokens q [B, H, T, Dk] over the cached keys and values: o [B, H, T, Dv].
 
-    Padded rows, and rows of sequences without a key, give zeros, whatever the keys and values beside them hold.  bfloat16 and float16, head dims in multiples of 8 up to 128, pages of a
-    multiple of 16 tokens, cache rows contiguous and 16-byte aligned.  What a page holds behind a sequence's last token does not matter; a
-    page number outside the cache is a mistake that is not looked for (some page of the cache is read)."""
+    Padded rows, and rows of sequences without a key, give zeros, whatever the keys and values beside them hold.  bfloat16 and float16, head
+    dims in multiples of 8 up to 128, pages of a multiple of 16 tokens, cache rows contiguous and 16-byte aligned.  What a page holds behind
+    a sequence's last token does not matter; a page number outside the cache is a mistake that is not looked for (some page of the cache is
+    read)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if sm_scale is None else sm_scale
     o = _lib.native.paged_attention(q, k_cache, v_cache, page_table, seq_len, window, n_sink, scale, n_new, False)
     if o is NotImplemented:
