@@ -29,7 +29,8 @@ EXPORTS = (
     "dlt_timing_enable", "dlt_timing_collect", "dlt_debug_copy",
     "dlt_swa_fwd_image", "dlt_swa_bwd_image", "dlt_swa_image_offsets", "dlt_swa_fwd_rot", "dlt_swa_bwd_rot",
     "dlt_swa_bwd_noalloc", "dlt_dry_run", "dlt_last_kernel_family",
-    "dlt_rope_axes", "dlt_window_workspace", "dlt_window_low_tokens", "dlt_window_fwd", "dlt_window_bwd", "dlt_paged_append", "dlt_paged_workspace", "dlt_paged_attn",
+    "dlt_rope_axes", "dlt_window_workspace", "dlt_window_low_tokens", "dlt_window_fwd", "dlt_window_bwd", "dlt_paged_append", "dlt_paged_workspace", "dlt_paged_attn", "dlt_page_assign",
+    "dlt_paged8_append", "dlt_paged8_workspace", "dlt_paged8_attn",
 )
 KERNEL_FAMILIES = ("none", "marching", "streaming", "tile", "flash", "generic", "band")   # DLT_FAMILY_* of include/dlt.h
 NOALLOC_MAX_DELTA = 1 << 20  # DLT_NOALLOC_MAX_DELTA of include/dlt.h
@@ -86,6 +87,12 @@ class PagedShape(Structure):
     _fields_ = [
         ("B", c_int32), ("H", c_int32), ("Hkv", c_int32), ("T", c_int32), ("dk", c_int32), ("dv", c_int32),
         ("page", c_int32), ("n_pages", c_int32), ("cols", c_int32), ("window", c_int32), ("n_sink", c_int32), ("sm_scale", c_float), ("dtype", c_int32),
+    ]
+
+
+class Scales8(Structure):
+    _fields_ = [
+        ("format", c_int32), ("block", c_int32), ("k_scale", c_void_p), ("v_scale", c_void_p), ("k_strides", c_int64 * 3), ("v_strides", c_int64 * 3),
     ]
 
 
@@ -178,6 +185,14 @@ def _declare(lib) -> None:
     lib.dlt_paged_workspace.argtypes = [POINTER(PagedShape), P64]
     lib.dlt_paged_attn.restype = c_int
     lib.dlt_paged_attn.argtypes = tensor * 4 + [c_void_p, c_int64, c_void_p, c_void_p, POINTER(PagedShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_paged8_append.restype = c_int
+    lib.dlt_paged8_append.argtypes = tensor * 6 + [POINTER(Scales8), c_void_p, c_int64, c_void_p, c_void_p, POINTER(RopeAxesDesc), POINTER(PagedShape), c_void_p]
+    lib.dlt_paged8_workspace.restype = c_int
+    lib.dlt_paged8_workspace.argtypes = [POINTER(PagedShape), POINTER(Scales8), P64]
+    lib.dlt_paged8_attn.restype = c_int
+    lib.dlt_paged8_attn.argtypes = tensor * 3 + [POINTER(Scales8)] + tensor + [c_void_p, c_int64, c_void_p, c_void_p, POINTER(PagedShape), c_void_p, c_int64, c_void_p]
+    lib.dlt_page_assign.restype = c_int
+    lib.dlt_page_assign.argtypes = [c_void_p, c_int64] + [c_void_p] * 3 + [c_int32] * 5 + [c_void_p] * 3
     lib.dlt_debug_copy.restype = c_int
     lib.dlt_debug_copy.argtypes = [c_void_p, c_void_p, c_int64, c_void_p]
     lib.dlt_timing_enable.restype = c_int

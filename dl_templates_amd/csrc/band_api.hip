@@ -333,7 +333,8 @@ void set_map(BandArgs& a) {
 // 579; 56 of 600 to 5000 154 / 160.  They would win, and not by much, where one context is far longer than the rest (65536 among 63 of 500: 1170 / 600, its
 // bytes take 77).  Both rules go by the table's width, since lengths stay on the device: 300 keys in a table for 8192 are planned as 8192 (9.4 us; 6.8 in a
 // table for 300).
-int plan_rows(BandArgs& a, bool forward) {
+// groups: kinds with several groups of waves on the same rows are there
+int plan_rows(BandArgs& a, bool forward, bool groups = true) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv;
   const bool paged = a.pg.cols != 0;
@@ -343,7 +344,7 @@ int plan_rows(BandArgs& a, bool forward) {
   if (forward && band_class(a.dk_, a.dv_) == 64 && chunks(128) <= 12) kind = BAND_ONE;
   const int64_t one = bh * blocks(64);
   const bool uneven = paged && 2 * one > cus && 2 * one <= 3 * cus && chunks(64) > 32;
-  if (forward && kind == BAND_ONE && one <= cus && !uneven) {
+  if (forward && groups && kind == BAND_ONE && one <= cus && !uneven) {
     if (bh * blocks(16) <= cus && chunks(16) <= (band_class(a.dk_, a.dv_) == 64 ? 16 : 10)) kind = BAND_FEW;
     else if (chunks(64) <= 12 || 2 * one > cus) kind = BAND_HALVES;
   }
@@ -535,6 +536,56 @@ extern "C" int dlt_paged_attn(const void* q, const int64_t q_strides[4], const v
   strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);
   a.pg.table = table; a.pg.seq = seq_len; a.pg.n_new = n_new; a.pg.ts = table_stride;
   rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged_64(a, shape->dtype, kind, stream) : dlt_band_paged_128(a, shape->dtype, kind, stream);
+  return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
+}
+
+// ---- the cache in 8 bits ----
+namespace {
+int check_rows8(const char* who, const char* name, const void* p, const int64_t* st) {
+  DLT_REQUIRE(st != nullptr && p != nullptr, "%s: %s is NULL", who, name);
+  DLT_REQUIRE(st[3] == 1 && (uintptr_t)p % 8 == 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0, "%s: rows of %s must be contiguous and start at multiples of 8 bytes", who,
+              name);
+  DLT_REQUIRE(st[0] >= 0 && st[1] >= 0 && st[2] >= 0, "%s: negative stride of %s", who, name);
+  if (17 * st[2] >= (int64_t)1 << 30) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: strides of %s are too large", who, name);
+  return DLT_OK;
+}
+}  // namespace
+
+extern "C" int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes) {
+  const char* who = "paged8_workspace";
+  DLT_REQUIRE(bytes != nullptr, "%s: bytes is NULL", who);
+  Band8Args a;
+  int rc = paged_problem(who, shape, a);
+  if (rc != DLT_OK || (rc = dlt_scales8_check(who, scales, shape->page)) != DLT_OK) return rc;
+  plan_rows(a, true, false);
+  *bytes = rows_bytes(a);
+  return DLT_OK;
+}
+
+extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4], const void* v_cache,
+                               const int64_t v_cache_strides[4], const dlt_scales8_t* scales, void* o, const int64_t o_strides[4], const int32_t* table, int64_t table_stride,
+                               const int32_t* seq_len, const int32_t* n_new, const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
+  const char* who = "paged8_attn";
+  hipStream_t stream = (hipStream_t)stream_;
+  Band8Args a;
+  int rc = paged_problem(who, shape, a);
+  if (rc != DLT_OK || (rc = dlt_scales8_check(who, scales, shape->page)) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "q", q, q_strides, a.Lq == 0, row_span(q_strides, a.G))) != DLT_OK) return rc;
+  if ((rc = check_rows8(who, "k_cache", k_cache, k_cache_strides)) != DLT_OK || (rc = check_rows8(who, "v_cache", v_cache, v_cache_strides)) != DLT_OK) return rc;
+  if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
+  DLT_REQUIRE(table != nullptr && seq_len != nullptr, "%s: table or seq_len is NULL", who);
+  DLT_REQUIRE(table_stride >= 0, "%s: negative table stride", who);
+  const int kind = plan_rows(a, true, false);
+  if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
+  if ((rc = check_grid(who, a)) != DLT_OK) return rc;
+  if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
+  a.q = q; a.k = k_cache; a.v = v_cache; a.out = o; a.part = (float*)ws;
+  strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);
+  a.pg.table = table; a.pg.seq = seq_len; a.pg.n_new = n_new; a.pg.ts = table_stride;
+  a.k_sc = (const uint8_t*)scales->k_scale; a.v_sc = (const uint8_t*)scales->v_scale;
+  for (int i = 0; i < 3; i++) { a.kss[i] = scales->k_strides[i]; a.vss[i] = scales->v_strides[i]; }
+  dlt_fastdiv_make((uint32_t)(scales->block / 16), a.mB, a.sB);
+  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged8_64(a, shape->dtype, scales->format, kind, stream) : dlt_band_paged8_128(a, shape->dtype, scales->format, kind, stream);
   return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
 }
 

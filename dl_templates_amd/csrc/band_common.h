@@ -9,6 +9,7 @@
 #pragma once
 #include "flash_dma_kernel.hpp"
 #include "kernargs.h"
+#include "page_cvt8.h"
 
 struct BandPages {          // keys and values in pages (paged calls); strides in elements
   const int32_t* table;     // [B, cols] page numbers
@@ -42,6 +43,16 @@ struct BandArgs {
   float scale_log2, grad_scale;   // grad_scale: of dQ and dK; 0 where every row sees one key, whose dS are zero but for roundings
   BandPages pg;
 };
+
+// Caches in 8 bits (page_cvt8.h): their strides are bytes
+struct Band8Args : BandArgs {
+  const uint8_t *k_sc, *v_sc;   // scales
+  int64_t kss[3], vss[3];       // page, head, block of the page
+  uint32_t mB, sB;              // division of a page's 16-token groups by those of a block
+};
+// F8: 0 16-bit numbers, 1 e4m3, 2 int8
+template <int F8> struct BandArgsOf { typedef Band8Args type; };
+template <> struct BandArgsOf<0> { typedef BandArgs type; };
 
 DLT_HD int64_t dlt_imin64(int64_t a, int64_t b) { return a < b ? a : b; }
 DLT_HD int64_t dlt_imax64(int64_t a, int64_t b) { return a > b ? a : b; }
@@ -212,6 +223,51 @@ struct BandStage {
 #pragma unroll 1
     for (int i = 0; i < NI; i++)
       if (!PAD || (int)piece(i) < npieces) dlt_copy16_to_lds(base, (uint32_t)dlt_imin(t0 + R::TPI * i, last) * sn2 + 16u * piece(i), dst + R::TPI * i * R::ROW);
+  }
+};
+
+// The same for 8-bit numbers: 16 tokens of one page HBM -> registers, and later -> LDS as 16-bit numbers, in the places that the copies above give them.  A lane has 16
+// numbers of a token.  Head dims that do not exist are written as zeros.
+template <int D, int FMT, typename TIO>
+struct BandStage8 {
+  typedef FlashDRow<D> R;
+  typedef u32x4 quad __attribute__((aligned(8)));
+  static constexpr int LPT = D / 16, TPI = 64 / LPT, NI = 16 / TPI;   // lanes of a token, tokens and number of loads
+  uint32_t off[NI];
+  int t0, c, full;   // full: 16-byte pieces that lie in the row; its last one may be half
+  bool half;
+  DLT_DEV void init(int lane, int dims, int64_t sn) {
+    t0 = lane / LPT;
+    c = lane % LPT;
+    full = dims >> 4;
+    half = (dims & 15) != 0 && c == full;
+#pragma unroll
+    for (int i = 0; i < NI; i++) off[i] = (uint32_t)(t0 + TPI * i) * (uint32_t)sn + 16u * (uint32_t)c;
+  }
+  DLT_DEV void fetch(const char* base, u32x4 (&x)[NI]) const {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      x[i] = u32x4{0u, 0u, 0u, 0u};
+      if (c < full) x[i] = *reinterpret_cast<const quad*>(base + off[i]);
+      else if (half) {
+        const u32x2 h = *reinterpret_cast<const u32x2*>(base + off[i]);
+        x[i][0] = h[0];
+        x[i][1] = h[1];
+      }
+    }
+  }
+  // tokens from `live` on are written as zeros
+  DLT_DEV void put(char* dst, const u32x4 (&x)[NI], float scale, int live) const {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      const int t = t0 + TPI * i;
+      const bool on = t < live;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const u32x4 v = cvt8_eight<FMT, TIO>(x[i][2 * u], x[i][2 * u + 1], scale);
+        lds_write16(dst + t * R::ROW + 16 * ((2 * c + u) ^ R::swz(t)), on ? v : u32x4{0u, 0u, 0u, 0u});
+      }
+    }
   }
 };
 

@@ -36,9 +36,31 @@ DLT_DEV int64_t band_key_off(const BandArgs& a, const int32_t* row, const int64_
   return page * st[0] + (in16 * 16 + (j & 15)) * st[2];
 }
 
+// A cached key or value in 8 bits, at the head's base: its numbers, the factor of their scale
+struct BandKey8 { const uint8_t* p; float scale; };
+DLT_DEV BandKey8 band_key8(const Band8Args& a, const int32_t* row, const void* base, const int64_t (&st)[3], const uint8_t* sc, const int64_t (&ss)[3], int j) {
+  int in16;
+  const int page = band_page(a.pg, row, j >> 4, in16);
+  return BandKey8{reinterpret_cast<const uint8_t*>(base) + (page * st[0] + (in16 * 16 + (j & 15)) * st[2]),
+                  cvt8_scale(sc[page * ss[0] + (int)dlt_fastdiv((uint32_t)in16, a.mB, a.sB) * ss[2]])};
+}
+template <int FMT, typename TIO>
+DLT_DEV float band_dot8(const TIO* x, const BandKey8& y, int dims) {
+  float s = 0.f;
+  for (int d = 0; d < dims; d += 8) {
+    float fx[8], fy[8];
+    const u32x2 w = *reinterpret_cast<const u32x2*>(y.p + d);
+    unpack8<TIO>(*reinterpret_cast<const u32x4*>(x + d), fx);
+    unpack8<TIO>(cvt8_eight<FMT, TIO>(w[0], w[1], y.scale), fy);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s = fmaf(fx[j], fy[j], s);
+  }
+  return s;
+}
+
 // One row again over the keys of chunks [i0, i1) that it sees: maximum (log2 units), sum, two dims of the unnormalised output
-template <typename TIO, bool PAGED, int CK>
-DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, const TIO* vb, const int32_t* pages, const BandWalk<CK>& W, int i0, int i1, int pos,
+template <typename TIO, bool PAGED, int CK, int F8 = 0>
+DLT_DEV void band_fwd_exact(const typename BandArgsOf<F8>::type& a, int h, const TIO* q, const TIO* kb, const TIO* vb, const int32_t* pages, const BandWalk<CK>& W, int i0, int i1, int pos,
                             int n_k, int lane, float& m, float& l, float (&acc)[2]) {
   m = -INFINITY;
   l = acc[0] = acc[1] = 0.f;
@@ -50,7 +72,9 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
       const bool sees = j < n_k && (CK >= 64 || lane < CK) && band_sees(pos, j, a.W, a.S);
       uint64_t todo = __builtin_amdgcn_ballot_w64(sees);
       if (todo == 0) continue;
-      const float s = sees ? band_dot(q, kb + band_key_off<PAGED>(a, pages, a.ks, j), a.dk_) * a.scale_log2 : -INFINITY;
+      float s = -INFINITY;
+      if constexpr (F8 == 0) s = sees ? band_dot(q, kb + band_key_off<PAGED>(a, pages, a.ks, j), a.dk_) * a.scale_log2 : -INFINITY;
+      else if (sees) s = band_dot8<F8 - 1, TIO>(q, band_key8(a, pages, kb, a.ks, a.k_sc + h * a.kss[1], a.kss, j), a.dk_) * a.scale_log2;
       const float m_new = fmaxf(m, band_wave_max(s));
       const float ref = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = m == -INFINITY ? 0.f : fast_exp2(m - ref);
@@ -62,15 +86,26 @@ DLT_DEV void band_fwd_exact(const BandArgs& a, const TIO* q, const TIO* kb, cons
         todo &= todo - 1;
         const float w = band_lane(p, u);
         l += w;
-        band_axpy(acc, w, vb + band_key_off<PAGED>(a, pages, a.vs, W.tok(x + u)), a.dv_, lane);
+        if constexpr (F8 == 0) band_axpy(acc, w, vb + band_key_off<PAGED>(a, pages, a.vs, W.tok(x + u)), a.dv_, lane);
+        else {
+          const BandKey8 v = band_key8(a, pages, vb, a.vs, a.v_sc + h * a.vss[1], a.vss, W.tok(x + u));
+          if (2 * lane < a.dv_) {
+            const unsigned p2 = cvt8_pair<F8 - 1, TIO>(*reinterpret_cast<const uint16_t*>(v.p + 2 * lane), v.scale, false);
+            acc[0] = fmaf(w, unpack_lo<TIO>(p2), acc[0]);
+            acc[1] = fmaf(w, unpack_hi<TIO>(p2), acc[1]);
+          }
+        }
       }
     }
 }
 
 // GR groups of NW waves own the same rows and take every GR-th chunk each; their results are joined at the end, through LDS.
-template <typename TIO, int D, int NP, int CK, int NW, int GR, bool PAGED, int PAD>
-__global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_kernel(const BandArgs a) {
-  dlt_kernargs_in<sizeof(BandArgs)>();
+// F8 (pages, GR = 1): keys and values in 8 bits.  A chunk comes through registers, becomes 16-bit numbers there, once for all rows of the workgroup, and lies in LDS as the
+// copies of a 16-bit chunk do; from there on nothing differs.
+template <typename TIO, int D, int NP, int CK, int NW, int GR, bool PAGED, int PAD, int F8 = 0>
+__global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_kernel(const typename BandArgsOf<F8>::type a) {
+  static_assert(F8 == 0 || (PAGED && GR == 1), "8-bit numbers: pages, one group of waves");
+  dlt_kernargs_in<sizeof(typename BandArgsOf<F8>::type)>();
   typedef BandBuf<D, CK> B;
   extern __shared__ __align__(16) char smem[];
   constexpr int KC = band_kc(D, PAD), VB = 2 * KC, NKB = CK / 32, OWN = 16 * NP * NW;
@@ -91,8 +126,9 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   const BandSeq sq = band_seq<PAGED>(a, b);
   const int n_rows = sq.n_q * a.G;                              // rows with a query; those behind get zeros
   const TIO* qb = reinterpret_cast<const TIO*>(a.q) + b * a.qs[0] + (int64_t)h * a.G * a.qs[1];
-  const TIO* kh = reinterpret_cast<const TIO*>(a.k) + (PAGED ? 0 : b * a.ks[0]) + h * a.ks[1];
-  const TIO* vh = reinterpret_cast<const TIO*>(a.v) + (PAGED ? 0 : b * a.vs[0]) + h * a.vs[1];
+  typedef typename std::conditional<F8 != 0, uint8_t, TIO>::type TKV;
+  const TKV* kh = reinterpret_cast<const TKV*>(a.k) + (PAGED ? 0 : b * a.ks[0]) + h * a.ks[1];
+  const TKV* vh = reinterpret_cast<const TKV*>(a.v) + (PAGED ? 0 : b * a.vs[0]) + h * a.vs[1];
   const int32_t* pages = PAGED ? a.pg.table + b * a.pg.ts : nullptr;
 
   // chunks of the block and of this share of it
@@ -106,7 +142,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   BandStage<D> stk, stv;
   stk.init(lane, a.dk_, a.ks[2]);
   stv.init(lane, a.dv_, a.vs[2]);
-  if constexpr (PAD) {
+  if constexpr (PAD && F8 == 0) {
 #pragma unroll
     for (int i = 0; i < NBUF * GR; i++) {
       flashd_zero_pads<D>(smem + i * B::BUF, CK, a.dk_ >> 3, tid, 64 * NW * GR);
@@ -163,9 +199,49 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       }
     }
   };
+  // 8-bit numbers: the wave's tokens of the chunk behind the next one are on their way in registers
+  typedef BandStage8<D, F8 == 2 ? DLT_INT8 : DLT_FP8_E4M3, TIO> S8;
+  S8 stk8, stv8;
+  u32x4 rk[NG][S8::NI], rv[NG][S8::NI];
+  int ek[NG], ev[NG];
+  Groups next8;
+  auto fetch8 = [&](const Groups& x) __attribute__((always_inline)) {
+    if constexpr (F8 != 0) {
+#pragma unroll
+      for (int u = 0; u < NG; u++) {
+        const int page = x.page[u], blk = (int)dlt_fastdiv((uint32_t)x.in16[u], a.mB, a.sB);
+        const int64_t row = 16 * x.in16[u];
+        stk8.fetch(reinterpret_cast<const char*>(kh) + (page * a.ks[0] + row * a.ks[2]), rk[u]);
+        stv8.fetch(reinterpret_cast<const char*>(vh) + (page * a.vs[0] + row * a.vs[2]), rv[u]);
+        ek[u] = a.k_sc[page * a.kss[0] + h * a.kss[1] + blk * a.kss[2]];
+        ev[u] = a.v_sc[page * a.vss[0] + h * a.vss[1] + blk * a.vss[2]];
+      }
+    }
+  };
+  auto put8 = [&](int i, char* buf) __attribute__((always_inline)) {
+    if constexpr (F8 != 0) {
+#pragma unroll
+      for (int u = 0; u < NG; u++) {
+        const int live = sq.n_k - W.tok(CK * i + wave * 16 * NG + 16 * u);   // tokens of the sequence; what lies behind them is written as zeros
+        char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
+        stk8.put(dst, rk[u], cvt8_scale(ek[u]), live);
+        stv8.put(dst + B::REG, rv[u], cvt8_scale(ev[u]), live);
+      }
+    }
+  };
   // Pages of the first chunks are looked up together: one trip to memory, not one a chunk (a token each of 8 sequences of up to 900, d = 64: 10.7 -> 10.1 us;
   // one sequence of 5000, d = 128: 10.1 -> 8.7; large grids alike).  Looked up behind the last chunk too: the table has a column for position 0.
-  if constexpr (PAGED) {
+  if constexpr (F8 != 0) {
+    stk8.init(lane, a.dk_, a.ks[2]);
+    stv8.init(lane, a.dv_, a.vs[2]);
+    const Groups x0 = lookup(i_beg), x1 = lookup(i_beg + 1);
+    next8 = lookup(i_beg + 2);
+    if (i_beg < i_end) {
+      fetch8(x0);
+      put8(i_beg, bufs);
+      if (i_beg + 1 < i_end) fetch8(x1);
+    }
+  } else if constexpr (PAGED) {
     Groups x[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) x[i] = lookup(i_beg + i * GR + grp);
@@ -209,11 +285,11 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   FlashDLane<D> L;
   flashd_lane_init(L, n, g);
 
-  swa2_wait_copies();
+  if constexpr (F8 == 0) swa2_wait_copies();
   pin_loaded(qf);
 #pragma unroll
   for (int i = 0; i < AHEAD; i++)
-    if (i_beg + i * GR + grp < i_end) settle(i_beg + i * GR + grp, bufs + i * B::BUF);
+    if (F8 == 0 && i_beg + i * GR + grp < i_end) settle(i_beg + i * GR + grp, bufs + i * B::BUF);
   __syncthreads();
 
   auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
@@ -321,6 +397,17 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   auto buf_of = [&](int i) { return bufs + (i >= NBUF ? i - NBUF : i) * B::BUF; };
   auto step = [&](auto mask_tag) __attribute__((always_inline)) {
     const int i = i_beg + it * GR + grp;
+    if constexpr (F8 != 0) {
+      // the next chunk to LDS, where the last one was; the one behind it on its way beside the products
+      if (i + 1 < i_end) put8(i + 1, buf_of(bi + 1));
+      if (i + 2 < i_end) fetch8(next8);
+      next8 = lookup(i + 3);
+      chunk(i, buf_of(bi), mask_tag);
+      bi = bi + 1 == NBUF ? 0 : bi + 1;
+      it++;
+      __syncthreads();
+      return;
+    }
     const bool more = i + AHEAD * GR < i_end;
     if (more) issue(i + AHEAD * GR, buf_of(bi + AHEAD), lookup(i + AHEAD * GR));
     if (GR == 1 || !decltype(mask_tag)::value || i < i_end) chunk(i, buf_of(bi), mask_tag);
@@ -408,7 +495,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
         const int r = wq0 + 16 * p + __builtin_ctz(todo);
         float m, l, o2[2];
-        band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
+        band_fwd_exact<TIO, PAGED, CK, F8>(a, h, band_row_ptr(qb, a.qs, a, r), reinterpret_cast<const TIO*>(kh), reinterpret_cast<const TIO*>(vh), pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
         __threadfence();   // behind the wave's own stores of the row
         if (2 * lane < a.dv_) *reinterpret_cast<float2*>(part + (int64_t)r * a.dv_ + 2 * lane) = float2{o2[0], o2[1]};
         if (lane == 0) *reinterpret_cast<float2*>(ml + 2 * r) = float2{m, l};
@@ -432,7 +519,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       for (unsigned todo = odd[p]; todo != 0; todo &= todo - 1) {
         const int w = 16 * p + __builtin_ctz(todo), r = wq0 + w;
         float m, l, o2[2];
-        band_fwd_exact<TIO, PAGED, CK>(a, band_row_ptr(qb, a.qs, a, r), kh, vh, pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
+        band_fwd_exact<TIO, PAGED, CK, F8>(a, h, band_row_ptr(qb, a.qs, a, r), reinterpret_cast<const TIO*>(kh), reinterpret_cast<const TIO*>(vh), pages, W, i_beg, i_end, sq.off + band_row(a, r).tok, sq.n_k, lane, m, l, o2);
         const float f = band_inverse(l, sq.off + band_row(a, r).tok);
 #pragma unroll
         for (int j = 0; j < 2; j++) o2[j] = low ? band_dropped<TIO>(o2[j] * f) : o2[j] * f;

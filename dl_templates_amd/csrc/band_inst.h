@@ -1,6 +1,7 @@
-// Included by band_{fwd,paged,dq,dkv}_<D>.hip with DLT_BAND_D (padded head dim) and DLT_BAND_PART (0: forward, 1: forward on pages, 2: dQ, 3: dK / dV)
+// Included by band_{fwd,paged,paged8,dq,dkv}_<D>.hip with DLT_BAND_D (padded head dim) and DLT_BAND_PART (0: forward, 1: forward on pages, 2: dQ, 3: dK / dV,
+// 4: forward on pages in 8 bits)
 // defined: kernels for one class of head dims, translation units of their own since they take long to compile.
-#if DLT_BAND_PART >= 2
+#if DLT_BAND_PART == 2 || DLT_BAND_PART == 3
 #include "band_bwd_kernel.h"
 #else
 #include "band_fwd_kernel.h"
@@ -14,8 +15,8 @@ namespace {
 constexpr int D = DLT_BAND_D;
 constexpr int band_lds(int bufs, int rows) { return bufs > rows * (2 * D + 16) ? bufs : rows * (2 * D + 16); }
 
-template <typename KernT>
-int band_go(KernT kern, const BandArgs& a, int64_t grid, int threads, int lds, int record, const char* who, hipStream_t stream) {
+template <typename KernT, typename ArgsT>
+int band_go(KernT kern, const ArgsT& a, int64_t grid, int threads, int lds, int record, const char* who, hipStream_t stream) {
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(kern), lds);
   if (rc != DLT_OK) return rc;
   dlt_timing_before(record, stream);
@@ -55,6 +56,23 @@ int DLT_BCAT(dlt_band_fwd_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind, 
 int DLT_BCAT(dlt_band_paged_, DLT_BAND_D)(const BandArgs& a, int dtype, int kind, hipStream_t stream) {
 #endif
   return dtype == DLT_BF16 ? band_fwd_np<bf16_t>(a, kind, stream) : band_fwd_np<f16_t>(a, kind, stream);
+}
+#elif DLT_BAND_PART == 4
+template <typename TIO, int NP, int F8>
+int band_fwd8(const Band8Args& a, hipStream_t stream) {
+  constexpr int lds = band_lds(band_nbuf(BandBuf<D, 64>::BUF) * BandBuf<D, 64>::BUF, 64 * NP);
+  // (pieces that do not exist are written as zeros: no kernel of its own for them but that of fewer blocks of head dims)
+  return band_go(D == 128 && dlt_imax(a.dk_, a.dv_) <= 96 ? band_fwd_kernel<TIO, D, NP, 64, 4, 1, true, D == 128 ? 2 : 0, F8> : band_fwd_kernel<TIO, D, NP, 64, 4, 1, true, 0, F8>,
+                 a, (int64_t)a.B * a.Hkv * a.nblk * a.shares, 256, lds, DLT_K_FWD, "paged8 forward launch", stream);
+}
+template <typename TIO>
+int band_fwd8_kind(const Band8Args& a, int format, int kind, hipStream_t stream) {
+  if (format == DLT_FP8_E4M3) return kind == BAND_TWO ? band_fwd8<TIO, 2, 1>(a, stream) : band_fwd8<TIO, 1, 1>(a, stream);
+  return kind == BAND_TWO ? band_fwd8<TIO, 2, 2>(a, stream) : band_fwd8<TIO, 1, 2>(a, stream);
+}
+}  // namespace
+int DLT_BCAT(dlt_band_paged8_, DLT_BAND_D)(const Band8Args& a, int dtype, int format, int kind, hipStream_t stream) {
+  return dtype == DLT_BF16 ? band_fwd8_kind<bf16_t>(a, format, kind, stream) : band_fwd8_kind<f16_t>(a, format, kind, stream);
 }
 #elif DLT_BAND_PART == 2
 template <typename TIO, int NP>

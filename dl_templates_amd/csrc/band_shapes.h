@@ -3,6 +3,7 @@
 #include "dlt_internal.hpp"
 
 struct BandArgs;
+struct Band8Args;
 constexpr int band_class(int dk, int dv) { return dk > 64 || dv > 64 ? 128 : 64; }
 // How a forward workgroup is made up: one wave's 16 rows, their keys over 4 waves; 64 rows, one block a wave, their keys over two groups of 4 waves; 64 rows on
 // 4 waves; 128 rows, two blocks a wave.  (The dQ kernel: BAND_ONE and BAND_TWO.)
@@ -11,6 +12,8 @@ int dlt_band_fwd_64(const BandArgs& a, int dtype, int kind, hipStream_t stream);
 int dlt_band_fwd_128(const BandArgs& a, int dtype, int kind, hipStream_t stream);
 int dlt_band_paged_64(const BandArgs& a, int dtype, int kind, hipStream_t stream);
 int dlt_band_paged_128(const BandArgs& a, int dtype, int kind, hipStream_t stream);
+int dlt_band_paged8_64(const Band8Args& a, int dtype, int format, int kind, hipStream_t stream);   // BAND_ONE, BAND_TWO
+int dlt_band_paged8_128(const Band8Args& a, int dtype, int format, int kind, hipStream_t stream);
 int dlt_band_bwd_q_64(const BandArgs& a, int dtype, int kind, hipStream_t stream);
 int dlt_band_bwd_q_128(const BandArgs& a, int dtype, int kind, hipStream_t stream);
 int dlt_band_bwd_kv_64(const BandArgs& a, int dtype, hipStream_t stream);

@@ -1,0 +1,204 @@
+// Pages of a cache handed to requests and taken back, from the lengths that the requests want (dlt_page_assign), for gfx950.
+//
+// With P(x) = ceil(x / page) request b needs max(P(want) - P(held), 0) pages or gives back max(P(held) - P(want), 0).  Exclusive sums of both over the requests, in
+// order, say everything else: page k of all that are needed is entry F + R - 1 - k of the stack "F free pages, then the R that come back, last request's last
+// page first", and request b is served iff its sum of needs, itself included, is at most F + R.  So every page and every slot is found by itself, from two sums, and
+// nothing is added atomically: equal calls give equal pages.
+//
+// Every workgroup forms the two sums of all requests (8 B of lengths each, from the L2) and keeps them in LDS, then takes a share of the new columns, of the
+// pages that come back and of the slots.  A table's row is read (a request that gives back) or written (one that gains), never both; the pool is read below F and
+// written from F on.  Lengths and the pool's count, which all workgroups read, are written by the last one to finish: a count of those that are done, in the
+// pool's second word, tells which that is; nobody waits.
+#include <algorithm>
+#include "dlt_internal.hpp"
+#include "kernargs.h"
+
+namespace {
+
+struct AssignArgs {
+  int32_t *table, *seq, *pool, *n_new, *slots;
+  const int32_t* want;
+  int64_t ts;
+  int32_t B, cols, page, n_pages, T;
+  uint32_t mp, sp, mt, st;   // divisions by page and T
+};
+
+struct Wish { int held, want, need, back; };
+// what request b holds and needs or gives back, in pages
+__device__ inline Wish wish_of(const AssignArgs& a, int b) {
+  Wish w;
+  const int room = a.cols * a.page;   // < 2^31
+  w.held = dlt_imax(0, dlt_imin(a.seq[b], room));
+  w.want = a.want[b];
+  w.need = w.back = 0;
+  if (w.want < 0) w.want = w.held;
+  if (w.want > room || (a.T >= 0 && w.want - w.held > a.T)) w.want = w.held;
+  const int p0 = (int)dlt_fastdiv((uint32_t)(w.held + a.page - 1), a.mp, a.sp), p1 = (int)dlt_fastdiv((uint32_t)(w.want + a.page - 1), a.mp, a.sp);
+  w.need = dlt_imax(p1 - p0, 0);
+  w.back = dlt_imax(p0 - p1, 0);
+  return w;
+}
+__device__ inline int pages_of(const AssignArgs& a, int tokens) { return (int)dlt_fastdiv((uint32_t)(tokens + a.page - 1), a.mp, a.sp); }
+
+// the last b with start[b] <= x; start[0] = 0, start[B] > x
+__device__ inline int owner_of(const int32_t* start, int B, int x) {
+  int lo = 0, hi = B;   // start[lo] <= x < start[hi]
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (start[m] <= x) lo = m;
+    else hi = m;
+  }
+  return lo;
+}
+
+struct Stack {
+  const AssignArgs& a;
+  const int32_t* back;   // exclusive sums of what comes back, [B + 1]
+  int F, R;
+  // r-th of the pages that come back: the last request's last page first
+  __device__ int returned(int r) const {
+    const int x = R - 1 - r, b = owner_of(back, a.B, x);
+    return a.table[b * a.ts + (pages_of(a, dlt_imax(a.want[b], 0)) + x - back[b])];
+  }
+  // k-th page that is taken
+  __device__ int taken(int k) const {
+    const int at = F + R - 1 - k;
+    return at < F ? a.pool[2 + at] : returned(at - F);
+  }
+};
+
+// inclusive sums of two numbers over the workgroup's threads, and their totals
+template <int NT>
+__device__ inline void scan2(int& x, int& y, int& sum_x, int& sum_y, int (*wave)[2]) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int ux = __shfl_up(x, d), uy = __shfl_up(y, d);
+    if (lane >= d) { x += ux; y += uy; }
+  }
+  if (lane == 63) { wave[w][0] = x; wave[w][1] = y; }
+  __syncthreads();
+  sum_x = sum_y = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) {
+    if (i == w) { x += sum_x; y += sum_y; }
+    sum_x += wave[i][0];
+    sum_y += wave[i][1];
+  }
+}
+
+template <int NT>
+__global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
+  dlt_kernargs_in<sizeof(AssignArgs)>();
+  extern __shared__ int32_t sums[];   // needs [B + 1], back [B + 1]
+  __shared__ int wave[NT / 64][2], most[NT / 64], last;
+  int32_t *need = sums, *back = sums + a.B + 1;
+  const int tid = threadIdx.x;
+
+  // sums of needs and of what comes back: a run of requests to a thread
+  const int per = (a.B + NT - 1) / NT, b0 = dlt_imin(tid * per, a.B), b1 = dlt_imin(b0 + per, a.B);
+  int n = 0, r = 0, sum_n, sum_r;
+  for (int b = b0; b < b1; b++) {
+    const Wish w = wish_of(a, b);
+    n += w.need;
+    r += w.back;
+  }
+  const int own_n = n, own_r = r;
+  const int F = dlt_imax(0, dlt_imin(a.pool[0], a.n_pages));
+  scan2<NT>(n, r, sum_n, sum_r, wave);
+  n -= own_n;
+  r -= own_r;
+  const int64_t room = (int64_t)F + sum_r;
+  int served = 0;   // pages taken
+  for (int b = b0; b < b1; b++) {
+    const Wish w = wish_of(a, b);
+    need[b] = n;
+    back[b] = r;
+    n += w.need;
+    r += w.back;
+    if (w.need > 0 && n <= room) served = n;
+  }
+  if (tid == 0) {
+    need[a.B] = sum_n;
+    back[a.B] = sum_r;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) served = dlt_imax(served, __shfl_xor(served, d));
+  if ((tid & 63) == 0) most[tid >> 6] = served;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) served = dlt_imax(served, most[i]);
+  const int left = (int)(room - served < a.n_pages ? room - served : a.n_pages);
+  const Stack stack{a, back, F, sum_r};
+  const int64_t at0 = (int64_t)blockIdx.x * NT + tid, step = (int64_t)gridDim.x * NT;
+
+  for (int64_t k = at0; k < served; k += step) {
+    const int b = owner_of(need, a.B, (int)k);
+    a.table[b * a.ts + (pages_of(a, wish_of(a, b).held) + (int)k - need[b])] = stack.taken((int)k);
+  }
+  for (int64_t i = at0; F + i < left; i += step) a.pool[2 + F + i] = stack.returned((int)i);
+  auto gain_of = [&](int b, const Wish& w) { return w.want > w.held && (w.need == 0 || need[b] + w.need <= room) ? w.want - w.held : 0; };
+  for (int64_t b = at0; b < a.B; b += step) a.n_new[b] = gain_of((int)b, wish_of(a, (int)b));
+  const int64_t slots = a.T > 0 ? (int64_t)a.B * a.T : 0;
+  for (int64_t i = at0; i < slots; i += step) {
+    const int b = (int)dlt_fastdiv((uint32_t)i, a.mt, a.st), t = (int)i - b * a.T;
+    const Wish w = wish_of(a, b);
+    int slot = -1;
+    if (t < gain_of(b, w)) {
+      const int p = w.held + t, col = (int)dlt_fastdiv((uint32_t)p, a.mp, a.sp), p0 = pages_of(a, w.held);
+      const int page = col < p0 ? a.table[b * a.ts + col] : stack.taken(need[b] + col - p0);
+      slot = page * a.page + (p - col * a.page);
+    }
+    a.slots[i] = slot;
+  }
+
+  if (gridDim.x > 1) {
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) last = atomicAdd(&a.pool[1], 1) == (int)gridDim.x - 1;
+    __syncthreads();
+    if (!last) return;
+    __threadfence();
+  } else {
+    __syncthreads();
+  }
+  for (int b = b0; b < b1; b++) {
+    const Wish w = wish_of(a, b);
+    const int now = w.want < w.held ? w.want : w.held + gain_of(b, w);
+    if (now != w.held) a.seq[b] = now;
+  }
+  if (tid == 0) {
+    a.pool[0] = left;
+    if (gridDim.x > 1) a.pool[1] = 0;
+  }
+}
+
+}  // namespace
+
+extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* seq_len, const int32_t* want, int32_t* pool, int32_t B, int32_t cols, int32_t page,
+                               int32_t n_pages, int32_t T, int32_t* n_new, int32_t* slots, void* stream_) {
+  const char* who = "page_assign";
+  hipStream_t stream = (hipStream_t)stream_;
+  DLT_REQUIRE(B >= 0 && cols > 0 && page > 0 && n_pages > 0 && T >= -1, "%s: B=%d cols=%d page=%d n_pages=%d T=%d", who, B, cols, page, n_pages, T);
+  if (B > DLT_ASSIGN_MAX) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: %d requests, at most %d are supported", who, B, DLT_ASSIGN_MAX);
+  if ((int64_t)B * cols > 0x3fffffff || (int64_t)cols * page > 0x3fffffff || n_pages > 0x3fffffff || (int64_t)n_pages * page > 0x7fffffff || (int64_t)B * T > 0x7fffffff)
+    return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many pages or tokens", who);
+  if (B == 0) return DLT_OK;
+  DLT_REQUIRE(table != nullptr && seq_len != nullptr && want != nullptr && pool != nullptr && n_new != nullptr && (slots != nullptr || T <= 0), "%s: a tensor is NULL", who);
+  DLT_REQUIRE(B == 1 || table_stride >= cols, "%s: rows of the table overlap (stride %lld, %d columns)", who, (long long)table_stride, cols);
+  AssignArgs a{};
+  a.table = table; a.seq = seq_len; a.pool = pool; a.n_new = n_new; a.slots = slots; a.want = want; a.ts = table_stride;
+  a.B = B; a.cols = cols; a.page = page; a.n_pages = n_pages; a.T = T;
+  dlt_fastdiv_make((uint32_t)page, a.mp, a.sp);
+  dlt_fastdiv_make((uint32_t)dlt_imax(T, 1), a.mt, a.st);
+  constexpr int NT = 256;
+  // slots, and columns that requests can gain at most
+  const int64_t work = (int64_t)B * dlt_imax(T, 1) + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work / (4 * NT), dlt_device_cus()));
+  const int lds = 2 * (B + 1) * 4;
+  const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
+  if (rc != DLT_OK) return rc;
+  hipLaunchKernelGGL(page_assign_kernel<NT>, dim3((unsigned)grid), dim3(NT), lds, stream, a);
+  DLT_CHECK_LAUNCH("page_assign launch");
+  return DLT_OK;
+}

@@ -27,6 +27,40 @@ DLT_HD int rope_axes_axis(const RopeAxes& r, int i, int& off, int& R) {
   return a;
 }
 
+// y0 = x0 c - x1 s, y1 = x0 s + x1 c
+__device__ inline float mix(float x, float c, float other, float s) {
+#pragma clang fp contract(off)
+  const float a = x * c, b = other * s;
+  return a + b;
+}
+
+// Rows of the tables for token t_ of sequence b at `place` in it (of row 0 where it has no position, so that loads need no branch), bit a of `on`: axis a turns it
+struct TableRows { const float* p[DLT_ROPE_AXES_MAX]; unsigned on; };
+__device__ inline TableRows table_rows(const RopeAxes& r, int b, int t_, int place, bool live) {
+  TableRows t;
+  t.on = 0;
+  int pos[DLT_ROPE_AXES_MAX];
+#pragma unroll
+  for (int a = 0; a < DLT_ROPE_AXES_MAX; a++) pos[a] = r.pos == nullptr ? place : a < r.n ? r.pos[a * r.pa + b * r.pb + t_ * r.pn] : -1;
+#pragma unroll
+  for (int a = 0; a < DLT_ROPE_AXES_MAX; a++) {
+    t.p[a] = r.tab[a] + dlt_imax(dlt_imin(pos[a], r.len[a] - 1), 0) * r.ts[a];
+    t.on |= (a < r.n && pos[a] >= 0 && live ? 1u : 0u) << a;
+  }
+  return t;
+}
+// row of a pair's axis, at the pair; its bit of `on`
+__device__ inline const float* pair_row(const RopeAxes& r, const TableRows& t, int pair, bool& on) {
+  const float* row = t.p[0];
+  unsigned bit = 1;
+  int off = 0;
+#pragma unroll
+  for (int a = 1; a < DLT_ROPE_AXES_MAX; a++)
+    if (a < r.n && pair >= r.end[a - 1]) { row = t.p[a]; off = r.end[a - 1]; bit = 1u << a; }
+  on = (t.on & bit) != 0;
+  return row + 2 * (pair - off);
+}
+
 // One call of the kernels in rope_axes.hip: rows of up to three tensors, token by token
 struct RotStream {
   const void* src;

@@ -16,13 +16,6 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 template <typename T> struct alignas(16) Vec8 { T v[8]; };
 
-// y0 = x0 c - x1 s, y1 = x0 s + x1 c
-__device__ inline float mix(float x, float c, float other, float s) {
-#pragma clang fp contract(off)
-  const float a = x * c, b = other * s;
-  return a + b;
-}
-
 // N elements from any address of the element's alignment
 template <int N, typename T>
 __device__ inline void load_run(T* v, const T* p) { __builtin_memcpy(v, p, N * sizeof(T)); }
@@ -115,35 +108,9 @@ DLT_HD int parts_of(const RopeAxes& r, int C) {
   return n;
 }
 
-// Rows of the tables for a token (of row 0 where it has no position, so that loads need no branch), bit a of `on`: axis a turns it
-struct TableRows { const float* p[DLT_ROPE_AXES_MAX]; unsigned on; };
-__device__ inline TableRows table_rows(const RopeAxes& r, const Token& k) {
-  TableRows t;
-  t.on = 0;
-  int pos[DLT_ROPE_AXES_MAX];
-#pragma unroll
-  for (int a = 0; a < DLT_ROPE_AXES_MAX; a++) pos[a] = r.pos == nullptr ? k.place : a < r.n ? r.pos[a * r.pa + k.b * r.pb + k.t * r.pn] : -1;
-#pragma unroll
-  for (int a = 0; a < DLT_ROPE_AXES_MAX; a++) {
-    t.p[a] = r.tab[a] + dlt_imax(dlt_imin(pos[a], r.len[a] - 1), 0) * r.ts[a];
-    t.on |= (a < r.n && pos[a] >= 0 && k.live ? 1u : 0u) << a;
-  }
-  return t;
-}
-// row of a pair's axis, at the pair; its bit of `on`
-__device__ inline const float* pair_row(const RopeAxes& r, const TableRows& t, int pair, bool& on) {
-  const float* row = t.p[0];
-  unsigned bit = 1;
-  int off = 0;
-#pragma unroll
-  for (int a = 1; a < DLT_ROPE_AXES_MAX; a++)
-    if (a < r.n && pair >= r.end[a - 1]) { row = t.p[a]; off = r.end[a - 1]; bit = 1u << a; }
-  on = (t.on & bit) != 0;
-  return row + 2 * (pair - off);
-}
 // (cos, sin) of a part's pairs, by slots; bit j of the result: slot j is rotated
 __device__ inline unsigned cos_sin(const RopeAxes& r, const Token& k, const RotPart& x, float (&c)[8], float (&s)[8]) {
-  const TableRows t = table_rows(r, k);
+  const TableRows t = table_rows(r, k.b, k.t, k.place, k.live);
   if (t.on == 0) return 0;
   float2 v[8];
   unsigned turn = 0;
@@ -331,7 +298,7 @@ __global__ __launch_bounds__(256) void rotate_rows_lds_kernel(RotArgs a, int par
   if (early) fetch(a.s[0], lo, hi);
 
   const Token k = token_of(a, b, t);
-  const TableRows rows = table_rows(a.r, k);
+  const TableRows rows = table_rows(a.r, k.b, k.t, k.place, k.live);
   float c[8], s[8];
   int other[8];
   unsigned turn = 0;
@@ -423,7 +390,7 @@ __global__ __launch_bounds__(256) void rotate_single_kernel(RotArgs a) {
   if (i < P) {
     int off, R;
     rope_axes_axis(a.r, i, off, R);
-    const float* row = pair_row(a.r, table_rows(a.r, k), i, turn);
+    const float* row = pair_row(a.r, table_rows(a.r, k.b, k.t, k.place, k.live), i, turn);
     c = row[0];
     s = a.r.inverse ? -row[1] : row[1];
     d0 = a.r.halves ? i : i + off;

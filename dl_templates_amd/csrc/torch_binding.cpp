@@ -830,7 +830,8 @@ struct Paged {
   const int32_t *table = nullptr, *seq = nullptr, *n_new = nullptr;
   int64_t ts = 0;
 };
-Paged paged_args(const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor* n_new, int64_t B, int64_t T, int64_t H) {
+// dtype: of the new tokens (-1: the cache's)
+Paged paged_args(const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& seq, const Tensor* n_new, int64_t B, int64_t T, int64_t H, int dtype = -1) {
   check_assert(kc.dim() == 4 && vc.dim() == 4 && kc.sizes().slice(0, 3) == vc.sizes().slice(0, 3), "caches must have shape [pages, heads, page, D], all but D alike");
   check_assert(kc.scalar_type() == vc.scalar_type(), "caches must have one dtype");
   require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), PyExc_TypeError,
@@ -853,7 +854,7 @@ Paged paged_args(const Tensor& kc, const Tensor& vc, const Tensor& table, const 
   p.s.B = (int32_t)B; p.s.H = (int32_t)H; p.s.Hkv = (int32_t)kc.size(1); p.s.T = (int32_t)T;
   p.s.dk = (int32_t)kc.size(3); p.s.dv = (int32_t)vc.size(3);
   p.s.page = (int32_t)kc.size(2); p.s.n_pages = (int32_t)kc.size(0); p.s.cols = (int32_t)table.size(1);
-  p.s.dtype = dtype_code(kc);
+  p.s.dtype = dtype < 0 ? dtype_code(kc) : dtype;
   return p;
 }
 
@@ -1213,6 +1214,161 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Caches of 8-bit numbers [pages, heads, page, D] and their scales [pages, heads, page / block]
+dlt_scales8_t scales_of(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs) {
+  require((kc.scalar_type() == at::kFloat8_e4m3fn || kc.scalar_type() == at::kChar) && vc.scalar_type() == kc.scalar_type(), PyExc_TypeError,
+          "caches must be float8_e4m3fn or int8, both alike");
+  require(ks.scalar_type() == at::kFloat8_e8m0fnu && vs.scalar_type() == at::kFloat8_e8m0fnu, PyExc_TypeError, "scales must be float8_e8m0fnu");
+  check_assert(kc.dim() == 4 && vc.dim() == 4, "caches must have shape [pages, heads, page, D], all but D alike");
+  check_assert(ks.dim() == 3 && vs.dim() == 3 && ks.sizes() == vs.sizes() && ks.sizes().slice(0, 2) == kc.sizes().slice(0, 2), "scales must have shape [pages, heads, blocks of a page]");
+  require(ks.size(2) > 0 && kc.size(2) % ks.size(2) == 0, PyExc_ValueError, "the blocks of a page must have one size");
+  require_gpu(kc, ks, vs);
+  dlt_scales8_t x{};
+  x.format = kc.scalar_type() == at::kChar ? DLT_INT8 : DLT_FP8_E4M3;
+  x.block = (int32_t)(kc.size(2) / ks.size(2));
+  x.k_scale = const_cast<void*>(ks.const_data_ptr());
+  x.v_scale = const_cast<void*>(vs.const_data_ptr());
+  for (int i = 0; i < 3; i++) {
+    x.k_strides[i] = ks.size(i) == 1 ? 0 : ks.stride(i);
+    x.v_strides[i] = vs.size(i) == 1 ? 0 : vs.stride(i);
+  }
+  return x;
+}
+// rows of 8-bit numbers that the kernels can read in 8-byte pieces
+bool rows8(const Tensor& x) {
+  bool ok = (x.stride(3) == 1 || x.size(3) == 1) && (uintptr_t)x.const_data_ptr() % 8 == 0;
+  for (int i = 0; i < 3; i++) ok = ok && (x.size(i) == 1 || (x.stride(i) % 8 == 0 && x.stride(i) >= 0));
+  return ok;
+}
+// rows in 16-byte pieces, else a copy
+Tensor as_pieces(const Tensor& x) {
+  if (x.dim() != 4 || x.numel() == 0) return x;
+  const int64_t n = 16 / (int64_t)x.element_size();
+  bool ok = (x.stride(3) == 1 || x.size(3) == 1) && (uintptr_t)x.const_data_ptr() % 16 == 0;
+  for (int i = 0; i < 3; i++) ok = ok && (x.size(i) == 1 || x.stride(i) % n == 0);
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+
+// (k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_len, n_new or None, pos or None, tables or None, layout number, q or None, any call or plain ones only) -> rotated q or None
+PyObject* py_paged8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 14, 14);
+  const Tensor &kc = tensor_arg(a[0]), &vc = tensor_arg(a[1]), &ks = tensor_arg(a[2]), &vs = tensor_arg(a[3]), &k0 = tensor_arg(a[4]), &v0 = tensor_arg(a[5]), &table = tensor_arg(a[6]),
+               &seq = tensor_arg(a[7]);
+  const Tensor n_new = a[8] == Py_None ? Tensor() : tensor_arg(a[8]), q0 = a[12] == Py_None ? Tensor() : tensor_arg(a[12]);
+  const bool rope = a[10] != Py_None;
+  Axes t;
+  if (rope) t = axes_arg(a[9], a[10], a[11]);
+  for (const Tensor* c : {&kc, &vc, &ks, &vs}) torch::autograd::check_inplace(*c, torch::autograd::compute_requires_grad(*c));
+  if (!bool_arg(a[13]) && !(plain(kc, vc, ks, vs, k0, v0, table, seq) && plain_each(n_new, q0) && plain_axes(t))) Py_RETURN_NOTIMPLEMENTED;
+  check_assert(k0.dim() == 4 && v0.dim() == 4 && k0.sizes().slice(0, 3) == v0.sizes().slice(0, 3), "k and v must have shape [B, heads, T, D], all but D alike");
+  dlt_scales8_t scales = scales_of(kc, vc, ks, vs);
+  check_assert(k0.size(1) == kc.size(1) && k0.size(3) == kc.size(3) && v0.size(3) == vc.size(3), "k and v must match their caches");
+  check_assert(k0.scalar_type() == v0.scalar_type(), "k and v must have one dtype");
+  check_assert(!q0.defined() || (q0.dim() == 4 && q0.size(0) == k0.size(0) && q0.size(2) == k0.size(2) && q0.size(3) == k0.size(3) && q0.scalar_type() == k0.scalar_type()),
+               "q must match k");
+  Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, k0.size(0), k0.size(2), q0.defined() ? q0.size(1) : 0, dtype_code(k0));
+  require_gpu(kc, k0, v0);
+  if (q0.defined()) require_gpu(kc, q0);
+  require(rows8(kc) && rows8(vc), PyExc_ValueError, "rows of the caches must be contiguous and start at multiples of 8 bytes");
+  const std::pair<const Tensor*, const char*> written[] = {{&kc, "k_cache"}, {&vc, "v_cache"}, {&ks, "k_scale"}, {&vs, "v_scale"}};
+  for (const auto& w : written) check_written(*w.first, w.second);
+  for (int i = 0; i < 4; i++)
+    for (int j = i + 1; j < 4; j++) check_two(*written[i].first, *written[j].first, "the caches and their scales");
+  Tensor q_out;
+  if (q0.defined()) {
+    c10::DeviceGuard guard(kc.device());
+    q_out = empty(q0.sizes(), q0.scalar_type(), q0);
+  }
+  if (p.s.B > 0) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::DeviceGuard guard(kc.device());
+    const Tensor k = as_pieces(k0), v = as_pieces(v0), q = q0.defined() ? as_pieces(q0) : q0;
+    dlt_rope_axes_t d;
+    if (rope) make_axes(t, k.size(0), k.size(2), kc, d);
+    check_rc(dlt_paged8_append(k.const_data_ptr(), st16(k).data(), v.const_data_ptr(), st16(v).data(), q.defined() ? q.const_data_ptr() : nullptr,
+                               q.defined() ? st16(q).data() : nullptr, q.defined() ? q_out.mutable_data_ptr() : nullptr, q.defined() ? st16(q_out).data() : nullptr,
+                               kc.mutable_data_ptr(), st16(kc).data(), vc.mutable_data_ptr(), st16(vc).data(), &scales, p.table, p.ts, p.seq, p.n_new, rope ? &d : nullptr, &p.s,
+                               stream_of(kc)));
+  }
+  for (const auto& w : written) torch::autograd::increment_version(*w.first);
+  if (!q_out.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(q_out);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, v_cache, k_scale, v_scale, page_table, seq_len, window or None, n_sink, scale, n_new or None, any call or plain ones only) -> o, no graph
+PyObject* py_paged8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 12, 12);
+  const Tensor &q0 = tensor_arg(a[0]), &kc = tensor_arg(a[1]), &vc = tensor_arg(a[2]), &ks = tensor_arg(a[3]), &vs = tensor_arg(a[4]), &table = tensor_arg(a[5]), &seq = tensor_arg(a[6]);
+  const Tensor n_new = a[10] == Py_None ? Tensor() : tensor_arg(a[10]);
+  if (!bool_arg(a[11]) && !(plain(q0, kc, vc, ks, vs, table, seq) && plain_each(n_new))) Py_RETURN_NOTIMPLEMENTED;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const dlt_scales8_t scales = scales_of(kc, vc, ks, vs);
+  check_assert(q0.dim() == 4 && q0.size(3) == kc.size(3), "q must have shape [B, heads, T, D] and match the cache");
+  Paged p = paged_args(kc, vc, table, seq, n_new.defined() ? &n_new : nullptr, q0.size(0), q0.size(2), q0.size(1), dtype_code(q0));
+  p.s.window = window_arg(a[7]);
+  p.s.n_sink = (int32_t)int_arg(a[8]);
+  p.s.sm_scale = (float)float_arg(a[9]);
+  require_gpu(kc, q0);
+  require(rows8(kc) && rows8(vc), PyExc_ValueError, "rows of the caches must be contiguous and start at multiples of 8 bytes");
+  c10::DeviceGuard guard(kc.device());
+  Tensor o = empty({q0.size(0), q0.size(1), q0.size(2), vc.size(3)}, q0.scalar_type(), q0);
+  if (o.numel() == 0) return THPVariable_Wrap(o);
+  const Tensor q = as_rows16(q0, group_of(q0, kc));
+  Workspace ws;
+  check_rc(dlt_paged8_workspace(&p.s, &scales, &ws.bytes));
+  if (ws.bytes > 0) {
+    ws.t = empty({ws.bytes / 4}, at::kFloat, q);
+    ws.ptr = ws.t.mutable_data_ptr();
+  }
+  check_rc(dlt_paged8_attn(q.const_data_ptr(), st16(q).data(), kc.const_data_ptr(), st16(kc).data(), vc.const_data_ptr(), st16(vc).data(), &scales, o.mutable_data_ptr(),
+                           st16(o).data(), p.table, p.ts, p.seq, p.n_new, &p.s, ws.ptr, ws.bytes, stream_of(q)));
+  return THPVariable_Wrap(o);
+  END_HANDLE_TH_ERRORS
+}
+
+// (page_table, seq_len, want, pool, page, n_tokens or None, any call or plain ones only) -> (n_new, slots or None)
+PyObject* py_page_assign(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 7, 7);
+  const Tensor &table = tensor_arg(a[0]), &seq = tensor_arg(a[1]), &want = tensor_arg(a[2]), &pool = tensor_arg(a[3]);
+  if (!bool_arg(a[6]) && !plain(table, seq, want, pool)) Py_RETURN_NOTIMPLEMENTED;
+  const int64_t page = int_arg(a[4]), T = a[5] == Py_None ? -1 : int_arg(a[5]);
+  auto ints = [](const Tensor& x) { return x.scalar_type() == at::kInt && x.dim() == 1 && (x.size(0) <= 1 || x.stride(0) == 1); };
+  require(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1), PyExc_TypeError,
+          "page_table must be an int32 tensor [B, pages of a sequence] with contiguous rows");
+  require(ints(seq) && ints(want), PyExc_TypeError, "seq_len and want must be contiguous 1-D int32 tensors");
+  require(ints(pool) && pool.size(0) > 2, PyExc_TypeError, "pool must be a contiguous 1-D int32 tensor [2 + pages]");
+  const int64_t B = table.size(0);
+  check_assert(seq.size(0) == B && want.size(0) == B, "page_table, seq_len and want must have a row for every request");
+  require(T >= 0 || a[5] == Py_None, PyExc_ValueError, "n_tokens must not be negative");
+  require(page > 0 && table.size(1) > 0, PyExc_ValueError, "pages need a token, and the table a column");
+  check_assert(B <= INT32_MAX && table.size(1) <= INT32_MAX && pool.size(0) <= INT32_MAX, "too many requests or pages");
+  require_gpu(table, seq, want, pool);
+  check_written(table, "page_table");
+  check_written(seq, "seq_len");
+  check_two(table, seq, "page_table and seq_len");
+  check_two(table, pool, "page_table and pool");
+  check_two(seq, pool, "seq_len and pool");
+  for (const Tensor* x : {&table, &seq, &pool}) require(!meet(want, *x), PyExc_RuntimeError, "want shares memory with a tensor that is written");
+  Tensor n_new, slots;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    c10::DeviceGuard guard(table.device());
+    n_new = empty({B}, at::kInt, table);
+    if (a[5] != Py_None) slots = empty({B, T}, at::kInt, table);
+    check_rc(dlt_page_assign(table.mutable_data_ptr<int32_t>(), table.size(0) > 1 ? table.stride(0) : table.size(1), seq.mutable_data_ptr<int32_t>(), want.const_data_ptr<int32_t>(),
+                             pool.mutable_data_ptr<int32_t>(), (int32_t)B, (int32_t)table.size(1), (int32_t)page, (int32_t)(pool.size(0) - 2), (int32_t)T,
+                             n_new.mutable_data_ptr<int32_t>(), slots.defined() && slots.numel() > 0 ? slots.mutable_data_ptr<int32_t>() : nullptr, stream_of(table)));
+  }
+  for (const Tensor* x : {&table, &seq, &pool}) torch::autograd::increment_version(*x);
+  if (!slots.defined()) return Py_BuildValue("(NO)", THPVariable_Wrap(n_new), Py_None);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(n_new), THPVariable_Wrap(slots));
+  END_HANDLE_TH_ERRORS
+}
+
 // (x[B', N, C], idx, row, col): rotated in place, returned
 PyObject* py_rope_apply(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -1298,7 +1454,7 @@ PyObject* py_pad_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define DLT_FN(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef METHODS[] = {DLT_FN(tiled_swa), DLT_FN(tiled_swa_fwd), DLT_FN(tiled_swa_rope), DLT_FN(tiled_swa_image), DLT_FN(flash), DLT_FN(swa_forward),
                          DLT_FN(swa_backward), DLT_FN(image_forward), DLT_FN(image_backward), DLT_FN(flash_forward), DLT_FN(flash_backward), DLT_FN(rope_apply), DLT_FN(rope_heads), DLT_FN(rope_inplace), DLT_FN(rope_pair),
-                         DLT_FN(pad_plan), DLT_FN(window), DLT_FN(window_forward), DLT_FN(window_backward), DLT_FN(rope_axes), DLT_FN(paged_append), DLT_FN(paged_attention),
+                         DLT_FN(pad_plan), DLT_FN(window), DLT_FN(window_forward), DLT_FN(window_backward), DLT_FN(rope_axes), DLT_FN(paged_append), DLT_FN(paged_attention), DLT_FN(page_assign), DLT_FN(paged8_append), DLT_FN(paged8_attention),
                          {nullptr, nullptr, 0, nullptr}};
 #undef DLT_FN
 

@@ -366,6 +366,50 @@ int dlt_paged_attn(const void* q, const int64_t q_strides[4], const void* k_cach
                    const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
                    const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
 
+/* ---- the same cache held in 8 bits ----------------------------------------------------------------
+ * Caches of 8-bit numbers c with a scale for each block of `block` tokens and head: the cache holds c times the scale of its block.  Scales are bytes, powers of two:
+ * byte e stands for 2^(e - 127), 255 for NaN; scale of page p, head h, block i of the page (rows i block .. (i + 1) block - 1) by strides[3].  A block is a
+ * multiple of 16 tokens, at most DLT_BLOCK8_MAX, that divides the page. */
+enum { DLT_FP8_E4M3 = 0, DLT_INT8 = 1 };   /* formats: OCP e4m3 (largest number 448, no infinities); whole numbers -127 .. 127 */
+#define DLT_BLOCK8_MAX 128
+typedef struct {
+  int32_t format, block;
+  void *k_scale, *v_scale;
+  int64_t k_strides[3], v_strides[3];   /* page, head, block of the page */
+} dlt_scales8_t;
+
+/* dlt_paged_append into such a cache.  Per block, head and tensor: e_need is the least e with |x| <= M 2^e for all of its new tokens' finite elements (M = 448, 127; -100
+ * at least), rotated in 32 bits; a block whose first token is new takes e_need, another the larger of its e and e_need, and where that is larger its older tokens'
+ * numbers are rounded anew.  Numbers are x 2^-e rounded to nearest, even ones at ties, and so bounded that DLT_FP16 inputs come back finite in fp16.  An element
+ * that is infinite or NaN becomes NaN: a number of e4m3, for int8 the scale of its block, which then stays NaN until the block's first token is new again.
+ * dk and dv multiples of 8 up to 128; rows of k, v, q, q_out, k_cache and v_cache contiguous, those of k, v, q and q_out at multiples of 16 bytes, of the caches at
+ * multiples of 8. */
+int dlt_paged8_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                      const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4],
+                      void* k_cache, const int64_t k_cache_strides[4], void* v_cache, const int64_t v_cache_strides[4],
+                      const dlt_scales8_t* scales, const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
+                      const dlt_rope_axes_t* rope, const dlt_paged_shape_t* shape, void* stream);
+
+/* dlt_paged_attn over such a cache: keys and values are read as numbers of q's type.  Cache rows contiguous, at multiples of 8 bytes. */
+int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes);
+int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4],
+                    const void* v_cache, const int64_t v_cache_strides[4], const dlt_scales8_t* scales, void* o, const int64_t o_strides[4],
+                    const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
+                    const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---- pages handed to requests ------------------------------------------------------------------
+ * pool: int32 [2 + n_pages], {number of free pages, 0 between calls, the free pages' numbers}.  Request b holds seq_len[b] tokens and wants want[b]: pages behind
+ * ceil(want / page) go back to the pool; what it lacks comes from there; want[b] < 0 leaves it alone.  Requests are served in order of b while the pool, with what
+ * came back in the same call, holds the pages of all that asked so far; from the first that it does not, requests that need a page get nothing and keep
+ * seq_len[b].  So do requests that want more than cols pages hold or, with T >= 0, more than T tokens more.  seq_len, table and pool are brought up to date in
+ * place (table: the columns of new pages), n_new[b] is how many tokens request b gained.  With T > 0 slots[b, t] (contiguous [B, T]) is the place of its new token t, page
+ * number times page plus the row, -1 where there is none.  Pages are taken from the top of the pool in order of request and column and put back in the opposite
+ * order, so a call that takes back what the last one gave leaves the pool as it was.  B at most DLT_ASSIGN_MAX; B * cols, cols * page and n_pages below 2^30, n_pages * page and
+ * B * T below 2^31.  Calls on one pool must not overlap. */
+#define DLT_ASSIGN_MAX 8192
+int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* seq_len, const int32_t* want, int32_t* pool, int32_t B, int32_t cols, int32_t page,
+                    int32_t n_pages, int32_t T, int32_t* n_new, int32_t* slots, void* stream);
+
 /* ---- per-kernel timing (measurement aid) ---------------------------------------------------
  * Counterpart of the reference's triton.testing.do_bench calls (src/tiled_swa.py:765-774,
  * src/flash_attn.py:592,606), at kernel granularity.  While enabled for the calling thread,
@@ -389,7 +433,7 @@ int dlt_debug_copy(void* dst, const void* src, int64_t bytes, void* stream);
  * autotuning, src/tiled_swa.py:570-573); here the host routes every call by shape, element type, strides and
  * alignment, and a C caller cannot see from the outside that, say, head dim 80 or a 9-token tile at head dim 96 lands on the
  * generic kernels (several times slower than the tuned ones).  dlt_last_kernel_family() returns the family the calling
- * thread's latest forward / backward call (dlt_swa_*, dlt_flash_*, dlt_window_*, dlt_paged_attn) was routed to.  With dlt_dry_run(1) (per thread) those
+ * thread's latest forward / backward call (dlt_swa_*, dlt_flash_*, dlt_window_*, dlt_paged_attn, dlt_paged8_attn) was routed to.  With dlt_dry_run(1) (per thread) those
  * calls validate their arguments and route, but launch nothing and touch no memory: pointers only need the alignment
  * of the real ones, so the query also works in a process without a GPU.
  *   MARCHING  token grids (b_size 1), head dim 32, windows up to 21 x 21, and 64, up to 13 x 13 (rotation: head dim 64, 8 rotary pairs, in
@@ -401,7 +445,7 @@ int dlt_debug_copy(void* dst, const void* src, int64_t bytes, void* stream);
  *   TILE      token grids, head dims in multiples of 32 up to 128, windows up to 21 columns (rotation in the tile loads)
  *   FLASH     dense / causal / tiles of 16 k tokens, 2-byte element types, head dims up to 128 (multiples of 8)
  *   GENERIC   everything else
- *   BAND      dlt_window_*, dlt_paged_attn */
+ *   BAND      dlt_window_*, dlt_paged_attn, dlt_paged8_attn */
 enum { DLT_FAMILY_NONE = 0, DLT_FAMILY_MARCHING = 1, DLT_FAMILY_STREAMING = 2, DLT_FAMILY_TILE = 3, DLT_FAMILY_FLASH = 4,
        DLT_FAMILY_GENERIC = 5, DLT_FAMILY_BAND = 6 };
 int dlt_dry_run(int on);

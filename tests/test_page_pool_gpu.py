@@ -1,0 +1,120 @@
+"""Pages handed to requests and taken back, against a loop over the requests (GPU)."""
+import random
+
+import pytest
+import torch
+
+from dl_templates_amd.page_pool import page_assign_, page_pool
+from tests import paged8_oracle as orc
+
+pytestmark = pytest.mark.gpu
+ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+
+
+class Both:
+    """The device's state and the loop's."""
+
+    def __init__(self, B, cols, page, n_pages):
+        self.page, self.n = page, n_pages
+        self.table, self.seq, self.free = [[7] * cols for _ in range(B)], [0] * B, list(range(n_pages - 1, -1, -1))
+        self.dev = [ints(self.table), ints(self.seq), page_pool(n_pages)]
+
+    def call(self, want, T=None):
+        n_new, slots = page_assign_(self.dev[0], self.dev[1], ints(want), self.dev[2], self.page, T)
+        w_new, w_slots = orc.assign(self.table, self.seq, want, self.free, self.page, T)
+        assert n_new.tolist() == w_new
+        assert (slots is None) == (T is None)
+        if T is not None:
+            assert slots.shape == (len(want), T) and slots.tolist() == w_slots
+        self.same()
+        return n_new
+
+    def same(self):
+        table, seq, pool = self.dev
+        assert seq.tolist() == self.seq and table.tolist() == self.table
+        assert pool[:2].tolist() == [len(self.free), 0] and pool[2:2 + len(self.free)].tolist() == self.free
+        held = [p for b, n in enumerate(self.seq) for p in self.table[b][:-(-n // self.page)]] + self.free
+        assert sorted(held) == list(range(self.n))
+
+
+# B, cols, page, pages of the pool, largest number of new tokens
+CASES = [(1, 1, 1, 1, 1), (1, 5, 16, 5, 80), (3, 4, 7, 5, 9), (64, 64, 64, 900, 1), (65, 9, 16, 300, 40), (257, 40, 3, 4000, 100), (700, 12, 16, 5000, 150), (8192, 2, 16, 9000, 3),
+         (1, 3000, 16, 2500, 40000), (5, 1000, 1, 3000, 900)]
+
+
+@pytest.mark.parametrize("case", CASES, ids=str)
+def test_against_a_loop(case):
+    B, cols, page, n, most = case
+    rng = random.Random(str(case))
+    s = Both(B, cols, page, n)
+    for step in range(8):
+        want = []
+        for b in range(B):
+            kind = rng.random()
+            want.append(-1 if kind < 0.1 else 0 if kind < 0.25 else rng.randint(0, s.seq[b]) if kind < 0.4 else s.seq[b] + rng.randint(0, most + (most > 1)))
+        s.call(want, None if step % 4 == 3 else most)
+
+
+def test_a_call_taken_back_leaves_the_pool_as_it_was():
+    rng = random.Random(1)
+    s = Both(300, 30, 16, 4000)
+    s.call([rng.randint(0, 300) for _ in range(300)])
+    for _ in range(3):
+        seq, pool = list(s.seq), s.dev[2].clone()
+        s.call([max(0, n + rng.randint(-100, 100)) for n in seq], 100)
+        s.call(seq)
+        assert torch.equal(s.dev[2][:2 + len(s.free)], pool[:2 + len(s.free)])
+
+
+def test_requests_behind_one_that_waits():
+    s = Both(5, 4, 16, 6)
+    # 2 pages, 3 pages, 2 pages (waits), 1 page (waits too), none
+    assert s.call([32, 48, 32, 16, 0]).tolist() == [32, 48, 0, 0, 0]
+    # within its page, given back in the same call, served by that
+    assert s.call([30, 0, 32, 16, 1]).tolist() == [0, 0, 32, 16, 1]
+    # more than the table's row, more than T tokens: as it was
+    assert s.call([65, 0, 64, -5, 3], 2).tolist() == [0, 0, 0, 0, 2]
+
+
+def test_a_pool_of_another_order_and_strided_rows():
+    wide = torch.full((4, 10), -3, dtype=torch.int32, device="cuda")
+    table, seq, pool = wide[:, 2:6], ints([0, 0, 0, 0]), ints([5, 0, 9, 8, 7, 6, 5, -1, -1, -1, -1, -1])
+    n_new, slots = page_assign_(table, seq, ints([17, 16, 0, 1]), pool, 16, 17)
+    assert n_new.tolist() == [17, 16, 0, 1] and seq.tolist() == [17, 16, 0, 1]
+    assert wide.tolist() == [[-3, -3, 5, 6] + [-3] * 6, [-3, -3, 7] + [-3] * 7, [-3] * 10, [-3, -3, 8] + [-3] * 7]
+    assert pool[:3].tolist() == [1, 0, 9] and slots[0].tolist() == list(range(80, 96)) + [96] and slots[3, :2].tolist() == [128, -1]
+
+
+def test_captured_and_replayed():
+    s = Both(100, 20, 16, 1200)
+    want, T = ints([0] * 100), 33
+    table, seq, pool = s.dev
+    page_assign_(table, seq, want, pool, 16, T)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        n_new, slots = page_assign_(table, seq, want, pool, 16, T)
+    rng = random.Random(2)
+    for _ in range(5):
+        w = [max(0, n + rng.randint(-40, 33)) for n in s.seq]
+        want.copy_(ints(w))
+        g.replay()
+        w_new, w_slots = orc.assign(s.table, s.seq, w, s.free, 16, T)
+        assert n_new.tolist() == w_new and slots.tolist() == w_slots
+        s.same()
+
+
+def test_another_stream():
+    s = Both(1000, 30, 16, 20000)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        s.call([(37 * b) % 480 for b in range(1000)], 480)
+    torch.cuda.current_stream().wait_stream(side)
+    s.same()
+
+
+def test_no_request():
+    empty = torch.empty(0, dtype=torch.int32, device="cuda")
+    n_new, slots = page_assign_(torch.empty(0, 4, dtype=torch.int32, device="cuda"), empty, empty.clone(), page_pool(3), 16, 5)
+    assert n_new.shape == (0,) and slots.shape == (0, 5)
