@@ -3,6 +3,7 @@
 #include <cmath>
 #include "band_common.h"
 #include "band_shapes.h"
+#include "page_few8_shapes.h"
 #include "rope_axes.h"
 
 namespace {
@@ -551,12 +552,33 @@ int check_rows8(const char* who, const char* name, const void* p, const int64_t*
 }
 }  // namespace
 
+namespace {
+// Up to 32 rows of a group: the kernels of page_few8.h.  The row of all steps is cut where a sequence may be long; a short one is a workgroup's whole
+// work, and needs no second launch.  false: not for them.
+bool plan_few8(Few8Args& a) {
+  if (a.rows > 32) return false;
+  const int64_t bh = (int64_t)a.B * a.Hkv, most = dlt_imin64((int64_t)a.W + a.S + a.Lq, a.Lk);   // keys that a sequence's rows can see
+  a.wgs = 0;
+  a.least = 2;
+  if (most > 1024 && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = (a.rows <= 16 ? 2 : 1) * dlt_device_cus();
+  a.by_heads.m = a.by_heads.s = 0;
+  dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);
+  return true;
+}
+int64_t few8_floats(const Few8Args& a) { return 2 * (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
+int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
+}  // namespace
+
 extern "C" int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes) {
   const char* who = "paged8_workspace";
   DLT_REQUIRE(bytes != nullptr, "%s: bytes is NULL", who);
-  Band8Args a;
+  Few8Args a;
   int rc = paged_problem(who, shape, a);
   if (rc != DLT_OK || (rc = dlt_scales8_check(who, scales, shape->page)) != DLT_OK) return rc;
+  if (plan_few8(a)) {
+    *bytes = few8_bytes(a);
+    return DLT_OK;
+  }
   plan_rows(a, true, false);
   *bytes = rows_bytes(a);
   return DLT_OK;
@@ -567,7 +589,7 @@ extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const 
                                const int32_t* seq_len, const int32_t* n_new, const dlt_paged_shape_t* shape, void* ws, int64_t ws_bytes, void* stream_) {
   const char* who = "paged8_attn";
   hipStream_t stream = (hipStream_t)stream_;
-  Band8Args a;
+  Few8Args a;
   int rc = paged_problem(who, shape, a);
   if (rc != DLT_OK || (rc = dlt_scales8_check(who, scales, shape->page)) != DLT_OK) return rc;
   if ((rc = check_rows(who, "q", q, q_strides, a.Lq == 0, row_span(q_strides, a.G))) != DLT_OK) return rc;
@@ -575,9 +597,10 @@ extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const 
   if ((rc = check_rows(who, "o", o, o_strides, a.Lq == 0, 0)) != DLT_OK) return rc;
   DLT_REQUIRE(table != nullptr && seq_len != nullptr, "%s: table or seq_len is NULL", who);
   DLT_REQUIRE(table_stride >= 0, "%s: negative table stride", who);
-  const int kind = plan_rows(a, true, false);
-  if ((rc = check_ws(who, ws, ws_bytes, rows_bytes(a))) != DLT_OK) return rc;
-  if ((rc = check_grid(who, a)) != DLT_OK) return rc;
+  const bool few = plan_few8(a);
+  const int kind = few ? 0 : plan_rows(a, true, false);
+  if ((rc = check_ws(who, ws, ws_bytes, few ? few8_bytes(a) : rows_bytes(a))) != DLT_OK) return rc;
+  if (!few && (rc = check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
   a.q = q; a.k = k_cache; a.v = v_cache; a.out = o; a.part = (float*)ws;
   strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);
@@ -585,7 +608,15 @@ extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const 
   a.k_sc = (const uint8_t*)scales->k_scale; a.v_sc = (const uint8_t*)scales->v_scale;
   for (int i = 0; i < 3; i++) { a.kss[i] = scales->k_strides[i]; a.vss[i] = scales->v_strides[i]; }
   dlt_fastdiv_make((uint32_t)(scales->block / 16), a.mB, a.sB);
-  rc = band_class(a.dk_, a.dv_) == 64 ? dlt_band_paged8_64(a, shape->dtype, scales->format, kind, stream) : dlt_band_paged8_128(a, shape->dtype, scales->format, kind, stream);
+  const bool small = band_class(a.dk_, a.dv_) == 64;
+  if (few) {
+    a.meta = (int32_t*)(a.part + few8_floats(a));
+    const int D = small ? 64 : 128;
+    bool full = a.dk_ == D && a.dv_ == D && (uintptr_t)k_cache % 16 == 0;
+    for (int i = 0; i < 3; i++) full = full && k_cache_strides[i] % 16 == 0;
+    return small ? dlt_few8_64(a, shape->dtype, scales->format, full, stream) : dlt_few8_128(a, shape->dtype, scales->format, full, stream);
+  }
+  rc = small ? dlt_band_paged8_64(a, shape->dtype, scales->format, kind, stream) : dlt_band_paged8_128(a, shape->dtype, scales->format, kind, stream);
   return rc != DLT_OK ? rc : join(a, false, shape->dtype, stream);
 }
 

@@ -1,0 +1,45 @@
+// Included by page_few8_<D>.hip with DLT_FEW8_D (padded head dim) defined.
+#include "page_few8.h"
+
+#define DLT_FCAT_(a, b) a##b
+#define DLT_FCAT(a, b) DLT_FCAT_(a, b)
+
+namespace {
+constexpr int D = DLT_FEW8_D;
+
+template <typename KernT>
+int few8_go(KernT kern, const Few8Args& a, int64_t grid, int lds, hipStream_t stream) {
+  const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(kern), lds);
+  if (rc != DLT_OK) return rc;
+  dlt_timing_before(DLT_K_FWD, stream);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, a);
+  dlt_timing_after(stream);
+  DLT_CHECK_LAUNCH("paged8 launch");
+  return DLT_OK;
+}
+template <typename TIO, int NP, int FMT>
+int few8_np(const Few8Args& a, bool full, hipStream_t stream) {
+  const int lds = 4 * NP * Few8<D>::WAVE_LDS;
+  if (a.wgs == 0) {
+    const int64_t grid = (int64_t)a.B * a.Hkv;
+    return full ? few8_go(few8_kernel<TIO, D, NP, FMT, true, false>, a, grid, lds, stream) : few8_go(few8_kernel<TIO, D, NP, FMT, false, false>, a, grid, lds, stream);
+  }
+  const int more = lds + 4 * (a.B + 1);
+  int rc = full ? few8_go(few8_kernel<TIO, D, NP, FMT, true, true>, a, a.wgs, more, stream) : few8_go(few8_kernel<TIO, D, NP, FMT, false, true>, a, a.wgs, more, stream);
+  if (rc != DLT_OK) return rc;
+  dlt_timing_before(DLT_K_FWD, stream);
+  hipLaunchKernelGGL(few8_join_kernel<TIO>, dim3((unsigned)a.rows, (unsigned)(a.B * a.Hkv)), dim3(256), 0, stream, a);
+  dlt_timing_after(stream);
+  DLT_CHECK_LAUNCH("paged8 sum launch");
+  return DLT_OK;
+}
+template <typename TIO>
+int few8_t(const Few8Args& a, int format, bool full, hipStream_t stream) {
+  if (format == DLT_FP8_E4M3) return a.rows <= 16 ? few8_np<TIO, 1, DLT_FP8_E4M3>(a, full, stream) : few8_np<TIO, 2, DLT_FP8_E4M3>(a, full, stream);
+  return a.rows <= 16 ? few8_np<TIO, 1, DLT_INT8>(a, full, stream) : few8_np<TIO, 2, DLT_INT8>(a, full, stream);
+}
+}  // namespace
+
+int DLT_FCAT(dlt_few8_, DLT_FEW8_D)(const Few8Args& a, int dtype, int format, bool full, hipStream_t stream) {
+  return dtype == DLT_BF16 ? few8_t<bf16_t>(a, format, full, stream) : few8_t<f16_t>(a, format, full, stream);
+}

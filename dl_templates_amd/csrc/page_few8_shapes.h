@@ -1,0 +1,12 @@
+// Arguments and launchers of the kernels of page_few8.h, by padded head dim.
+#pragma once
+#include "band_common.h"
+
+struct Few8Args : Band8Args {
+  int32_t wgs, least;   // workgroups; steps that one takes at least
+  int32_t* meta;        // of each (batch, kv head): first workgroup, how many
+};
+constexpr int FEW8_B_MAX = 4096;   // sequences whose steps are listed in LDS
+// full: both tensors have that many dims and K's rows lie at multiples of 16 bytes
+int dlt_few8_64(const Few8Args& a, int dtype, int format, bool full, hipStream_t stream);
+int dlt_few8_128(const Few8Args& a, int dtype, int format, bool full, hipStream_t stream);
