@@ -6,29 +6,34 @@
 
 namespace {
 constexpr int D = DLT_FEW8_D;
+constexpr int FEW8_JOIN_WGS = 1024;   // rows of a call that are joined by a workgroup each
 
 template <typename KernT>
-int few8_go(KernT kern, const Few8Args& a, int64_t grid, int lds, hipStream_t stream) {
+int few8_go(KernT kern, const Few8Args& a, int64_t grid, int waves, int lds, hipStream_t stream) {
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(kern), lds);
   if (rc != DLT_OK) return rc;
   dlt_timing_before(DLT_K_FWD, stream);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds, stream, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * waves), lds, stream, a);
   dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("paged8 launch");
   return DLT_OK;
 }
+template <typename TIO, int NP, int FMT, int NW, bool BAL>
+int few8_nw(const Few8Args& a, bool full, int64_t grid, hipStream_t stream) {
+  const int lds = NW * NP * Few8<D>::WAVE_LDS;
+  return full ? few8_go(few8_kernel<TIO, D, NP, FMT, true, NW, BAL>, a, grid, NW, lds, stream) : few8_go(few8_kernel<TIO, D, NP, FMT, false, NW, BAL>, a, grid, NW, lds, stream);
+}
 template <typename TIO, int NP, int FMT>
 int few8_np(const Few8Args& a, bool full, hipStream_t stream) {
-  const int lds = 4 * NP * Few8<D>::WAVE_LDS;
-  if (a.wgs == 0) {
-    const int64_t grid = (int64_t)a.B * a.Hkv;
-    return full ? few8_go(few8_kernel<TIO, D, NP, FMT, true, false>, a, grid, lds, stream) : few8_go(few8_kernel<TIO, D, NP, FMT, false, false>, a, grid, lds, stream);
-  }
-  const int more = lds + 4 * (a.B + 1);
-  int rc = full ? few8_go(few8_kernel<TIO, D, NP, FMT, true, true>, a, a.wgs, more, stream) : few8_go(few8_kernel<TIO, D, NP, FMT, false, true>, a, a.wgs, more, stream);
+  if constexpr (NP == 1)
+    if (a.wgs == 0 && a.waves == 16) return few8_nw<TIO, NP, FMT, 16, false>(a, full, (int64_t)a.B * a.Hkv, stream);
+  if (a.wgs == 0) return few8_nw<TIO, NP, FMT, 4, false>(a, full, (int64_t)a.B * a.Hkv, stream);
+  const int rc = few8_nw<TIO, NP, FMT, 4, true>(a, full, a.wgs, stream);
   if (rc != DLT_OK) return rc;
   dlt_timing_before(DLT_K_FWD, stream);
-  hipLaunchKernelGGL(few8_join_kernel<TIO>, dim3((unsigned)a.rows, (unsigned)(a.B * a.Hkv)), dim3(256), 0, stream, a);
+  const unsigned bh = (unsigned)(a.B * a.Hkv);
+  if ((int64_t)bh * a.rows <= FEW8_JOIN_WGS) hipLaunchKernelGGL((few8_join_kernel<TIO, true>), dim3((unsigned)a.rows, bh), dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((few8_join_kernel<TIO, false>), dim3((unsigned)(a.rows + 3) / 4, bh), dim3(256), 0, stream, a);
   dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("paged8 sum launch");
   return DLT_OK;
