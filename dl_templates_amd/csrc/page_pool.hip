@@ -5,7 +5,7 @@
 // page first", and request b is served iff its sum of needs, itself included, is at most F + R.  So every page and every slot is found by itself, from two sums, and
 // nothing is added atomically: equal calls give equal pages.
 //
-// Every workgroup forms the two sums of all requests (8 B of lengths each, from the L2) and keeps them in LDS, then takes a share of the new columns, of the
+// Every workgroup forms the two sums of all requests (8 B of lengths each, from the L2) and keeps them in LDS with what every request holds and gains, then takes a share of the new columns, of the
 // pages that come back and of the slots.  A table's row is read (a request that gives back) or written (one that gains), never both; the pool is read below F and
 // written from F on.  Lengths and the pool's count, which all workgroups read, are written by the last one to finish: a count of those that are done, in the
 // pool's second word, tells which that is; nobody waits.
@@ -53,12 +53,12 @@ __device__ inline int owner_of(const int32_t* start, int B, int x) {
 
 struct Stack {
   const AssignArgs& a;
-  const int32_t* back;   // exclusive sums of what comes back, [B + 1]
+  const int32_t *back, *held, *gain;   // exclusive sums of what comes back, [B + 1]; of every request
   int F, R;
   // r-th of the pages that come back: the last request's last page first
   __device__ int returned(int r) const {
     const int x = R - 1 - r, b = owner_of(back, a.B, x);
-    return a.table[b * a.ts + (pages_of(a, dlt_imax(a.want[b], 0)) + x - back[b])];
+    return a.table[b * a.ts + (pages_of(a, held[b] + gain[b]) + x - back[b])];
   }
   // k-th page that is taken
   __device__ int taken(int k) const {
@@ -90,9 +90,9 @@ __device__ inline void scan2(int& x, int& y, int& sum_x, int& sum_y, int (*wave)
 template <int NT>
 __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   dlt_kernargs_in<sizeof(AssignArgs)>();
-  extern __shared__ int32_t sums[];   // needs [B + 1], back [B + 1]
+  extern __shared__ int32_t sums[];   // needs [B + 1], back [B + 1], held [B], gains [B]: tokens gained, or given back where negative
   __shared__ int wave[NT / 64][2], most[NT / 64], last;
-  int32_t *need = sums, *back = sums + a.B + 1;
+  int32_t *need = sums, *back = need + a.B + 1, *held = back + a.B + 1, *gain = held + a.B;
   const int tid = threadIdx.x;
 
   // sums of needs and of what comes back: a run of requests to a thread
@@ -116,6 +116,8 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
     back[b] = r;
     n += w.need;
     r += w.back;
+    held[b] = w.held;
+    gain[b] = w.need > 0 && n > room ? 0 : w.want - w.held;
     if (w.need > 0 && n <= room) served = n;
   }
   if (tid == 0) {
@@ -129,44 +131,58 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
 #pragma unroll
   for (int i = 0; i < NT / 64; i++) served = dlt_imax(served, most[i]);
   const int left = (int)(room - served < a.n_pages ? room - served : a.n_pages);
-  const Stack stack{a, back, F, sum_r};
+  const Stack stack{a, back, held, gain, F, sum_r};
   const int64_t at0 = (int64_t)blockIdx.x * NT + tid, step = (int64_t)gridDim.x * NT;
 
   for (int64_t k = at0; k < served; k += step) {
     const int b = owner_of(need, a.B, (int)k);
-    a.table[b * a.ts + (pages_of(a, wish_of(a, b).held) + (int)k - need[b])] = stack.taken((int)k);
+    a.table[b * a.ts + (pages_of(a, held[b]) + (int)k - need[b])] = stack.taken((int)k);
   }
   for (int64_t i = at0; F + i < left; i += step) a.pool[2 + F + i] = stack.returned((int)i);
-  auto gain_of = [&](int b, const Wish& w) { return w.want > w.held && (w.need == 0 || need[b] + w.need <= room) ? w.want - w.held : 0; };
-  for (int64_t b = at0; b < a.B; b += step) a.n_new[b] = gain_of((int)b, wish_of(a, (int)b));
+  for (int64_t b = at0; b < a.B; b += step) a.n_new[b] = dlt_imax(gain[b], 0);
+  // slots, four in a row of all to a thread: they share their request and mostly their page
   const int64_t slots = a.T > 0 ? (int64_t)a.B * a.T : 0;
-  for (int64_t i = at0; i < slots; i += step) {
-    const int b = (int)dlt_fastdiv((uint32_t)i, a.mt, a.st), t = (int)i - b * a.T;
-    const Wish w = wish_of(a, b);
-    int slot = -1;
-    if (t < gain_of(b, w)) {
-      const int p = w.held + t, col = (int)dlt_fastdiv((uint32_t)p, a.mp, a.sp), p0 = pages_of(a, w.held);
-      const int page = col < p0 ? a.table[b * a.ts + col] : stack.taken(need[b] + col - p0);
-      slot = page * a.page + (p - col * a.page);
+  // (from the last workgroup on: on a small call others have the columns)
+  for (int64_t i = 4 * ((int64_t)(gridDim.x - 1 - blockIdx.x) * NT + tid); i < slots; i += 4 * step) {
+    int b = (int)dlt_fastdiv((uint32_t)i, a.mt, a.st), t = (int)i - b * a.T, page = -1, until = 0;   // `page` holds tokens below `until` of request b
+    int has = held[b], more = gain[b], out[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      if (t == a.T) {
+        t = until = 0;
+        if (++b == a.B) break;
+        has = held[b];
+        more = gain[b];
+      }
+      const int p = has + t;
+      out[k] = -1;
+      if (t < more) {
+        if (p >= until) {
+          const int col = (int)dlt_fastdiv((uint32_t)p, a.mp, a.sp), p0 = pages_of(a, has);
+          page = col < p0 ? a.table[b * a.ts + col] : stack.taken(need[b] + col - p0);
+          until = (col + 1) * a.page;
+        }
+        out[k] = (page + 1) * a.page - (until - p);
+      }
+      t++;
     }
-    a.slots[i] = slot;
+    if (i + 4 <= slots) *reinterpret_cast<int4*>(a.slots + i) = int4{out[0], out[1], out[2], out[3]};
+    else
+      for (int k = 0; i + k < slots; k++) a.slots[i + k] = out[k];
   }
 
   if (gridDim.x > 1) {
-    __threadfence();
+    // every load of this workgroup has returned: its lengths may be written now.  (Nothing that a workgroup writes is read by another.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (tid == 0) last = atomicAdd(&a.pool[1], 1) == (int)gridDim.x - 1;
+    if (tid == 0) last = __hip_atomic_fetch_add(&a.pool[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     __syncthreads();
     if (!last) return;
-    __threadfence();
   } else {
     __syncthreads();
   }
-  for (int b = b0; b < b1; b++) {
-    const Wish w = wish_of(a, b);
-    const int now = w.want < w.held ? w.want : w.held + gain_of(b, w);
-    if (now != w.held) a.seq[b] = now;
-  }
+  for (int b = tid; b < a.B; b += NT)
+    if (gain[b] != 0) a.seq[b] = held[b] + gain[b];
   if (tid == 0) {
     a.pool[0] = left;
     if (gridDim.x > 1) a.pool[1] = 0;
@@ -185,6 +201,7 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
     return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many pages or tokens", who);
   if (B == 0) return DLT_OK;
   DLT_REQUIRE(table != nullptr && seq_len != nullptr && want != nullptr && pool != nullptr && n_new != nullptr && (slots != nullptr || T <= 0), "%s: a tensor is NULL", who);
+  DLT_REQUIRE((uintptr_t)slots % 16 == 0, "%s: slots must start at a multiple of 16 bytes", who);
   DLT_REQUIRE(B == 1 || table_stride >= cols, "%s: rows of the table overlap (stride %lld, %d columns)", who, (long long)table_stride, cols);
   AssignArgs a{};
   a.table = table; a.seq = seq_len; a.pool = pool; a.n_new = n_new; a.slots = slots; a.want = want; a.ts = table_stride;
@@ -192,10 +209,12 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
   dlt_fastdiv_make((uint32_t)page, a.mp, a.sp);
   dlt_fastdiv_make((uint32_t)dlt_imax(T, 1), a.mt, a.st);
   constexpr int NT = 256;
-  // slots, and columns that requests can gain at most
-  const int64_t work = (int64_t)B * dlt_imax(T, 1) + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols);
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work / (4 * NT), dlt_device_cus()));
-  const int lds = 2 * (B + 1) * 4;
+  // slots by fours, and columns that requests can gain (give back, without a limit to the slots): one of them to a thread, but no more than two workgroups a CU, each of
+  // which is another atomic on the pool's word: 1000 requests, 4000 slots each, 256 / 512 / 1024 workgroups 30 / 22 / 25 us (with lengths read again for every slot)
+  const int64_t work = (int64_t)B * dlt_imax(T, 1) / 4 + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols), cus = dlt_device_cus();
+  // (small calls up to eight, so that columns and slots are not one after the other: 64 requests, one token more, 6.5 -> 6.0 us)
+  const int64_t grid = std::max<int64_t>(1, std::max<int64_t>(std::min<int64_t>(work / 16, 8), std::min<int64_t>(work / NT, (T >= 0 ? 2 : 1) * cus)));
+  const int lds = 4 * (B + 1) * 4;
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
   if (rc != DLT_OK) return rc;
   hipLaunchKernelGGL(page_assign_kernel<NT>, dim3((unsigned)grid), dim3(NT), lds, stream, a);

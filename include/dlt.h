@@ -402,7 +402,7 @@ int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const void* k_cac
  * ceil(want / page) go back to the pool; what it lacks comes from there; want[b] < 0 leaves it alone.  Requests are served in order of b while the pool, with what
  * came back in the same call, holds the pages of all that asked so far; from the first that it does not, requests that need a page get nothing and keep
  * seq_len[b].  So do requests that want more than cols pages hold or, with T >= 0, more than T tokens more.  seq_len, table and pool are brought up to date in
- * place (table: the columns of new pages), n_new[b] is how many tokens request b gained.  With T > 0 slots[b, t] (contiguous [B, T]) is the place of its new token t, page
+ * place (table: the columns of new pages), n_new[b] is how many tokens request b gained.  With T > 0 slots[b, t] (contiguous [B, T], 16-byte aligned) is the place of its new token t, page
  * number times page plus the row, -1 where there is none.  Pages are taken from the top of the pool in order of request and column and put back in the opposite
  * order, so a call that takes back what the last one gave leaves the pool as it was.  B at most DLT_ASSIGN_MAX; B * cols, cols * page and n_pages below 2^30, n_pages * page and
  * B * T below 2^31.  Calls on one pool must not overlap. */
