@@ -5,9 +5,11 @@
 // out of its subnormals, whole numbers lose at most half a step of the new scale, less than a step over all growths (1/2 + 1/4 + ..).
 //
 // An item is a block, a head and a tensor (K or V): its tokens are fetched once, rotated in 32 bits, held in registers until their largest element is known, and written as
-// 8-bit numbers.  8 dims to a lane, as many rows to a wave as fit.  Few new tokens a block: a wave to an item (nothing waits for another wave); else four waves, which
-// exchange their maxima through LDS.  Rows of q are rotated by workgroups of their own in the same launch, a wave to some tokens, the heads one after the other under
+// 8-bit numbers, some heads one after the other under one fetch of cos and sin, the next head's rows on their way.  8 dims to a lane, as many rows to a wave as fit.  Few new tokens a block: a wave to an item (nothing waits for another wave); else four or eight, which
+// exchange their maxima through LDS (blocks of 128, d = 128, by four waves with twice the rows in registers: 60 us for 36).  Rows of q are rotated by workgroups of their own in the same launch, a wave to some tokens, the heads one after the other under
 // one fetch of cos and sin.
+//
+// Memory bound: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 30 us, 4.5 TB/s; a token each of 64 sequences 5 us on the GPU, latency: length, page, row.
 #include <algorithm>
 #include "attn_common.hpp"
 #include "page_cvt8.h"
@@ -31,23 +33,29 @@ struct App8Args {
   int32_t page, n_pages, cols, block;
   int32_t nb;               // blocks that T tokens of a sequence can touch
   int32_t kv_blocks;        // workgroups of keys and values; behind them those of q
+  int32_t hk, kv_heads, kv_chunks;   // heads of K or V that an item walks; of K, rounded up to whole runs; runs of K and V
   int32_t hq, q_chunks;     // heads of q that a wave walks, such chunks
   int32_t whole;            // a lane's 8 dims are one run of pairs of one axis
   const int32_t *table, *seq, *n_new;
   int64_t tbs;
   RopeAxes r;
-  uint32_t mT, sT, mb, sb, mp, sp;   // divisions by T, block, page
+  uint32_t mT, sT, mb, sb, mp, sp, mc, sc, mn, sn;   // divisions by T, block, page, runs of heads, blocks of a sequence
 };
 
+// 8 elements as they come
 template <typename T>
-DLT_DEV void load8(float (&f)[8], const T* p) {   // 16-byte aligned
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+struct Raw8 { u32x4 w[sizeof(T) / 2]; };
+template <typename T>
+DLT_DEV void fetch8(Raw8<T>& r, const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) { f[i] = a[i]; f[4 + i] = b[i]; }
-  } else {
-    unpack8<T>(*reinterpret_cast<const u32x4*>(p), f);
-  }
+  for (int i = 0; i < (int)(sizeof(T) / 2); i++) r.w[i] = *reinterpret_cast<const u32x4*>(p + 8 * i / (sizeof(T) / 2));
+}
+template <typename T>
+DLT_DEV void widen8(float (&f)[8], const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) f[i] = __uint_as_float(r.w[i >> 2][i & 3]);
+  } else unpack8<T>(r.w[0], f);
 }
 
 // A lane's 8 dims d0 .. d0 + 7 of a token: cos, sin (with the sign of their dim's half), where their partners are, which of them turn
@@ -106,26 +114,36 @@ DLT_DEV Turn turn_of(const RopeAxes& r, int d0, int b, int t, int place, bool li
   }
   return x;
 }
-// the row's 8 dims, rotated
+// A row's 8 dims and their partners
 template <typename T, bool WHOLE>
-DLT_DEV void rotated(float (&y)[8], const RopeAxes& r, const T* row, int d0, const Turn& x) {
-  load8(y, row + d0);
-  if (x.on == 0) return;
-  float w[8];
-  if constexpr (WHOLE) {
-    load8(w, row + x.other);
-  } else {
+struct Pair8 {
+  Raw8<T> own, far;
+  DLT_DEV void fetch(const RopeAxes& r, const T* row, int d0, const Turn& x) {
+    fetch8(own, row + d0);
+    if (x.on == 0) return;
+    if constexpr (WHOLE) {
+      fetch8(far, row + x.other);
+    } else {
+      T v[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      int pair, other = d0 + j;
-      bool first;
-      if (d0 + j < 2 * r.pairs) half_of(r, d0 + j, pair, other, first);
-      w[j] = (float)row[other];
+      for (int j = 0; j < 8; j++) {
+        int pair, other = d0 + j;
+        bool first;
+        if (d0 + j < 2 * r.pairs) half_of(r, d0 + j, pair, other, first);
+        v[j] = row[other];
+      }
+      __builtin_memcpy(&far, v, sizeof(far));
     }
   }
+  DLT_DEV void rotated(float (&y)[8], const Turn& x) const {
+    widen8<T>(y, own);
+    if (x.on == 0) return;
+    float w[8];
+    widen8<T>(w, far);
 #pragma unroll
-  for (int j = 0; j < 8; j++) y[j] = x.on >> j & 1 ? mix(y[j], x.c[j], w[j], x.s[j]) : y[j];
-}
+    for (int j = 0; j < 8; j++) y[j] = x.on >> j & 1 ? mix(y[j], x.c[j], w[j], x.s[j]) : y[j];
+  }
+};
 
 // Rows of q: tokens of all sequences in a row, `rpw` to a wave, `hq` heads to a wave
 template <typename T, bool WHOLE>
@@ -143,44 +161,55 @@ DLT_DEV void rotate_q(const App8Args& a, int item, int lane) {
   if (a.r.n > 0) x = turn_of<WHOLE>(a.r, d0, b, t, (int)(at < -1 ? -1 : at), t < n_new);
   const T* src = reinterpret_cast<const T*>(a.q) + b * a.qs[0] + t * a.qs[2];
   T* dst = reinterpret_cast<T*>(a.q_out) + b * a.qos[0] + t * a.qos[2] + d0;
-#pragma unroll 2
-  for (int h = h0; h < h1; h++) {
-    if (x.on == 0) {   // as it is, bit for bit
-      u32x4 v[sizeof(T) / 2];
-      __builtin_memcpy(v, src + h * a.qs[1] + d0, sizeof(v));
+  constexpr int UNR = 4;   // heads on their way together
+  for (int h = h0; h < h1; h += UNR) {
+    Pair8<T, WHOLE> v[UNR];
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(T) / 2); i++) __builtin_nontemporal_store(v[i], reinterpret_cast<u32x4*>(dst + h * a.qos[1]) + i);
-      continue;
-    }
-    float y[8];
-    rotated<T, WHOLE>(y, a.r, src + h * a.qs[1], d0, x);
-    if constexpr (sizeof(T) == 4) {
-      __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, reinterpret_cast<f32x4*>(dst + h * a.qos[1]));
-      __builtin_nontemporal_store(f32x4{y[4], y[5], y[6], y[7]}, reinterpret_cast<f32x4*>(dst + h * a.qos[1]) + 1);
-    } else {
-      __builtin_nontemporal_store(pack8<T>(y), reinterpret_cast<u32x4*>(dst + h * a.qos[1]));
+    for (int u = 0; u < UNR; u++) v[u].fetch(a.r, src + dlt_imin(h + u, h1 - 1) * a.qs[1], d0, x);
+#pragma unroll
+    for (int u = 0; u < UNR; u++) {
+      if (h + u >= h1) continue;
+      Raw8<T> out = v[u].own;   // as it is, bit for bit, where nothing turns
+      if (x.on != 0) {
+        float y[8];
+        v[u].rotated(y, x);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) out.w[i >> 2][i & 3] = __float_as_uint(y[i]);
+        } else out.w[0] = pack8<T>(y);
+      }
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(T) / 2); i++) __builtin_nontemporal_store(out.w[i], reinterpret_cast<u32x4*>(dst + (h + u) * a.qos[1]) + i);
     }
   }
 }
 
+// Waves a CU that the heads an item (or a wave of q) walks have to leave: more heads fetch cos and sin, lengths and pages less often.  us, 4 / 8 / 16 / 32 waves of keys and
+// values: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 34.6 / 33.7 / 35.3 / 41.1, of 16 29.4 / 29.5 / 32.5 / 36.2; 7 of up to 2047, 16 + 8 + 8, d = 64,
+// blocks of 16 22.4 / 18.3 / 19.6 / 24.0.  4 / 8 / 16 waves of q beside 8 of those: 36.7 / 33.7 / 30.0; 30.5 / 29.5 / 27.5; 18.7 / 18.3 / 17.6.
+constexpr int APP8_WAVES = 8, APP8_Q_WAVES = 16;
+
 // NW waves to an item, MAXP rows of registers to a lane
 template <typename T, int FMT, bool WHOLE, int NW, int MAXP>
-__global__ __launch_bounds__(256) void paged8_append_kernel(const App8Args a) {
+__global__ __launch_bounds__(NW == 8 ? 512 : 256) void paged8_append_kernel(const App8Args a) {
   dlt_kernargs_in<sizeof(App8Args)>();
-  __shared__ unsigned big[4];
+  __shared__ unsigned big[2][8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if ((int)blockIdx.x >= a.kv_blocks) {
-    rotate_q<T, WHOLE>(a, ((int)blockIdx.x - a.kv_blocks) * 4 + wave, lane);
+    rotate_q<T, WHOLE>(a, ((int)blockIdx.x - a.kv_blocks) * (NW == 8 ? 8 : 4) + wave, lane);
     return;
   }
-  // item: heads innermost, then K and V, blocks, sequences
-  int item = NW == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
-  const int mine = NW == 4 ? wave : 0;
-  const int heads = 2 * a.Hkv;
-  const int bj = item / heads;
+  // item: runs of `hk` heads of K and V innermost, then blocks, sequences
+  const int item = NW > 1 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, mine = NW > 1 ? wave : 0;
+  const int bj = (int)dlt_fastdiv((uint32_t)item, a.mc, a.sc);
   if (bj >= a.B * a.nb) return;   // (NW = 1: no wave waits for another)
-  const int hs = item - bj * heads, h = hs >= a.Hkv ? hs - a.Hkv : hs, b = bj / a.nb, j = bj - b * a.nb;
-  const App8Side& s = a.s[hs >= a.Hkv ? 1 : 0];
+  const int b = (int)dlt_fastdiv((uint32_t)bj, a.mn, a.sn), j = bj - b * a.nb;
+  int h = (item - bj * a.kv_chunks) * a.hk;
+  const bool vals = h >= a.kv_heads;   // heads of V behind those of K, in chunks of their own
+  if (vals) h -= a.kv_heads;
+  const int h1 = dlt_imin(h + a.hk, a.Hkv);
+  const App8Side& s = a.s[vals ? 1 : 0];
+  const bool rot = !vals && a.r.n > 0;
 
   // new tokens lo .. hi - 1 of the sequence, n0 .. n1 - 1 of them in the block
   const int n_new = a.n_new != nullptr ? dlt_imax(0, dlt_imin(a.n_new[b], a.T)) : a.T;
@@ -190,86 +219,104 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const App8Args a) {
   const int blk = (int)dlt_fastdiv((uint32_t)lo, a.mb, a.sb) + j, base = blk * a.block;
   const int n0 = dlt_imax(lo, base), n1 = dlt_imin(hi, base + a.block);
   if (n0 >= n1) return;
-  const int col = (int)dlt_fastdiv((uint32_t)base, a.mp, a.sp), page = a.table[b * a.tbs + col], row0 = base - col * a.page;
-  if (page < 0 || page >= a.n_pages) return;
+  const int col = (int)dlt_fastdiv((uint32_t)base, a.mp, a.sp), row0 = base - col * a.page;
+  const int page = a.table[b * a.tbs + col];   // on its way beside the rows
 
   const int D = s.D, parts = D >> 3, rpw = 64 / parts, in = lane / parts, d0 = 8 * (lane - in * parts);
   const bool lane_on = in < rpw;
-  uint8_t* dst = s.dst + (page * s.ds[0] + h * s.ds[1] + row0 * s.ds[2]);
-  uint8_t* sc = s.scale + (page * s.es[0] + h * s.es[1] + (int)dlt_fastdiv((uint32_t)row0, a.mb, a.sb) * s.es[2]);
-  const bool older = base < n0;
-  const int e_old = older ? *sc : 0;
-
-  float y[MAXP][8];
-  unsigned amax = 0;   // bits of the largest finite magnitude; bit 31: an element that is none
-#pragma unroll
-  for (int p = 0; p < MAXP; p++) {
+  Turn turn[MAXP];   // cos and sin of the lane's rows, for all heads
+  auto turn_at = [&](int p) __attribute__((always_inline)) {
     const int tok = n0 + (p * NW + mine) * rpw + in;
+    if (rot && lane_on && tok < n1) return turn_of<WHOLE>(a.r, d0, b, (int)(tok - held), tok, true);
+    Turn x;
+    x.on = 0;
+    x.other = d0;
+    return x;
+  };
 #pragma unroll
-    for (int i = 0; i < 8; i++) y[p][i] = 0.f;
-    if (lane_on && tok < n1) {
-      const int t = (int)(tok - held);
-      const T* src = reinterpret_cast<const T*>(s.src) + (b * s.ss[0] + h * s.ss[1] + t * s.ss[2]);
-      if (s.rot && a.r.n > 0) {
-        const Turn x = turn_of<WHOLE>(a.r, d0, b, t, tok, true);
-        rotated<T, WHOLE>(y[p], a.r, src, d0, x);
-      } else {
-        load8(y[p], src + d0);
-      }
+  for (int p = 0; p < MAXP; p++) turn[p] = turn_at(p);
+  Pair8<T, WHOLE> x[MAXP];
+  auto fetch = [&](int head) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < MAXP; p++) {
+      const int tok = n0 + (p * NW + mine) * rpw + in;
+      if (lane_on && tok < n1) x[p].fetch(a.r, reinterpret_cast<const T*>(s.src) + (b * s.ss[0] + head * s.ss[1] + (int)(tok - held) * s.ss[2]), d0, turn[p]);
+    }
+  };
+  fetch(h);
+  if (page < 0 || page >= a.n_pages) return;
+
+#pragma unroll 1
+  for (int round = 0; h < h1; h++, round ^= 1) {
+    uint8_t* dst = s.dst + (page * s.ds[0] + h * s.ds[1] + row0 * s.ds[2]);
+    uint8_t* sc = s.scale + (page * s.es[0] + h * s.es[1] + (int)dlt_fastdiv((uint32_t)row0, a.mb, a.sb) * s.es[2]);
+    const bool older = base < n0;
+    const int e_old = older ? *sc : 0;
+
+    float y[MAXP][8];
+    unsigned m = 0, odd_bits = 0;   // of the largest finite magnitude; nonzero: an element that is none
+#pragma unroll
+    for (int p = 0; p < MAXP; p++) {
+      const int tok = n0 + (p * NW + mine) * rpw + in;
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[p][i] = 0.f;
+      if (lane_on && tok < n1) x[p].rotated(y[p], turn[p]);
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const unsigned m = __float_as_uint(y[p][i]) & 0x7fffffffu;
-        amax = m < 0x7f800000u ? (amax & 0x80000000u) | ((amax & 0x7fffffffu) > m ? (amax & 0x7fffffffu) : m) : amax | 0x80000000u;
+        const unsigned v = __float_as_uint(y[p][i]) & 0x7fffffffu;
+        const bool fin = v < 0x7f800000u;
+        odd_bits |= fin ? 0u : 1u;
+        m = fin && v > m ? v : m;
       }
     }
-  }
-  const bool odd_lane = (amax >> 31) != 0;
-  unsigned m = amax & 0x7fffffffu;
+    if (h + 1 < h1) fetch(h + 1);   // beside what follows
 #pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) {
-    const unsigned o = (unsigned)__shfl_xor((int)m, k);
-    m = m > o ? m : o;
-  }
-  bool odd = __builtin_amdgcn_ballot_w64(odd_lane) != 0;
-  if constexpr (NW == 4) {
-    asm volatile("" ::"v"(e_old));   // read before another wave may write it
-    if (lane == 0) big[wave] = m | (odd ? 0x80000000u : 0u);
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const unsigned o = big[w];
-      odd = odd || (o >> 31) != 0;
-      m = m > (o & 0x7fffffffu) ? m : (o & 0x7fffffffu);
+    for (int k = 32; k >= 1; k >>= 1) {
+      const unsigned o = (unsigned)__shfl_xor((int)m, k);
+      m = m > o ? m : o;
     }
-  }
-  const int need = cvt8_exponent<FMT>(m);          // biased
-  const int e = dlt_imax(need, e_old);             // 255, NaN, stays
-  const int e_new = FMT == DLT_INT8 && odd ? 255 : e;
-  const float inv = e >= 254 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
-  const float most = sizeof(T) == 2 && std::is_same<T, f16_t>::value ? cvt8_most_f16<FMT>(e) : cvt8_most<FMT>();
-  // older tokens of the block at a larger scale
-  if (older && e > e_old && e_new != 255) {
-    keep_branch();
-    const float by = e - e_old > 60 ? 0.f : __uint_as_float((unsigned)(127 - (e - e_old)) << 23);
-    for (int r = mine * rpw + in; r < n0 - base; r += NW * rpw) {
-      if (!lane_on) break;
-      uint8_t* p = dst + r * s.ds[2] + d0;
-      float f[8];
-      cvt8_get8<FMT>(*reinterpret_cast<const u32x2*>(p), f);
+    bool odd = __builtin_amdgcn_ballot_w64(odd_bits != 0) != 0;
+    if constexpr (NW > 1) {
+      asm volatile("" ::"v"(e_old));   // read before another wave may write it
+      if (lane == 0) big[round][wave] = m | (odd ? 0x80000000u : 0u);
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] *= by;
-      *reinterpret_cast<u32x2*>(p) = cvt8_put8<FMT>(f, most);
+      for (int w = 0; w < NW; w++) {
+        const unsigned o = big[round][w];
+        odd = odd || (o >> 31) != 0;
+        m = m > (o & 0x7fffffffu) ? m : (o & 0x7fffffffu);
+      }
     }
-  }
-  if (mine == 0 && lane == 0 && (!older || e_new != e_old)) *sc = (uint8_t)e_new;
+    const int need = cvt8_exponent<FMT>(m);          // biased
+    const int e = dlt_imax(need, e_old);             // 255, NaN, stays
+    const int e_new = FMT == DLT_INT8 && odd ? 255 : e;
+    const float inv = e >= 254 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
+    const float most = std::is_same<T, f16_t>::value ? cvt8_most_f16<FMT>(e) : cvt8_most<FMT>();
+    // older tokens of the block at a larger scale
+    if (older && e > e_old && e_new != 255) {
+      keep_branch();
+      const float by = e - e_old > 60 ? 0.f : __uint_as_float((unsigned)(127 - (e - e_old)) << 23);
+      if (lane_on)
+#pragma unroll 4
+        for (int r = mine * rpw + in; r < n0 - base; r += NW * rpw) {
+          uint8_t* p = dst + r * s.ds[2] + d0;
+          float f[8];
+          cvt8_get8<FMT>(*reinterpret_cast<const u32x2*>(p), f);
 #pragma unroll
-  for (int p = 0; p < MAXP; p++) {
-    const int r = n0 - base + (p * NW + mine) * rpw + in;
-    if (lane_on && r < n1 - base) {
-      float f[8];
+          for (int i = 0; i < 8; i++) f[i] *= by;
+          *reinterpret_cast<u32x2*>(p) = cvt8_put8<FMT>(f, most);
+        }
+    }
+    if (mine == 0 && lane == 0 && (!older || e_new != e_old)) *sc = (uint8_t)e_new;
 #pragma unroll
-      for (int i = 0; i < 8; i++) f[i] = y[p][i] * inv;
-      *reinterpret_cast<u32x2*>(dst + r * s.ds[2] + d0) = cvt8_put8<FMT>(f, most);
+    for (int p = 0; p < MAXP; p++) {
+      const int r = n0 - base + (p * NW + mine) * rpw + in;
+      if (lane_on && r < n1 - base) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = y[p][i] * inv;
+        *reinterpret_cast<u32x2*>(dst + r * s.ds[2] + d0) = cvt8_put8<FMT>(f, most);
+      }
     }
   }
 }
@@ -277,11 +324,12 @@ __global__ __launch_bounds__(256) void paged8_append_kernel(const App8Args a) {
 template <typename T, int FMT, bool WHOLE>
 int launch(const App8Args& a, int nw, int passes, int64_t grid, hipStream_t stream) {
   dlt_timing_before(DLT_K_ROPE, stream);
-  const dim3 g((unsigned)grid), t(256);
+  const dim3 g((unsigned)grid), t(nw == 8 ? 512 : 256);
   if (nw == 1) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 1, 2>), g, t, 0, stream, a);
-  else if (passes <= 1) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 4, 1>), g, t, 0, stream, a);
-  else if (passes <= 4) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 4, 4>), g, t, 0, stream, a);
-  else hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 4, 8>), g, t, 0, stream, a);
+  else if (nw == 4 && passes == 1) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 4, 1>), g, t, 0, stream, a);
+  else if (nw == 4) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 4, 2>), g, t, 0, stream, a);
+  else if (passes <= 2) hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 8, 2>), g, t, 0, stream, a);
+  else hipLaunchKernelGGL((paged8_append_kernel<T, FMT, WHOLE, 8, 4>), g, t, 0, stream, a);
   dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("paged8_append launch");
   return DLT_OK;
@@ -362,21 +410,29 @@ extern "C" int dlt_paged8_append(const void* k, const int64_t k_strides[4], cons
   dlt_fastdiv_make((uint32_t)a.page, a.mp, a.sp);
   a.whole = 1;
   for (int i = 0; i < a.r.n; i++) a.whole = a.whole && a.r.end[i] % 8 == 0;
-  // a wave to an item while two rounds of its rows hold what a block can get
+  // waves of an item: as many as hold what a block can get in two rounds of their rows (up to four for eight waves: 128 rows of 128 dims)
   const int rows = 64 / (std::max(s->dk, s->dv) / 8), most = std::min(s->T, a.block);
-  const int nw = most <= 2 * rows ? 1 : 4, passes = (most + nw * rows - 1) / (nw * rows);
+  const int nw = most <= 2 * rows ? 1 : most <= 8 * rows ? 4 : 8, passes = (most + nw * rows - 1) / (nw * rows);
   a.nb = (s->T + a.block - 2) / a.block + 1;
-  const int64_t items = (int64_t)s->B * a.nb * 2 * s->Hkv;
-  a.kv_blocks = (int32_t)std::min<int64_t>((items + (4 / nw) - 1) / (4 / nw), 0x7fffffff);
+  // heads of an item: all of K's or V's while that leaves APP8_WAVES a CU, fewer otherwise
+  const int64_t blocks = (int64_t)s->B * a.nb, waves_kv = APP8_WAVES * (int64_t)dlt_device_cus();
+  a.hk = s->Hkv;
+  while (a.hk > 1 && blocks * nw * 2 * ((s->Hkv + a.hk - 1) / a.hk) < waves_kv) a.hk = (a.hk + 1) / 2;
+  const int runs = (s->Hkv + a.hk - 1) / a.hk;
+  a.kv_heads = runs * a.hk;
+  a.kv_chunks = 2 * runs;
+  dlt_fastdiv_make((uint32_t)a.kv_chunks, a.mc, a.sc);
+  dlt_fastdiv_make((uint32_t)a.nb, a.mn, a.sn);
+  const int64_t items = blocks * a.kv_chunks;
+  a.kv_blocks = (int32_t)std::min<int64_t>(nw > 1 ? items : (items + 3) / 4, 0x7fffffff);
   int64_t grid = a.kv_blocks;
   if (s->H > 0) {
     const int64_t groups = ((int64_t)s->B * s->T + 64 / (s->dk / 8) - 1) / (64 / (s->dk / 8));
-    // all heads to a wave while that leaves two workgroups a CU, fewer otherwise
-    const int64_t waves = 8 * (int64_t)dlt_device_cus();
+    const int64_t waves = APP8_Q_WAVES * (int64_t)dlt_device_cus();
     a.hq = s->H;
     while (a.hq > 1 && groups * ((s->H + a.hq - 1) / a.hq) < waves) a.hq = (a.hq + 1) / 2;
     a.q_chunks = (s->H + a.hq - 1) / a.hq;
-    grid += (groups * a.q_chunks + 3) / 4;
+    grid += nw == 8 ? (groups * a.q_chunks + 7) / 8 : (groups * a.q_chunks + 3) / 4;
   }
   if (items > 0x7fffff00 || grid > 0x7fffffff || (int64_t)s->B * s->T > 0x7fffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too much work for one launch", who);
   switch (s->dtype) {
