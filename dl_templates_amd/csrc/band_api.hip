@@ -574,6 +574,23 @@ bool plan_few8(Few8Args& a) {
 }
 int64_t few8_floats(const Few8Args& a) { return (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
 int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
+
+// More rows than that: as plan_rows has it, without its kinds of several groups of waves, and with 128 rows a workgroup, which become 16-bit keys and values half as often, also
+// where their keys have to be shared for two workgroups a CU, while a share has chunks enough: 12, or 8 where blocks of 64 rows would not fill the chip either.  us, by
+// 64 rows / 128: 8 kv heads of 4 query heads, d = 128, 8192 keys, 128 queries 53 / 48, 256 84 / 66, 512 151 / 104, 1024 272 / 180; 8 sequences of 64 queries on up to 4000 93 / 70;
+// but 32 queries 27 / 32, 64 36 / 37.5, 1024 under a window of 1024 42 / 56.
+int plan_rows8(BandArgs& a) {
+  const int cus = dlt_device_cus();
+  const int64_t bh = (int64_t)a.B * a.Hkv, blocks = (a.rows + 127) / 128, wgs = bh * blocks;
+  const int chunks = (int)dlt_imin64((int64_t)a.W + a.S + 128 / a.G + 1, a.Lk) / 64 + 1;
+  const int64_t n = wgs > 0 ? (2 * cus + wgs / 2) / wgs : 1, least = bh * ((a.rows + 63) / 64) >= cus ? 12 : 8;
+  const int64_t bytes = bh * a.rows * (a.dv_ + 2) * 4;
+  if (a.rows <= 128 || n <= 1 || n > BAND_SHARES_MAX || chunks / n < least || n * bytes > DLT_WINDOW_WORKSPACE_MAX) return plan_rows(a, true, false);
+  a.nblk = (int)blocks;
+  a.shares = (int)n;
+  set_map(a);
+  return BAND_TWO;
+}
 }  // namespace
 
 extern "C" int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes) {
@@ -586,7 +603,7 @@ extern "C" int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_sc
     *bytes = few8_bytes(a);
     return DLT_OK;
   }
-  plan_rows(a, true, false);
+  plan_rows8(a);
   *bytes = rows_bytes(a);
   return DLT_OK;
 }
@@ -605,7 +622,7 @@ extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const 
   DLT_REQUIRE(table != nullptr && seq_len != nullptr, "%s: table or seq_len is NULL", who);
   DLT_REQUIRE(table_stride >= 0, "%s: negative table stride", who);
   const bool few = plan_few8(a);
-  const int kind = few ? 0 : plan_rows(a, true, false);
+  const int kind = few ? 0 : plan_rows8(a);
   if ((rc = check_ws(who, ws, ws_bytes, few ? few8_bytes(a) : rows_bytes(a))) != DLT_OK) return rc;
   if (!few && (rc = check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;

@@ -256,18 +256,20 @@ struct BandStage8 {
       }
     }
   }
-  // tokens from `live` on are written as zeros
-  DLT_DEV void put(char* dst, const u32x4 (&x)[NI], float scale, int live) const {
+  DLT_DEV void put(char* dst, const u32x4 (&x)[NI], float scale) const {
 #pragma unroll
     for (int i = 0; i < NI; i++) {
       const int t = t0 + TPI * i;
-      const bool on = t < live;
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const u32x4 v = cvt8_eight<FMT, TIO>(x[i][2 * u], x[i][2 * u + 1], scale);
-        lds_write16(dst + t * R::ROW + 16 * ((2 * c + u) ^ R::swz(t)), on ? v : u32x4{0u, 0u, 0u, 0u});
-      }
+      for (int u = 0; u < 2; u++) lds_write16(dst + t * R::ROW + 16 * ((2 * c + u) ^ R::swz(t)), cvt8_eight<FMT, TIO>(x[i][2 * u], x[i][2 * u + 1], scale));
     }
+  }
+  // tokens from `live` on become zeros
+  DLT_DEV void clear(u32x4 (&x)[NI], int live) const {
+#pragma unroll
+    for (int i = 0; i < NI; i++)
+#pragma unroll
+      for (int u = 0; u < 4; u++) x[i][u] = t0 + TPI * i < live ? x[i][u] : 0u;
   }
 };
 

@@ -205,11 +205,25 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   u32x4 rk[NG][S8::NI], rv[NG][S8::NI];
   int ek[NG], ev[NG];
   Groups next8;
+  // pages as the table has them, through the scalar cache: a wait for a vector load would be one for the keys and values that were asked for before it
+  auto lookup8 = [&](int i) __attribute__((always_inline)) {
+    Groups x;
+    if constexpr (F8 != 0) {
+#pragma unroll
+      for (int u = 0; u < NG; u++) {
+        const int t16 = dlt_imax(0, dlt_imin(W.tok(CK * i + wave * 16 * NG + 16 * u), sq.n_k - 1)) >> 4;
+        const int pi = __builtin_amdgcn_readfirstlane((int)dlt_fastdiv((uint32_t)t16, a.pg.m16, a.pg.s16));
+        x.in16[u] = t16 - pi * a.pg.p16;
+        x.page[u] = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)pages)[pi];
+      }
+    }
+    return x;
+  };
   auto fetch8 = [&](const Groups& x) __attribute__((always_inline)) {
     if constexpr (F8 != 0) {
 #pragma unroll
       for (int u = 0; u < NG; u++) {
-        const int page = x.page[u], blk = (int)dlt_fastdiv((uint32_t)x.in16[u], a.mB, a.sB);
+        const int page = dlt_imax(0, dlt_imin(x.page[u], a.pg.n_pages - 1)), blk = (int)dlt_fastdiv((uint32_t)x.in16[u], a.mB, a.sB);
         const int64_t row = 16 * x.in16[u];
         stk8.fetch(reinterpret_cast<const char*>(kh) + (page * a.ks[0] + row * a.ks[2]), rk[u]);
         stv8.fetch(reinterpret_cast<const char*>(vh) + (page * a.vs[0] + row * a.vs[2]), rv[u]);
@@ -222,10 +236,15 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
     if constexpr (F8 != 0) {
 #pragma unroll
       for (int u = 0; u < NG; u++) {
-        const int live = sq.n_k - W.tok(CK * i + wave * 16 * NG + 16 * u);   // tokens of the sequence; what lies behind them is written as zeros
+        const int live = sq.n_k - W.tok(CK * i + wave * 16 * NG + 16 * u);   // tokens of the sequence
+        if (live < 16) {   // pages hold anything behind them: those values, which no row sees, are cleared, and so are scales of blocks of nothing else
+          keep_branch();
+          stv8.clear(rv[u], live);
+          if (live <= 0) ev[u] = 127;
+        }
         char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
-        stk8.put(dst, rk[u], cvt8_scale(ek[u]), live);
-        stv8.put(dst + B::REG, rv[u], cvt8_scale(ev[u]), live);
+        stk8.put(dst, rk[u], cvt8_scale(ek[u]));
+        stv8.put(dst + B::REG, rv[u], cvt8_scale(ev[u]));
       }
     }
   };
@@ -234,8 +253,8 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   if constexpr (F8 != 0) {
     stk8.init(lane, a.dk_, a.ks[2]);
     stv8.init(lane, a.dv_, a.vs[2]);
-    const Groups x0 = lookup(i_beg), x1 = lookup(i_beg + 1);
-    next8 = lookup(i_beg + 2);
+    const Groups x0 = lookup8(i_beg), x1 = lookup8(i_beg + 1);
+    next8 = lookup8(i_beg + 2);
     if (i_beg < i_end) {
       fetch8(x0);
       put8(i_beg, bufs);
@@ -401,7 +420,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       // the next chunk to LDS, where the last one was; the one behind it on its way beside the products
       if (i + 1 < i_end) put8(i + 1, buf_of(bi + 1));
       if (i + 2 < i_end) fetch8(next8);
-      next8 = lookup(i + 3);
+      next8 = lookup8(i + 3);
       chunk(i, buf_of(bi), mask_tag);
       bi = bi + 1 == NBUF ? 0 : bi + 1;
       it++;
