@@ -553,6 +553,8 @@ int check_rows8(const char* who, const char* name, const void* p, const int64_t*
 }  // namespace
 
 namespace {
+int64_t few8_floats(const Few8Args& a) { return (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
+int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
 // Up to 32 rows of a group: the kernels of page_few8.h (false: not for them).  A workgroup to each head where that is good enough, since it needs no second launch:
 // contexts of up to 1024 keys (8 sequences of up to 1000, 8 kv heads, d = 128, 11.3 us either way), and of up to 2560 where the heads fill the CUs (us, whole heads / runs: 64
 // sequences of up to 2000, 8 kv heads, d = 128, 35.0 / 38.2; 32 under a window of 1024 15.9 / 21.3; but 32 of up to 4000 48 / 43, 16 under a window of 4096, 128 heads, 50 /
@@ -569,12 +571,10 @@ bool plan_few8(Few8Args& a) {
   // 16 waves while a head has a tile for each at most and workgroups a CU for each: one token on 300 keys, 8 heads, d = 64, 8.0 -> 7.2 us
   a.waves = a.rows <= 16 && bh <= cus && most <= 16 * (band_class(a.dk_, a.dv_) == 64 ? 64 : 32) ? 16 : 4;
   if (most > (bh >= cus ? 2560 : 1024) && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = a.want + (int)bh;
+  if (few8_bytes(a) > DLT_WINDOW_WORKSPACE_MAX) a.wgs = 0;
   dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);
   return true;
 }
-int64_t few8_floats(const Few8Args& a) { return (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
-int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
-
 // More rows than that: as plan_rows has it, without its kinds of several groups of waves, and with 128 rows a workgroup, which become 16-bit keys and values half as often, also
 // where their keys have to be shared for two workgroups a CU, while a share has chunks enough: 12, or 8 where blocks of 64 rows would not fill the chip either.  us, by
 // 64 rows / 128: 8 kv heads of 4 query heads, d = 128, 8192 keys, 128 queries 53 / 48, 256 84 / 66, 512 151 / 104, 1024 272 / 180; 8 sequences of 64 queries on up to 4000 93 / 70;

@@ -208,12 +208,12 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
   a.B = B; a.cols = cols; a.page = page; a.n_pages = n_pages; a.T = T;
   dlt_fastdiv_make((uint32_t)page, a.mp, a.sp);
   dlt_fastdiv_make((uint32_t)dlt_imax(T, 1), a.mt, a.st);
-  constexpr int NT = 256;
-  // slots by fours, and columns that requests can gain (give back, without a limit to the slots): one of them to a thread, but no more than two workgroups a CU, each of
-  // which is another atomic on the pool's word: 1000 requests, 4000 slots each, 256 / 512 / 1024 workgroups 30 / 22 / 25 us (with lengths read again for every slot)
+  constexpr int NT = 1024;
+  // Slots by fours, and columns that requests can gain (give back, without a limit to the slots), 256 of them to a workgroup, up to a workgroup a CU.  Each is another atomic
+  // on the pool's word, so they are large: 1000 requests, 4000 slots each, and back, 256 of 1024 threads 15.0 + 8.2 us, 128 17.8 + 8.2, 512 of 256 18.8 + 8.6.
   const int64_t work = (int64_t)B * dlt_imax(T, 1) / 4 + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols), cus = dlt_device_cus();
   // (small calls up to eight, so that columns and slots are not one after the other: 64 requests, one token more, 6.5 -> 6.0 us)
-  const int64_t grid = std::max<int64_t>(1, std::max<int64_t>(std::min<int64_t>(work / 16, 8), std::min<int64_t>(work / NT, (T >= 0 ? 2 : 1) * cus)));
+  const int64_t grid = std::max<int64_t>(1, std::max<int64_t>(std::min<int64_t>(work / 16, 8), std::min<int64_t>(work / 256, cus)));
   const int lds = 4 * (B + 1) * 4;
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
   if (rc != DLT_OK) return rc;

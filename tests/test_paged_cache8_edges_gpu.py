@@ -275,6 +275,47 @@ def test_inference_mode_and_no_graph():
         assert page_assign_(t, s, ints([20]), p, 16, 32)[0].tolist() == [20]
 
 
+@pytest.mark.parametrize("layout", ["blocks", "halves"])
+@pytest.mark.parametrize("sections", [(8, 16, 8), (5, 11, 0)])
+def test_given_positions_of_several_axes(layout, sections):
+    """Positions that are handed in, one set for all sequences or one each, some of them negative: keys and queries turn by those, not by their places."""
+    gen = torch.Generator().manual_seed(9)
+    B, H, Hkv, T, page, d, lens, new = 2, 4, 2, 21, 32, 64, [50, 30], [21, 13]
+    kc, vc, ks, vs, table = pool(gen, B, Hkv, page, 16, lens, d, d, FP8)
+    k, v, q = (torch.randn(B, h, T, d, generator=gen).to(BF) for h in (Hkv, Hkv, H))
+    tables = [orc.table(40, r) for r in sections]
+    for shape in ((3, T), (3, B, T)):
+        pos = torch.randint(-3, 40, shape, generator=gen).int()
+        live = torch.tensor([[t < n for t in range(T)] for n in new])
+        each = torch.where(live, pos if pos.dim() == 3 else pos[:, None], -1).int()      # padding does not turn
+        rk, rq = orc.rotate(k, each, tables, layout), orc.rotate(q, each, tables, layout)
+        got = [x.cuda() for x in (kc, vc, ks, vs)]
+        out = paged8_append_(*got, k.cuda(), v.cuda(), table.cuda(), ints(lens), ints(new), (pos.cuda(), [t.cuda() for t in tables], layout), q.cuda())
+        c, e, tol, near = orc8.append(kc, ks, rk[0], k.double().abs().amax(-1, keepdim=True).expand_as(k) * 2, table, lens, new, BF)
+        assert not near.any() and torch.equal(got[2].cpu().view(torch.uint8).int(), e)
+        assert ((got[0].cpu().float().double() - c).abs() <= tol).all()
+        orc.check(out.cpu(), rq, "queries")
+
+
+def test_a_block_of_nan_stays_until_it_is_begun_again():
+    """int8: one NaN makes its block's scale NaN; tokens that join keep it so, and the block's next first token ends it."""
+    kc, vc = (torch.zeros(1, 1, 32, 64, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.full((1, 1, 2), 100, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu) for _ in range(2))
+    x = torch.ones(1, 1, 4, 64, dtype=BF, device="cuda")
+    bad = x.clone()
+    bad[0, 0, 2, 9] = float("inf")
+    bits = lambda: ks.view(torch.uint8).flatten().tolist()  # noqa: E731
+    paged8_append_(kc, vc, ks, vs, bad, x, ints([[0]]), ints([4]))
+    assert bits() == [255, 100] and vs.view(torch.uint8).flatten().tolist()[0] == 127 - 6
+    paged8_append_(kc, vc, ks, vs, x, x, ints([[0]]), ints([8]))
+    assert bits() == [255, 100]
+    q = torch.ones(1, 1, 2, 64, dtype=BF, device="cuda")
+    assert torch.isnan(paged8_attention(q, kc, vc, ks, vs, ints([[0]]), ints([8]))).all()
+    paged8_append_(kc, vc, ks, vs, x, x, ints([[0]]), ints([4]))
+    assert bits() == [127 - 6, 100]
+    assert (paged8_attention(q, kc, vc, ks, vs, ints([[0]]), ints([4])) == 1).all()
+
+
 class Server:
     """Requests that come, take tokens (some of them guessed and taken back) and end, over the three operators.  What a sequence was given is kept beside it."""
 
