@@ -556,7 +556,7 @@ namespace {
 int64_t few8_floats(const Few8Args& a) { return (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
 int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
 // Up to 32 rows of a group: the kernels of page_few8.h (false: not for them).  A workgroup to each head where that is good enough, since it needs no second launch:
-// contexts of up to 1024 keys (8 sequences of up to 1000, 8 kv heads, d = 128, 11.3 us either way), and of up to 2560 where the heads fill the CUs (us, whole heads / runs: 64
+// contexts of up to 1024 keys (8 sequences of up to 1000, 8 kv heads, d = 128, 10.5 us either way), and of up to 2560 where the heads fill the CUs (us, whole heads / runs: 64
 // sequences of up to 2000, 8 kv heads, d = 128, 35.0 / 38.2; 32 under a window of 1024 15.9 / 21.3; but 32 of up to 4000 48 / 43, 16 under a window of 4096, 128 heads, 50 /
 // 32).  Both rules go by the table's width and the window, since lengths stay on the device.
 // Runs: two workgroups a CU, one where the steps are few (few8_run) or a workgroup has two blocks of rows: 16 sequences, one of 32768 and 15 of 500, 4 kv heads, 18.0 us with
@@ -568,8 +568,9 @@ bool plan_few8(Few8Args& a) {
   a.wgs = 0;
   a.want = (a.rows <= 16 ? 2 : 1) * cus;
   a.want_few = cus;
-  // 16 waves while a head has a tile for each at most and workgroups a CU for each: one token on 300 keys, 8 heads, d = 64, 8.0 -> 7.2 us
-  a.waves = a.rows <= 16 && bh <= cus && most <= 16 * (band_class(a.dk_, a.dv_) == 64 ? 64 : 32) ? 16 : 4;
+  // eight waves where there is no more than a workgroup a CU (us, four / eight / sixteen: one token on 300 keys, 8 heads, d = 64, 6.9 / 6.8 / 7.1, on 1000, d = 128, 11.8 / 10.7 /
+  // 11.9; 32 sequences of up to 500, 8 heads, d = 128, 9.5 / 9.2 / 10.1)
+  a.waves = a.rows <= 16 && bh <= cus ? 8 : 4;
   if (most > (bh >= cus ? 2560 : 1024) && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = a.want + (int)bh;
   if (few8_bytes(a) > DLT_WINDOW_WORKSPACE_MAX) a.wgs = 0;
   dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);

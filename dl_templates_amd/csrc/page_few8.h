@@ -133,8 +133,8 @@ DLT_DEV u32x4 few8_values(unsigned a, unsigned b, float scale_a, float scale_b) 
 
 // FULL: both tensors have D dims, K's rows lie at multiples of 16 bytes.  BAL: a run of steps to a workgroup, else a (batch, kv head).
 template <typename TIO, int D, int NP, int FMT, bool FULL, int NW, bool BAL>
-__global__ __launch_bounds__(64 * NW, NW == 16 ? 4 : NP == 1 ? 3 : 2) void few8_kernel(const Few8Args a) {
-  static_assert(NW == 4 || (NW == 16 && !BAL), "a step is four tiles");
+__global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_kernel(const Few8Args a) {
+  static_assert(NW == 4 || !BAL, "a step is four tiles");
   dlt_kernargs_in<sizeof(Few8Args)>();
   typedef Few8<D> F;
   constexpr int NG = F::NG, VB = F::VB, KC = F::KC, VW = F::VW, TK = F::TK;

@@ -26,7 +26,7 @@ int few8_nw(const Few8Args& a, bool full, int64_t grid, hipStream_t stream) {
 template <typename TIO, int NP, int FMT>
 int few8_np(const Few8Args& a, bool full, hipStream_t stream) {
   if constexpr (NP == 1)
-    if (a.wgs == 0 && a.waves == 16) return few8_nw<TIO, NP, FMT, 16, false>(a, full, (int64_t)a.B * a.Hkv, stream);
+    if (a.wgs == 0 && a.waves == 8) return few8_nw<TIO, NP, FMT, 8, false>(a, full, (int64_t)a.B * a.Hkv, stream);
   if (a.wgs == 0) return few8_nw<TIO, NP, FMT, 4, false>(a, full, (int64_t)a.B * a.Hkv, stream);
   const int rc = few8_nw<TIO, NP, FMT, 4, true>(a, full, a.wgs, stream);
   if (rc != DLT_OK) return rc;
