@@ -568,9 +568,9 @@ bool plan_few8(Few8Args& a) {
   a.wgs = 0;
   a.want = (a.rows <= 16 ? 2 : 1) * cus;
   a.want_few = cus;
-  // eight waves where there is no more than a workgroup a CU (us, four / eight / sixteen: one token on 300 keys, 8 heads, d = 64, 6.9 / 6.8 / 7.1, on 1000, d = 128, 11.8 / 10.7 /
-  // 11.9; 32 sequences of up to 500, 8 heads, d = 128, 9.5 / 9.2 / 10.1)
-  a.waves = a.rows <= 16 && bh <= cus ? 8 : 4;
+  // eight waves to a head where heads make less than two workgroups a CU (us, four / eight / sixteen: one token on 300 keys, 8 heads, d = 64, 6.9 / 6.8 / 7.1, on 1000, d = 128,
+  // 11.8 / 10.7 / 11.9; 32 sequences of up to 500, 8 heads, d = 128, 9.5 / 9.2 / 10.1; 48 under a window of 2048, 8 heads, d = 64, 28.5 / 25.3; but 64 of up to 2000 35 / 39)
+  a.waves = a.rows <= 16 && bh < 2 * cus ? 8 : 4;
   if (most > (bh >= cus ? 2560 : 1024) && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = a.want + (int)bh;
   if (few8_bytes(a) > DLT_WINDOW_WORKSPACE_MAX) a.wgs = 0;
   dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);
