@@ -233,36 +233,45 @@ struct BandStage8 {
   typedef FlashDRow<D> R;
   typedef u32x4 quad __attribute__((aligned(8)));
   static constexpr int LPT = D / 16, TPI = 64 / LPT, NI = 16 / TPI;   // lanes of a token, tokens and number of loads
-  uint32_t off[NI];
+  uint32_t off, at;   // of the lane's first piece in memory and in LDS
+  int64_t sn;
   int t0, c, full;   // full: 16-byte pieces that lie in the row; its last one may be half
   bool half;
-  DLT_DEV void init(int lane, int dims, int64_t sn) {
+  DLT_DEV void init(int lane, int dims, int64_t sn_) {
     t0 = lane / LPT;
     c = lane % LPT;
     full = dims >> 4;
     half = (dims & 15) != 0 && c == full;
-#pragma unroll
-    for (int i = 0; i < NI; i++) off[i] = (uint32_t)(t0 + TPI * i) * (uint32_t)sn + 16u * (uint32_t)c;
+    sn = sn_;
+    off = (uint32_t)t0 * (uint32_t)sn + 16u * (uint32_t)c;
+    at = t0 * R::ROW + 16 * ((2 * c) ^ R::swz(t0));   // swz(t0 + TPI) = swz(t0)
   }
   DLT_DEV void fetch(const char* base, u32x4 (&x)[NI]) const {
+    uint32_t o = off;
+    asm volatile("" : "+v"(o));   // a 32-bit offset beside a wave-uniform address, not a 64-bit one kept for every load
+    if (full == LPT) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) x[i] = *reinterpret_cast<const quad*>(base + TPI * i * sn + o);
+      return;
+    }
+    keep_branch();
 #pragma unroll
     for (int i = 0; i < NI; i++) {
       x[i] = u32x4{0u, 0u, 0u, 0u};
-      if (c < full) x[i] = *reinterpret_cast<const quad*>(base + off[i]);
+      if (c < full) x[i] = *reinterpret_cast<const quad*>(base + TPI * i * sn + o);
       else if (half) {
-        const u32x2 h = *reinterpret_cast<const u32x2*>(base + off[i]);
+        const u32x2 h = *reinterpret_cast<const u32x2*>(base + TPI * i * sn + o);
         x[i][0] = h[0];
         x[i][1] = h[1];
       }
     }
   }
+  // piece J of 2 NI
+  template <int J>
   DLT_DEV void put(char* dst, const u32x4 (&x)[NI], float scale) const {
-#pragma unroll
-    for (int i = 0; i < NI; i++) {
-      const int t = t0 + TPI * i;
-#pragma unroll
-      for (int u = 0; u < 2; u++) lds_write16(dst + t * R::ROW + 16 * ((2 * c + u) ^ R::swz(t)), cvt8_eight<FMT, TIO>(x[i][2 * u], x[i][2 * u + 1], scale));
-    }
+    constexpr int i = J / 2, u = J % 2;
+    static_assert(i < NI, "a piece of the lane");
+    lds_write16(dst + (u == 0 ? at : D == 128 ? at + 16 : at ^ 16) + TPI * i * R::ROW, cvt8_eight<FMT, TIO>(x[i][2 * u], x[i][2 * u + 1], scale));
   }
   // tokens from `live` on become zeros
   DLT_DEV void clear(u32x4 (&x)[NI], int live) const {

@@ -199,68 +199,56 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       }
     }
   };
-  // 8-bit numbers: the wave's tokens of the chunk behind the next one are on their way in registers
+  // 8-bit numbers: the wave's 16 tokens of the chunk behind the next one are on their way in registers.  Pages of 64 chunks are looked up at once, a lane each: a load of one
+  // page a chunk, scalar or not, is a trip to memory that waits in the products end on.
   typedef BandStage8<D, F8 == 2 ? DLT_INT8 : DLT_FP8_E4M3, TIO> S8;
+  static_assert(F8 == 0 || NG == 1, "16 tokens of a chunk a wave");
   S8 stk8, stv8;
-  u32x4 rk[NG][S8::NI], rv[NG][S8::NI];
-  int ek[NG], ev[NG];
-  Groups next8;
-  // pages as the table has them, through the scalar cache: a wait for a vector load would be one for the keys and values that were asked for before it
-  auto lookup8 = [&](int i) __attribute__((always_inline)) {
-    Groups x;
+  u32x4 rk[S8::NI], rv[S8::NI];
+  int ek, ev, page64;
+  // (tokens behind the last one are taken back to it; the table has a column for position 0)
+  auto fetch8 = [&](int i) __attribute__((always_inline)) {
     if constexpr (F8 != 0) {
-#pragma unroll
-      for (int u = 0; u < NG; u++) {
-        const int t16 = dlt_imax(0, dlt_imin(W.tok(CK * i + wave * 16 * NG + 16 * u), sq.n_k - 1)) >> 4;
-        const int pi = __builtin_amdgcn_readfirstlane((int)dlt_fastdiv((uint32_t)t16, a.pg.m16, a.pg.s16));
-        x.in16[u] = t16 - pi * a.pg.p16;
-        x.page[u] = ((const __attribute__((address_space(4))) int32_t*)(uintptr_t)pages)[pi];
-      }
-    }
-    return x;
-  };
-  auto fetch8 = [&](const Groups& x) __attribute__((always_inline)) {
-    if constexpr (F8 != 0) {
-#pragma unroll
-      for (int u = 0; u < NG; u++) {
-        const int page = dlt_imax(0, dlt_imin(x.page[u], a.pg.n_pages - 1)), blk = (int)dlt_fastdiv((uint32_t)x.in16[u], a.mB, a.sB);
-        const int64_t row = 16 * x.in16[u];
-        stk8.fetch(reinterpret_cast<const char*>(kh) + (page * a.ks[0] + row * a.ks[2]), rk[u]);
-        stv8.fetch(reinterpret_cast<const char*>(vh) + (page * a.vs[0] + row * a.vs[2]), rv[u]);
-        ek[u] = a.k_sc[page * a.kss[0] + h * a.kss[1] + blk * a.kss[2]];
-        ev[u] = a.v_sc[page * a.vss[0] + h * a.vss[1] + blk * a.vss[2]];
-      }
+      auto group = [&](int c) __attribute__((always_inline)) { return dlt_imax(0, dlt_imin(W.tok(CK * c + wave * 16), sq.n_k - 1)) >> 4; };
+      const int u = (i - i_beg) & 63;
+      if (u == 0) page64 = pages[dlt_fastdiv((uint32_t)group(i + lane), a.pg.m16, a.pg.s16)];
+      const int t16 = group(i), in16 = t16 - (int)dlt_fastdiv((uint32_t)t16, a.pg.m16, a.pg.s16) * a.pg.p16, blk = (int)dlt_fastdiv((uint32_t)in16, a.mB, a.sB);
+      const int page = dlt_imax(0, dlt_imin(__builtin_amdgcn_readlane(page64, u), a.pg.n_pages - 1));
+      const int64_t row = 16 * in16;
+      stk8.fetch(reinterpret_cast<const char*>(kh) + (page * a.ks[0] + row * a.ks[2]), rk);
+      stv8.fetch(reinterpret_cast<const char*>(vh) + (page * a.vs[0] + row * a.vs[2]), rv);
+      ek = a.k_sc[page * a.kss[0] + h * a.kss[1] + blk * a.kss[2]];
+      ev = a.v_sc[page * a.vss[0] + h * a.vss[1] + blk * a.vss[2]];
     }
   };
-  auto put8 = [&](int i, char* buf) __attribute__((always_inline)) {
-    if constexpr (F8 != 0) {
-#pragma unroll
-      for (int u = 0; u < NG; u++) {
-        const int live = sq.n_k - W.tok(CK * i + wave * 16 * NG + 16 * u);   // tokens of the sequence
-        if (live < 16) {   // pages hold anything behind them: those values, which no row sees, are cleared, and so are scales of blocks of nothing else
-          keep_branch();
-          stv8.clear(rv[u], live);
-          if (live <= 0) ev[u] = 127;
-        }
-        char* dst = buf + (wave * 16 * NG + 16 * u) * 2 * D;
-        stk8.put(dst, rk[u], cvt8_scale(ek[u]));
-        stv8.put(dst + B::REG, rv[u], cvt8_scale(ev[u]));
-      }
+  // before chunk i goes to LDS: pages hold anything behind the last token; those values, which no row sees, are cleared, and so are scales of blocks of nothing else
+  auto settle8 = [&](int i) __attribute__((always_inline)) {
+    const int live = sq.n_k - W.tok(CK * i + wave * 16);
+    if (live < 16) {
+      keep_branch();
+      stv8.clear(rv, live);
+      if (live <= 0) ev = 127;
     }
   };
-  // Pages of the first chunks are looked up together: one trip to memory, not one a chunk (a token each of 8 sequences of up to 900, d = 64: 10.7 -> 10.1 us;
-  // one sequence of 5000, d = 128: 10.1 -> 8.7; large grids alike).  Looked up behind the last chunk too: the table has a column for position 0.
+  constexpr int PUTS = F8 != 0 ? 4 * S8::NI : 0;   // 16-byte writes of a wave
+  auto put8 = [&](char* buf, auto jc) __attribute__((always_inline)) {
+    constexpr int j = decltype(jc)::value;
+    char* dst = buf + wave * 16 * 2 * D;
+    if constexpr (j < 2 * S8::NI) stk8.template put<j>(dst, rk, cvt8_scale(ek));
+    else stv8.template put<j - 2 * S8::NI>(dst + B::REG, rv, cvt8_scale(ev));
+  };
   if constexpr (F8 != 0) {
     stk8.init(lane, a.dk_, a.ks[2]);
     stv8.init(lane, a.dv_, a.vs[2]);
-    const Groups x0 = lookup8(i_beg), x1 = lookup8(i_beg + 1);
-    next8 = lookup8(i_beg + 2);
     if (i_beg < i_end) {
-      fetch8(x0);
-      put8(i_beg, bufs);
-      if (i_beg + 1 < i_end) fetch8(x1);
+      fetch8(i_beg);
+      settle8(i_beg);
+      swa2_for<0, PUTS>([&](auto jc) __attribute__((always_inline)) { put8(bufs, jc); });
+      if (i_beg + 1 < i_end) fetch8(i_beg + 1);
     }
   } else if constexpr (PAGED) {
+    // Pages of the first chunks are looked up together: one trip to memory, not one a chunk (a token each of 8 sequences of up to 900, d = 64: 10.7 -> 10.1 us;
+    // one sequence of 5000, d = 128: 10.1 -> 8.7; large grids alike).  Looked up behind the last chunk too: the table has a column for position 0.
     Groups x[AHEAD];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++) x[i] = lookup(i_beg + i * GR + grp);
@@ -300,9 +288,9 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   }
   const float scale = a.scale_log2;
   const unsigned one2 = pack2<TIO>(1.f, 1.f);
-  const u32x4 ones = n == 0 ? u32x4{one2, one2, one2, one2} : u32x4{0u, 0u, 0u, 0u};
-  FlashDLane<D> L;
-  flashd_lane_init(L, n, g);
+  const u32x4 row_of_ones = n == 0 ? u32x4{one2, one2, one2, one2} : u32x4{0u, 0u, 0u, 0u};
+  FlashDLane<D> lanes;
+  flashd_lane_init(lanes, n, g);
 
   if constexpr (F8 == 0) swa2_wait_copies();
   pin_loaded(qf);
@@ -311,12 +299,26 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
     if (F8 == 0 && i_beg + i * GR + grp < i_end) settle(i_beg + i * GR + grp, bufs + i * B::BUF);
   __syncthreads();
 
-  auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag) __attribute__((always_inline)) {
+  // beside(k): what runs beside the k-th operand's products
+  auto consume = [&](const int x, Swa2Lds __restrict__ cur, auto mask_tag, auto beside) __attribute__((always_inline)) {
     constexpr bool MASK = decltype(mask_tag)::value;
     Swa2Lds sK = cur, sV = cur + B::REG;
     constexpr int N1 = NKB * 2 * KC, NT = N1 + NKB * VB;
     constexpr int RD = 1;   // LDS reads ahead of the matrix instruction (2 to 6: no faster)
     u32x4 ring[RD + 1];
+    // 8-bit numbers under way take registers that places in LDS would fill: those are formed from one, a[c] = a[0] ^ 64 c and tr[d] = tr[0] ^ 32 d, and so is the row of ones
+    FlashDLane<D> L = lanes;
+    u32x4 ones = row_of_ones;
+    if constexpr (F8 != 0) {
+      int a0 = lanes.a[0], t0 = lanes.tr[0];
+      unsigned o = row_of_ones[0];
+      asm volatile("" : "+v"(a0), "+v"(t0), "+v"(o));
+#pragma unroll
+      for (int c = 0; c < D / 32; c++) L.a[c] = a0 ^ 64 * c;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) L.tr[d] = t0 ^ 32 * d;
+      ones = u32x4{o, o, o, o};
+    }
     auto rd = [&](auto kc) __attribute__((always_inline)) {
       constexpr int k = decltype(kc)::value;
       if constexpr (k < N1) {
@@ -345,6 +347,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
         constexpr int kb = k / (2 * KC), mb = (k / KC) % 2, r = k % KC;
 #pragma unroll
         for (int p = 0; p < NP; p++) s[p] = Mma<TIO>::mfma(op, qf[p][r], r == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[p]);
+        beside(kc);
         if constexpr (r == KC - 1) {
 #pragma unroll
           for (int p = 0; p < NP; p++)
@@ -403,10 +406,10 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
       }
     });
   };
-  auto chunk = [&](int i, char* buf, auto mask_tag) __attribute__((always_inline)) {
+  auto chunk = [&](int i, char* buf, auto mask_tag, auto beside) __attribute__((always_inline)) {
     const int x = CK * i;
     if (decltype(mask_tag)::value && (x > pb || (x + CK - 1 <= pa - a.W && x >= a.S))) return;   // no row of the wave sees any of it
-    consume(x, (Swa2Lds)buf, mask_tag);
+    consume(x, (Swa2Lds)buf, mask_tag, beside);
   };
   int f0, f1;
   W.whole(first, last, a.W, i_beg, i_end, f0, f1);
@@ -417,11 +420,21 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   auto step = [&](auto mask_tag) __attribute__((always_inline)) {
     const int i = i_beg + it * GR + grp;
     if constexpr (F8 != 0) {
-      // the next chunk to LDS, where the last one was; the one behind it on its way beside the products
-      if (i + 1 < i_end) put8(i + 1, buf_of(bi + 1));
-      if (i + 2 < i_end) fetch8(next8);
-      next8 = lookup8(i + 3);
-      chunk(i, buf_of(bi), mask_tag);
+      // The next chunk goes to LDS, where the last one was, beside the products of S, which leave the vector units idle; in masked chunks before them (beside them the compiler
+      // runs out of registers: whole-number caches 115 -> 135 us).  Behind the last chunk nothing reads what is written.  512 tokens over 8192, 32 heads on 8, d = 128, all
+      // pieces ahead of the products -> this: 110 -> 98 us (int8 115 -> 108), 2048 tokens 330 -> 275.
+      settle8(i + 1);
+      char* const next = buf_of(bi + 1);
+      if constexpr (decltype(mask_tag)::value) {
+        swa2_for<0, PUTS>([&](auto jc) __attribute__((always_inline)) { put8(next, jc); });
+        chunk(i, buf_of(bi), mask_tag, [](auto) __attribute__((always_inline)) {});
+      } else {
+        chunk(i, buf_of(bi), mask_tag, [&](auto kc) __attribute__((always_inline)) {
+          constexpr int k = decltype(kc)::value, every = NKB * 2 * KC / PUTS;
+          if constexpr (k % every == every - 1 && k / every < PUTS) put8(next, std::integral_constant<int, k / every>{});
+        });
+      }
+      if (i + 2 < i_end) fetch8(i + 2);
       bi = bi + 1 == NBUF ? 0 : bi + 1;
       it++;
       __syncthreads();
@@ -429,7 +442,7 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
     }
     const bool more = i + AHEAD * GR < i_end;
     if (more) issue(i + AHEAD * GR, buf_of(bi + AHEAD), lookup(i + AHEAD * GR));
-    if (GR == 1 || !decltype(mask_tag)::value || i < i_end) chunk(i, buf_of(bi), mask_tag);
+    if (GR == 1 || !decltype(mask_tag)::value || i < i_end) chunk(i, buf_of(bi), mask_tag, [](auto) __attribute__((always_inline)) {});
     if (more) flashd_wait_copies<(AHEAD - 1) * PER_CHUNK>();
     else swa2_wait_copies();
     bi = bi + 1 == NBUF ? 0 : bi + 1;

@@ -399,3 +399,17 @@ def test_a_captured_step(fmt, T):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)), i
         a.check(out)
         b.check(want)
+
+
+@pytest.mark.parametrize("T, d, dtype, fmt, window, n_sink", [(40, 64, HF, I8, None, 0), (130, 128, BF, FP8, None, 0), (40, 128, HF, FP8, 4300, 70), (130, 64, BF, I8, 4222, 1)])
+def test_a_workgroup_with_more_than_64_chunks(T, d, dtype, fmt, window, n_sink):
+    """64 sequences whose tables name the same pages: every workgroup walks the whole context of 4500 tokens."""
+    gen = torch.Generator().manual_seed(70)
+    case = (1, 8, 8, T, 64, 32, [4500], None, d, d, window, n_sink, dtype, fmt)
+    kc, vc, ks, vs, table = cache_for(case, gen)
+    q = torch.randn(1, 8, T, d, generator=gen).to(dtype)
+    scale = 0.3 / math.sqrt(d)
+    o = paged8_attention(q.cuda().expand(64, -1, -1, -1).contiguous(), *(x.cuda() for x in (kc, vc, ks, vs)), table.cuda().expand(64, -1).contiguous(), ints([4500] * 64), window, n_sink,
+                         scale)
+    assert (o == o[:1]).all()
+    check(case, o[:1].cpu(), q, (kc, vc, ks, vs, table), [T], scale)
