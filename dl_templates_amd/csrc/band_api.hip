@@ -578,8 +578,8 @@ bool plan_few8(Few8Args& a) {
 }
 // More rows than that: as plan_rows has it, without its kinds of several groups of waves, and with 128 rows a workgroup, which become 16-bit keys and values half as often, also
 // where their keys have to be shared for two workgroups a CU, while a share has chunks enough: 12, or 8 where blocks of 64 rows would not fill the chip either.  us, by
-// 64 rows / 128: 8 kv heads of 4 query heads, d = 128, 8192 keys, 128 queries 53 / 48, 256 84 / 66, 512 151 / 104, 1024 272 / 180; 8 sequences of 64 queries on up to 4000 93 / 70;
-// but 32 queries 27 / 32, 64 36 / 37.5, 1024 under a window of 1024 42 / 56.
+// 64 rows / 128: 8 kv heads of 4 query heads, d = 128, 8192 keys, 128 queries 48 / 46, 256 73 / 64, 512 130 / 98, 1024 216 / 168; 8 sequences of 64 queries on up to 4000 82 / 65;
+// but 32 queries 27 / 33, 64 34 / 37, 1024 under a window of 1024 39 / 55.
 int plan_rows8(BandArgs& a) {
   const int cus = dlt_device_cus();
   const int64_t bh = (int64_t)a.B * a.Hkv, blocks = (a.rows + 127) / 128, wgs = bh * blocks;

@@ -5,11 +5,13 @@
 // out of its subnormals, whole numbers lose at most half a step of the new scale, less than a step over all growths (1/2 + 1/4 + ..).
 //
 // An item is a block, a head and a tensor (K or V): its tokens are fetched once, rotated in 32 bits, held in registers until their largest element is known, and written as
-// 8-bit numbers, some heads one after the other under one fetch of cos and sin, the next head's rows on their way.  8 dims to a lane, as many rows to a wave as fit.  Few new tokens a block: a wave to an item (nothing waits for another wave); else four or eight, which
-// exchange their maxima through LDS (blocks of 128, d = 128, by four waves with twice the rows in registers: 60 us for 36).  Rows of q are rotated by workgroups of their own in the same launch, a wave to some tokens, the heads one after the other under
-// one fetch of cos and sin.
+// 8-bit numbers, some heads one after the other under one fetch of cos and sin, the next head's rows on their way.  8 dims to a lane, as many rows to a wave as fit.
+// Few new tokens a block: a wave to an item (nothing waits for another wave); else four or eight, which exchange their maxima through LDS (blocks of 128, d = 128, by four
+// waves with twice the rows in registers: 60 us for 36).  Rows of q are rotated by workgroups of their own in the same launch, a wave to some tokens, the heads one after
+// the other under one fetch of cos and sin.
 //
-// Memory bound: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 30 us, 4.5 TB/s; a token each of 64 sequences 5 us on the GPU, latency: length, page, row.
+// Memory bound: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 30 us, 4.5 TB/s; 7 of up to 2047, 16 + 8 + 8, d = 64, blocks of 16 17 to 19 us, 80 MB with
+// the rows of q that hold no token.  A token each of 64 sequences: 5 us on the GPU, latency: length, page, row.
 #include <algorithm>
 #include "attn_common.hpp"
 #include "page_cvt8.h"

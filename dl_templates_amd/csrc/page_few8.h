@@ -3,8 +3,8 @@
 // Bound by the cache's bytes.  A wave takes tiles of 32 tokens (64 at D = 64) by itself: K and V go from memory to its registers, the next tile while this one is
 // worked on, and nothing passes through LDS or waits for another wave.  S^T = K Q^T: a lane's 8-bit numbers are a run of a token's dims, which become an operand as they are
 // converted (the order of the dims is free as long as q has it too).  P^T leaves that product as the operand of the next one, O^T += V^T P^T, whose other operand wants the
-// tokens of a dim side by side: a lane fetches the same few dims of 8 tokens, and 4 x 4 bytes are turned with 8 byte permutes.  Conversions are a tenth of the vector issue
-// slots that the bytes' time leaves.
+// tokens of a dim side by side: a lane fetches the same few dims of 8 tokens, and 4 x 4 bytes are turned with 8 byte permutes.  A tile is 12 loads of a lane, 24 matrix
+// instructions and about 250 vector ones at D = 128, a third of the time that its 8 KB take at the rate of memory.
 // P enters its product in two parts, its rounding and the rest, which costs 8 matrix instructions of 24 that nothing waits for: the only rounding to 16 bits is the
 // output's (relative error 0.0024 -> 0.0017 in bf16, that of the output's rounding).
 //

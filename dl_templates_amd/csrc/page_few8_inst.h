@@ -6,7 +6,10 @@
 
 namespace {
 constexpr int D = DLT_FEW8_D;
-constexpr int FEW8_JOIN_WGS = 1024;   // rows of a call that are joined by a workgroup each
+// Up to so many rows of a call are joined by a workgroup each, if a head has 8 runs or more; others by a wave each.  us, wave / workgroup: 96 rows, 64 runs a head (2 sequences
+// of 100000, 4 kv heads) 44 / 37; 32 rows, 64 runs 13.6 / 11.5; 512 rows, 16 runs (4 of 20000, 4 tokens, 8 kv heads) 26.5 / 25.7; 512 rows, 4 runs (16 of up to 4000) 22.5 / 24.0;
+// 1024 rows, 2 runs 40.4 / 43.1.
+constexpr int FEW8_JOIN_WGS = 1024;
 
 template <typename KernT>
 int few8_go(KernT kern, const Few8Args& a, int64_t grid, int waves, int lds, hipStream_t stream) {
@@ -32,7 +35,7 @@ int few8_np(const Few8Args& a, bool full, hipStream_t stream) {
   if (rc != DLT_OK) return rc;
   dlt_timing_before(DLT_K_FWD, stream);
   const unsigned bh = (unsigned)(a.B * a.Hkv);
-  if ((int64_t)bh * a.rows <= FEW8_JOIN_WGS) hipLaunchKernelGGL((few8_join_kernel<TIO, true>), dim3((unsigned)a.rows, bh), dim3(256), 0, stream, a);
+  if ((int64_t)bh * a.rows <= FEW8_JOIN_WGS && 8 * bh <= a.want) hipLaunchKernelGGL((few8_join_kernel<TIO, true>), dim3((unsigned)a.rows, bh), dim3(256), 0, stream, a);
   else hipLaunchKernelGGL((few8_join_kernel<TIO, false>), dim3((unsigned)(a.rows + 3) / 4, bh), dim3(256), 0, stream, a);
   dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("paged8 sum launch");
