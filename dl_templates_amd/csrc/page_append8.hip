@@ -417,9 +417,9 @@ extern "C" int dlt_paged8_append(const void* k, const int64_t k_strides[4], cons
   const int nw = most <= 2 * rows ? 1 : most <= 8 * rows ? 4 : 8, passes = (most + nw * rows - 1) / (nw * rows);
   a.nb = (s->T + a.block - 2) / a.block + 1;
   // heads of an item: all of K's or V's while that leaves APP8_WAVES a CU, fewer otherwise
-  const int64_t blocks = (int64_t)s->B * a.nb, waves_kv = APP8_WAVES * (int64_t)dlt_device_cus();
+  const int64_t cus = dlt_device_cus(), blocks = (int64_t)s->B * a.nb;
   a.hk = s->Hkv;
-  while (a.hk > 1 && blocks * nw * 2 * ((s->Hkv + a.hk - 1) / a.hk) < waves_kv) a.hk = (a.hk + 1) / 2;
+  while (a.hk > 1 && blocks * nw * 2 * ((s->Hkv + a.hk - 1) / a.hk) < APP8_WAVES * cus) a.hk = (a.hk + 1) / 2;
   const int runs = (s->Hkv + a.hk - 1) / a.hk;
   a.kv_heads = runs * a.hk;
   a.kv_chunks = 2 * runs;
@@ -430,9 +430,8 @@ extern "C" int dlt_paged8_append(const void* k, const int64_t k_strides[4], cons
   int64_t grid = a.kv_blocks;
   if (s->H > 0) {
     const int64_t groups = ((int64_t)s->B * s->T + 64 / (s->dk / 8) - 1) / (64 / (s->dk / 8));
-    const int64_t waves = APP8_Q_WAVES * (int64_t)dlt_device_cus();
     a.hq = s->H;
-    while (a.hq > 1 && groups * ((s->H + a.hq - 1) / a.hq) < waves) a.hq = (a.hq + 1) / 2;
+    while (a.hq > 1 && groups * ((s->H + a.hq - 1) / a.hq) < APP8_Q_WAVES * cus) a.hq = (a.hq + 1) / 2;
     a.q_chunks = (s->H + a.hq - 1) / a.hq;
     grid += nw == 8 ? (groups * a.q_chunks + 7) / 8 : (groups * a.q_chunks + 3) / 4;
   }
