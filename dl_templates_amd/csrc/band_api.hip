@@ -555,10 +555,11 @@ int check_rows8(const char* who, const char* name, const void* p, const int64_t*
 namespace {
 int64_t few8_floats(const Few8Args& a) { return (int64_t)a.wgs * a.rows * (a.dv_ + 2); }   // behind them the heads' workgroups
 int64_t few8_bytes(const Few8Args& a) { return a.wgs == 0 ? 0 : 4 * few8_floats(a) + 8 * (int64_t)a.B * a.Hkv; }
-// Up to 32 rows of a group: the kernels of page_few8.h (false: not for them).  A workgroup to each head where that is good enough, since it needs no second launch:
-// contexts of up to 1024 keys (8 sequences of up to 1000, 8 kv heads, d = 128, 10.5 us either way), and of up to 2560 where the heads fill the CUs (us, whole heads / runs: 64
-// sequences of up to 2000, 8 kv heads, d = 128, 35.0 / 38.2; 32 under a window of 1024 15.9 / 21.3; but 32 of up to 4000 48 / 43, 16 under a window of 4096, 128 heads, 50 /
-// 32).  Both rules go by the table's width and the window, since lengths stay on the device.
+// Up to 32 rows of a group: the kernels of page_few8.h (false: not for them).  A workgroup to each head where that is good enough, since it needs no second launch: where a
+// sequence's rows see up to 1152 keys, and up to 2560 where heads are half as many as CUs or more (us, whole heads / runs, d = 128 if not said: 64 sequences of up to 2000, 8 kv heads,
+// 35.0 / 38.2; 128, 192 heads under a window of 2048 18.4 / 20.2, 21.1 / 28.3, 192 at d = 64 16.4 / 23.1; 64 and 192 heads under one of 1024 12.9 / 14.2, 13.5 / 18.9; but 32
+// sequences of up to 4000 48 / 43, 64, 128, 192 heads under a window of 4096 29.0 / 20.4, 33.6 / 29.8, 38.3 / 40.2).  The rule goes by the table's width and the window, since
+// lengths stay on the device.  Runs that are the same number for every head, found without the lengths of others: no faster (384 heads under a window of 2048, d = 64: 29 / 26).
 // Runs: two workgroups a CU, one where the steps are few (few8_run) or a workgroup has two blocks of rows: 16 sequences, one of 32768 and 15 of 500, 4 kv heads, 18.0 us with
 // two, 15.9 with one; one of 20000, 8 kv heads, 16.4 / 15.6; but 64 of up to 8192 116 / 128.  With three: 119 for those, two of 100000 39 -> 42.
 bool plan_few8(Few8Args& a) {
@@ -571,7 +572,7 @@ bool plan_few8(Few8Args& a) {
   // eight waves to a head where heads make less than two workgroups a CU (us, four / eight / sixteen: one token on 300 keys, 8 heads, d = 64, 6.9 / 6.8 / 7.1, on 1000, d = 128,
   // 11.8 / 10.7 / 11.9; 32 sequences of up to 500, 8 heads, d = 128, 9.5 / 9.2 / 10.1; 48 under a window of 2048, 8 heads, d = 64, 28.5 / 25.3; but 64 of up to 2000 35 / 39)
   a.waves = a.rows <= 16 && bh < 2 * cus ? 8 : 4;
-  if (most > (bh >= cus ? 2560 : 1024) && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = a.want + (int)bh;
+  if (most > (2 * bh >= cus ? 2560 : 1152) && a.B <= FEW8_B_MAX && bh <= 65535 && bh * (a.Lk / 128 + 2) < 1 << 30) a.wgs = a.want + (int)bh;
   if (few8_bytes(a) > DLT_WINDOW_WORKSPACE_MAX) a.wgs = 0;
   dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);
   return true;
