@@ -10,7 +10,7 @@
 // below F and written from F on.  Lengths and the pool's count, which all workgroups read, are written by the last one to finish: a count of those that are done, in the
 // pool's second word, tells which that is; nobody waits.
 //
-// Bound by latency: 64 requests, a token more and back, 6.2 + 4.8 us on the GPU (lengths, sums, pages, rows, the count of those that are done); 1000 requests, 4000 slots each,
+// Bound by latency: 64 requests, a token more and back, 5.2 + 4.7 us on the GPU (lengths, sums, pages, rows); 1000 requests, 4000 slots each,
 // 16 MB of slots written, and back, 14.8 + 8.1: the sums of 1000 requests are formed in each of 256 workgroups, whose counts meet in one word (about 10 ns each).
 #include <algorithm>
 #include "dlt_internal.hpp"
@@ -135,18 +135,20 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   for (int i = 0; i < NT / 64; i++) served = dlt_imax(served, most[i]);
   const int left = (int)(room - served < a.n_pages ? room - served : a.n_pages);
   const Stack stack{a, back, held, gain, F, sum_r};
-  const int64_t at0 = (int64_t)blockIdx.x * NT + tid, step = (int64_t)gridDim.x * NT;
+  // Every kind of work begins with waves of its own: on a small call, one workgroup, none waits for another kind's memory (64 requests, a token more: 6.0 us by eight
+  // workgroups, 5.2 by this one)
+  const int64_t wg0 = (int64_t)blockIdx.x * NT, step = (int64_t)gridDim.x * NT;
 
-  for (int64_t k = at0; k < served; k += step) {
+  for (int64_t k = wg0 + tid; k < served; k += step) {
     const int b = owner_of(need, a.B, (int)k);
     a.table[b * a.ts + (pages_of(a, held[b]) + (int)k - need[b])] = stack.taken((int)k);
   }
-  for (int64_t i = at0; F + i < left; i += step) a.pool[2 + F + i] = stack.returned((int)i);
-  for (int64_t b = at0; b < a.B; b += step) a.n_new[b] = dlt_imax(gain[b], 0);
+  for (int64_t i = wg0 + (tid ^ NT / 4); F + i < left; i += step) a.pool[2 + F + i] = stack.returned((int)i);
+  for (int64_t b = wg0 + (tid ^ NT / 8); b < a.B; b += step) a.n_new[b] = dlt_imax(gain[b], 0);
   // slots, four in a row of all to a thread: they share their request and mostly their page
   const int64_t slots = a.T > 0 ? (int64_t)a.B * a.T : 0;
   // (from the last workgroup on: on a small call others have the columns)
-  for (int64_t i = 4 * ((int64_t)(gridDim.x - 1 - blockIdx.x) * NT + tid); i < slots; i += 4 * step) {
+  for (int64_t i = 4 * ((int64_t)(gridDim.x - 1 - blockIdx.x) * NT + (tid ^ NT / 2)); i < slots; i += 4 * step) {
     int b = (int)dlt_fastdiv((uint32_t)i, a.mt, a.st), t = (int)i - b * a.T, page = -1, until = 0;   // `page` holds tokens below `until` of request b
     int has = held[b], more = gain[b], out[4];
 #pragma unroll
@@ -215,8 +217,7 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
   // Slots by fours, and columns that requests can gain (give back, without a limit to the slots), 256 of them to a workgroup, up to a workgroup a CU.  Each is another atomic
   // on the pool's word, so they are large: 1000 requests, 4000 slots each, and back, 256 of 1024 threads 15.0 + 8.2 us, 128 17.8 + 8.2, 512 of 256 18.8 + 8.6.
   const int64_t work = (int64_t)B * dlt_imax(T, 1) / 4 + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols), cus = dlt_device_cus();
-  // (small calls up to eight, so that columns and slots are not one after the other: 64 requests, one token more, 6.5 -> 6.0 us)
-  const int64_t grid = std::max<int64_t>(1, std::max<int64_t>(std::min<int64_t>(work / 16, 8), std::min<int64_t>(work / 256, cus)));
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work / 256, cus));
   const int lds = 4 * (B + 1) * 4;
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
   if (rc != DLT_OK) return rc;
