@@ -101,8 +101,9 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   // sums of needs and of what comes back: a run of requests to a thread
   const int per = (a.B + NT - 1) / NT, b0 = dlt_imin(tid * per, a.B), b1 = dlt_imin(b0 + per, a.B);
   int n = 0, r = 0, sum_n, sum_r;
+  Wish w{};
   for (int b = b0; b < b1; b++) {
-    const Wish w = wish_of(a, b);
+    w = wish_of(a, b);
     n += w.need;
     r += w.back;
   }
@@ -114,7 +115,7 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   const int64_t room = (int64_t)F + sum_r;
   int served = 0;   // pages taken
   for (int b = b0; b < b1; b++) {
-    const Wish w = wish_of(a, b);
+    if (per > 1) w = wish_of(a, b);
     need[b] = n;
     back[b] = r;
     n += w.need;
