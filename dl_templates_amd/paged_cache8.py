@@ -59,7 +59,8 @@ def paged8_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.
 
 def paged8_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, page_table: torch.Tensor,
                      seq_len: torch.Tensor, window: int = None, n_sink: int = 0, sm_scale: float = None, n_new: torch.Tensor = None) -> torch.Tensor:
-    """``paged_attention`` over an 8-bit cache: o [B, H, T, Dv] of q [B, H, T, Dk], bfloat16 or float16, keys and values read as numbers of q's type.
+    """``paged_attention`` over an 8-bit cache: o [B, H, T, Dv] of q [B, H, T, Dk], bfloat16 or float16, keys and values read as numbers of q's type.  For
+    float16 queries the cache must hold no number beyond 65504; an append of float16 tokens sees to that.
 
     Padded rows, and rows of sequences without a key, give zeros, whatever the keys and values beside them hold.  Head dims in multiples of 8 up to 128, cache rows contiguous
     and 8-byte aligned.  What a page holds behind a sequence's last token, its scales included, does not matter; a page number outside the cache is a mistake that is not

@@ -390,7 +390,8 @@ int dlt_paged8_append(const void* k, const int64_t k_strides[4], const void* v, 
                       const dlt_scales8_t* scales, const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
                       const dlt_rope_axes_t* rope, const dlt_paged_shape_t* shape, void* stream);
 
-/* dlt_paged_attn over such a cache: keys and values are read as numbers of q's type.  Cache rows contiguous, at multiples of 8 bytes. */
+/* dlt_paged_attn over such a cache: keys and values are read as numbers of q's type, which for DLT_FP16 have to be 65504 at most (an append of DLT_FP16 sees to
+ * that).  Cache rows contiguous, at multiples of 8 bytes. */
 int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes);
 int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4],
                     const void* v_cache, const int64_t v_cache_strides[4], const dlt_scales8_t* scales, void* o, const int64_t o_strides[4],
