@@ -568,12 +568,13 @@ __global__ __launch_bounds__(256) void few8_join_kernel(const Few8Args a) {
       m = m_new;
 #pragma unroll
       for (int k = 0; k < TOGETHER; k++) {
-        // with a weight of 0 too: an infinite or NaN part holds such a value of a key that the row sees.  (No branch around the last part again: the loads would
-        // be moved behind it, one after the other.)
-        const float f = i0 + EACH * k < who.y ? few8_weight(x[k], m) : 0.f;
-        l = fmaf(x[k].y, f, l);
-        o0 = fmaf(v[k].x, f, o0);
-        o1 = fmaf(v[k].y, f, o1);
+        // with a weight of 0 too: an infinite or NaN part holds such a value of a key that the row sees.  The last part again is left out, not given a weight of 0: it may be
+        // infinite.  (No branch around it: the loads would be moved behind it, one after the other.)
+        const bool one = i0 + EACH * k < who.y;
+        const float f = few8_weight(x[k], m);
+        l = one ? fmaf(x[k].y, f, l) : l;
+        o0 = one ? fmaf(v[k].x, f, o0) : o0;
+        o1 = one ? fmaf(v[k].y, f, o1) : o1;
       }
     }
   if constexpr (WG) {

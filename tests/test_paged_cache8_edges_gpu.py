@@ -413,3 +413,30 @@ def test_a_workgroup_with_more_than_64_chunks(T, d, dtype, fmt, window, n_sink):
                          scale)
     assert (o == o[:1]).all()
     check(case, o[:1].cpu(), q, (kc, vc, ks, vs, table), [T], scale)
+
+
+@pytest.mark.parametrize("T, lens", [(1, [5000]), (3, [20001]), (1, [3000] * 40), (40, [5000])])
+@pytest.mark.parametrize("fmt", [FP8, I8])
+def test_infinite_values_where_parts_are_joined(T, lens, fmt):
+    """A block of values past the type's largest number, in one dim, at a sequence's end: that dim is infinite, the others are what they are."""
+    gen = torch.Generator().manual_seed(90)
+    B, Hkv, d, page = len(lens), 2, 128, 64
+    case = (B, 2 * Hkv, Hkv, T, page, 16, lens, None, d, d, None, 0, BF, fmt)
+
+    def end(kc, vc, ks, vs, table):
+        for b, n in enumerate(lens):
+            t = n - T - 1   # every row sees it
+            block, p = t % page // 16, int(table[b, t // page])
+            c = vc[p, 0, 16 * block:16 * block + 16].view(torch.uint8)
+            c.zero_()
+            c[:, 5] = 0x7e if fmt == FP8 else 127
+            vs[p, 0].view(torch.uint8)[block] = 254
+
+    o, q, parts, new, scale = attend(case, gen, change=[end])
+    assert torch.isposinf(o[:, :2, :, 5]).all() and torch.isfinite(o[:, 2:]).all()
+    kc, vc, ks, vs, table = parts
+    for b, n in enumerate(lens):
+        k, v = gathered(kc, ks, table, b, n, BF)[None], gathered(vc, vs, table, b, n, BF)[None]
+        v[:, 0, :, 5] = 0   # the infinities are looked at above: a dense product in 64 bits multiplies hidden ones by 0
+        o[b, :2, :, 5] = 0
+        orc.check(o[b:b + 1], orc.window(q[b:b + 1], k, v, None, 0, scale)["o"], f"sequence {b}")
