@@ -415,7 +415,7 @@ def test_a_workgroup_with_more_than_64_chunks(T, d, dtype, fmt, window, n_sink):
     check(case, o[:1].cpu(), q, (kc, vc, ks, vs, table), [T], scale)
 
 
-@pytest.mark.parametrize("T, lens", [(1, [5000]), (3, [20001]), (1, [3000] * 40), (40, [5000])])
+@pytest.mark.parametrize("T, lens", [(1, [5000]), (3, [20001]), (1, [3000] * 40), (40, [5000]), (1, [300]), (5, [1000] * 3), (1, [64] * 300)])
 @pytest.mark.parametrize("fmt", [FP8, I8])
 def test_infinite_values_where_parts_are_joined(T, lens, fmt):
     """A block of values past the type's largest number, in one dim, at a sequence's end: that dim is infinite, the others are what they are."""
@@ -440,3 +440,50 @@ def test_infinite_values_where_parts_are_joined(T, lens, fmt):
         v[:, 0, :, 5] = 0   # the infinities are looked at above: a dense product in 64 bits multiplies hidden ones by 0
         o[b, :2, :, 5] = 0
         orc.check(o[b:b + 1], orc.window(q[b:b + 1], k, v, None, 0, scale)["o"], f"sequence {b}")
+
+
+@pytest.mark.parametrize("fmt", [FP8, I8])
+def test_traced_calls_depend_on_their_inputs(fmt):
+    def inputs(seed):
+        s = Server(fmt, BF, seed, 7)
+        s.inputs()
+        s.want.clamp_(min=1)
+        return s.table, s.seq, s.want, s.pool, s.kc, s.vc, s.ks, s.vs, s.k, s.v, s.q
+    tables = [orc.table(320, 32).cuda()]
+
+    def step(table, seq, want, pool, kc, vc, ks, vs, k, v, q):
+        n_new, slots = page_assign_(table, seq, want, pool, 32, 7)
+        r = paged8_append_(kc, vc, ks, vs, k, v, table, seq, n_new, (None, tables, "halves"), q)
+        return n_new, slots, r, paged8_attention(r, kc, vc, ks, vs, table, seq, 100, 5, None, n_new)
+
+    def fill(table, seq, want, pool, kc, vc, ks, vs, k, v, q):
+        before = seq + 0
+        n_new, slots = page_assign_(table, seq, want, pool, 32)
+        assert slots is None and paged8_append_(kc, vc, ks, vs, k, v, table, seq, n_new) is None
+        return before, seq + 0, n_new, paged8_attention(q, kc, vc, ks, vs, table, seq, None, 0, None, n_new)
+    for f in (step, fill):
+        traced = torch.jit.trace(f, inputs(30), check_trace=False)
+        for seed in (31, 32, 33, 34):
+            a, b = inputs(seed), inputs(seed)
+            got, want = traced(*a), f(*b)
+            assert all(torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8)) for x, y in zip(tuple(got) + a, tuple(want) + b)), (f.__name__, seed)
+
+
+def test_calls_are_timed():
+    """With per-launch timing on, calls do what they do without it, and every launch leaves a record."""
+    from dl_templates_amd import _lib
+    gen = torch.Generator().manual_seed(40)
+    cases = [(1, 8, 2, 1, 64, 64, [300], None, 64, 64, None, 0, BF, FP8), (2, 8, 2, 1, 64, 64, [5000, 700], None, 128, 128, None, 0, HF, I8),
+             (1, 8, 2, 100, 32, 32, [700], None, 128, 128, None, 0, BF, I8)]
+    for case in cases:
+        B, H, Hkv, T, page, block, lens, _, dk, dv, _, _, dtype, fmt = case
+        kc, vc, ks, vs, table = (x.cuda() for x in cache_for(case, gen))
+        q = torch.randn(B, H, T, dk, generator=gen).to(dtype).cuda()
+        want = paged8_attention(q, kc, vc, ks, vs, table, ints(lens))
+        _lib.timing_enable(True)
+        try:
+            got = paged8_attention(q, kc, vc, ks, vs, table, ints(lens))
+            records = _lib.timing_collect()
+        finally:
+            _lib.timing_enable(False)
+        assert torch.equal(got, want) and len(records) >= 1
