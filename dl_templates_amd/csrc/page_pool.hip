@@ -7,11 +7,11 @@
 //
 // Every workgroup forms the two sums of all requests (8 B of lengths each, from the L2) and keeps them in LDS with what every request holds and gains, then takes a share of
 // the new columns, of the pages that come back and of the slots.  A table's row is read (a request that gives back) or written (one that gains), never both; the pool is read
-// below F and written from F on.  Lengths and the pool's count, which all workgroups read, are written by the last one to finish: a count of those that are done, in the
-// pool's second word, tells which that is; nobody waits.
+// below F and written from F on.  Lengths and the pool's count, which all workgroups read before all else, are written by the last one to have read them: a count in the
+// pool's second word tells which that is; nobody waits.
 //
-// Bound by latency: 64 requests, a token more and back, 5.2 + 4.7 us on the GPU (lengths, sums, pages, rows); 1000 requests, 4000 slots each,
-// 16 MB of slots written, and back, 14.8 + 8.1: the sums of 1000 requests are formed in each of 256 workgroups, whose counts meet in one word (about 10 ns each).
+// Bound by latency: 64 requests, a token more and back, 4.9 + 4.4 us on the GPU (lengths, sums, pages, rows); 1000 requests, 4000 slots each,
+// 16 MB of slots written, and back, 13.7 + 7.9: the sums of 1000 requests are formed in every workgroup, whose counts meet in one word (about 10 ns each).
 #include <algorithm>
 #include "dlt_internal.hpp"
 #include "kernargs.h"
@@ -27,12 +27,12 @@ struct AssignArgs {
 };
 
 struct Wish { int held, want, need, back; };
-// what request b holds and needs or gives back, in pages
-__device__ inline Wish wish_of(const AssignArgs& a, int b) {
+// what a request of `seq` tokens that wants `want` holds and needs or gives back, in pages
+__device__ inline Wish wish_of(const AssignArgs& a, int seq, int want) {
   Wish w;
   const int room = a.cols * a.page;   // < 2^31
-  w.held = dlt_imax(0, dlt_imin(a.seq[b], room));
-  w.want = a.want[b];
+  w.held = dlt_imax(0, dlt_imin(seq, room));
+  w.want = want;
   w.need = w.back = 0;
   if (w.want < 0) w.want = w.held;
   if (w.want > room || (a.T >= 0 && w.want - w.held > a.T)) w.want = w.held;
@@ -101,11 +101,30 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   // sums of needs and of what comes back: a run of requests to a thread
   const int per = (a.B + NT - 1) / NT, b0 = dlt_imin(tid * per, a.B), b1 = dlt_imin(b0 + per, a.B);
   int n = 0, r = 0, sum_n, sum_r;
+  constexpr int PER = DLT_ASSIGN_MAX / NT;
+  int seq[PER], want[PER];
   Wish w{};
-  for (int b = b0; b < b1; b++) {
-    w = wish_of(a, b);
-    n += w.need;
-    r += w.back;
+  if (per == 1) {
+    if (b0 < b1) w = wish_of(a, a.seq[b0], a.want[b0]);
+    n = w.need;
+    r = w.back;
+  } else {   // their lengths together, not one after the other (8000 requests, a token more and back: 46 -> 38 us)
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      seq[k] = want[k] = 0;
+      if (k < per) {
+        const int b = dlt_imin(b0 + k, a.B - 1);
+        seq[k] = a.seq[b];
+        want[k] = a.want[b];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < PER; k++)
+      if (b0 + k < b1) {
+        w = wish_of(a, seq[k], want[k]);
+        n += w.need;
+        r += w.back;
+      }
   }
   const int own_n = n, own_r = r;
   const int F = dlt_imax(0, dlt_imin(a.pool[0], a.n_pages));
@@ -114,8 +133,7 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   r -= own_r;
   const int64_t room = (int64_t)F + sum_r;
   int served = 0;   // pages taken
-  for (int b = b0; b < b1; b++) {
-    if (per > 1) w = wish_of(a, b);
+  auto keep = [&](int b) __attribute__((always_inline)) {
     need[b] = n;
     back[b] = r;
     n += w.need;
@@ -123,6 +141,16 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
     held[b] = w.held;
     gain[b] = w.need > 0 && n > room ? 0 : w.want - w.held;
     if (w.need > 0 && n <= room) served = n;
+  };
+  if (per == 1) {
+    if (b0 < b1) keep(b0);
+  } else {
+#pragma unroll
+    for (int k = 0; k < PER; k++)
+      if (b0 + k < b1) {
+        w = wish_of(a, seq[k], want[k]);
+        keep(b0 + k);
+      }
   }
   if (tid == 0) {
     need[a.B] = sum_n;
@@ -134,6 +162,14 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NT / 64; i++) served = dlt_imax(served, most[i]);
+  // Every load of lengths and of the pool's count by this workgroup has returned: as far as it is concerned they may be written.  Counted here, beside the work, and looked at behind
+  // it (4000 requests, a token more and back, 22.4 -> 21.2 us); by many workgroups, which would queue up here (10 ns each), behind it too (1000 requests, 4000 slots 21.9 -> 21.0).
+  const bool early = gridDim.x <= 64;
+  int before = 0;
+  auto count = [&]() __attribute__((always_inline)) {
+    if (tid == 0) before = __hip_atomic_fetch_add(&a.pool[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  };
+  if (gridDim.x > 1 && early) count();
   const int left = (int)(room - served < a.n_pages ? room - served : a.n_pages);
   const Stack stack{a, back, held, gain, F, sum_r};
   // Every kind of work begins with waves of its own: on a small call, one workgroup, none waits for another kind's memory (64 requests, a token more: 6.0 us by eight
@@ -177,15 +213,12 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
       for (int k = 0; i + k < slots; k++) a.slots[i + k] = out[k];
   }
 
+  // the last workgroup to be counted writes them.  (Nothing else that a workgroup writes is read by another.)
   if (gridDim.x > 1) {
-    // every load of this workgroup has returned: its lengths may be written now.  (Nothing that a workgroup writes is read by another.)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0) last = __hip_atomic_fetch_add(&a.pool[1], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    if (!early) count();
+    if (tid == 0) last = before == (int)gridDim.x - 1;
     __syncthreads();
     if (!last) return;
-  } else {
-    __syncthreads();
   }
   for (int b = tid; b < a.B; b += NT)
     if (gain[b] != 0) a.seq[b] = held[b] + gain[b];
@@ -215,10 +248,11 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
   dlt_fastdiv_make((uint32_t)page, a.mp, a.sp);
   dlt_fastdiv_make((uint32_t)dlt_imax(T, 1), a.mt, a.st);
   constexpr int NT = 1024;
-  // Slots by fours, and columns that requests can gain (give back, without a limit to the slots), 256 of them to a workgroup, up to a workgroup a CU.  Each is another atomic
-  // on the pool's word, so they are large: 1000 requests, 4000 slots each, and back, 256 of 1024 threads 15.0 + 8.2 us, 128 17.8 + 8.2, 512 of 256 18.8 + 8.6.
-  const int64_t work = (int64_t)B * dlt_imax(T, 1) / 4 + (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols), cus = dlt_device_cus();
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(work / 256, cus));
+  // 256 requests, as many threads of slots by fours, or 4096 columns that requests can gain (give back, without a limit to the slots) to a workgroup, up to a workgroup a CU.  Each is
+  // another addition to the pool's word, so they are large.  us, 1000 requests, 4000 slots each, by 32 / 64 / 128 / 256 workgroups 37.3 / 23.6 / 16.9 / 14.0, and back, a million
+  // columns that may be given, 7.9 / 7.7 / 8.1 / 9.7.
+  const int64_t slots4 = (int64_t)B * dlt_imax(T, 0) / 4, columns = (int64_t)B * (T >= 0 ? dlt_imin(T / page + 2, cols) : cols), cus = dlt_device_cus();
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((B + slots4) / 256 + columns / 4096, cus));
   const int lds = 4 * (B + 1) * 4;
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
   if (rc != DLT_OK) return rc;
