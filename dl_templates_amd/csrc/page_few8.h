@@ -292,7 +292,8 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
       for (int u = 0; u < NG; u++) {
         tok[u] = W.tok(TK * tile + 16 * u);
         ek[u] = __builtin_amdgcn_readlane(ek_l, at * NG + u);
-        ev[u] = __builtin_amdgcn_readlane(ev_l, at * NG + u);
+        const int e = __builtin_amdgcn_readlane(ev_l, at * NG + u);
+        ev[u] = tok[u] < sq.n_k ? e : 127;   // of a block of nothing that the sequence holds: anything
       }
       float t[NP][NG][4];
 #pragma unroll
@@ -373,16 +374,14 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
           pl[p][kb] = pack8<PT>(r);
         }
       }
-      if (tok[NG - 1] + 16 > sq.n_k) {   // pages hold anything behind the last key: those values, which no row sees, are cleared, and so are scales of blocks of nothing else
+      if (tok[NG - 1] + 16 > sq.n_k) {   // pages hold anything behind the last key: those values, which no row sees, are cleared
         keep_branch();
 #pragma unroll
-        for (int u = 0; u < NG; u++) {
-          if (tok[u] >= sq.n_k) ev[u] = 127;
+        for (int u = 0; u < NG; u++)
 #pragma unroll
           for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int w = 0; w < VW; w++) vr[u][j][w] = tok[u] + 4 * g + j < sq.n_k ? vr[u][j][w] : 0u;
-        }
       }
 #pragma unroll
       for (int kb = 0; kb < F::NT; kb++)
