@@ -292,7 +292,7 @@ __global__ __launch_bounds__(NW == 8 ? 512 : 256) void paged8_append_kernel(cons
     const int need = cvt8_exponent<FMT>(m);          // biased
     const int e = dlt_imax(need, e_old);             // 255, NaN, stays
     const int e_new = FMT == DLT_INT8 && odd ? 255 : e;
-    const float inv = e >= 254 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
+    const float inv = cvt8_inverse(e);
     const float most = std::is_same<T, f16_t>::value ? cvt8_most_f16<FMT>(e) : cvt8_most<FMT>();
     // older tokens of the block at a larger scale
     if (older && e > e_old && e_new != 255) {

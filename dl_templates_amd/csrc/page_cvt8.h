@@ -8,6 +8,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 int dlt_scales8_check(const char* who, const dlt_scales8_t* s, int page);
 
 constexpr int CVT8_LEAST = 127 - 100;   // of the exponents that an append gives
+// 1 / 2^(e - 127); a scale that is NaN: 0
+DLT_DEV float cvt8_inverse(int e) { return e >= 254 ? (e == 254 ? 0x1p-127f : 0.f) : __uint_as_float((unsigned)(254 - e) << 23); }
 // least biased exponent at which the magnitude with these bits fits
 template <int FMT>
 DLT_DEV int cvt8_exponent(unsigned bits) {
@@ -21,7 +23,7 @@ DLT_DEV constexpr float cvt8_most() { return FMT == DLT_FP8_E4M3 ? 448.f : 127.f
 // the largest number whose value at scale e is finite in fp16 (65504 and below)
 template <int FMT>
 DLT_DEV float cvt8_most_f16(int e) {
-  const float inv = e >= 254 ? 0.f : __uint_as_float((unsigned)(254 - e) << 23);
+  const float inv = cvt8_inverse(e);
   return FMT == DLT_FP8_E4M3 ? fminf(448.f, 61440.f * inv) : fminf(127.f, floorf(65504.f * inv));
 }
 
