@@ -71,7 +71,8 @@ DLT_DEV u32x2 cvt8_put8(const float (&v)[8], float most) {
 
 // Two neighbouring 8-bit numbers (the low two bytes, or the high two) times the scale with biased exponent e as a pair of 16-bit values.  e4m3: one instruction, which takes
 // the scale's exponent.  int8: a whole number to 32 bits, times the scale, packed; exact.
-DLT_DEV float cvt8_scale(int e) { return __uint_as_float((unsigned)e << 23 | (e == 255 ? 0x400000u : 0u)); }   // 255: NaN
+// (both ends of a byte need the bit below the exponent's: 0 is 2^-127, a subnormal number, 255 NaN)
+DLT_DEV float cvt8_scale(int e) { return __uint_as_float((unsigned)e << 23 | ((e + 1 & 0xfe) == 0 ? 0x400000u : 0u)); }
 template <int FMT, typename TIO>
 DLT_DEV unsigned cvt8_pair(unsigned w, float scale, bool hi);
 template <> DLT_DEV unsigned cvt8_pair<DLT_FP8_E4M3, bf16_t>(unsigned w, float scale, bool hi) {

@@ -1,13 +1,47 @@
 """The paged cache in 8 bits where numbers end: scales at both ends of their byte (GPU)."""
+import math
+
 import pytest
 import torch
 
-from dl_templates_amd.paged_cache8 import paged8_append_
+from dl_templates_amd.paged_cache8 import paged8_append_, paged8_attention
 from tests import paged8_oracle as orc8
-from tests.test_paged_cache8_gpu import BF, F32, FP8, HF, I8, ints, pool
+from tests.test_paged_cache8_edges_gpu import check
+from tests.test_paged_cache8_gpu import BF, F32, FP8, HF, I8, cache_for, ints, pool
 
 pytestmark = pytest.mark.gpu
 bytes_of = lambda x: x.view(torch.uint8)  # noqa: E731
+
+
+@pytest.mark.parametrize("fmt", [FP8, I8])
+def test_ones_at_the_first_and_the_last_scale(fmt):
+    one = torch.ones(1, 1, 64, 64).to(fmt).cuda()
+    sc = lambda v: torch.full((1, 1, 1), v, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)  # noqa: E731
+    for e, n, T in ((0, 1, 1), (0, 9, 1), (0, 64, 40), (254, 1, 1), (254, 1, 40)):   # (two of 2^127 would leave 32 bits)
+        q = torch.zeros(1, 2, T, 64, dtype=BF, device="cuda")
+        new = ints([min(n, T)])
+        o = paged8_attention(q, one, one, sc(127), sc(e), ints([[0]]), ints([n]), n_new=new)[:, :, :min(n, T)]
+        assert (o.double() == 2.0 ** (e - 127)).all(), (fmt, e, n, T)
+
+
+# rows in whole heads, in runs, and more of them; values that differ from key to key by what softmax gives them
+LOW = [(2, 4, 2, 1, 32, 16, [700, 90], None, 64, 64, None, 0, BF), (2, 8, 2, 3, 64, 32, [3900, 800], None, 128, 128, None, 0, BF), (1, 8, 2, 30, 64, 64, [900], None, 128, 128, 300, 10, BF)]
+
+
+@pytest.mark.parametrize("case", LOW, ids=["heads", "runs", "rows"])
+@pytest.mark.parametrize("fmt", [FP8, I8])
+def test_keys_at_the_least_scales(case, fmt):
+    """The same for keys, under queries so large (2^112 and about) that their scores are ordinary ones."""
+    case = case + (fmt,)
+    gen = torch.Generator().manual_seed(22)
+    kc, vc, ks, vs, table = cache_for(case, gen)
+    u = bytes_of(ks)
+    u[u != 255] = torch.randint(0, 3, u[u != 255].shape, generator=gen).to(torch.uint8)
+    B, H, _, T, _, _, lens, _, dk, _, window, n_sink, dtype, _ = case
+    q = (torch.randn(B, H, T, dk, generator=gen).clamp(-3.9, 3.9) * 2.0 ** 112).to(dtype)
+    scale = 64.0 / math.sqrt(dk)   # numbers of 100 times 2^-126 times 2^112: 2^-7 a pair of a query's and a key's dims
+    o = paged8_attention(q.cuda(), *(x.cuda() for x in (kc, vc, ks, vs)), table.cuda(), ints(lens), window, n_sink, scale).cpu()
+    check(case, o, q, (kc, vc, ks, vs, table), [T] * B, scale)
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
