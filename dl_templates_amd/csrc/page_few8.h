@@ -104,6 +104,12 @@ DLT_DEV void few8_turn(const unsigned (&r)[4], unsigned (&t)[4]) {
   t[3] = __builtin_amdgcn_perm(y1, x1, 0x07060302);
 }
 
+// Whole numbers: P times the scale of its key's values enters its product in bfloat16, whose least numbers are 2^-133; scales go down to 2^-127, and a key's share of a sum to
+// far less than its P of 1.  So P is taken times 2^32, and the sums times 2^-32 when they are done: at the least scale a P of 2^-38 still counts.  From scales of about 2^80 on that
+// does not fit 32 bits any more: those rows come out infinite or NaN and are formed again one by one, without it.
+constexpr int FEW8_LIFT = 32;
+DLT_DEV float few8_lifted(int e) { return __uint_as_float((unsigned)dlt_imin(e + FEW8_LIFT, 255) << 23); }   // 255 and beyond the exponents: infinite
+
 // Operands of 8 numbers.  e4m3: one instruction for two, which also takes the scale.  Whole numbers enter the products as they are, exact in both types, and their scales
 // multiply scores and P instead; values, and P, enter as bfloat16 whatever q's type is, whose exponents hold every scale (P's two parts keep 16 bits of it).
 DLT_DEV unsigned few8_ints_bf16(unsigned w, bool hi) {   // whole numbers in 32 bits have no bits set below bfloat16's
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
           if constexpr (FMT == DLT_INT8) {
             // values enter as whole numbers, their scales here: a block of 16 tokens has one
 #pragma unroll
-            for (int j = 0; j < 8; j++) e[j] *= cvt8_scale(ev[2 * kb + (j >> 2)]);
+            for (int j = 0; j < 8; j++) e[j] *= few8_lifted(ev[2 * kb + (j >> 2)]);
           }
           ph[p][kb] = pack8<PT>(e);
           unpack8<PT>(ph[p][kb], r);
@@ -414,7 +420,11 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
     for (int p = 0; p < NP; p++) {
       char* mine = smem + (wave * NP + p) * F::WAVE_LDS;
 #pragma unroll
-      for (int d = 0; d < VB; d++) *reinterpret_cast<f32x4*>(mine + 1024 * d + 16 * lane) = acc[p][d];
+      for (int d = 0; d < VB; d++) {
+        f32x4 x = acc[p][d];
+        if constexpr (FMT == DLT_INT8) x *= __uint_as_float((unsigned)(127 - FEW8_LIFT) << 23);
+        *reinterpret_cast<f32x4*>(mine + 1024 * d + 16 * lane) = x;
+      }
       const float l = wave_sum4(l_run[p]);
       if (g == 0) *reinterpret_cast<float2*>(mine + 1024 * VB + 8 * n) = float2{m_run[p] * scale, l};
     }

@@ -30,6 +30,22 @@ LOW = [(2, 4, 2, 1, 32, 16, [700, 90], None, 64, 64, None, 0, BF), (2, 8, 2, 3, 
 
 @pytest.mark.parametrize("case", LOW, ids=["heads", "runs", "rows"])
 @pytest.mark.parametrize("fmt", [FP8, I8])
+def test_values_at_the_least_scales(case, fmt):
+    """Scales of 2^-127 to 2^-121 on the values: no key's share of a sum is lost, however small its probability."""
+    case = case + (fmt,)
+    gen = torch.Generator().manual_seed(21)
+    kc, vc, ks, vs, table = cache_for(case, gen)
+    u = bytes_of(vs)
+    u[u != 255] = torch.randint(0, 7, u[u != 255].shape, generator=gen).to(torch.uint8)
+    B, H, _, T, _, _, lens, _, dk, _, window, n_sink, dtype, _ = case
+    q = torch.randn(B, H, T, dk, generator=gen).to(dtype)
+    scale = 1.0 / math.sqrt(dk)
+    o = paged8_attention(q.cuda(), *(x.cuda() for x in (kc, vc, ks, vs)), table.cuda(), ints(lens), window, n_sink, scale).cpu()
+    check(case, o, q, (kc, vc, ks, vs, table), [T] * B, scale)
+
+
+@pytest.mark.parametrize("case", LOW, ids=["heads", "runs", "rows"])
+@pytest.mark.parametrize("fmt", [FP8, I8])
 def test_keys_at_the_least_scales(case, fmt):
     """The same for keys, under queries so large (2^112 and about) that their scores are ordinary ones."""
     case = case + (fmt,)
