@@ -414,6 +414,24 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
       __builtin_amdgcn_sched_barrier(0);
     }
 
+    // Whole-number keys meet q without their scales.  From 2^114 on (inputs of bfloat16 only) such a sum of up to 128 products of up to 2^7 each can leave 32 bits, and an infinity
+    // with the sign of a small probability would not be seen in the sums: rows with such an element of q are formed again, from keys with their scales.
+    bool huge[NP];
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+      huge[p] = false;
+      if constexpr (FMT == DLT_INT8 && std::is_same<TIO, bf16_t>::value) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 most = {0, 0};
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, qf[p][c][i] & 0x7fff7fffu));
+        constexpr unsigned short limit = (127 + 114) << 7;
+        huge[p] = most[0] >= limit || most[1] >= limit;
+      }
+    }
+
     // ---- the waves' results, joined: four waves take a quarter of the blocks of output dims each
     if (tid < NP) odd_rows[tid] = 0u;
 #pragma unroll
@@ -458,7 +476,7 @@ __global__ __launch_bounds__(64 * NW, NW > 4 ? 4 : NP == 1 ? 3 : 2) void few8_ke
           for (int i = 0; i < 4; i++) o[p][d][i] = fmaf(v[i], f, o[p][d][i]);
         }
       }
-      bool bad = band_odd(ol[p]);
+      bool bad = band_odd(ol[p]) || huge[p];
 #pragma unroll
       for (int d = 0; d < OB; d++)
 #pragma unroll

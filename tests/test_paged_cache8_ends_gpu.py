@@ -1,4 +1,4 @@
-"""The paged cache in 8 bits where numbers end: scales at both ends of their byte (GPU)."""
+"""The paged cache in 8 bits where numbers end: scales at both ends of their byte, queries near the type's largest number (GPU)."""
 import math
 
 import pytest
@@ -81,3 +81,23 @@ def test_tokens_join_a_block_of_any_scale(old, fmt, dtype):
     for i, (c, e, _, near) in enumerate(want):
         assert torch.equal(bytes_of(got[2 + i].cpu()).int(), e)
         assert torch.equal(got[i].cpu().float().double(), c)
+
+
+@pytest.mark.parametrize("case", LOW, ids=["heads", "runs", "rows"])
+@pytest.mark.parametrize("fmt", [FP8, I8])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_queries_near_the_largest_number(case, fmt, sign):
+    """Queries of 2^122 over keys of 2^-121: products without the keys' scales would leave 32 bits.  Scores are about -3 or 3, all of one sign, unequal from key to key."""
+    case = case + (fmt,)
+    gen = torch.Generator().manual_seed(24)
+    kc, vc, ks, vs, table = cache_for(case, gen)
+    kc.copy_((kc.float().abs().nan_to_num(1.0) % 64 + 64).to(fmt))
+    u = bytes_of(ks)
+    u[u != 255] = 0
+    B, H, _, T, _, _, lens, _, dk, _, window, n_sink, dtype, _ = case
+    q = torch.randn(B, H, T, dk, generator=gen).abs().clamp(0.1, 3.9)
+    q[:, ::2] *= 2.0 ** -14   # beside rows that need nothing of the kind
+    q = (q * (sign * 2.0 ** 122)).to(dtype)
+    scale = 2.0 / dk   # 96 2^-127 2^122 0.8 dk times that: 4.8; rows of even heads: none to speak of
+    o = paged8_attention(q.cuda(), *(x.cuda() for x in (kc, vc, ks, vs)), table.cuda(), ints(lens), window, n_sink, scale).cpu()
+    check(case, o, q, (kc, vc, ks, vs, table), [T] * B, scale)
