@@ -159,11 +159,14 @@ __global__ __launch_bounds__(NT) void page_assign_kernel(AssignArgs a) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) served = dlt_imax(served, __shfl_xor(served, d));
   if ((tid & 63) == 0) most[tid >> 6] = served;
+  asm volatile("" ::"v"(F));   // waves without a request need it only behind the count: a barrier waits for no load from memory
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < NT / 64; i++) served = dlt_imax(served, most[i]);
   // Every load of lengths and of the pool's count by this workgroup has returned: as far as it is concerned they may be written.  Counted here, beside the work, and looked at behind
   // it (4000 requests, a token more and back, 22.4 -> 21.2 us); by many workgroups, which would queue up here (10 ns each), behind it too (1000 requests, 4000 slots 21.9 -> 21.0).
+  // Nothing that one workgroup writes is read by another, so the addition needs no release and acquire, which would write caches back and empty them (1000 requests, 4000 slots and back
+  // 20.0 -> 27.1; 4000 requests, a token more and back, 21.7 -> 22.6): what has to come before it are loads, and those are waited for.
   const bool early = gridDim.x <= 64;
   int before = 0;
   auto count = [&]() __attribute__((always_inline)) {

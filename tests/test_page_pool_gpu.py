@@ -143,3 +143,28 @@ def test_tables_of_a_16_bit_cache():
             x = given[b][0][None]
             assert x.shape[3] == s.seq[b]
             long_orc.check(o[b:b + 1, :, :m], long_orc.window(q[b:b + 1, :, :m], x[:, 0], x[:, 1], None, 0, 0.1)["o"], f"request {b}")
+
+
+@pytest.mark.parametrize("B, T", [(5, 3000), (300, 200), (300, 700), (1000, 60), (1500, 30)])
+def test_many_calls_by_many_workgroups(B, T):
+    """Waves without a request beside those that have some, up to 64 workgroups and more: pages handed out and taken back again and again, each time as in the first one."""
+    rng = random.Random(4)
+    page, cols = 16, 200
+    held = [rng.randint(0, cols * page - T) for _ in range(B)]
+    want = [n + rng.randint(0, T) if rng.random() < 0.6 else rng.randint(0, n) for n in held]
+    s = Both(B, cols, page, B * cols)
+    s.call(held)
+    table, seq, pool = s.dev
+    up, down, seen = ints(want), ints(held), []
+    for _ in range(60):
+        state = []
+        for w, t in ((up, T), (down, None)):
+            n_new, slots = page_assign_(table, seq, w, pool, page, t)
+            state += [n_new, slots, seq.clone(), table.clone(), pool.clone()]
+        seen.append(state)
+    s.call(want, T)   # against the loop
+    for i, state in enumerate(seen):
+        left = 2 + int(state[4][0])
+        assert torch.equal(state[2], up) and torch.equal(state[7], down) and left == 2 + len(s.free)
+        for j, (x, first) in enumerate(zip(state, seen[0])):
+            assert x is None or torch.equal(x[:left] if j in (4, 9) else x, first[:left] if j in (4, 9) else first), (i, j)
