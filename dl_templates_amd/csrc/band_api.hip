@@ -577,6 +577,11 @@ bool plan_few8(Few8Args& a) {
   dlt_fastdiv_make((uint32_t)a.Hkv, a.by_heads.m, a.by_heads.s);
   return true;
 }
+// a launch holds fewer than 2^32 threads
+int check_few8(const char* who, const Few8Args& a) {
+  if ((a.wgs != 0 ? a.wgs : (int64_t)a.B * a.Hkv) * 64 * a.waves > 0xffffffff) return dlt_set_error(DLT_ERR_UNSUPPORTED, "%s: too many workgroups", who);
+  return DLT_OK;
+}
 // More rows than that: as plan_rows has it, without its kinds of several groups of waves, and with 128 rows a workgroup, which become 16-bit keys and values half as often, also
 // where their keys have to be shared for two workgroups a CU, while a share has chunks enough: 12, or 8 where blocks of 64 rows would not fill the chip either.  us, by
 // 64 rows / 128: 8 kv heads of 4 query heads, d = 128, 8192 keys, 128 queries 48 / 46, 256 73 / 64, 512 130 / 98, 1024 216 / 168; 8 sequences of 64 queries on up to 4000 82 / 65;
@@ -626,7 +631,7 @@ extern "C" int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const 
   const bool few = plan_few8(a);
   const int kind = few ? 0 : plan_rows8(a);
   if ((rc = check_ws(who, ws, ws_bytes, few ? few8_bytes(a) : rows_bytes(a))) != DLT_OK) return rc;
-  if (!few && (rc = check_grid(who, a)) != DLT_OK) return rc;
+  if ((rc = few ? check_few8(who, a) : check_grid(who, a)) != DLT_OK) return rc;
   if (dlt_route_note(DLT_FAMILY_BAND) || a.Lq == 0) return DLT_OK;
   a.q = q; a.k = k_cache; a.v = v_cache; a.out = o; a.part = (float*)ws;
   strides3(a.qs, q_strides); strides3(a.ks, k_cache_strides); strides3(a.vs, v_cache_strides); strides3(a.os, o_strides);

@@ -199,3 +199,11 @@ def test_the_loop_that_hands_out_pages():
     # the first ends: its pages come back, the last one first, and go to the second (two more) and the third
     assert orc8.assign(table, seq, [0, 33, 1], free, 16, None) == ([0, 28, 1], [[], [], []])
     assert seq == [0, 33, 1] and free == [] and table == [[0, 1, -1], [2, 0, 1], [3, -1, -1]]
+
+
+def test_more_heads_than_a_launch_holds(L):
+    """Up to 32 rows of a group have a workgroup to a (batch, kv head) or a run: their number must not wrap (2^20 x 2^12 heads came out as a launch of none)."""
+    for B, Hkv in ((1 << 20, 1 << 12), (1 << 24, 1), ((1 << 31) - 1, 3)):
+        for G in (1, 20):
+            assert attend(L, B=B, H=G * Hkv, Hkv=Hkv, dk=8, dv=8) == 2 and "workgroups" in err(L), (B, Hkv, G)
+    assert attend(L, B=(1 << 24) - 1, H=1, Hkv=1, dk=8, dv=8) == 0, err(L)
