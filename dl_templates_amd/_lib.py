@@ -34,7 +34,7 @@ EXPORTS = (
 )
 KERNEL_FAMILIES = ("none", "marching", "streaming", "tile", "flash", "generic", "band")   # DLT_FAMILY_* of include/dlt.h
 NOALLOC_MAX_DELTA = 1 << 20  # DLT_NOALLOC_MAX_DELTA of include/dlt.h
-KERNEL_NAMES = ("rope2d", "attn_fwd", "attn_delta", "attn_bwd_kv", "attn_bwd_q")
+KERNEL_NAMES = ("rope2d", "attn_fwd", "attn_delta", "attn_bwd_kv", "attn_bwd_q", "page_assign")
 
 
 class DltError(RuntimeError):

@@ -259,7 +259,9 @@ extern "C" int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* se
   const int lds = 4 * (B + 1) * 4;
   const int rc = dlt_ensure_lds(reinterpret_cast<const void*>(page_assign_kernel<NT>), lds);
   if (rc != DLT_OK) return rc;
+  dlt_timing_before(DLT_K_PAGES, stream);
   hipLaunchKernelGGL(page_assign_kernel<NT>, dim3((unsigned)grid), dim3(NT), lds, stream, a);
+  dlt_timing_after(stream);
   DLT_CHECK_LAUNCH("page_assign launch");
   return DLT_OK;
 }

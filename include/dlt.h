@@ -414,13 +414,14 @@ int dlt_page_assign(int32_t* table, int64_t table_stride, int32_t* seq_len, cons
 /* ---- per-kernel timing (measurement aid) ---------------------------------------------------
  * Counterpart of the reference's triton.testing.do_bench calls (src/tiled_swa.py:765-774,
  * src/flash_attn.py:592,606), at kernel granularity.  While enabled for the calling thread,
- * every kernel the library launches, but for dlt_page_assign's, is bracketed by a pair of hipEvents recorded on the
+ * every kernel the library launches is bracketed by a pair of hipEvents recorded on the
  * launch stream.  A backward launch that forms dq, dk and dv together (tiles of 16 tokens with a 3 x 3
  * window, head dim 32 / 64; narrow grids at 32 excepted) is recorded as DLT_K_BWD_KV, without a
- * DLT_K_BWD_Q beside it.  A flash pass split with a workspace gives a second record of its kind for the sum.  dlt_timing_collect waits for the recorded events, writes up to `max`
+ * DLT_K_BWD_Q beside it.  A call whose keys are shared by workgroups (with a workspace) gives a second record of its kind for the sum; appends are recorded as
+ * DLT_K_ROPE.  dlt_timing_collect waits for the recorded events, writes up to `max`
  * records in launch order, stores the number available in *n and clears the list.
  * Enabling creates events lazily (host-side handles only, no device allocation). */
-enum { DLT_K_ROPE = 0, DLT_K_FWD = 1, DLT_K_DELTA = 2, DLT_K_BWD_KV = 3, DLT_K_BWD_Q = 4, DLT_K_COUNT = 5 };
+enum { DLT_K_ROPE = 0, DLT_K_FWD = 1, DLT_K_DELTA = 2, DLT_K_BWD_KV = 3, DLT_K_BWD_Q = 4, DLT_K_PAGES = 5, DLT_K_COUNT = 6 };
 typedef struct {
   int32_t kernel; /* DLT_K_* */
   float ms;

@@ -505,3 +505,32 @@ def test_scales_behind_a_sequence_leave_every_bit(T, lens, d, fmt):
             u[u == 255] = byte   # cache_for leaves NaN there and nowhere else
         out.append(paged8_attention(q, *(x.cuda() for x in parts), table.cuda(), ints(lens), None, 0, 0.1))
     assert all(torch.equal(x, out[0]) for x in out) and torch.isfinite(out[0]).all()
+
+
+def records_of(call):
+    """(what the call gives, names of the launches that it leaves on record)"""
+    from dl_templates_amd import _lib
+    _lib.timing_enable(True)
+    try:
+        out = call()
+        records = _lib.timing_collect()
+    finally:
+        _lib.timing_enable(False)
+    assert all(ms > 0 for _, ms in records)
+    return out, [n for n, _ in records]
+
+
+@pytest.mark.parametrize("T, lens, d, launches", [(1, [300], 64, 1), (1, [5000, 700], 128, 2), (6, [5000, 700], 128, 2), (100, [200], 128, 1), (40, [5000], 64, 2), (100, [5000], 128, 2)])
+@pytest.mark.parametrize("fmt", [FP8, I8])
+def test_every_launch_leaves_a_record(T, lens, d, launches, fmt):
+    """Whole heads and unshared rows are one launch, runs and shared keys two; an append and a call for pages one each."""
+    B = len(lens)
+    case = (B, 8, 2, T, 64, 64, lens, None, d, d, None, 0, BF, fmt)
+    kc, vc, ks, vs, table = (x.cuda() for x in cache_for(case, torch.Generator().manual_seed(41)))
+    k, v, q = (torch.randn(B, h, T, d, dtype=BF, device="cuda") for h in (2, 2, 8))
+    assert records_of(lambda: paged8_append_(kc, vc, ks, vs, k, v, table, ints(lens), None, None, q))[1] == ["rope2d"]
+    o, names = records_of(lambda: paged8_attention(q, kc, vc, ks, vs, table, ints(lens)))
+    assert names == ["attn_fwd"] * launches and torch.equal(o, paged8_attention(q, kc, vc, ks, vs, table, ints(lens)))
+    pages, seq = page_pool(64), ints([0] * B)
+    (n_new, _), names = records_of(lambda: page_assign_(torch.zeros(B, 9, dtype=torch.int32, device="cuda"), seq, ints([77] * B), pages, 16))
+    assert names == ["page_assign"] and n_new.tolist() == [77] * B
