@@ -234,8 +234,9 @@ __global__ __launch_bounds__(64 * NW * GR, NW * GR == 4 ? 2 : 1) void band_fwd_k
   auto put8 = [&](char* buf, auto jc) __attribute__((always_inline)) {
     constexpr int j = decltype(jc)::value;
     char* dst = buf + wave * 16 * 2 * D;
-    if constexpr (j < 2 * S8::NI) stk8.template put<j>(dst, rk, cvt8_scale(ek));
-    else stv8.template put<j - 2 * S8::NI>(dst + B::REG, rv, cvt8_scale(ev));
+    // (one scale for the wave: formed by the scalar unit; 512 tokens over 8192, int8 / e4m3 108.5 / 99.8 -> 105.6 / 95 us)
+    if constexpr (j < 2 * S8::NI) stk8.template put<j>(dst, rk, cvt8_scale(__builtin_amdgcn_readfirstlane(ek)));
+    else stv8.template put<j - 2 * S8::NI>(dst + B::REG, rv, cvt8_scale(__builtin_amdgcn_readfirstlane(ev)));
   };
   if constexpr (F8 != 0) {
     stk8.init(lane, a.dk_, a.ks[2]);
