@@ -10,7 +10,7 @@
 // waves with twice the rows in registers: 60 us for 36).  Rows of q are rotated by workgroups of their own in the same launch, a wave to some tokens, the heads one after
 // the other under one fetch of cos and sin.
 //
-// Memory bound: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 30 us, 4.5 TB/s; 7 of up to 2047, 16 + 8 + 8, d = 64, blocks of 16 17 to 19 us, 80 MB with
+// Memory bound: 4 sequences of 1500 tokens, 32 + 8 + 8 heads, d = 128, blocks of 64 30 us, 4.5 TB/s (from fp32 59, 4.4 TB/s); 7 of up to 2047, 16 + 8 + 8, d = 64, blocks of 16 17 to 19 us, 80 MB with
 // the rows of q that hold no token.  A token each of 64 sequences: 5 us on the GPU, latency: length, page, row.
 #include <algorithm>
 #include "attn_common.hpp"

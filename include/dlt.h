@@ -382,7 +382,7 @@ typedef struct {
  * at least), rotated in 32 bits; a block whose first token is new takes e_need, another the larger of its e and e_need, and where that is larger its older tokens'
  * numbers are rounded anew.  Numbers are x 2^-e rounded to nearest, even ones at ties, and so bounded that DLT_FP16 inputs come back finite in fp16.  An element
  * that is infinite or NaN becomes NaN: a number of e4m3, for int8 the scale of its block, which then stays NaN until the block's first token is new again.
- * dk and dv multiples of 8 up to 128; rows of k, v, q, q_out, k_cache and v_cache contiguous, those of k, v, q and q_out at multiples of 16 bytes, of the caches at
+ * A block gets tokens of one sequence in a call.  dk and dv multiples of 8 up to 128; rows of k, v, q, q_out, k_cache and v_cache contiguous, those of k, v, q and q_out at multiples of 16 bytes, of the caches at
  * multiples of 8. */
 int dlt_paged8_append(const void* k, const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
                       const void* q, const int64_t q_strides[4], void* q_out, const int64_t q_out_strides[4],
@@ -390,8 +390,8 @@ int dlt_paged8_append(const void* k, const int64_t k_strides[4], const void* v, 
                       const dlt_scales8_t* scales, const int32_t* table, int64_t table_stride, const int32_t* seq_len, const int32_t* n_new,
                       const dlt_rope_axes_t* rope, const dlt_paged_shape_t* shape, void* stream);
 
-/* dlt_paged_attn over such a cache: keys and values are read as numbers of q's type, which for DLT_FP16 have to be 65504 at most (an append of DLT_FP16 sees to
- * that).  Cache rows contiguous, at multiples of 8 bytes. */
+/* dlt_paged_attn over such a cache: keys and values are read as numbers of q's type (those of DLT_INT8, in calls of up to 32 rows a kv head, as they are), which for
+ * DLT_FP16 have to be 65504 at most (an append of DLT_FP16 sees to that).  Cache rows contiguous, at multiples of 8 bytes. */
 int dlt_paged8_workspace(const dlt_paged_shape_t* shape, const dlt_scales8_t* scales, int64_t* bytes);
 int dlt_paged8_attn(const void* q, const int64_t q_strides[4], const void* k_cache, const int64_t k_cache_strides[4],
                     const void* v_cache, const int64_t v_cache_strides[4], const dlt_scales8_t* scales, void* o, const int64_t o_strides[4],
